@@ -45,6 +45,8 @@ COMPONENTS = {
     "general_delta": ("general_delta.cu",),
     "linear": ("linear_attn.cu",),
     "ssd": ("ssd.cu",),
+    # training: the loss behind the output layer
+    "token_loss": ("token_loss.cu",),
 }
 
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -154,6 +154,12 @@ COMPONENT_SIGS = {
         "ipex_ssd_chunks": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, vp, vp, ci, ci, vp, vp, vp,
                             ci, ci, ci, ci, ci, ci, vp, vp],
     },
+    "token_loss": {
+        "ipex_token_logprobs": [vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, i64, ci, ci, i64, cf, ci, vp, vp],
+        "ipex_token_logprobs_grad": [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, ci, i64, cf, ci, vp],
+        "ipex_distill": [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, ci, ci, cf, ci, vp, vp],
+        "ipex_distill_grad": [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, ci, ci, cf, ci, vp],
+    },
     "linear": {
         "ipex_linear_chunks_ok": [ci, ci, ci],
         "ipex_linear_fused_ok": [ci],
