@@ -45,7 +45,8 @@ COMPONENTS = {
     "general_delta": ("general_delta.cu",),
     "linear": ("linear_attn.cu",),
     "ssd": ("ssd.cu",),
-    # training: the loss behind the output layer
+    # training: attention with a gradient, the loss behind the output layer
+    "train_attn": ("attn_train_tcgen05.cu",),
     "token_loss": ("token_loss.cu",),
 }
 

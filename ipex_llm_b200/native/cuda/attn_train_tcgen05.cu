@@ -1,0 +1,1169 @@
+// Attention with a gradient on the 5th-generation tensor cores, sm_100a: forward keeps one number a row (the logarithm of the
+// soft-max's sum), backward computes the probabilities from it again.
+//
+//   s_ij = scale q_i . k_j     P_ij = e^(s_ij - L_i)     o_i = sum_j P_ij v_j          L_i = log sum_j e^(s_ij) over seen keys
+//   dP_ij = dO_i . v_j         delta_i = dO_i . o_i      dS_ij = P_ij (dP_ij - delta_i)
+//   dq_i = scale sum_j dS_ij k_j      dk_j = scale sum_i dS_ij q_i      dv_j = sum_i P_ij dO_i
+//
+// Query i sees key j if the key is not hidden and, when causal, j <= i + Skv - Sq, and with a window also
+// j > i + Skv - Sq - window.  A row that sees nothing gives zeros and gets no gradient.  Key heads are shared by Hq / Hkv
+// query heads; their gradients are summed over those inside one CTA, in a fixed order: no result depends on an order of atomics.
+//
+// Tiles are 128 x 128.  All operands come by TMA from 4-D maps (width, rows, heads, sequences) of the tensors as they lie, in
+// the 128-byte swizzle; what lies outside of a sequence, or past a head's width, reads as zero.  One tile in shared memory
+// serves as a K-major operand (rows are M or N: q, k in s; dO, v in dP) and as an MN-major one (rows are summed over: v in o,
+// k in dq, q and dO in dk and dv).  Probabilities and dS go back to tensor memory in 16 bits, over the scores that they were
+// made from, and are the products' first operand there.
+//
+// The products are issued by one warp in an order that leaves the soft-max of one tile under the products of another:
+//   forward     two tiles of queries with four warps each, one thread to a row, take turns
+//   dk and dv   transposed scores (rows are keys), so that P^T and dS^T are what the products want; s of the next step runs
+//               under this step's dS, dP of the next under the next P
+//   dq          a pass of its own over the keys, which computes s and dP once more (7 products in all where 5 would do): the
+//               sums then need no atomics, whose order would change results, and no 32-bit dq in global memory
+//
+// In fp16 the range of dS is what is short, not its precision: P is taken times 2^12, and dP - delta times a power of two that a
+// bound on |dO_i| |v_j| gives for each group of heads, so that the largest dS comes near 2^15.  Both go out of the results again.
+//
+// Every wait is bounded; one that runs out raises the CTA's abort flag, all roles leave, and the error word gets 71 (loader), 72
+// (products), 73 (soft-max).  No cluster multicast.
+#include "common/utils.cuh"
+#include "tcgen05_common.cuh"
+
+namespace {
+
+using namespace tc5;
+
+constexpr int kT = 128;           // rows of a tile of queries or keys
+constexpr int kThreads = 320;     // eight warps of arithmetic, the loader, the products
+constexpr uint32_t kTmemCols = 512;
+constexpr int kShiftF16 = 12;     // P is stored times 2^12 in fp16
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Four-dimensional tile load: 64 columns from x on of 128 rows from y on of head h, sequence b.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* tm, int x, int y, int h, int b, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(h), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
+// A tile of D columns: D / 64 blocks of [128 rows x 128 bytes] behind one another.
+template <int D>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* tm, int row, int h, int b, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) tma_load_4d(dst + c * (kT * 128), tm, c * 64, row, h, b, bar);
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// 32 lanes x 32 columns without the wait, and the wait; values are there only behind it.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(float (&v)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+f"(v[j]));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] . B[smem]; issued by one thread.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+// The same tile read with its rows as the summed-over dimension (MN-major): 64 columns of 128 bytes are one swizzle atom wide,
+// atoms of further columns follow after a block of 128 rows (leading offset), groups of eight rows after 1024 bytes (stride).
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)((kT * 128) >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+constexpr uint32_t kBMajorMN = 1u << 16;
+
+// acc = A . B^T over D columns, both tiles K-major.
+template <int D>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      umma_f16(d, a + c * (kT * 128 >> 4) + 2 * kk, b + c * (kT * 128 >> 4) + 2 * kk, idesc, (c | kk) != 0);
+}
+// acc (+)= A . B over 128 rows of B: A in tensor memory, 16 bits; its second half begins `half` columns behind the first.
+__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t a, int half, uint64_t b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    umma_ts(d, a + (kk < 4 ? kk * 8 : half + (kk - 4) * 8), b + kk * (16 * 128 >> 4), idesc, accumulate || kk != 0);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 32 columns of a row out of tensor memory, times `f`, to 16-bit memory; columns from `width` on do not exist.
+template <typename T>
+__device__ __forceinline__ void put_row32(T* dst, const float (&v)[32], float f, int col, int width) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (col + 8 * q >= width) break;
+    uint4 w;
+    w.x = pack2<T>(v[8 * q] * f, v[8 * q + 1] * f);
+    w.y = pack2<T>(v[8 * q + 2] * f, v[8 * q + 3] * f);
+    w.z = pack2<T>(v[8 * q + 4] * f, v[8 * q + 5] * f);
+    w.w = pack2<T>(v[8 * q + 6] * f, v[8 * q + 7] * f);
+    *reinterpret_cast<uint4*>(dst + col + 8 * q) = w;
+  }
+}
+
+struct Shape {
+  int B, Hq, Hkv, Sq, Skv, D;
+  int causal, window;        // window 0: none
+  int q_pad;                 // row stride of the statistics: Sq rounded up to 128
+  int k_words;               // 32-bit words of a sequence's mask of keys
+  const uint32_t* mask;      // [B, k_words] or null: bit j: key j is real
+  float scale, scale_log2;
+  int* err;
+};
+
+// Bits [lo, hi) of the 32 from bit `at` on.
+__device__ __forceinline__ uint32_t range_bits(int lo, int hi, int at) {
+  lo = min(max(lo - at, 0), 32);
+  hi = min(max(hi - at, 0), 32);
+  const uint32_t below_hi = hi >= 32 ? 0xFFFFFFFFu : (1u << hi) - 1;
+  const uint32_t below_lo = lo >= 32 ? 0xFFFFFFFFu : (1u << lo) - 1;
+  return below_hi & ~below_lo;
+}
+
+// Blocks of keys that rows [q0, q0 + 128) may see.
+__device__ __forceinline__ void key_blocks(const Shape& s, int q0, int& j0, int& j1) {
+  const int off = s.Skv - s.Sq, last = min(q0 + kT, s.Sq) - 1;
+  const int hi = last < q0 ? 0 : s.causal ? min(s.Skv, last + off + 1) : s.Skv;
+  const int lo = s.window > 0 ? max(0, q0 + off - s.window + 1) : 0;
+  j0 = lo / kT;
+  j1 = hi > lo ? (hi + kT - 1) / kT : j0;
+}
+// The keys of a row: [lo, hi).
+__device__ __forceinline__ void row_keys(const Shape& s, int q, int& lo, int& hi) {
+  const int off = s.Skv - s.Sq;
+  hi = s.causal ? min(s.Skv, q + off + 1) : s.Skv;
+  lo = s.window > 0 ? max(0, q + off - s.window + 1) : 0;
+}
+
+// What a CTA takes down in every case.
+__device__ __forceinline__ void finish(uint32_t tmem_base, int warp) {
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 9) tmem_dealloc(tmem_base, kTmemCols);
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+struct FwdArgs {
+  Shape s;
+  void* out;          // [B, Sq, Hq, D]
+  float* nlse;        // [B, Hq, q_pad]: -L log2(e) (+ the shift of fp16); -inf for rows that see nothing and past Sq
+  float shift;
+};
+
+template <int D>
+struct FwdSmem {
+  static constexpr int kTile = kT * D * 2;
+  static constexpr int kStages = D == 128 ? 5 : 6;
+  static constexpr int kBars = (2 + kStages) * kTile;
+  static constexpr int kSize = 1024 + kBars + 256;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdArgs a) {
+  using L = FwdSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + 2 * L::kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* q_full = bars;
+  uint64_t* kv_full = bars + 1;
+  uint64_t* kv_empty = kv_full + L::kStages;
+  uint64_t* s_full = kv_empty + L::kStages;    // [2]
+  uint64_t* p_full = s_full + 2;               // [2]
+  uint64_t* o_full = p_full + 2;               // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const Shape& s = a.s;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int h = blockIdx.x, b = blockIdx.z, kvh = h / (s.Hq / s.Hkv);
+  // the longest rows first
+  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 2 * kT;
+  int j0[2], j1[2];
+  key_blocks(s, q0, j0[0], j1[0]);
+  key_blocks(s, q0 + kT, j0[1], j1[1]);
+  const int ja = j1[1] > j0[1] ? (j1[0] > j0[0] ? min(j0[0], j0[1]) : j0[1]) : j0[0];
+  const int jb = j1[1] > j0[1] ? max(j1[0], j1[1]) : j1[0];
+  const int n_tiles = q0 + kT < s.Sq ? 2 : 1;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, kTmemCols);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 8) {
+    // ---------------- loader: keys and values of a block take a stage each, in turn ----------------
+    if (lane == 0 && ja < jb) {
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      mbar_expect_tx(q_full, n_tiles * L::kTile);
+      for (int t = 0; t < n_tiles; ++t) load_tile<D>(sQ + t * L::kTile, &tm_q, q0 + t * kT, h, b, q_full);
+      bool ok = true;
+      int n = 0;
+      for (int j = ja; j < jb && ok; ++j)
+        for (int w = 0; w < 2 && ok; ++w, ++n) {
+          const int st = n % L::kStages;
+          if (!mbar_wait(&kv_empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+          mbar_expect_tx(&kv_full[st], L::kTile);
+          load_tile<D>(sKV + st * L::kTile, w ? &tm_v : &tm_k, j * kT, kvh, b, &kv_full[st]);
+        }
+      if (!ok) {
+        mbar_wait_quiet(q_full, 0, 1 << 12);
+        for (int i = n - L::kStages < 0 ? 0 : n - L::kStages; i < n; ++i)
+          mbar_wait_quiet(&kv_full[i % L::kStages], i / L::kStages & 1, 1 << 12);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---------------- products ----------------
+    const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
+    const uint64_t qd = make_desc_sw128(smem_u32(sQ)), kd = make_desc_sw128(smem_u32(sKV)), vd = make_desc_mn(smem_u32(sKV));
+    bool ok = ja >= jb || warp_wait(q_full, 0, abort_flag);
+    auto scores = [&](int t, int j) {            // of a tile that sees block j
+      if (elect_one()) {
+        mma_rows<D>(tmem + t * kT, qd + t * (L::kTile >> 4), kd + (uint64_t)(2 * (j - ja) % L::kStages * (L::kTile >> 4)), idesc_s);
+        umma_commit(&s_full[t]);
+      }
+      __syncwarp();
+    };
+    auto has = [&](int t, int j) { return j >= j0[t] && j < j1[t]; };
+    auto wait_kv = [&](int n) { return warp_wait(&kv_full[n % L::kStages], n / L::kStages & 1, abort_flag); };
+    auto free_kv = [&](int n) {
+      if (elect_one()) umma_commit(&kv_empty[n % L::kStages]);
+      __syncwarp();
+    };
+    if (ok && ja < jb) {
+      ok = wait_kv(0);
+      tcgen05_fence_after();
+      for (int t = 0; t < 2 && ok; ++t)
+        if (has(t, ja)) scores(t, ja);
+      if (ok) free_kv(0);
+    }
+    for (int j = ja; j < jb && ok; ++j) {
+      const int n = 2 * (j - ja);
+      ok = wait_kv(n + 1);
+      if (ok && j + 1 < jb) ok = wait_kv(n + 2);
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (has(t, j)) {
+          ok = warp_wait(&p_full[t], j - j0[t] & 1, abort_flag);
+          if (!ok) break;
+          tcgen05_fence_after();
+          if (elect_one()) {
+            mma_sum(tmem + 2 * kT + t * kT, tmem + t * kT, 32, vd + (uint64_t)((n + 1) % L::kStages * (L::kTile >> 4)), idesc_o,
+                    j > j0[t]);
+            umma_commit(&o_full[t]);
+          }
+          __syncwarp();
+        }
+        // over the probabilities that the product in front has read
+        if (j + 1 < jb && has(t, j + 1)) scores(t, j + 1);
+      }
+      if (!ok) break;
+      free_kv(n + 1);
+      if (j + 1 < jb) free_kv(n + 2);
+    }
+    if (!ok && lane == 0) report(s.err, 72);
+    __syncwarp();
+  } else {
+    // ---------------- soft-max: a thread to a row ----------------
+    const int t = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + t * kT, tO = tmem + lanes + 2 * kT + t * kT;
+    const int q = q0 + t * kT + r;
+    int klo, khi;
+    row_keys(s, q, klo, khi);
+    const float c = s.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = j0[t]; j < j1[t]; ++j) {
+      const int it = j - j0[t], k0 = j * kT;
+      if (!warp_wait(&s_full[t], it & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      tcgen05_fence_after();
+      float v[kT];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32(tS + 32 * i, v + 32 * i);
+      uint32_t see[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        see[i] = range_bits(klo - k0, khi - k0, 32 * i);
+        if (s.mask != nullptr) see[i] &= __ldg(s.mask + (int64_t)b * s.k_words + j * 4 + i);
+      }
+      const bool all = (see[0] & see[1] & see[2] & see[3]) == 0xFFFFFFFFu;
+      tmem_ld_wait(v);
+      if (!__all_sync(0xffffffffu, all)) {
+#pragma unroll
+        for (int i = 0; i < kT; ++i) v[i] = see[i >> 5] >> (i & 31) & 1 ? v[i] : -INFINITY;
+      }
+      float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+      for (int i = 4; i < kT; i += 4)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], v[i + u]);
+      const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      // The reference moves only when it falls behind by a factor of 2^8: until then sums and products stay below 2^8 times
+      // what they would be, far from the end of their range, and the outputs need not be read.
+      const bool move = (top - m) * c > 8.f;
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? ex2((m - top) * c) : 1.f;
+        l *= f;
+        if (move) m = top;
+        if (it > 0) {
+          if (!warp_wait(&o_full[t], (it - 1) & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+          tcgen05_fence_after();
+#pragma unroll
+          for (int cc = 0; cc < D; cc += 32) {
+            float o[32];
+            tmem_ld32(tO + cc, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            tmem_st32(tO + cc, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+      }
+      const float mc = m == -INFINITY ? 0.f : -m * c;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float p0 = ex2(fmaf(v[64 * g + 2 * i], c, mc)), p1 = ex2(fmaf(v[64 * g + 2 * i + 1], c, mc));
+          sum[i & 1] += p0;
+          sum[2 + (i & 1)] += p1;
+          pk[i] = pack2<T>(p0, p1);
+        }
+        tmem_st32(tS + 32 * g, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tcgen05_fence_before();
+      mbar_arrive(&p_full[t]);
+    }
+    const int n = j1[t] - j0[t];
+    if (ok && n > 0) {
+      ok = warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
+      if (!ok && lane == 0) report(s.err, 73);
+      tcgen05_fence_after();
+    }
+    if (ok && q0 + t * kT < s.Sq) {
+      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : NAN;   // a row without keys: zeros
+      if (a.nlse != nullptr) {
+        const bool none = q >= s.Sq || m == -INFINITY;
+        a.nlse[((int64_t)b * s.Hq + h) * s.q_pad + q] = none ? -INFINITY : a.shift - m * c - log2f(l);
+      }
+      T* dst = reinterpret_cast<T*>(a.out) + (((int64_t)b * s.Sq + q) * s.Hq + h) * s.D;
+#pragma unroll
+      for (int cc = 0; cc < D; cc += 32) {
+        float o[32];
+        if (n > 0) {
+          tmem_ld32(tO + cc, o);
+          tmem_ld_wait(o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (q < s.Sq) put_row32<T>(dst, o, inv, cc, s.D);
+      }
+    }
+  }
+  finish(tmem, warp);
+}
+
+// ------------------------------------------------------------------------------------------------ before the backward pass
+// delta_i = dO_i . o_i, a warp to a row (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
+// heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
+struct PrepArgs {
+  const void* out;         // [B, Sq, Hq, D]
+  const void* grad;        // by strides
+  const void* v;
+  int64_t g_b, g_h, g_s, v_b, v_h, v_s;
+  float* delta;            // [B, Hq, q_pad]
+  uint32_t* bound;         // [B, Hkv, 2] zeros, or null
+  int B, Hq, Hkv, Sq, Skv, D, q_pad;
+};
+
+template <typename T>
+__device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
+  const T *a = reinterpret_cast<const T*>(&x), *b = reinterpret_cast<const T*>(&y);
+  float d = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) d = fmaf(to_float<T>(a[i]), to_float<T>(b[i]), d);
+  return d;
+}
+
+// 16 lanes to a row (up to 128 columns, eight each): two rows to a warp.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
+  const int64_t rows_q = (int64_t)a.B * a.Hq * a.q_pad, rows_v = a.bound != nullptr ? (int64_t)a.B * a.Hkv * a.Skv : 0;
+  const int sub = threadIdx.x & 15;
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+  const bool in = 8 * sub < a.D;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  float d = 0.f, n = 0.f;
+  int64_t group = -1;
+  if (row < rows_q) {
+    const int64_t bh = row / a.q_pad, q = row % a.q_pad;
+    const int64_t b = bh / a.Hq, h = bh % a.Hq;
+    group = (b * a.Hkv + h / (a.Hq / a.Hkv)) * 2;
+    if (in && q < a.Sq) {
+      const uint4 g = *reinterpret_cast<const uint4*>((const T*)a.grad + b * a.g_b + h * a.g_h + q * a.g_s + 8 * sub);
+      const uint4 o = *reinterpret_cast<const uint4*>((const T*)a.out + ((b * a.Sq + q) * a.Hq + h) * a.D + 8 * sub);
+      d = dot8<T>(g, o);
+      if (a.bound != nullptr) n = dot8<T>(g, g);
+    }
+  } else if (row < rows_q + rows_v) {
+    const int64_t at = row - rows_q, bh = at / a.Skv, k = at % a.Skv;
+    const int64_t b = bh / a.Hkv, h = bh % a.Hkv;
+    group = bh * 2 + 1;
+    const uint4 w = in ? *reinterpret_cast<const uint4*>((const T*)a.v + b * a.v_b + h * a.v_h + k * a.v_s + 8 * sub) : zero;
+    n = dot8<T>(w, w);
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    d += __shfl_xor_sync(0xffffffffu, d, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (sub == 0 && row < rows_q) a.delta[row] = d;
+  if (sub == 0 && a.bound != nullptr && group >= 0 && n > __uint_as_float(a.bound[group])) atomicMax(&a.bound[group], __float_as_uint(n));
+}
+
+// fp16: the power of two for dP - delta.  |dP_ij - delta_i| <= 2 max |dO_i| max |v_j| (o_i is a mean of the v_j).
+__device__ __forceinline__ float grad_factor(const uint32_t* bound, int group, float shift) {
+  if (bound == nullptr) return 1.f;
+  const float n2 = 4.f * __uint_as_float(bound[2 * group]) * __uint_as_float(bound[2 * group + 1]);
+  if (!(n2 > 0.f && n2 < INFINITY)) return 1.f;
+  const int e = (int)floorf(15.f - 0.5f * log2f(n2) - shift);
+  return exp2f((float)min(max(e, -100), 100));
+}
+
+struct BwdArgs {
+  Shape s;
+  const float* nlse;      // [B, Hq, q_pad]
+  const float* delta;     // [B, Hq, q_pad]
+  const uint32_t* bound;  // [B, Hkv, 2] or null
+  void* dq;               // [B, Sq, Hq, D]
+  void* dk;               // [B, Skv, Hkv, D]
+  void* dv;
+  float shift;
+};
+
+// ------------------------------------------------------------------------------------------------ dk and dv
+template <int D>
+struct BwdSmem {
+  static constexpr int kTile = kT * D * 2;
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kStat = (2 + 2 * kStages) * kTile;       // nlse and delta of a stage's queries
+  static constexpr int kBars = kStat + kStages * 1024;
+  static constexpr int kSize = 1024 + kBars + 256;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
+                const __grid_constant__ BwdArgs a) {
+  using L = BwdSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + L::kTile;
+  uint8_t* sQG = smem + 2 * L::kTile;            // stages of [q | dO]
+  float* stat = reinterpret_cast<float*>(smem + L::kStat);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* kv_full = bars;
+  uint64_t* full = bars + 1;
+  uint64_t* empty = full + L::kStages;
+  uint64_t* s_full = empty + L::kStages;
+  uint64_t* p_full = s_full + 1;
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_full = s_full + 3;
+  uint64_t* done = s_full + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const Shape& s = a.s;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int kvh = blockIdx.x, b = blockIdx.z, group = s.Hq / s.Hkv;
+  const int k0 = blockIdx.y * kT;                // the first keys are seen by most queries, and come first
+  const int off = s.Skv - s.Sq;
+  // blocks of queries that may see these keys
+  const int qlo = s.causal ? max(0, k0 - off) : 0;
+  const int qhi = s.window > 0 ? min((int64_t)s.Sq, (int64_t)min(k0 + kT, s.Skv) - 1 + s.window - off) : s.Sq;
+  const int i0 = qlo / kT, ni = qhi > qlo ? (qhi + kT - 1) / kT - i0 : 0;
+  const int total = ni * group;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 256);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 256);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, kTmemCols);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot, tP = tmem + kT, tV = tmem + 2 * kT, tK = tmem + 3 * kT;
+
+  if (warp == 8) {
+    if (lane == 0 && total > 0) {
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_g);
+      mbar_expect_tx(kv_full, 2 * L::kTile);
+      load_tile<D>(sK, &tm_k, k0, kvh, b, kv_full);
+      load_tile<D>(sV, &tm_v, k0, kvh, b, kv_full);
+      bool ok = true;
+      int n = 0;
+      for (; n < total; ++n) {
+        const int st = n % L::kStages, h = kvh * group + n / ni, q0 = (i0 + n % ni) * kT;
+        if (!mbar_wait(&empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        mbar_expect_tx(&full[st], 2 * L::kTile + 1024);
+        load_tile<D>(sQG + 2 * st * L::kTile, &tm_q, q0, h, b, &full[st]);
+        load_tile<D>(sQG + (2 * st + 1) * L::kTile, &tm_g, q0, h, b, &full[st]);
+        const int64_t row = ((int64_t)b * s.Hq + h) * s.q_pad + q0;
+        bulk_load(stat + st * 256, a.nlse + row, 512, &full[st]);
+        bulk_load(stat + st * 256 + 128, a.delta + row, 512, &full[st]);
+      }
+      if (!ok) {
+        mbar_wait_quiet(kv_full, 0, 1 << 12);
+        for (int i = n - L::kStages < 0 ? 0 : n - L::kStages; i < n; ++i)
+          mbar_wait_quiet(&full[i % L::kStages], i / L::kStages & 1, 1 << 12);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
+    const uint64_t kd = make_desc_sw128(smem_u32(sK)), vd = make_desc_sw128(smem_u32(sV));
+    const uint64_t qg_rows = make_desc_sw128(smem_u32(sQG)), qg_sum = make_desc_mn(smem_u32(sQG));
+    auto at = [&](int n, int which) { return (uint64_t)((2 * (n % L::kStages) + which) * (L::kTile >> 4)); };
+    auto wait_full = [&](int n) { return warp_wait(&full[n % L::kStages], n / L::kStages & 1, abort_flag); };
+    auto scores = [&](int n) {                  // k q^T
+      if (elect_one()) {
+        mma_rows<D>(tmem, kd, qg_rows + at(n, 0), idesc_s);
+        umma_commit(s_full);
+      }
+      __syncwarp();
+    };
+    auto grads = [&](int n) {                   // v dO^T
+      if (elect_one()) {
+        mma_rows<D>(tP, vd, qg_rows + at(n, 1), idesc_s);
+        umma_commit(dp_full);
+      }
+      __syncwarp();
+    };
+    bool ok = total == 0 || (warp_wait(kv_full, 0, abort_flag) && wait_full(0));
+    if (ok && total > 0) {
+      tcgen05_fence_after();
+      scores(0);
+      grads(0);
+    }
+    for (int n = 0; n < total && ok; ++n) {
+      ok = warp_wait(p_full, n & 1, abort_flag);
+      if (!ok) break;
+      tcgen05_fence_after();
+      if (elect_one()) mma_sum(tV, tmem, 64, qg_sum + at(n, 1), idesc_o, n > 0);
+      __syncwarp();
+      if (n + 1 < total) {
+        ok = wait_full(n + 1);
+        if (!ok) break;
+        tcgen05_fence_after();
+        scores(n + 1);
+      }
+      ok = warp_wait(ds_full, n & 1, abort_flag);
+      if (!ok) break;
+      tcgen05_fence_after();
+      if (elect_one()) {
+        mma_sum(tK, tP, 64, qg_sum + at(n, 0), idesc_o, n > 0);
+        umma_commit(n + 1 < total ? &empty[n % L::kStages] : done);
+      }
+      __syncwarp();
+      if (n + 1 < total) grads(n + 1);
+    }
+    if (!ok && lane == 0) report(s.err, 72);
+    __syncwarp();
+  } else {
+    // ---------------- a key (and half of the queries) to a thread ----------------
+    const int r = threadIdx.x & 127, hf = warp >> 2;
+    const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16) + hf * 64;
+    const int k = k0 + r;
+    const float c = s.scale_log2;
+    const float f = a.bound != nullptr ? grad_factor(a.bound, b * s.Hkv + kvh, a.shift) : 1.f;
+    bool ok = true;
+    for (int n = 0; n < total; ++n) {
+      const int st = n % L::kStages, q0 = (i0 + n % ni) * kT;
+      const uint32_t par = n & 1;
+      if (!warp_wait(&full[st], n / L::kStages & 1, abort_flag) || !warp_wait(s_full, par, abort_flag)) {
+        ok = false;
+        if (lane == 0) report(s.err, 73);
+        break;
+      }
+      tcgen05_fence_after();
+      float p[64];
+      tmem_ld32(tmem + lanes, p);
+      tmem_ld32(tmem + lanes + 32, p + 32);
+      const float4* nl = reinterpret_cast<const float4*>(stat + st * 256 + hf * 64);
+      const float4* dl = nl + 32;
+      // this key is seen by queries [lo, hi)
+      const int lo = s.causal ? k - off - q0 : -kT, hi = s.window > 0 ? min((int64_t)kT, (int64_t)k - off - q0 + s.window) : kT;
+      const uint32_t see0 = range_bits(lo, hi, hf * 64), see1 = range_bits(lo, hi, hf * 64 + 32);
+      const bool all = (see0 & see1) == 0xFFFFFFFFu;
+      tmem_ld_wait(p);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float4 w = nl[i];
+        p[4 * i] = ex2(fmaf(p[4 * i], c, w.x));
+        p[4 * i + 1] = ex2(fmaf(p[4 * i + 1], c, w.y));
+        p[4 * i + 2] = ex2(fmaf(p[4 * i + 2], c, w.z));
+        p[4 * i + 3] = ex2(fmaf(p[4 * i + 3], c, w.w));
+      }
+      if (!__all_sync(0xffffffffu, all)) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) p[i] = (i < 32 ? see0 : see1) >> (i & 31) & 1 ? p[i] : 0.f;
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+      tmem_st32(tmem + lanes, pk);
+      tmem_st_wait();
+      tcgen05_fence_before();
+      mbar_arrive(p_full);
+      if (!warp_wait(dp_full, par, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      tcgen05_fence_after();
+      float d[64];
+      tmem_ld32(tP + lanes, d);
+      tmem_ld32(tP + lanes + 32, d + 32);
+      tmem_ld_wait(d);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float4 w = dl[i];
+        d[4 * i] = p[4 * i] * (d[4 * i] - w.x);
+        d[4 * i + 1] = p[4 * i + 1] * (d[4 * i + 1] - w.y);
+        d[4 * i + 2] = p[4 * i + 2] * (d[4 * i + 2] - w.z);
+        d[4 * i + 3] = p[4 * i + 3] * (d[4 * i + 3] - w.w);
+      }
+      if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) d[i] *= f;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(d[2 * i], d[2 * i + 1]);
+      tmem_st32(tP + lanes, pk);
+      tmem_st_wait();
+      tcgen05_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && total > 0) {
+      ok = warp_wait(done, 0, abort_flag);
+      if (!ok && lane == 0) report(s.err, 73);
+      tcgen05_fence_after();
+    }
+    if (ok) {
+      // half of the columns to a thread: dv, then dk
+      bool real = k < s.Skv && total > 0;
+      if (real && s.mask != nullptr) real = s.mask[(int64_t)b * s.k_words + (k >> 5)] >> (k & 31) & 1;
+      const int64_t row = (((int64_t)b * s.Skv + k) * s.Hkv + kvh) * s.D;
+      const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16;
+      const float un = exp2f(-a.shift);
+#pragma unroll
+      for (int cc = 0; cc < D / 2; cc += 32) {
+        const int col = hf * (D / 2) + cc;
+        float o[32];
+        if (total > 0) {
+          tmem_ld32(tV + mine + col, o);
+          tmem_ld_wait(o);
+        }
+        if (!real) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (k < s.Skv) put_row32<T>(reinterpret_cast<T*>(a.dv) + row, o, un, col, s.D);
+        if (total > 0) {
+          tmem_ld32(tK + mine + col, o);
+          tmem_ld_wait(o);
+        }
+        if (!real) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (k < s.Skv) put_row32<T>(reinterpret_cast<T*>(a.dk) + row, o, s.scale * un / f, col, s.D);
+      }
+    }
+  }
+  finish(tmem, warp);
+}
+
+// ------------------------------------------------------------------------------------------------ dq
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
+               const __grid_constant__ BwdArgs a) {
+  using L = BwdSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sG = smem + L::kTile;
+  uint8_t* sKV = smem + 2 * L::kTile;            // stages of [k | v]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* q_full = bars;
+  uint64_t* full = bars + 1;
+  uint64_t* empty = full + L::kStages;
+  uint64_t* s_full = empty + L::kStages;         // [2]
+  uint64_t* dp_full = s_full + 2;
+  uint64_t* ds_full = s_full + 3;
+  uint64_t* done = s_full + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const Shape& s = a.s;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int h = blockIdx.x, b = blockIdx.z, kvh = h / (s.Hq / s.Hkv);
+  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kT;
+  int j0, j1;
+  key_blocks(s, q0, j0, j1);
+  const int total = j1 - j0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 256);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, kTmemCols);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  // two tiles of scores in turn, dP (and dS over it), the sum
+  const uint32_t tmem = *tmem_slot, tP = tmem + 2 * kT, tQ = tmem + 3 * kT;
+
+  if (warp == 8) {
+    if (lane == 0 && total > 0) {
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      mbar_expect_tx(q_full, 2 * L::kTile);
+      load_tile<D>(sQ, &tm_q, q0, h, b, q_full);
+      load_tile<D>(sG, &tm_g, q0, h, b, q_full);
+      bool ok = true;
+      int n = 0;
+      for (; n < total; ++n) {
+        const int st = n % L::kStages;
+        if (!mbar_wait(&empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        mbar_expect_tx(&full[st], 2 * L::kTile);
+        load_tile<D>(sKV + 2 * st * L::kTile, &tm_k, (j0 + n) * kT, kvh, b, &full[st]);
+        load_tile<D>(sKV + (2 * st + 1) * L::kTile, &tm_v, (j0 + n) * kT, kvh, b, &full[st]);
+      }
+      if (!ok) {
+        mbar_wait_quiet(q_full, 0, 1 << 12);
+        for (int i = n - L::kStages < 0 ? 0 : n - L::kStages; i < n; ++i)
+          mbar_wait_quiet(&full[i % L::kStages], i / L::kStages & 1, 1 << 12);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
+    const uint64_t qd = make_desc_sw128(smem_u32(sQ)), gd = make_desc_sw128(smem_u32(sG));
+    const uint64_t kv_rows = make_desc_sw128(smem_u32(sKV)), kv_sum = make_desc_mn(smem_u32(sKV));
+    auto at = [&](int n, int which) { return (uint64_t)((2 * (n % L::kStages) + which) * (L::kTile >> 4)); };
+    auto wait_full = [&](int n) { return warp_wait(&full[n % L::kStages], n / L::kStages & 1, abort_flag); };
+    auto scores = [&](int n) {                  // q k^T
+      if (elect_one()) {
+        mma_rows<D>(tmem + (n & 1) * kT, qd, kv_rows + at(n, 0), idesc_s);
+        umma_commit(&s_full[n & 1]);
+      }
+      __syncwarp();
+    };
+    auto grads = [&](int n) {                   // dO v^T
+      if (elect_one()) {
+        mma_rows<D>(tP, gd, kv_rows + at(n, 1), idesc_s);
+        umma_commit(dp_full);
+      }
+      __syncwarp();
+    };
+    bool ok = total == 0 || (warp_wait(q_full, 0, abort_flag) && wait_full(0));
+    if (ok && total > 0) {
+      tcgen05_fence_after();
+      scores(0);
+      grads(0);
+    }
+    for (int n = 0; n < total && ok; ++n) {
+      // the next scores' tile was read before dS of the step before this one was handed over
+      if (n + 1 < total) {
+        ok = wait_full(n + 1);
+        if (!ok) break;
+        tcgen05_fence_after();
+        scores(n + 1);
+      }
+      ok = warp_wait(ds_full, n & 1, abort_flag);
+      if (!ok) break;
+      tcgen05_fence_after();
+      if (elect_one()) {
+        mma_sum(tQ, tP, 64, kv_sum + at(n, 0), idesc_o, n > 0);
+        umma_commit(n + 1 < total ? &empty[n % L::kStages] : done);
+      }
+      __syncwarp();
+      if (n + 1 < total) grads(n + 1);
+    }
+    if (!ok && lane == 0) report(s.err, 72);
+    __syncwarp();
+  } else {
+    // ---------------- half of a query's keys to a thread ----------------
+    const int r = threadIdx.x & 127, hf = warp >> 2;
+    const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + hf * 64;
+    const int q = q0 + r;
+    int klo, khi;
+    row_keys(s, q, klo, khi);
+    const float c = s.scale_log2;
+    const float f = a.bound != nullptr ? grad_factor(a.bound, b * s.Hkv + kvh, a.shift) : 1.f;
+    const int64_t at = ((int64_t)b * s.Hq + h) * s.q_pad + q;
+    const float nl = a.nlse[at], dl = a.delta[at] * -f;
+    bool ok = true;
+    for (int n = 0; n < total; ++n) {
+      const int kb = (j0 + n) * kT + hf * 64;
+      if (!warp_wait(&s_full[n & 1], n >> 1 & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      tcgen05_fence_after();
+      float p[64];
+      tmem_ld32(tmem + lanes + (n & 1) * kT, p);
+      tmem_ld32(tmem + lanes + (n & 1) * kT + 32, p + 32);
+      uint32_t see0 = range_bits(klo, khi, kb), see1 = range_bits(klo, khi, kb + 32);
+      if (s.mask != nullptr) {
+        const uint32_t* w = s.mask + (int64_t)b * s.k_words + (kb >> 5);
+        see0 &= __ldg(w);
+        see1 &= __ldg(w + 1);
+      }
+      const bool all = (see0 & see1) == 0xFFFFFFFFu;
+      tmem_ld_wait(p);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(p[i], c, nl));
+      if (!__all_sync(0xffffffffu, all)) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) p[i] = (i < 32 ? see0 : see1) >> (i & 31) & 1 ? p[i] : 0.f;
+      }
+      if (!warp_wait(dp_full, n & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      tcgen05_fence_after();
+      float d[64];
+      tmem_ld32(tP + lanes, d);
+      tmem_ld32(tP + lanes + 32, d + 32);
+      tmem_ld_wait(d);
+      uint32_t pk[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        pk[i] = pack2<T>(p[2 * i] * fmaf(d[2 * i], f, dl), p[2 * i + 1] * fmaf(d[2 * i + 1], f, dl));
+      tmem_st32(tP + lanes, pk);
+      tmem_st_wait();
+      tcgen05_fence_before();
+      mbar_arrive(ds_full);
+    }
+    if (ok && total > 0) {
+      ok = warp_wait(done, 0, abort_flag);
+      if (!ok && lane == 0) report(s.err, 73);
+      tcgen05_fence_after();
+    }
+    if (ok) {
+      T* dst = reinterpret_cast<T*>(a.dq) + (((int64_t)b * s.Sq + q) * s.Hq + h) * s.D;
+      const float un = s.scale * exp2f(-a.shift) / f;
+#pragma unroll
+      for (int cc = 0; cc < D / 2; cc += 32) {
+        const int col = hf * (D / 2) + cc;
+        float o[32];
+        if (total > 0) {
+          tmem_ld32(tQ + mine + col, o);
+          tmem_ld_wait(o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (q < s.Sq) put_row32<T>(dst, o, un, col, s.D);
+      }
+    }
+  }
+  finish(tmem, warp);
+}
+
+// ------------------------------------------------------------------------------------------------ hidden keys
+// The mask of keys as bits, and keys and values with zeros in hidden rows, so that what those hold (infinities, NaN) takes no
+// part in products where they are summed over.
+struct HideArgs {
+  const uint8_t* mask;     // [B, Skv] by strides
+  int64_t m_b, m_s;
+  const void *k, *v;
+  int64_t k_b, k_h, k_s, v_b, v_h, v_s;
+  uint4 *ko, *vo;          // [B, Skv, Hkv, D]
+  uint32_t* words;         // [B, k_words]
+  int Hkv, Skv, D, k_words;
+};
+
+__global__ void __launch_bounds__(256) attn_hide_kernel(HideArgs a) {
+  __shared__ uint32_t word;
+  const int b = blockIdx.y, s0 = blockIdx.x * 32, tid = threadIdx.x;
+  if (tid < 32) {
+    const bool real = s0 + tid < a.Skv && a.mask[b * a.m_b + (s0 + tid) * a.m_s] != 0;
+    const uint32_t w = __ballot_sync(0xffffffffu, real);
+    if (tid == 0) {
+      word = w;
+      a.words[(int64_t)b * a.k_words + blockIdx.x] = w;
+    }
+  }
+  __syncthreads();
+  const uint32_t w = word;
+  const int per = a.D / 8, row = a.Hkv * per, n = min(32, a.Skv - s0) * row;
+  for (int i = tid; i < n; i += 256) {
+    const int sl = i / row, h = i % row / per, c = i % per * 8;
+    const bool real = w >> sl & 1;
+    const int64_t at = ((int64_t)b * a.Skv + s0) * row + i;
+    const uint16_t* k = reinterpret_cast<const uint16_t*>(a.k) + b * a.k_b + h * a.k_h + (int64_t)(s0 + sl) * a.k_s + c;
+    const uint16_t* v = reinterpret_cast<const uint16_t*>(a.v) + b * a.v_b + h * a.v_h + (int64_t)(s0 + sl) * a.v_s + c;
+    a.ko[at] = real ? *reinterpret_cast<const uint4*>(k) : make_uint4(0, 0, 0, 0);
+    a.vo[at] = real ? *reinterpret_cast<const uint4*>(v) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+// [sequences, heads, rows, D] by strides in elements: rows of D (a multiple of 8) elements.
+struct Tensor4 {
+  const void* p;
+  int64_t b, h, s;
+};
+
+bool encode(CUtensorMap* tm, CUtensorMapDataType dt, const Tensor4& t, int D, int rows, int heads, int B) {
+  EncodeTiledFn enc = tensor_map_encoder();
+  if (enc == nullptr) return false;
+  // strides of dimensions of size 1 are never taken, but have to be multiples of 16 bytes
+  const int64_t s = rows > 1 ? t.s : D, h = heads > 1 ? t.h : D, b = B > 1 ? t.b : D;
+  if ((reinterpret_cast<uintptr_t>(t.p) & 15) || t.p == nullptr || s <= 0 || h <= 0 || b <= 0 || ((s | h | b) & 7)) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)s * 2, (cuuint64_t)h * 2, (cuuint64_t)b * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)kT, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(tm, dt, 4, const_cast<void*>(t.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The driver's encoder wants a current context, which a thread that has launched nothing yet (autograd's) need not have.
+bool bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
+bool shape_ok(int B, int Hq, int Hkv, int Sq, int Skv, int D, int window, float scale) {
+  return B >= 1 && B <= 65535 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq <= (1 << 20) && Sq >= 1 && Skv >= 1 &&
+         Sq <= (1 << 23) && Skv <= (1 << 23) && D >= 8 && D <= 128 && D % 8 == 0 && window >= 0 && scale > 0.f && scale < 1e30f;
+}
+
+Shape make_shape(int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window, const uint32_t* mask, float scale, int* err) {
+  Shape s;
+  s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.Sq = Sq; s.Skv = Skv; s.D = D; s.causal = causal; s.window = window;
+  s.q_pad = (Sq + kT - 1) / kT * kT;
+  s.k_words = (Skv + kT - 1) / kT * (kT / 32);
+  s.mask = mask; s.scale = scale; s.scale_log2 = scale * 1.4426950408889634f; s.err = err;
+  return s;
+}
+
+template <typename T> constexpr CUtensorMapDataType map_type() {
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+template <typename T> constexpr float shift_of() { return std::is_same<T, __half>::value ? (float)kShiftF16 : 0.f; }
+
+// One CTA to an SM whatever the tiles take: each allocates all of the tensor memory.
+constexpr int one_cta(int bytes) { return bytes > 120 * 1024 ? bytes : 120 * 1024; }
+
+template <typename T, int D>
+int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, void* out, float* nlse, cudaStream_t stream) {
+  CUtensorMap tq, tk, tv;
+  const CUtensorMapDataType dt = map_type<T>();
+  if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
+      !encode(&tv, dt, v, s.D, s.Skv, s.Hkv, s.B))
+    return (int)cudaErrorInvalidValue;
+  constexpr int smem = one_cta(FwdSmem<D>::kSize);
+  static SmemLimit limit;
+  const cudaError_t e = limit((const void*)attn_fwd_kernel<T, D>, smem);
+  if (e != cudaSuccess) return (int)e;
+  FwdArgs a = {s, out, nlse, shift_of<T>()};
+  const dim3 grid(s.Hq, (s.Sq + 2 * kT - 1) / (2 * kT), s.B);
+  attn_fwd_kernel<T, D><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a);
+  return (int)cudaGetLastError();
+}
+
+template <typename T, int D>
+int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, const Tensor4& g, const void* out,
+            const float* nlse, float* delta, uint32_t* bound, void* dq, void* dk, void* dv, cudaStream_t stream) {
+  CUtensorMap tq, tk, tv, tg;
+  const CUtensorMapDataType dt = map_type<T>();
+  if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
+      !encode(&tv, dt, v, s.D, s.Skv, s.Hkv, s.B) || !encode(&tg, dt, g, s.D, s.Sq, s.Hq, s.B))
+    return (int)cudaErrorInvalidValue;
+  constexpr int smem = one_cta(BwdSmem<D>::kSize);
+  static SmemLimit limit_kv, limit_q;
+  cudaError_t e = limit_kv((const void*)attn_dkv_kernel<T, D>, smem);
+  if (e == cudaSuccess) e = limit_q((const void*)attn_dq_kernel<T, D>, smem);
+  if (e != cudaSuccess) return (int)e;
+  PrepArgs p = {out, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, delta, bound, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
+  const int64_t rows = (int64_t)s.B * s.Hq * s.q_pad + (bound != nullptr ? (int64_t)s.B * s.Hkv * s.Skv : 0);
+  if (rows / 16 + 1 > 0x7FFFFFFF) return (int)cudaErrorInvalidValue;
+  attn_prep_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(p);
+  BwdArgs a = {s, nlse, delta, bound, dq, dk, dv, shift_of<T>()};
+  attn_dkv_kernel<T, D><<<dim3(s.Hkv, (s.Skv + kT - 1) / kT, s.B), kThreads, smem, stream>>>(tq, tk, tv, tg, a);
+  attn_dq_kernel<T, D><<<dim3(s.Hq, (s.Sq + kT - 1) / kT, s.B), kThreads, smem, stream>>>(tq, tk, tv, tg, a);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// q [B, Hq, Sq, D], k and v [B, Hkv, Skv, D] by the strides of sequences, heads and rows (elements; multiples of 8, rows
+// contiguous, pointers 16-byte aligned), fp16 or bf16, D a multiple of 8 up to 128.  window > 0 needs causal.  mask_words: the
+// real keys' bits [B, ceil(Skv / 128) * 4] or null (ipex_attn_hide writes them).  out [B, Sq, Hq, D] contiguous; nlse [B, Hq, Sq
+// rounded up to 128] (16-byte aligned) for the backward pass, or null.  Returns a cudaError_t.
+IPEX_API int ipex_attn_train_fwd(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
+                                 int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, const uint32_t* mask_words,
+                                 void* out, float* nlse, int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window,
+                                 float scale, int dtype, int* err, void* stream) {
+  if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || (reinterpret_cast<uintptr_t>(out) & 15) ||
+      (Sq + 2 * kT - 1) / (2 * kT) > 65535)
+    return (int)cudaErrorInvalidValue;
+  const Shape s = make_shape(B, Hq, Hkv, Sq, Skv, D, causal, window, mask_words, scale, err);
+  const Tensor4 tq = {q, q_b, q_h, q_s}, tk = {k, k_b, k_h, k_s}, tv = {v, v_b, v_h, v_s};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == DT_F16)
+    return D <= 64 ? run_fwd<__half, 64>(s, tq, tk, tv, out, nlse, st) : run_fwd<__half, 128>(s, tq, tk, tv, out, nlse, st);
+  if (dtype == DT_BF16)
+    return D <= 64 ? run_fwd<__nv_bfloat16, 64>(s, tq, tk, tv, out, nlse, st)
+                   : run_fwd<__nv_bfloat16, 128>(s, tq, tk, tv, out, nlse, st);
+  return (int)cudaErrorInvalidValue;
+}
+
+// g: the gradient of out, by strides like q.  delta [B, Hq, Sq rounded up to 128] (16-byte aligned) is scratch; bound [B, Hkv, 2]
+// zeros for fp16, null for bf16.  dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
+IPEX_API int ipex_attn_train_bwd(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
+                                 int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, const uint32_t* mask_words,
+                                 const void* out, const float* nlse, const void* g, int64_t g_b, int64_t g_h, int64_t g_s,
+                                 float* delta, uint32_t* bound, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq,
+                                 int Skv, int D, int causal, int window, float scale, int dtype, int* err, void* stream) {
+  if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || nlse == nullptr || delta == nullptr ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(nlse) | reinterpret_cast<uintptr_t>(delta) |
+        reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) ||
+      (Sq + kT - 1) / kT > 65535 || (Skv + kT - 1) / kT > 65535 || (dtype == DT_F16) != (bound != nullptr))
+    return (int)cudaErrorInvalidValue;
+  const Shape s = make_shape(B, Hq, Hkv, Sq, Skv, D, causal, window, mask_words, scale, err);
+  const Tensor4 tq = {q, q_b, q_h, q_s}, tk = {k, k_b, k_h, k_s}, tv = {v, v_b, v_h, v_s}, tg = {g, g_b, g_h, g_s};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == DT_F16)
+    return D <= 64 ? run_bwd<__half, 64>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st)
+                   : run_bwd<__half, 128>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st);
+  if (dtype == DT_BF16)
+    return D <= 64 ? run_bwd<__nv_bfloat16, 64>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st)
+                   : run_bwd<__nv_bfloat16, 128>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st);
+  return (int)cudaErrorInvalidValue;
+}
+
+// mask [B, Skv] of bytes by strides (0: hidden); k, v by strides as above; k_out, v_out [B, Skv, Hkv, D] contiguous, words [B,
+// ceil(Skv / 128) * 4].
+IPEX_API int ipex_attn_hide(const uint8_t* mask, int64_t m_b, int64_t m_s, const void* k, int64_t k_b, int64_t k_h, int64_t k_s,
+                            const void* v, int64_t v_b, int64_t v_h, int64_t v_s, void* k_out, void* v_out, uint32_t* words, int B,
+                            int Hkv, int Skv, int D, void* stream) {
+  if (B < 1 || B > 65535 || Hkv < 1 || Skv < 1 || Skv > (1 << 23) || D < 8 || D > 128 || D % 8 ||
+      ((k_b | k_h | k_s | v_b | v_h | v_s) & 7) ||
+      ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) |
+        reinterpret_cast<uintptr_t>(v_out)) & 15))
+    return (int)cudaErrorInvalidValue;
+  HideArgs a = {mask, m_b, m_s, k, v, k_b, k_h, k_s, v_b, v_h, v_s, (uint4*)k_out, (uint4*)v_out, words, Hkv, Skv, D,
+                (Skv + kT - 1) / kT * (kT / 32)};
+  attn_hide_kernel<<<dim3(a.k_words, B), 256, 0, (cudaStream_t)stream>>>(a);
+  return (int)cudaGetLastError();
+}

@@ -154,6 +154,13 @@ COMPONENT_SIGS = {
         "ipex_ssd_chunks": [vp, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, vp, vp, ci, ci, vp, vp, vp,
                             ci, ci, ci, ci, ci, ci, vp, vp],
     },
+    "train_attn": {
+        "ipex_attn_train_fwd": [vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci,
+                                cf, ci, vp, vp],
+        "ipex_attn_train_bwd": [vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, i64, i64, i64, vp, vp,
+                                vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, cf, ci, vp, vp],
+        "ipex_attn_hide": [vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, ci, ci, ci, ci, vp],
+    },
     "token_loss": {
         "ipex_token_logprobs": [vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, i64, ci, ci, i64, cf, ci, vp, vp],
         "ipex_token_logprobs_grad": [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, ci, i64, cf, ci, vp],
