@@ -38,6 +38,10 @@ constexpr int kT = 128;           // rows of a tile of queries or keys
 constexpr int kThreads = 320;     // eight warps of arithmetic, the loader, the products
 constexpr uint32_t kTmemCols = 512;
 constexpr int kShiftF16 = 12;     // P is stored times 2^12 in fp16
+// delta_i is the difference of all dP_ij of a row: with the rounded o its error reaches every dS_ij of the row with the same sign
+// and adds a third to the error of dq and dk (measured: 1.53 times the final rounding's instead of 1.42).  So what rounding takes
+// from o is kept too, rounded once more, times 2^11 so that it does not fall among fp16's subnormals.
+constexpr float kLowScale = 2048.f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -209,6 +213,7 @@ __device__ __forceinline__ void finish(uint32_t tmem_base, int warp) {
 struct FwdArgs {
   Shape s;
   void* out;          // [B, Sq, Hq, D]
+  void* low;          // what rounding took from it, times kLowScale, for the backward pass; or null
   float* nlse;        // [B, Hq, q_pad]: -L log2(e) (+ the shift of fp16); -inf for rows that see nothing and past Sq
   float shift;
 };
@@ -445,7 +450,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
-        if (q < s.Sq) put_row32<T>(dst, o, inv, cc, s.D);
+        if (q < s.Sq) {
+          put_row32<T>(dst, o, inv, cc, s.D);
+          if (a.low != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = o[i] * inv;
+              o[i] = x - to_float<T>(from_float<T>(x));
+            }
+            put_row32<T>(reinterpret_cast<T*>(a.low) + (dst - reinterpret_cast<T*>(a.out)), o, kLowScale, cc, s.D);
+          }
+        }
       }
     }
   }
@@ -457,6 +472,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
 struct PrepArgs {
   const void* out;         // [B, Sq, Hq, D]
+  const void* low;
   const void* grad;        // by strides
   const void* v;
   int64_t g_b, g_h, g_s, v_b, v_h, v_s;
@@ -490,8 +506,9 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
     group = (b * a.Hkv + h / (a.Hq / a.Hkv)) * 2;
     if (in && q < a.Sq) {
       const uint4 g = *reinterpret_cast<const uint4*>((const T*)a.grad + b * a.g_b + h * a.g_h + q * a.g_s + 8 * sub);
-      const uint4 o = *reinterpret_cast<const uint4*>((const T*)a.out + ((b * a.Sq + q) * a.Hq + h) * a.D + 8 * sub);
-      d = dot8<T>(g, o);
+      const int64_t at = ((b * a.Sq + q) * a.Hq + h) * a.D + 8 * sub;
+      const uint4 o = *reinterpret_cast<const uint4*>((const T*)a.out + at), lo = *reinterpret_cast<const uint4*>((const T*)a.low + at);
+      d = dot8<T>(g, o) + dot8<T>(g, lo) * (1.f / kLowScale);
       if (a.bound != nullptr) n = dot8<T>(g, g);
     }
   } else if (row < rows_q + rows_v) {
@@ -992,19 +1009,19 @@ struct HideArgs {
 
 __global__ void __launch_bounds__(256) attn_hide_kernel(HideArgs a) {
   __shared__ uint32_t word;
-  const int b = blockIdx.y, s0 = blockIdx.x * 32, tid = threadIdx.x;
+  const int b = blockIdx.z, s0 = blockIdx.x * 32, tid = threadIdx.x;
   if (tid < 32) {
     const bool real = s0 + tid < a.Skv && a.mask[b * a.m_b + (s0 + tid) * a.m_s] != 0;
     const uint32_t w = __ballot_sync(0xffffffffu, real);
     if (tid == 0) {
       word = w;
-      a.words[(int64_t)b * a.k_words + blockIdx.x] = w;
+      if (blockIdx.y == 0) a.words[(int64_t)b * a.k_words + blockIdx.x] = w;
     }
   }
   __syncthreads();
   const uint32_t w = word;
   const int per = a.D / 8, row = a.Hkv * per, n = min(32, a.Skv - s0) * row;
-  for (int i = tid; i < n; i += 256) {
+  for (int i = blockIdx.y * 256 + tid; i < n; i += 256 * gridDim.y) {
     const int sl = i / row, h = i % row / per, c = i % per * 8;
     const bool real = w >> sl & 1;
     const int64_t at = ((int64_t)b * a.Skv + s0) * row + i;
@@ -1065,7 +1082,8 @@ template <typename T> constexpr float shift_of() { return std::is_same<T, __half
 constexpr int one_cta(int bytes) { return bytes > 120 * 1024 ? bytes : 120 * 1024; }
 
 template <typename T, int D>
-int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, void* out, float* nlse, cudaStream_t stream) {
+int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, void* out, void* low, float* nlse,
+            cudaStream_t stream) {
   CUtensorMap tq, tk, tv;
   const CUtensorMapDataType dt = map_type<T>();
   if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
@@ -1075,7 +1093,7 @@ int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
   static SmemLimit limit;
   const cudaError_t e = limit((const void*)attn_fwd_kernel<T, D>, smem);
   if (e != cudaSuccess) return (int)e;
-  FwdArgs a = {s, out, nlse, shift_of<T>()};
+  FwdArgs a = {s, out, low, nlse, shift_of<T>()};
   const dim3 grid(s.Hq, (s.Sq + 2 * kT - 1) / (2 * kT), s.B);
   attn_fwd_kernel<T, D><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a);
   return (int)cudaGetLastError();
@@ -1083,7 +1101,7 @@ int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
 
 template <typename T, int D>
 int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, const Tensor4& g, const void* out,
-            const float* nlse, float* delta, uint32_t* bound, void* dq, void* dk, void* dv, cudaStream_t stream) {
+            const void* low, const float* nlse, float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
   CUtensorMap tq, tk, tv, tg;
   const CUtensorMapDataType dt = map_type<T>();
   if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
@@ -1094,7 +1112,13 @@ int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
   cudaError_t e = limit_kv((const void*)attn_dkv_kernel<T, D>, smem);
   if (e == cudaSuccess) e = limit_q((const void*)attn_dq_kernel<T, D>, smem);
   if (e != cudaSuccess) return (int)e;
-  PrepArgs p = {out, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, delta, bound, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
+  uint32_t* bound = nullptr;
+  if (std::is_same<T, __half>::value) {
+    bound = reinterpret_cast<uint32_t*>(delta + (int64_t)s.B * s.Hq * s.q_pad);
+    e = cudaMemsetAsync(bound, 0, (size_t)s.B * s.Hkv * 8, stream);
+    if (e != cudaSuccess) return (int)e;
+  }
+  PrepArgs p = {out, low, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, delta, bound, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
   const int64_t rows = (int64_t)s.B * s.Hq * s.q_pad + (bound != nullptr ? (int64_t)s.B * s.Hkv * s.Skv : 0);
   if (rows / 16 + 1 > 0x7FFFFFFF) return (int)cudaErrorInvalidValue;
   attn_prep_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(p);
@@ -1108,47 +1132,50 @@ int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
 
 // q [B, Hq, Sq, D], k and v [B, Hkv, Skv, D] by the strides of sequences, heads and rows (elements; multiples of 8, rows
 // contiguous, pointers 16-byte aligned), fp16 or bf16, D a multiple of 8 up to 128.  window > 0 needs causal.  mask_words: the
-// real keys' bits [B, ceil(Skv / 128) * 4] or null (ipex_attn_hide writes them).  out [B, Sq, Hq, D] contiguous; nlse [B, Hq, Sq
+// real keys' bits [B, ceil(Skv / 128) * 4] or null (ipex_attn_hide writes them).  out [B, Sq, Hq, D] contiguous; low, the same
+// shape, and nlse [B, Hq, Sq
 // rounded up to 128] (16-byte aligned) for the backward pass, or null.  Returns a cudaError_t.
 IPEX_API int ipex_attn_train_fwd(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
                                  int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, const uint32_t* mask_words,
-                                 void* out, float* nlse, int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window,
-                                 float scale, int dtype, int* err, void* stream) {
-  if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || (reinterpret_cast<uintptr_t>(out) & 15) ||
+                                 void* out, void* low, float* nlse, int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal,
+                                 int window, float scale, int dtype, int* err, void* stream) {
+  if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || out == nullptr ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(low) | reinterpret_cast<uintptr_t>(nlse)) & 15) ||
       (Sq + 2 * kT - 1) / (2 * kT) > 65535)
     return (int)cudaErrorInvalidValue;
   const Shape s = make_shape(B, Hq, Hkv, Sq, Skv, D, causal, window, mask_words, scale, err);
   const Tensor4 tq = {q, q_b, q_h, q_s}, tk = {k, k_b, k_h, k_s}, tv = {v, v_b, v_h, v_s};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == DT_F16)
-    return D <= 64 ? run_fwd<__half, 64>(s, tq, tk, tv, out, nlse, st) : run_fwd<__half, 128>(s, tq, tk, tv, out, nlse, st);
+    return D <= 64 ? run_fwd<__half, 64>(s, tq, tk, tv, out, low, nlse, st) : run_fwd<__half, 128>(s, tq, tk, tv, out, low, nlse, st);
   if (dtype == DT_BF16)
-    return D <= 64 ? run_fwd<__nv_bfloat16, 64>(s, tq, tk, tv, out, nlse, st)
-                   : run_fwd<__nv_bfloat16, 128>(s, tq, tk, tv, out, nlse, st);
+    return D <= 64 ? run_fwd<__nv_bfloat16, 64>(s, tq, tk, tv, out, low, nlse, st)
+                   : run_fwd<__nv_bfloat16, 128>(s, tq, tk, tv, out, low, nlse, st);
   return (int)cudaErrorInvalidValue;
 }
 
-// g: the gradient of out, by strides like q.  delta [B, Hq, Sq rounded up to 128] (16-byte aligned) is scratch; bound [B, Hkv, 2]
-// zeros for fp16, null for bf16.  dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
+// g: the gradient of out, by strides like q.  work: scratch, 16-byte aligned, as many floats as nlse has and 2 B Hkv.  dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
 IPEX_API int ipex_attn_train_bwd(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
                                  int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, const uint32_t* mask_words,
-                                 const void* out, const float* nlse, const void* g, int64_t g_b, int64_t g_h, int64_t g_s,
-                                 float* delta, uint32_t* bound, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq,
+                                 const void* out, const void* low, const float* nlse, const void* g, int64_t g_b, int64_t g_h,
+                                 int64_t g_s, float* work, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq,
                                  int Skv, int D, int causal, int window, float scale, int dtype, int* err, void* stream) {
-  if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || nlse == nullptr || delta == nullptr ||
-      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(nlse) | reinterpret_cast<uintptr_t>(delta) |
+  if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || out == nullptr || low == nullptr ||
+      nlse == nullptr || work == nullptr || dq == nullptr || dk == nullptr || dv == nullptr ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(low) | reinterpret_cast<uintptr_t>(nlse) |
+        reinterpret_cast<uintptr_t>(work) |
         reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) ||
-      (Sq + kT - 1) / kT > 65535 || (Skv + kT - 1) / kT > 65535 || (dtype == DT_F16) != (bound != nullptr))
+      (Sq + kT - 1) / kT > 65535 || (Skv + kT - 1) / kT > 65535)
     return (int)cudaErrorInvalidValue;
   const Shape s = make_shape(B, Hq, Hkv, Sq, Skv, D, causal, window, mask_words, scale, err);
   const Tensor4 tq = {q, q_b, q_h, q_s}, tk = {k, k_b, k_h, k_s}, tv = {v, v_b, v_h, v_s}, tg = {g, g_b, g_h, g_s};
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == DT_F16)
-    return D <= 64 ? run_bwd<__half, 64>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st)
-                   : run_bwd<__half, 128>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st);
+    return D <= 64 ? run_bwd<__half, 64>(s, tq, tk, tv, tg, out, low, nlse, work, dq, dk, dv, st)
+                   : run_bwd<__half, 128>(s, tq, tk, tv, tg, out, low, nlse, work, dq, dk, dv, st);
   if (dtype == DT_BF16)
-    return D <= 64 ? run_bwd<__nv_bfloat16, 64>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st)
-                   : run_bwd<__nv_bfloat16, 128>(s, tq, tk, tv, tg, out, nlse, delta, bound, dq, dk, dv, st);
+    return D <= 64 ? run_bwd<__nv_bfloat16, 64>(s, tq, tk, tv, tg, out, low, nlse, work, dq, dk, dv, st)
+                   : run_bwd<__nv_bfloat16, 128>(s, tq, tk, tv, tg, out, low, nlse, work, dq, dk, dv, st);
   return (int)cudaErrorInvalidValue;
 }
 
@@ -1158,12 +1185,14 @@ IPEX_API int ipex_attn_hide(const uint8_t* mask, int64_t m_b, int64_t m_s, const
                             const void* v, int64_t v_b, int64_t v_h, int64_t v_s, void* k_out, void* v_out, uint32_t* words, int B,
                             int Hkv, int Skv, int D, void* stream) {
   if (B < 1 || B > 65535 || Hkv < 1 || Skv < 1 || Skv > (1 << 23) || D < 8 || D > 128 || D % 8 ||
-      ((k_b | k_h | k_s | v_b | v_h | v_s) & 7) ||
+      mask == nullptr || k == nullptr || v == nullptr || k_out == nullptr || v_out == nullptr || words == nullptr || ((k_b | k_h | k_s | v_b | v_h | v_s) & 7) ||
       ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) |
         reinterpret_cast<uintptr_t>(v_out)) & 15))
     return (int)cudaErrorInvalidValue;
   HideArgs a = {mask, m_b, m_s, k, v, k_b, k_h, k_s, v_b, v_h, v_s, (uint4*)k_out, (uint4*)v_out, words, Hkv, Skv, D,
                 (Skv + kT - 1) / kT * (kT / 32)};
-  attn_hide_kernel<<<dim3(a.k_words, B), 256, 0, (cudaStream_t)stream>>>(a);
+  // two vectors of k and of v to a thread
+  const int shares = (32 * Hkv * (D / 8) + 511) / 512;
+  attn_hide_kernel<<<dim3(a.k_words, shares < 65535 ? shares : 65535, B), 256, 0, (cudaStream_t)stream>>>(a);
   return (int)cudaGetLastError();
 }

@@ -696,6 +696,7 @@ IPEX_API int ipex_token_logprobs(const void* logits, int64_t s0, int64_t s1, int
                                  float* entropy, float* stats, float* top_logprob, int64_t* top_id, int64_t rows, int V, int top,
                                  int64_t ignore, float temp, int dtype, int* err, void* stream) {
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || top < 0 || top > kMaxTop || top > V || !temp_ok(temp) ||
+      targets == nullptr || logprob == nullptr || (top > 0 && (top_logprob == nullptr || top_id == nullptr)) ||
       (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
   ProbArgs a = {{logits, s0, s1, n1, V}, targets, logprob, entropy, stats, top_logprob, top_id, top, 0, ignore, temp, 1.f / temp, err};
@@ -712,8 +713,8 @@ IPEX_API int ipex_token_logprobs(const void* logits, int64_t s0, int64_t s1, int
 IPEX_API int ipex_token_logprobs_grad(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* targets,
                                       const float* stats, const float* g, const float* g_entropy, void* dlogits, int64_t rows,
                                       int V, int64_t ignore, float temp, int dtype, void* stream) {
-  if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || !temp_ok(temp) || dlogits == nullptr || stats == nullptr ||
-      (reinterpret_cast<uintptr_t>(stats) & 15))
+  if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || !temp_ok(temp) ||
+      targets == nullptr || dlogits == nullptr || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
   ProbGradArgs a = {{logits, s0, s1, n1, V}, targets, stats, g, g_entropy, dlogits, ignore, 1.f / temp, 0};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
@@ -730,7 +731,7 @@ IPEX_API int ipex_distill(const void* logits, int64_t s0, int64_t s1, int64_t n1
                           const float* lse, float* loss, float* stats, int64_t rows, int V, int K, float temp, int dtype, int* err,
                           void* stream) {
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
-      (lse != nullptr && V > (1 << 20)) || (reinterpret_cast<uintptr_t>(stats) & 15))
+      ids == nullptr || values == nullptr || loss == nullptr || (lse != nullptr && V > (1 << 20)) || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
   DistillArgs a = {{logits, s0, s1, n1, V}, ids, values, lse, loss, stats, K, 0, temp, 1.f / temp, err};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
@@ -748,8 +749,8 @@ IPEX_API int ipex_distill(const void* logits, int64_t s0, int64_t s1, int64_t n1
 IPEX_API int ipex_distill_grad(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* ids, const float* values,
                                const float* stats, const float* g, void* dlogits, int64_t rows, int V, int K, float temp, int dtype,
                                void* stream) {
-  if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) || dlogits == nullptr ||
-      stats == nullptr || g == nullptr || (reinterpret_cast<uintptr_t>(stats) & 15))
+  if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
+      ids == nullptr || values == nullptr || dlogits == nullptr || stats == nullptr || g == nullptr || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
   DistillGradArgs a = {{logits, s0, s1, n1, V}, ids, values, stats, g, dlogits, K, 0, temp, 1.f / temp};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);

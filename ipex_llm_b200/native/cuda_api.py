@@ -155,10 +155,10 @@ COMPONENT_SIGS = {
                             ci, ci, ci, ci, ci, ci, vp, vp],
     },
     "train_attn": {
-        "ipex_attn_train_fwd": [vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci,
-                                cf, ci, vp, vp],
-        "ipex_attn_train_bwd": [vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, i64, i64, i64, vp, vp,
-                                vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, cf, ci, vp, vp],
+        "ipex_attn_train_fwd": [vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci,
+                                ci, cf, ci, vp, vp],
+        "ipex_attn_train_bwd": [vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, i64, i64, vp, vp,
+                                vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, cf, ci, vp, vp],
         "ipex_attn_hide": [vp, i64, i64, vp, i64, i64, i64, vp, i64, i64, i64, vp, vp, vp, ci, ci, ci, ci, vp],
     },
     "token_loss": {

@@ -7,6 +7,7 @@ any strides between rows.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import NamedTuple, Optional
 
@@ -40,55 +41,66 @@ def _rows(logits: torch.Tensor):
         logits = logits.contiguous()
     if logits.dim() == 3:
         return logits, logits.stride(0), logits.stride(1), logits.shape[1]
-    return logits, 0, logits.stride(0) if logits.dim() == 2 else 0, max(1, logits[..., 0].numel())
+    return logits, 0, logits.stride(0) if logits.dim() == 2 else 0, logits.shape[0] if logits.dim() == 2 else 1
 
 
-def _check_logits(logits: torch.Tensor, what: str):
-    invalidInputError(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{what}: logits need a vocabulary dimension, got shape "
-                                                                   f"{tuple(logits.shape)}")
-    kinds = (torch.float16, torch.bfloat16, torch.float32) + (() if logits.is_cuda else (torch.float64,))
-    invalidInputError(logits.dtype in kinds, f"{what}: logits of type {logits.dtype} are not supported")
-    invalidInputError(logits.shape[-1] <= 1 << 30, f"{what}: a vocabulary of {logits.shape[-1]} is too large")
-    invalidInputError(not logits.is_cuda or logits.numel() // logits.shape[-1] <= 1 << 27, f"{what}: too many rows")
+def _on(dev: torch.device):
+    """A guard for launches on another device than the current one."""
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
-def _check_temperature(temperature: float, what: str):
-    invalidInputError(1e-6 <= temperature <= 1e6, f"{what}: the temperature should lie between 1e-6 and 1e6, got {temperature}")
+_HERE = contextlib.nullcontext()
+
+
+def _check_logits(logits: torch.Tensor, temperature: float, what: str):
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= 1 << 30:
+        invalidInputError(False, f"{what}: logits need a vocabulary of 1 to 2^30 tokens, got shape {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32) and (logits.is_cuda or logits.dtype != torch.float64):
+        invalidInputError(False, f"{what}: logits of type {logits.dtype} are not supported")
+    if logits.is_cuda and logits.numel() // logits.shape[-1] > 1 << 27:
+        invalidInputError(False, f"{what}: more than 2^27 rows")
+    if not 1e-6 <= temperature <= 1e6:
+        invalidInputError(False, f"{what}: the temperature should lie between 1e-6 and 1e6, got {temperature}")
 
 
 def _check_like(t: torch.Tensor, shape, device, what: str, whole: bool):
-    invalidInputError(tuple(t.shape) == tuple(shape), f"{what} should have shape {tuple(shape)}, got {tuple(t.shape)}")
-    invalidInputError(t.device == device, f"{what} should be on {device}, like the logits, got {t.device}")
-    kind = not (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool) if whole else t.is_floating_point()
-    invalidInputError(kind, f"{what} should hold {'token ids' if whole else 'floating-point numbers'}, got {t.dtype}")
+    if t.shape != shape:
+        invalidInputError(False, f"{what} should have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        invalidInputError(False, f"{what} should be on {device}, like the logits, got {t.device}")
+    if (t.is_floating_point() == whole) or t.is_complex() or t.dtype == torch.bool:
+        invalidInputError(False, f"{what} should hold {'token ids' if whole else 'floating-point numbers'}, got {t.dtype}")
+
+
+def _token_logprobs(logits, targets, temperature, entropy, top, ignore, keep):
+    """The results, and with ``keep`` each row's statistics for the backward pass."""
+    x, s0, s1, n1 = _rows(logits)
+    shape, V, dev = targets.shape, logits.shape[-1], logits.device
+    rows = targets.numel()
+    logprob = torch.empty(shape, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(logprob) if entropy else None
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if keep else None
+    top_lp = torch.empty((*shape, top), dtype=torch.float32, device=dev) if top else None
+    top_id = torch.empty((*shape, top), dtype=torch.int64, device=dev) if top else None
+    if rows:
+        with _on(dev):
+            rc = stream_lib("token_loss").ipex_token_logprobs(
+                ptr(x), s0, s1, n1, ptr(targets), ptr(logprob), ptr(ent), ptr(stats), ptr(top_lp), ptr(top_id), rows, V, top, ignore,
+                temperature, api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
+        api.check(rc, "token_logprobs")
+    return (logprob, ent, top_lp, top_id), stats
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, temperature, entropy, top, ignore):
         ctx.set_materialize_grads(False)
-        x, s0, s1, n1 = _rows(logits.detach())
-        shape, V, dev = targets.shape, logits.shape[-1], logits.device
-        rows = targets.numel()
-        targets = targets.to(torch.int64).contiguous()
-        f32 = dict(dtype=torch.float32, device=dev)
-        logprob = torch.empty(shape, **f32)
-        ent = torch.empty(shape, **f32) if entropy else None
-        stats = torch.empty(rows, 4, **f32) if ctx.needs_input_grad[0] else None
-        top_lp = torch.empty(*shape, top, **f32) if top else None
-        top_id = torch.empty(*shape, top, dtype=torch.int64, device=dev) if top else None
-        if rows:
-            with torch.cuda.device(dev):
-                rc = stream_lib("token_loss").ipex_token_logprobs(
-                    ptr(x), s0, s1, n1, ptr(targets), ptr(logprob), ptr(ent), ptr(stats), ptr(top_lp), ptr(top_id), rows, V, top,
-                    ignore, temperature, api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
-            api.check(rc, "token_logprobs")
+        out, stats = _token_logprobs(logits, targets, temperature, entropy, top, ignore, True)
         if top:
-            ctx.mark_non_differentiable(top_lp, top_id)
-        if stats is not None:
-            ctx.save_for_backward(logits, targets, stats)
+            ctx.mark_non_differentiable(*out[2:])
+        ctx.save_for_backward(logits, targets, stats)
         ctx.temperature, ctx.ignore = temperature, ignore
-        return logprob, ent, top_lp, top_id
+        return out
 
     @staticmethod
     @once_differentiable
@@ -97,13 +109,15 @@ class _TokenLogprobs(torch.autograd.Function):
             return (None,) * 6
         logits, targets, stats = ctx.saved_tensors
         x, s0, s1, n1 = _rows(logits)
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g, g_ent = (None if t is None else t.float().contiguous() for t in (g, g_ent))
-        if targets.numel():
-            with torch.cuda.device(logits.device):
+        dev, rows = logits.device, targets.numel()
+        dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        g = None if g is None else g.float().contiguous()
+        g_ent = None if g_ent is None else g_ent.float().contiguous()
+        if rows:
+            with _on(dev):
                 rc = stream_lib("token_loss").ipex_token_logprobs_grad(
-                    ptr(x), s0, s1, n1, ptr(targets), ptr(stats), ptr(g), ptr(g_ent), ptr(dx), targets.numel(), x.shape[-1],
-                    ctx.ignore, ctx.temperature, api.dtype_code(x.dtype), current_stream())
+                    ptr(x), s0, s1, n1, ptr(targets), ptr(stats), ptr(g), ptr(g_ent), ptr(dx), rows, x.shape[-1], ctx.ignore,
+                    ctx.temperature, api.dtype_code(x.dtype), current_stream())
             api.check(rc, "token_logprobs_grad")
         return dx, None, None, None, None, None
 
@@ -147,37 +161,43 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: flo
 
     16-bit and 32-bit logits; the gradient has the logits' type.
     """
-    _check_logits(logits, "token_logprobs")
-    _check_temperature(temperature, "token_logprobs")
+    _check_logits(logits, temperature, "token_logprobs")
     _check_like(targets, logits.shape[:-1], logits.device, "token_logprobs: targets", True)
-    invalidInputError(0 <= top <= min(MAX_TOP, logits.shape[-1]),
-                      f"token_logprobs: top should be between 0 and {min(MAX_TOP, logits.shape[-1])}, got {top}")
+    most = min(MAX_TOP, logits.shape[-1])
+    if not 0 <= top <= most:
+        invalidInputError(False, f"token_logprobs: top should be between 0 and {most}, got {top}")
     if logits.is_cuda:
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, float(temperature), bool(entropy), int(top),
-                                                   int(ignore_index)))
+        args = (logits, targets.to(torch.int64).contiguous(), float(temperature), bool(entropy), int(top), int(ignore_index))
+        if logits.requires_grad and torch.is_grad_enabled():
+            return TokenLogprobs(*_TokenLogprobs.apply(*args))
+        return TokenLogprobs(*_token_logprobs(*args, False)[0])
     outside = (targets != ignore_index) & ((targets < 0) | (targets >= logits.shape[-1]))
-    invalidInputError(not bool(outside.any()), "token_logprobs: a target lies outside of the vocabulary")
+    if bool(outside.any()):
+        invalidInputError(False, "token_logprobs: a target lies outside of the vocabulary")
     return TokenLogprobs(*_token_logprobs_plain(logits, targets.long(), temperature, entropy, top, ignore_index))
+
+
+def _distill(logits, ids, values, lse, temperature, keep):
+    """The loss, and with ``keep`` each row's statistics for the backward pass."""
+    x, s0, s1, n1 = _rows(logits)
+    dev, V, K = logits.device, logits.shape[-1], ids.shape[-1]
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
+    rows = loss.numel()
+    stats = torch.empty((rows, 8), dtype=torch.float32, device=dev) if keep else None
+    if rows:
+        with _on(dev):
+            rc = stream_lib("token_loss").ipex_distill(
+                ptr(x), s0, s1, n1, ptr(ids), ptr(values), ptr(lse), ptr(loss), ptr(stats), rows, V, K, temperature,
+                api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
+        api.check(rc, "distill")
+    return loss, stats
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, values, lse, temperature):
-        x, s0, s1, n1 = _rows(logits.detach())
-        V, K, dev = logits.shape[-1], ids.shape[-1], logits.device
-        ids, values = ids.to(torch.int64).contiguous(), values.detach().float().contiguous()
-        lse = None if lse is None else lse.detach().float().contiguous()
-        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-        rows = loss.numel()
-        stats = torch.empty(rows, 8, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
-        if rows:
-            with torch.cuda.device(dev):
-                rc = stream_lib("token_loss").ipex_distill(
-                    ptr(x), s0, s1, n1, ptr(ids), ptr(values), ptr(lse), ptr(loss), ptr(stats), rows, V, K, temperature,
-                    api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
-            api.check(rc, "distill")
-        if stats is not None:
-            ctx.save_for_backward(logits, ids, values, stats)
+        loss, stats = _distill(logits, ids, values, lse, temperature, True)
+        ctx.save_for_backward(logits, ids, values, stats)
         ctx.temperature = temperature
         return loss
 
@@ -186,13 +206,14 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, g):
         logits, ids, values, stats = ctx.saved_tensors
         x, s0, s1, n1 = _rows(logits)
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dev = logits.device
+        dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         g = g.float().contiguous()
         if g.numel():
-            with torch.cuda.device(logits.device):
+            with _on(dev):
                 rc = stream_lib("token_loss").ipex_distill_grad(
-                    ptr(x), s0, s1, n1, ptr(ids), ptr(values), ptr(stats), ptr(g), ptr(dx), g.numel(), x.shape[-1],
-                    ids.shape[-1], ctx.temperature, api.dtype_code(x.dtype), current_stream())
+                    ptr(x), s0, s1, n1, ptr(ids), ptr(values), ptr(stats), ptr(g), ptr(dx), g.numel(), x.shape[-1], ids.shape[-1],
+                    ctx.temperature, api.dtype_code(x.dtype), current_stream())
             api.check(rc, "distill_grad")
         return dx, None, None, None, None
 
@@ -233,20 +254,25 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
 
     The gradient goes to the logits alone (in their type: 16 or 32 bits); the teacher is a constant.
     """
-    _check_logits(logits, "distill_loss")
-    _check_temperature(temperature, "distill_loss")
-    invalidInputError(teacher_ids.dim() == logits.dim() and 1 <= teacher_ids.shape[-1] <= MAX_TEACHER,
-                      f"distill_loss: teacher_ids should hold 1 to {MAX_TEACHER} tokens for each row, got shape "
-                      f"{tuple(teacher_ids.shape)}")
-    shape = (*logits.shape[:-1], teacher_ids.shape[-1])
+    _check_logits(logits, temperature, "distill_loss")
+    if teacher_ids.dim() != logits.dim() or not 1 <= teacher_ids.shape[-1] <= MAX_TEACHER:
+        invalidInputError(False, f"distill_loss: teacher_ids should hold 1 to {MAX_TEACHER} tokens for each row, got shape "
+                                 f"{tuple(teacher_ids.shape)}")
+    rows = logits.shape[:-1]
+    shape = (*rows, teacher_ids.shape[-1])
     _check_like(teacher_ids, shape, logits.device, "distill_loss: teacher_ids", True)
     _check_like(teacher_logits, shape, logits.device, "distill_loss: teacher_logits", False)
-    if teacher_logsumexp is not None:
-        _check_like(teacher_logsumexp, logits.shape[:-1], logits.device, "distill_loss: teacher_logsumexp", False)
-        invalidInputError(logits.shape[-1] <= MAX_TAIL_VOCAB,
-                          f"distill_loss: teacher_logsumexp takes vocabularies up to {MAX_TAIL_VOCAB}")
+    lse = teacher_logsumexp
+    if lse is not None:
+        _check_like(lse, rows, logits.device, "distill_loss: teacher_logsumexp", False)
+        if logits.shape[-1] > MAX_TAIL_VOCAB:
+            invalidInputError(False, f"distill_loss: teacher_logsumexp takes vocabularies up to {MAX_TAIL_VOCAB}")
     if logits.is_cuda:
-        return _Distill.apply(logits, teacher_ids, teacher_logits, teacher_logsumexp, float(temperature))
-    invalidInputError(not bool((teacher_ids >= logits.shape[-1]).any()), "distill_loss: an id lies outside of the vocabulary")
-    lse = None if teacher_logsumexp is None else teacher_logsumexp.detach()
-    return _distill_plain(logits, teacher_ids.long(), teacher_logits.detach(), lse, temperature)
+        args = (logits, teacher_ids.to(torch.int64).contiguous(), teacher_logits.detach().float().contiguous(),
+                None if lse is None else lse.detach().float().contiguous(), float(temperature))
+        if logits.requires_grad and torch.is_grad_enabled():
+            return _Distill.apply(*args)
+        return _distill(*args, False)[0]
+    if bool((teacher_ids >= logits.shape[-1]).any()):
+        invalidInputError(False, "distill_loss: an id lies outside of the vocabulary")
+    return _distill_plain(logits, teacher_ids.long(), teacher_logits.detach(), None if lse is None else lse.detach(), temperature)

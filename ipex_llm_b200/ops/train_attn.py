@@ -5,6 +5,7 @@ On a CUDA tensor the package's own kernels run, on the current stream of the ten
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Optional
 
@@ -17,64 +18,82 @@ from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
 
 MAX_DIM = 128
+MAX_TOKENS = 1 << 22
 _TILE = 128
 
 
-def _fit(t: torch.Tensor) -> torch.Tensor:
-    """The tensor as the kernels' 4-D maps take it: rows contiguous, other strides positive multiples of 16 bytes."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and \
-        all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3]))
-    return t if ok else t.contiguous()
+def _fit(t: torch.Tensor):
+    """The tensor as the kernels' 4-D maps take it, rows contiguous and other strides positive multiples of 16 bytes (copied
+    where it is not), behind its pointer and strides.  The stride of a dimension of size 1 is never taken: 8 stands for it."""
+    (B, H, S, _), (b, h, s, d) = t.shape, t.stride()
+    b, h, s = b if B > 1 else 8, h if H > 1 else 8, s if S > 1 else 8
+    at = t.data_ptr()
+    if d != 1 or at & 15 or (b | h | s) & 7 or not (b and h and s):
+        return _fit(t.contiguous())
+    return at, b, h, s, t
 
 
-def _strided(t: torch.Tensor):
-    """Pointer and strides; that of a dimension of size 1 is never taken."""
-    return (ptr(t), *(8 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])))
+def _on(dev: torch.device):
+    """A guard for launches on another device than the current one."""
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _forward(q, k, v, key_mask, scale, causal, window, keep: bool):
+    """The outputs [B, Sq, Hq, D] and, with ``keep``, what the backward pass needs."""
+    lib, dev = stream_lib("train_attn"), q.device
+    B, Hq, Sq, D = q.shape
+    Hkv, Skv = k.shape[1], k.shape[2]
+    *q_at, q = _fit(q)
+    *k_at, k = _fit(k)
+    *v_at, v = _fit(v)
+    sizes = (B, Hq, Hkv, Sq, Skv, D, int(causal), window, scale, api.dtype_code(q.dtype))
+    out = torch.empty((B, Sq, Hq, D), dtype=q.dtype, device=dev)
+    stats = low = words = None
+    if keep:
+        stats = torch.empty((B, Hq, -(-Sq // _TILE) * _TILE), dtype=torch.float32, device=dev)
+        low = torch.empty_like(out)
+    with _on(dev):
+        st, err = current_stream(), ptr(error_flag(dev))
+        if key_mask is not None:
+            words = torch.empty((B, -(-Skv // _TILE) * (_TILE // 32)), dtype=torch.int32, device=dev)
+            k, v = torch.empty((2, B, Skv, Hkv, D), dtype=q.dtype, device=dev).transpose(2, 3).unbind(0)
+            api.check(lib.ipex_attn_hide(ptr(key_mask), *key_mask.stride(), *k_at, *v_at, ptr(k), ptr(v), ptr(words), B, Hkv, Skv, D,
+                                         st), "attn_hide")
+            *k_at, k = _fit(k)
+            *v_at, v = _fit(v)
+        api.check(lib.ipex_attn_train_fwd(*q_at, *k_at, *v_at, ptr(words), ptr(out), ptr(low), ptr(stats), *sizes, err, st),
+                  "attn_train_fwd")
+    return out, (q, k, v, out, low, stats, words), sizes
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_mask, scale, causal, window):
-        lib, dev = stream_lib("train_attn"), q.device
-        B, Hq, Sq, D = q.shape
-        Hkv, Skv = k.shape[1], k.shape[2]
-        grad = any(ctx.needs_input_grad[:3])
-        q, k, v = _fit(q.detach()), _fit(k.detach()), _fit(v.detach())
-        sizes = (B, Hq, Hkv, Sq, Skv, D, int(causal), window, scale, api.dtype_code(q.dtype))
-        out = torch.empty(B, Sq, Hq, D, dtype=q.dtype, device=dev)
-        stats = torch.empty(B, Hq, -(-Sq // _TILE) * _TILE, dtype=torch.float32, device=dev) if grad else None
-        words = None
-        with torch.cuda.device(dev):
-            st = current_stream()
-            if key_mask is not None:
-                words = torch.empty(B, -(-Skv // _TILE) * (_TILE // 32), dtype=torch.int32, device=dev)
-                kv = torch.empty(2, B, Skv, Hkv, D, dtype=q.dtype, device=dev)
-                api.check(lib.ipex_attn_hide(ptr(key_mask), *key_mask.stride(), *_strided(k), *_strided(v), ptr(kv[0]), ptr(kv[1]),
-                                             ptr(words), B, Hkv, Skv, D, st), "attn_hide")
-                k, v = kv[0].transpose(1, 2), kv[1].transpose(1, 2)
-            api.check(lib.ipex_attn_train_fwd(*_strided(q), *_strided(k), *_strided(v), ptr(words), ptr(out), ptr(stats), *sizes,
-                                              ptr(error_flag(dev)), st), "attn_train_fwd")
-        if grad:
-            ctx.save_for_backward(q, k, v, out, stats, words)
-            ctx.sizes = sizes
+        out, kept, ctx.sizes = _forward(q, k, v, key_mask, scale, causal, window, True)
+        ctx.save_for_backward(*kept)
         return out.transpose(1, 2)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, out, stats, words = ctx.saved_tensors
+        q, k, v, out, low, stats, words = ctx.saved_tensors
         B, Hq, Hkv, Sq, Skv, D = ctx.sizes[:6]
         dev = q.device
-        g = _fit(g)
-        dq = torch.empty(B, Sq, Hq, D, dtype=q.dtype, device=dev)
-        dk = torch.empty(B, Skv, Hkv, D, dtype=q.dtype, device=dev)
-        dv = torch.empty(B, Skv, Hkv, D, dtype=q.dtype, device=dev)
-        delta = torch.empty_like(stats)
-        with torch.cuda.device(dev):
-            bound = torch.zeros(B, Hkv, 2, dtype=torch.int32, device=dev) if q.dtype == torch.float16 else None
+        *q_at, q = _fit(q)
+        *k_at, k = _fit(k)
+        *v_at, v = _fit(v)
+        *g_at, g = _fit(g)
+        dq = torch.empty_like(out)
+        dk = torch.empty((B, Skv, Hkv, D), dtype=q.dtype, device=dev)
+        dv = torch.empty_like(dk)
+        work = torch.empty(stats.numel() + 2 * B * Hkv, dtype=torch.float32, device=dev)
+        with _on(dev):
             rc = stream_lib("train_attn").ipex_attn_train_bwd(
-                *_strided(q), *_strided(k), *_strided(v), ptr(words), ptr(out), ptr(stats), *_strided(g), ptr(delta), ptr(bound),
-                ptr(dq), ptr(dk), ptr(dv), *ctx.sizes, ptr(error_flag(dev)), current_stream())
+                *q_at, *k_at, *v_at, ptr(words), ptr(out), ptr(low), ptr(stats), *g_at, ptr(work), ptr(dq), ptr(dk), ptr(dv),
+                *ctx.sizes, ptr(error_flag(dev)), current_stream())
         api.check(rc, "attn_train_bwd")
         return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None, None
 
@@ -119,33 +138,36 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     copied).  Scores, sums and gradients are summed in 32 bits; probabilities and their gradients are rounded to 16 bits
     where they enter a product.  The results do not depend on the order in which anything runs.
     """
-    invalidInputError(q.dim() == 4 and k.dim() == 4 and tuple(k.shape) == tuple(v.shape),
-                      f"attention: q, k and v should be [batch, heads, tokens, dim], k and v alike; got {tuple(q.shape)}, "
-                      f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        invalidInputError(False, f"attention: q, k and v should be [batch, heads, tokens, dim], k and v alike; got {tuple(q.shape)}, "
+                                 f"{tuple(k.shape)} and {tuple(v.shape)}")
     B, Hq, Sq, D = q.shape
-    Hkv, Skv = k.shape[1], k.shape[2]
-    invalidInputError(k.shape[0] == B and k.shape[3] == D and Hkv >= 1 and Hq >= 1 and Hq % Hkv == 0,
-                      f"attention: keys {tuple(k.shape)} do not fit queries {tuple(q.shape)}")
-    invalidInputError(q.dtype == k.dtype == v.dtype and q.device == k.device == v.device,
-                      "attention: q, k and v should have one type and lie on one device")
-    scale = D ** -0.5 if scale is None else float(scale)
-    invalidInputError(0.0 < scale < 1e30, f"attention: the scale has to be positive and finite, got {scale}")
-    window = int(window)
-    invalidInputError(0 <= window < 1 << 31 and (causal or window == 0),
-                      f"attention: a window of {window} tokens needs causal attention and has to be positive (0: none)")
+    _, Hkv, Skv, _ = k.shape
+    if k.shape[0] != B or k.shape[3] != D or D < 1 or Hkv < 1 or Hq < 1 or Hq % Hkv != 0:
+        invalidInputError(False, f"attention: keys {tuple(k.shape)} do not fit queries {tuple(q.shape)}")
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
+        invalidInputError(False, "attention: q, k and v should have one type and lie on one device")
+    scale, window = D ** -0.5 if scale is None else float(scale), int(window)
+    if not 0.0 < scale < 1e30:
+        invalidInputError(False, f"attention: the scale has to be positive and finite, got {scale}")
+    if not 0 <= window < 1 << 31 or (window and not causal):
+        invalidInputError(False, f"attention: a window of {window} tokens needs causal attention and has to be positive (0: none)")
     if key_mask is not None:
-        invalidInputError(tuple(key_mask.shape) == (B, Skv) and key_mask.device == q.device and
-                          not (key_mask.is_floating_point() or key_mask.is_complex()),
-                          f"attention: key_mask should be [{B}, {Skv}] truth values on {q.device}, got {tuple(key_mask.shape)} of "
-                          f"{key_mask.dtype} on {key_mask.device}")
+        if key_mask.shape != (B, Skv) or key_mask.device != q.device or key_mask.is_floating_point() or key_mask.is_complex():
+            invalidInputError(False, f"attention: key_mask should be [{B}, {Skv}] truth values on {q.device}, got "
+                                     f"{tuple(key_mask.shape)} of {key_mask.dtype} on {key_mask.device}")
         key_mask = key_mask if key_mask.dtype == torch.bool else key_mask != 0
     if not q.is_cuda:
-        invalidInputError(q.is_floating_point(), f"attention: inputs of type {q.dtype} are not supported")
+        invalidInputError(q.is_floating_point(), "attention: inputs should be floating-point numbers")
         return _attention_plain(q, k, v, key_mask, scale, causal, window)
-    invalidInputError(q.dtype in (torch.float16, torch.bfloat16), f"attention: {q.dtype} is not supported on the GPU (float16 and "
-                                                                  "bfloat16 are)")
-    invalidInputError(8 <= D <= MAX_DIM and D % 8 == 0, f"attention: heads of {D} are not supported (multiples of 8 up to 128 are)")
-    invalidInputError(B <= 65535 and max(Sq, Skv) < 1 << 23, "attention: too many sequences or tokens")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        invalidInputError(False, f"attention: {q.dtype} is not supported on the GPU (float16 and bfloat16 are)")
+    if D > MAX_DIM or D % 8:
+        invalidInputError(False, f"attention: heads of {D} are not supported (multiples of 8 up to {MAX_DIM} are)")
+    if B > 65535 or Sq > MAX_TOKENS or Skv > MAX_TOKENS:
+        invalidInputError(False, f"attention: {B} sequences of {Sq} queries and {Skv} keys are too many (65535 of {MAX_TOKENS} are not)")
     if q.numel() == 0 or k.numel() == 0:
         return q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0.0) + (k.sum() + v.sum()) * 0
-    return _Attention.apply(q, k, v, key_mask, scale, bool(causal), window)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, key_mask, scale, bool(causal), window)
+    return _forward(q, k, v, key_mask, scale, bool(causal), window, False)[0].transpose(1, 2)
