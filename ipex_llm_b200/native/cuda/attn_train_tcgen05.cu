@@ -15,12 +15,19 @@
 // k in dq, q and dO in dk and dv).  Probabilities and dS go back to tensor memory in 16 bits, over the scores that they were
 // made from, and are the products' first operand there.
 //
-// The products are issued by one warp in an order that leaves the soft-max of one tile under the products of another:
-//   forward     two tiles of queries with four warps each, one thread to a row, take turns
+// The products are issued by one warp in an order that leaves the arithmetic of one tile under the products of another:
+//   forward     two tiles of queries with eight warps each take turns, two threads to a row
 //   dk and dv   transposed scores (rows are keys), so that P^T and dS^T are what the products want; s of the next step runs
 //               under this step's dS, dP of the next under the next P
 //   dq          a pass of its own over the keys, which computes s and dP once more (7 products in all where 5 would do): the
 //               sums then need no atomics, whose order would change results, and no 32-bit dq in global memory
+// Sixteen warps of arithmetic hide each other's latencies: with eight, two to a scheduler, an exponential's chain (product,
+// special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks.
+//
+// In the transposed scores L_i and delta_i belong to columns, not to the threads' rows.  Read from shared memory, four numbers a
+// request, they took a third of its bandwidth, which the products need.  So they are summed by the products too: one more step
+// of 16 columns, in which a query's row holds -L_i / scale (or -delta_i) in three pieces of 16 bits, and every key's row the
+// pieces' weights.
 //
 // In fp16 the range of dS is what is short, not its precision: P is taken times 2^12, and dP - delta times a power of two that a
 // bound on |dO_i| |v_j| gives for each group of heads, so that the largest dS comes near 2^15.  Both go out of the results again.
@@ -35,7 +42,9 @@ namespace {
 using namespace tc5;
 
 constexpr int kT = 128;           // rows of a tile of queries or keys
-constexpr int kThreads = 320;     // eight warps of arithmetic, the loader, the products
+constexpr int kArith = 16;        // warps of arithmetic
+constexpr int kLoader = kArith, kIssuer = kArith + 1;
+constexpr int kThreads = 32 * (kArith + 2);
 constexpr uint32_t kTmemCols = 512;
 constexpr int kShiftF16 = 12;     // P is stored times 2^12 in fp16
 // delta_i is the difference of all dP_ij of a row: with the rounded o its error reaches every dS_ij of the row with the same sign
@@ -81,6 +90,15 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
 template <int N>
 __device__ __forceinline__ void tmem_ld_wait(float (&v)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -96,6 +114,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
       "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
       "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -123,6 +149,16 @@ __device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
   return d;
 }
 constexpr uint32_t kBMajorMN = 1u << 16;
+// 16 columns of a K-major operand without a swizzle: rows of eight columns, 16 bytes, lie behind one another; the second eight
+// columns begin `second` bytes behind the first (leading offset), eight rows take 128 bytes (stride).
+__device__ __forceinline__ uint64_t make_desc_rows16(uint32_t smem_addr, uint32_t second) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(second >> 4) << 16;
+  d |= (uint64_t)(128 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  return d;
+}
 
 // acc = A . B^T over D columns, both tiles K-major.
 template <int D>
@@ -133,11 +169,20 @@ __device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint64_t b, uin
     for (int kk = 0; kk < 4; ++kk)
       umma_f16(d, a + c * (kT * 128 >> 4) + 2 * kk, b + c * (kT * 128 >> 4) + 2 * kk, idesc, (c | kk) != 0);
 }
-// acc (+)= A . B over 128 rows of B: A in tensor memory, 16 bits; its second half begins `half` columns behind the first.
-__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t a, int half, uint64_t b, uint32_t idesc, bool accumulate) {
+// acc (+)= A . B over 128 rows of B: A in tensor memory, 16 bits, each 2 * RUN of its columns (RUN of tensor memory) packed into
+// the front of the PITCH columns of scores that they were made from.
+template <int RUN, int PITCH>
+__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    umma_ts(d, a + (kk < 4 ? kk * 8 : half + (kk - 4) * 8), b + kk * (16 * 128 >> 4), idesc, accumulate || kk != 0);
+    umma_ts(d, a + kk * 8 / RUN * PITCH + kk * 8 % RUN, b + kk * (16 * 128 >> 4), idesc, accumulate || kk != 0);
+}
+// What a warp has written to tensor memory goes to the products: one arrival a warp.
+__device__ __forceinline__ void hand_over(uint64_t* bar, int lane) {
+  tmem_st_wait();
+  tcgen05_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
 }
 
 template <typename T>
@@ -206,7 +251,7 @@ __device__ __forceinline__ void row_keys(const Shape& s, int q, int& lo, int& hi
 __device__ __forceinline__ void finish(uint32_t tmem_base, int warp) {
   tcgen05_fence_before();
   __syncthreads();
-  if (warp == 9) tmem_dealloc(tmem_base, kTmemCols);
+  if (warp == kIssuer) tmem_dealloc(tmem_base, kTmemCols);
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -221,9 +266,10 @@ struct FwdArgs {
 template <int D>
 struct FwdSmem {
   static constexpr int kTile = kT * D * 2;
-  static constexpr int kStages = D == 128 ? 5 : 6;
-  static constexpr int kBars = (2 + kStages) * kTile;
-  static constexpr int kSize = 1024 + kBars + 256;
+  static constexpr int kStages = D == 128 ? 4 : 6;
+  static constexpr int kXch = (2 + kStages) * kTile;            // maxima and sums of half rows, two of each
+  static constexpr int kBars = kXch + 2 * 2 * 2 * kT * 4;
+  static constexpr int kSize = 1024 + kBars + 512;
 };
 
 template <typename T, int D>
@@ -242,7 +288,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* s_full = kv_empty + L::kStages;    // [2]
   uint64_t* p_full = s_full + 2;               // [2]
   uint64_t* o_full = p_full + 2;               // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* x_full = o_full + 2;               // [8]: the two warps of 32 rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(x_full + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const Shape& s = a.s;
@@ -265,19 +312,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], kArith / 2);
       mbar_init(&o_full[i], 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(&x_full[i], 2);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == kIssuer) tmem_alloc(tmem_slot, kTmemCols);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 8) {
+  if (warp == kLoader) {
     // ---------------- loader: keys and values of a block take a stage each, in turn ----------------
     if (lane == 0 && ja < jb) {
       prefetch_tmap(&tm_q);
@@ -301,7 +349,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kIssuer) {
     // ---------------- products ----------------
     const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
     const uint64_t qd = make_desc_sw128(smem_u32(sQ)), kd = make_desc_sw128(smem_u32(sKV)), vd = make_desc_mn(smem_u32(sKV));
@@ -336,7 +384,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (!ok) break;
           tcgen05_fence_after();
           if (elect_one()) {
-            mma_sum(tmem + 2 * kT + t * kT, tmem + t * kT, 32, vd + (uint64_t)((n + 1) % L::kStages * (L::kTile >> 4)), idesc_o,
+            mma_sum<64, 64>(tmem + 2 * kT + t * kT, tmem + t * kT, vd + (uint64_t)((n + 1) % L::kStages * (L::kTile >> 4)), idesc_o,
                     j > j0[t]);
             umma_commit(&o_full[t]);
           }
@@ -352,41 +400,52 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
   } else {
-    // ---------------- soft-max: a thread to a row ----------------
-    const int t = warp >> 2, r = threadIdx.x & 127;
+    // ---------------- soft-max: two threads to a row, 64 columns each ----------------
+    const int t = warp >> 3, hf = warp >> 2 & 1, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + t * kT, tO = tmem + lanes + 2 * kT + t * kT;
+    uint64_t* x_bar = &x_full[t * 4 + (warp & 3)];
+    float* xch = reinterpret_cast<float*>(smem + L::kXch) + t * 4 * kT;   // [2 turns][2 halves][128]
     const int q = q0 + t * kT + r;
     int klo, khi;
     row_keys(s, q, klo, khi);
     const float c = s.scale_log2;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = j0[t]; j < j1[t]; ++j) {
-      const int it = j - j0[t], k0 = j * kT;
-      if (!warp_wait(&s_full[t], it & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+    const int n = j1[t] - j0[t];
+    for (int it = 0; it < n; ++it) {
+      const int k0 = (j0[t] + it) * kT + hf * 64;
+      if (!warp_wait(&s_full[t], it & 1, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
-      float v[kT];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(tS + 32 * i, v + 32 * i);
-      uint32_t see[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        see[i] = range_bits(klo - k0, khi - k0, 32 * i);
-        if (s.mask != nullptr) see[i] &= __ldg(s.mask + (int64_t)b * s.k_words + j * 4 + i);
+      float v[64];
+      tmem_ld32(tS + hf * 64, v);
+      tmem_ld32(tS + hf * 64 + 32, v + 32);
+      uint32_t see0 = range_bits(klo, khi, k0), see1 = range_bits(klo, khi, k0 + 32);
+      if (s.mask != nullptr) {
+        const uint32_t* w = s.mask + (int64_t)b * s.k_words + (k0 >> 5);
+        see0 &= __ldg(w);
+        see1 &= __ldg(w + 1);
       }
-      const bool all = (see[0] & see[1] & see[2] & see[3]) == 0xFFFFFFFFu;
       tmem_ld_wait(v);
-      if (!__all_sync(0xffffffffu, all)) {
+      if (!__all_sync(0xffffffffu, (see0 & see1) == 0xFFFFFFFFu)) {
 #pragma unroll
-        for (int i = 0; i < kT; ++i) v[i] = see[i >> 5] >> (i & 31) & 1 ? v[i] : -INFINITY;
+        for (int i = 0; i < 64; ++i) v[i] = (i < 32 ? see0 : see1) >> (i & 31) & 1 ? v[i] : -INFINITY;
       }
       float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-      for (int i = 4; i < kT; i += 4)
+      for (int i = 4; i < 64; i += 4)
 #pragma unroll
         for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], v[i + u]);
-      const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      // The other half's maximum.  Behind this the other warp has read its scores too, which this one's probabilities may cover.
+      float* turn = xch + (it & 1) * 2 * kT;
+      turn[hf * kT + r] = top;
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x_bar);
+      if (!warp_wait(x_bar, it & 1, abort_flag)) { ok = false; break; }
+      tcgen05_fence_after();
+      top = fmaxf(m, fmaxf(top, turn[(hf ^ 1) * kT + r]));
       // The reference moves only when it falls behind by a factor of 2^8: until then sums and products stay below 2^8 times
       // what they would be, far from the end of their range, and the outputs need not be read.
       const bool move = (top - m) * c > 8.f;
@@ -395,53 +454,53 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         l *= f;
         if (move) m = top;
         if (it > 0) {
-          if (!warp_wait(&o_full[t], (it - 1) & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+          if (!warp_wait(&o_full[t], (it - 1) & 1, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
 #pragma unroll
-          for (int cc = 0; cc < D; cc += 32) {
-            float o[32];
-            tmem_ld32(tO + cc, o);
+          for (int cc = 0; cc < D / 2; cc += 16) {       // 16 at a time: the scores stay in registers
+            float o[16];
+            tmem_ld16(tO + hf * (D / 2) + cc, o);
             tmem_ld_wait(o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
-            tmem_st32(tO + cc, reinterpret_cast<const uint32_t*>(o));
+            for (int i = 0; i < 16; ++i) o[i] *= f;
+            tmem_st16(tO + hf * (D / 2) + cc, reinterpret_cast<const uint32_t*>(o));
           }
         }
       }
       const float mc = m == -INFINITY ? 0.f : -m * c;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t pk[32];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float p0 = ex2(fmaf(v[64 * g + 2 * i], c, mc)), p1 = ex2(fmaf(v[64 * g + 2 * i + 1], c, mc));
-          sum[i & 1] += p0;
-          sum[2 + (i & 1)] += p1;
-          pk[i] = pack2<T>(p0, p1);
-        }
-        tmem_st32(tS + 32 * g, pk);
+      for (int i = 0; i < 32; ++i) {
+        const float p0 = ex2(fmaf(v[2 * i], c, mc)), p1 = ex2(fmaf(v[2 * i + 1], c, mc));
+        sum[i & 1] += p0;
+        sum[2 + (i & 1)] += p1;
+        pk[i] = pack2<T>(p0, p1);
       }
+      tmem_st32(tS + 32 * hf, pk);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tcgen05_fence_before();
-      mbar_arrive(&p_full[t]);
+      hand_over(&p_full[t], lane);
     }
-    const int n = j1[t] - j0[t];
     if (ok && n > 0) {
-      ok = warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
-      if (!ok && lane == 0) report(s.err, 73);
+      // the row's sum, and the last product
+      float* turn = xch + (n & 1) * 2 * kT;
+      turn[hf * kT + r] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x_bar);
+      ok = warp_wait(x_bar, n & 1, abort_flag) && warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
       tcgen05_fence_after();
+      if (ok) l += turn[(hf ^ 1) * kT + r];
     }
+    if (!ok && lane == 0) report(s.err, 73);
     if (ok && q0 + t * kT < s.Sq) {
       const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : NAN;   // a row without keys: zeros
-      if (a.nlse != nullptr) {
+      if (a.nlse != nullptr && hf == 0) {
         const bool none = q >= s.Sq || m == -INFINITY;
         a.nlse[((int64_t)b * s.Hq + h) * s.q_pad + q] = none ? -INFINITY : a.shift - m * c - log2f(l);
       }
       T* dst = reinterpret_cast<T*>(a.out) + (((int64_t)b * s.Sq + q) * s.Hq + h) * s.D;
 #pragma unroll
-      for (int cc = 0; cc < D; cc += 32) {
+      for (int cc = hf * 32; cc < D; cc += 64) {
         float o[32];
         if (n > 0) {
           tmem_ld32(tO + cc, o);
@@ -470,13 +529,39 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // ------------------------------------------------------------------------------------------------ before the backward pass
 // delta_i = dO_i . o_i, a warp to a row (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
 // heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
+// Three pieces of 16 bits whose weighted sum is x, in a row of eight numbers: the third takes what the first two leave, below
+// 2^-24 of x.  fp16's weights spread the pieces over its range: numbers up to 2^23, to 2^-43.
+template <typename T> struct Pieces;
+template <> struct Pieces<__nv_bfloat16> {
+  static __device__ float weight(int) { return 1.f; }
+};
+template <> struct Pieces<__half> {
+  static __device__ float weight(int i) { return i == 0 ? 256.f : i == 1 ? 0x1p-6f : 0x1p-18f; }
+};
+template <typename T>
+__device__ __forceinline__ uint4 in_pieces(float x) {
+  __align__(16) T v[8];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const float w = Pieces<T>::weight(i);
+    v[i] = from_float<T>(x / w);
+    x -= to_float<T>(v[i]) * w;
+  }
+#pragma unroll
+  for (int i = 3; i < 8; ++i) v[i] = from_float<T>(0.f);
+  return *reinterpret_cast<const uint4*>(v);
+}
+
 struct PrepArgs {
   const void* out;         // [B, Sq, Hq, D]
   const void* low;
   const void* grad;        // by strides
   const void* v;
   int64_t g_b, g_h, g_s, v_b, v_h, v_s;
+  const float* nlse;       // [B, Hq, q_pad]
   float* delta;            // [B, Hq, q_pad]
+  uint4* pieces;           // [B, Hq, q_pad / 128][2][128]: of -L / scale and of -delta; rows that see nothing: 0
+  float inv_scale_log2;
   uint32_t* bound;         // [B, Hkv, 2] zeros, or null
   int B, Hq, Hkv, Sq, Skv, D, q_pad;
 };
@@ -523,7 +608,13 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
     d += __shfl_xor_sync(0xffffffffu, d, o);
     n += __shfl_xor_sync(0xffffffffu, n, o);
   }
-  if (sub == 0 && row < rows_q) a.delta[row] = d;
+  if (sub == 0 && row < rows_q) {
+    a.delta[row] = d;
+    const float nl = a.nlse[row];
+    uint4* at = a.pieces + row / kT * (2 * kT) + row % kT;
+    at[0] = in_pieces<T>(nl == -INFINITY ? 0.f : nl * a.inv_scale_log2);
+    at[kT] = in_pieces<T>(-d);
+  }
   if (sub == 0 && a.bound != nullptr && group >= 0 && n > __uint_as_float(a.bound[group])) atomicMax(&a.bound[group], __float_as_uint(n));
 }
 
@@ -540,6 +631,7 @@ struct BwdArgs {
   Shape s;
   const float* nlse;      // [B, Hq, q_pad]
   const float* delta;     // [B, Hq, q_pad]
+  const uint4* pieces;
   const uint32_t* bound;  // [B, Hkv, 2] or null
   void* dq;               // [B, Sq, Hq, D]
   void* dk;               // [B, Skv, Hkv, D]
@@ -552,8 +644,9 @@ template <int D>
 struct BwdSmem {
   static constexpr int kTile = kT * D * 2;
   static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int kStat = (2 + 2 * kStages) * kTile;       // nlse and delta of a stage's queries
-  static constexpr int kBars = kStat + kStages * 1024;
+  static constexpr int kPieces = (2 + 2 * kStages) * kTile;     // of -L / scale and -delta of a stage's queries
+  static constexpr int kWeights = kPieces + kStages * 4096;     // 16 columns of the pieces' weights, eight of them zeros
+  static constexpr int kBars = kWeights + 4096;
   static constexpr int kSize = 1024 + kBars + 256;
 };
 
@@ -568,7 +661,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint8_t* sK = smem;
   uint8_t* sV = smem + L::kTile;
   uint8_t* sQG = smem + 2 * L::kTile;            // stages of [q | dO]
-  float* stat = reinterpret_cast<float*>(smem + L::kStat);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* kv_full = bars;
   uint64_t* full = bars + 1;
@@ -599,20 +691,27 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_init(&empty[i], 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(p_full, 256);
+    mbar_init(p_full, kArith);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 256);
+    mbar_init(ds_full, kArith);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, kTmemCols);
+  if (threadIdx.x < 256) {
+    __align__(16) T w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = from_float<T>(threadIdx.x < kT && i < 3 ? Pieces<T>::weight(i) : 0.f);
+    reinterpret_cast<uint4*>(smem + L::kWeights)[threadIdx.x] = *reinterpret_cast<const uint4*>(w);
+    fence_proxy_async_smem();
+  }
+  if (warp == kIssuer) tmem_alloc(tmem_slot, kTmemCols);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot, tP = tmem + kT, tV = tmem + 2 * kT, tK = tmem + 3 * kT;
 
-  if (warp == 8) {
+  if (warp == kLoader) {
     if (lane == 0 && total > 0) {
       prefetch_tmap(&tm_q);
       prefetch_tmap(&tm_g);
@@ -624,12 +723,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       for (; n < total; ++n) {
         const int st = n % L::kStages, h = kvh * group + n / ni, q0 = (i0 + n % ni) * kT;
         if (!mbar_wait(&empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
-        mbar_expect_tx(&full[st], 2 * L::kTile + 1024);
+        mbar_expect_tx(&full[st], 2 * L::kTile + 4096);
         load_tile<D>(sQG + 2 * st * L::kTile, &tm_q, q0, h, b, &full[st]);
         load_tile<D>(sQG + (2 * st + 1) * L::kTile, &tm_g, q0, h, b, &full[st]);
-        const int64_t row = ((int64_t)b * s.Hq + h) * s.q_pad + q0;
-        bulk_load(stat + st * 256, a.nlse + row, 512, &full[st]);
-        bulk_load(stat + st * 256 + 128, a.delta + row, 512, &full[st]);
+        bulk_load(smem + L::kPieces + st * 4096, a.pieces + (((int64_t)b * s.Hq + h) * s.q_pad + q0) * 2, 4096, &full[st]);
       }
       if (!ok) {
         mbar_wait_quiet(kv_full, 0, 1 << 12);
@@ -638,15 +735,18 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kIssuer) {
     const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
     const uint64_t kd = make_desc_sw128(smem_u32(sK)), vd = make_desc_sw128(smem_u32(sV));
     const uint64_t qg_rows = make_desc_sw128(smem_u32(sQG)), qg_sum = make_desc_mn(smem_u32(sQG));
+    const uint64_t weights = make_desc_rows16(smem_u32(smem + L::kWeights), 2048);
+    const uint64_t pieces = make_desc_rows16(smem_u32(smem + L::kPieces), 0);   // their second eight columns: the first once more
     auto at = [&](int n, int which) { return (uint64_t)((2 * (n % L::kStages) + which) * (L::kTile >> 4)); };
     auto wait_full = [&](int n) { return warp_wait(&full[n % L::kStages], n / L::kStages & 1, abort_flag); };
     auto scores = [&](int n) {                  // k q^T
       if (elect_one()) {
         mma_rows<D>(tmem, kd, qg_rows + at(n, 0), idesc_s);
+        umma_f16(tmem, weights, pieces + (n % L::kStages * 4096 >> 4), idesc_s, true);
         umma_commit(s_full);
       }
       __syncwarp();
@@ -654,6 +754,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     auto grads = [&](int n) {                   // v dO^T
       if (elect_one()) {
         mma_rows<D>(tP, vd, qg_rows + at(n, 1), idesc_s);
+        umma_f16(tP, weights, pieces + (n % L::kStages * 4096 + 2048 >> 4), idesc_s, true);
         umma_commit(dp_full);
       }
       __syncwarp();
@@ -668,7 +769,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       ok = warp_wait(p_full, n & 1, abort_flag);
       if (!ok) break;
       tcgen05_fence_after();
-      if (elect_one()) mma_sum(tV, tmem, 64, qg_sum + at(n, 1), idesc_o, n > 0);
+      if (elect_one()) mma_sum<16, 32>(tV, tmem, qg_sum + at(n, 1), idesc_o, n > 0);
       __syncwarp();
       if (n + 1 < total) {
         ok = wait_full(n + 1);
@@ -680,7 +781,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (!ok) break;
       tcgen05_fence_after();
       if (elect_one()) {
-        mma_sum(tK, tP, 64, qg_sum + at(n, 0), idesc_o, n > 0);
+        mma_sum<16, 32>(tK, tP, qg_sum + at(n, 0), idesc_o, n > 0);
         umma_commit(n + 1 < total ? &empty[n % L::kStages] : done);
       }
       __syncwarp();
@@ -689,110 +790,77 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
   } else {
-    // ---------------- a key (and half of the queries) to a thread ----------------
-    const int r = threadIdx.x & 127, hf = warp >> 2;
-    const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16) + hf * 64;
+    // ---------------- a key and a quarter of the queries to a thread ----------------
+    const int qd = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + qd * 32;
     const int k = k0 + r;
     const float c = s.scale_log2;
     const float f = a.bound != nullptr ? grad_factor(a.bound, b * s.Hkv + kvh, a.shift) : 1.f;
     bool ok = true;
     for (int n = 0; n < total; ++n) {
-      const int st = n % L::kStages, q0 = (i0 + n % ni) * kT;
+      const int q0 = (i0 + n % ni) * kT;
       const uint32_t par = n & 1;
-      if (!warp_wait(&full[st], n / L::kStages & 1, abort_flag) || !warp_wait(s_full, par, abort_flag)) {
-        ok = false;
-        if (lane == 0) report(s.err, 73);
-        break;
-      }
+      if (!warp_wait(s_full, par, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
-      float p[64];
+      float p[32];
       tmem_ld32(tmem + lanes, p);
-      tmem_ld32(tmem + lanes + 32, p + 32);
-      const float4* nl = reinterpret_cast<const float4*>(stat + st * 256 + hf * 64);
-      const float4* dl = nl + 32;
       // this key is seen by queries [lo, hi)
       const int lo = s.causal ? k - off - q0 : -kT, hi = s.window > 0 ? min((int64_t)kT, (int64_t)k - off - q0 + s.window) : kT;
-      const uint32_t see0 = range_bits(lo, hi, hf * 64), see1 = range_bits(lo, hi, hf * 64 + 32);
-      const bool all = (see0 & see1) == 0xFFFFFFFFu;
+      const uint32_t see = range_bits(lo, hi, qd * 32);
       tmem_ld_wait(p);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float4 w = nl[i];
-        p[4 * i] = ex2(fmaf(p[4 * i], c, w.x));
-        p[4 * i + 1] = ex2(fmaf(p[4 * i + 1], c, w.y));
-        p[4 * i + 2] = ex2(fmaf(p[4 * i + 2], c, w.z));
-        p[4 * i + 3] = ex2(fmaf(p[4 * i + 3], c, w.w));
-      }
-      if (!__all_sync(0xffffffffu, all)) {
+      for (int i = 0; i < 32; ++i) p[i] = ex2(p[i] * c);
+      if (!__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) p[i] = (i < 32 ? see0 : see1) >> (i & 31) & 1 ? p[i] : 0.f;
+        for (int i = 0; i < 32; ++i) p[i] = see >> i & 1 ? p[i] : 0.f;
       }
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
-      tmem_st32(tmem + lanes, pk);
-      tmem_st_wait();
-      tcgen05_fence_before();
-      mbar_arrive(p_full);
-      if (!warp_wait(dp_full, par, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      for (int i = 0; i < 16; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+      tmem_st16(tmem + lanes, pk);
+      hand_over(p_full, lane);
+      if (!warp_wait(dp_full, par, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
-      float d[64];
+      float d[32];
       tmem_ld32(tP + lanes, d);
-      tmem_ld32(tP + lanes + 32, d + 32);
       tmem_ld_wait(d);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float4 w = dl[i];
-        d[4 * i] = p[4 * i] * (d[4 * i] - w.x);
-        d[4 * i + 1] = p[4 * i + 1] * (d[4 * i + 1] - w.y);
-        d[4 * i + 2] = p[4 * i + 2] * (d[4 * i + 2] - w.z);
-        d[4 * i + 3] = p[4 * i + 3] * (d[4 * i + 3] - w.w);
+        float x = p[2 * i] * d[2 * i], y = p[2 * i + 1] * d[2 * i + 1];
+        if constexpr (std::is_same<T, __half>::value) {
+          x *= f;
+          y *= f;
+        }
+        pk[i] = pack2<T>(x, y);
       }
-      if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) d[i] *= f;
-      }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) pk[i] = pack2<T>(d[2 * i], d[2 * i + 1]);
-      tmem_st32(tP + lanes, pk);
-      tmem_st_wait();
-      tcgen05_fence_before();
-      mbar_arrive(ds_full);
+      tmem_st16(tP + lanes, pk);
+      hand_over(ds_full, lane);
     }
     if (ok && total > 0) {
       ok = warp_wait(done, 0, abort_flag);
-      if (!ok && lane == 0) report(s.err, 73);
       tcgen05_fence_after();
     }
+    if (!ok && lane == 0) report(s.err, 73);
     if (ok) {
-      // half of the columns to a thread: dv, then dk
       bool real = k < s.Skv && total > 0;
       if (real && s.mask != nullptr) real = s.mask[(int64_t)b * s.k_words + (k >> 5)] >> (k & 31) & 1;
       const int64_t row = (((int64_t)b * s.Skv + k) * s.Hkv + kvh) * s.D;
-      const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16;
       const float un = exp2f(-a.shift);
+      // 32 columns at a time: those of dv, then those of dk
 #pragma unroll
-      for (int cc = 0; cc < D / 2; cc += 32) {
-        const int col = hf * (D / 2) + cc;
+      for (int i = qd; i < 2 * D / 32; i += 4) {
+        const bool is_v = i < D / 32;
+        const int col = i % (D / 32) * 32;
         float o[32];
         if (total > 0) {
-          tmem_ld32(tV + mine + col, o);
+          tmem_ld32((is_v ? tV : tK) + mine + col, o);
           tmem_ld_wait(o);
         }
         if (!real) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
         }
-        if (k < s.Skv) put_row32<T>(reinterpret_cast<T*>(a.dv) + row, o, un, col, s.D);
-        if (total > 0) {
-          tmem_ld32(tK + mine + col, o);
-          tmem_ld_wait(o);
-        }
-        if (!real) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
-        if (k < s.Skv) put_row32<T>(reinterpret_cast<T*>(a.dk) + row, o, s.scale * un / f, col, s.D);
+        if (k < s.Skv) put_row32<T>(reinterpret_cast<T*>(is_v ? a.dv : a.dk) + row, o, is_v ? un : s.scale * un / f, col, s.D);
       }
     }
   }
@@ -839,19 +907,19 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, 256);
+    mbar_init(ds_full, kArith);
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, kTmemCols);
+  if (warp == kIssuer) tmem_alloc(tmem_slot, kTmemCols);
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
   // two tiles of scores in turn, dP (and dS over it), the sum
   const uint32_t tmem = *tmem_slot, tP = tmem + 2 * kT, tQ = tmem + 3 * kT;
 
-  if (warp == 8) {
+  if (warp == kLoader) {
     if (lane == 0 && total > 0) {
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
@@ -874,7 +942,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == kIssuer) {
     const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
     const uint64_t qd = make_desc_sw128(smem_u32(sQ)), gd = make_desc_sw128(smem_u32(sG));
     const uint64_t kv_rows = make_desc_sw128(smem_u32(sKV)), kv_sum = make_desc_mn(smem_u32(sKV));
@@ -912,7 +980,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (!ok) break;
       tcgen05_fence_after();
       if (elect_one()) {
-        mma_sum(tQ, tP, 64, kv_sum + at(n, 0), idesc_o, n > 0);
+        mma_sum<16, 32>(tQ, tP, kv_sum + at(n, 0), idesc_o, n > 0);
         umma_commit(n + 1 < total ? &empty[n % L::kStages] : done);
       }
       __syncwarp();
@@ -921,9 +989,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
   } else {
-    // ---------------- half of a query's keys to a thread ----------------
-    const int r = threadIdx.x & 127, hf = warp >> 2;
-    const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + hf * 64;
+    // ---------------- a quarter of a query's keys to a thread ----------------
+    const int qd = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + qd * 32;
     const int q = q0 + r;
     int klo, khi;
     row_keys(s, q, klo, khi);
@@ -933,62 +1001,48 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const float nl = a.nlse[at], dl = a.delta[at] * -f;
     bool ok = true;
     for (int n = 0; n < total; ++n) {
-      const int kb = (j0 + n) * kT + hf * 64;
-      if (!warp_wait(&s_full[n & 1], n >> 1 & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      const int kb = (j0 + n) * kT + qd * 32;
+      if (!warp_wait(&s_full[n & 1], n >> 1 & 1, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
-      float p[64];
+      float p[32];
       tmem_ld32(tmem + lanes + (n & 1) * kT, p);
-      tmem_ld32(tmem + lanes + (n & 1) * kT + 32, p + 32);
-      uint32_t see0 = range_bits(klo, khi, kb), see1 = range_bits(klo, khi, kb + 32);
-      if (s.mask != nullptr) {
-        const uint32_t* w = s.mask + (int64_t)b * s.k_words + (kb >> 5);
-        see0 &= __ldg(w);
-        see1 &= __ldg(w + 1);
-      }
-      const bool all = (see0 & see1) == 0xFFFFFFFFu;
+      uint32_t see = range_bits(klo, khi, kb);
+      if (s.mask != nullptr) see &= __ldg(s.mask + (int64_t)b * s.k_words + (kb >> 5));
       tmem_ld_wait(p);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(p[i], c, nl));
-      if (!__all_sync(0xffffffffu, all)) {
+      for (int i = 0; i < 32; ++i) p[i] = ex2(fmaf(p[i], c, nl));
+      if (!__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) p[i] = (i < 32 ? see0 : see1) >> (i & 31) & 1 ? p[i] : 0.f;
+        for (int i = 0; i < 32; ++i) p[i] = see >> i & 1 ? p[i] : 0.f;
       }
-      if (!warp_wait(dp_full, n & 1, abort_flag)) { ok = false; if (lane == 0) report(s.err, 73); break; }
+      if (!warp_wait(dp_full, n & 1, abort_flag)) { ok = false; break; }
       tcgen05_fence_after();
-      float d[64];
+      float d[32];
       tmem_ld32(tP + lanes, d);
-      tmem_ld32(tP + lanes + 32, d + 32);
       tmem_ld_wait(d);
-      uint32_t pk[32];
+      uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
+      for (int i = 0; i < 16; ++i)
         pk[i] = pack2<T>(p[2 * i] * fmaf(d[2 * i], f, dl), p[2 * i + 1] * fmaf(d[2 * i + 1], f, dl));
-      tmem_st32(tP + lanes, pk);
-      tmem_st_wait();
-      tcgen05_fence_before();
-      mbar_arrive(ds_full);
+      tmem_st16(tP + lanes, pk);
+      hand_over(ds_full, lane);
     }
     if (ok && total > 0) {
       ok = warp_wait(done, 0, abort_flag);
-      if (!ok && lane == 0) report(s.err, 73);
       tcgen05_fence_after();
     }
-    if (ok) {
+    if (!ok && lane == 0) report(s.err, 73);
+    if (ok && qd < D / 32) {
       T* dst = reinterpret_cast<T*>(a.dq) + (((int64_t)b * s.Sq + q) * s.Hq + h) * s.D;
-      const float un = s.scale * exp2f(-a.shift) / f;
+      float o[32];
+      if (total > 0) {
+        tmem_ld32(tQ + mine + qd * 32, o);
+        tmem_ld_wait(o);
+      } else {
 #pragma unroll
-      for (int cc = 0; cc < D / 2; cc += 32) {
-        const int col = hf * (D / 2) + cc;
-        float o[32];
-        if (total > 0) {
-          tmem_ld32(tQ + mine + col, o);
-          tmem_ld_wait(o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
-        if (q < s.Sq) put_row32<T>(dst, o, un, col, s.D);
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
       }
+      if (q < s.Sq) put_row32<T>(dst, o, s.scale * exp2f(-a.shift) / f, qd * 32, s.D);
     }
   }
   finish(tmem, warp);
@@ -1061,7 +1115,7 @@ bool bind_context() {
 
 bool shape_ok(int B, int Hq, int Hkv, int Sq, int Skv, int D, int window, float scale) {
   return B >= 1 && B <= 65535 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq <= (1 << 20) && Sq >= 1 && Skv >= 1 &&
-         Sq <= (1 << 23) && Skv <= (1 << 23) && D >= 8 && D <= 128 && D % 8 == 0 && window >= 0 && scale > 0.f && scale < 1e30f;
+         Sq <= (1 << 23) && Skv <= (1 << 23) && D >= 8 && D <= 128 && D % 8 == 0 && window >= 0 && scale >= 1e-4f && scale <= 1e4f;
 }
 
 Shape make_shape(int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window, const uint32_t* mask, float scale, int* err) {
@@ -1101,7 +1155,7 @@ int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
 
 template <typename T, int D>
 int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, const Tensor4& g, const void* out,
-            const void* low, const float* nlse, float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
+            const void* low, const float* nlse, float* work, void* dq, void* dk, void* dv, cudaStream_t stream) {
   CUtensorMap tq, tk, tv, tg;
   const CUtensorMapDataType dt = map_type<T>();
   if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
@@ -1114,15 +1168,17 @@ int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
   if (e != cudaSuccess) return (int)e;
   uint32_t* bound = nullptr;
   if (std::is_same<T, __half>::value) {
-    bound = reinterpret_cast<uint32_t*>(delta + (int64_t)s.B * s.Hq * s.q_pad);
+    bound = reinterpret_cast<uint32_t*>(work + (int64_t)s.B * s.Hq * s.q_pad * 9);
     e = cudaMemsetAsync(bound, 0, (size_t)s.B * s.Hkv * 8, stream);
     if (e != cudaSuccess) return (int)e;
   }
-  PrepArgs p = {out, low, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, delta, bound, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
+  uint4* pieces = reinterpret_cast<uint4*>(work);
+  float* delta = work + (int64_t)s.B * s.Hq * s.q_pad * 8;
+  PrepArgs p = {out, low, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, nlse, delta, pieces, 1.f / s.scale_log2, bound, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
   const int64_t rows = (int64_t)s.B * s.Hq * s.q_pad + (bound != nullptr ? (int64_t)s.B * s.Hkv * s.Skv : 0);
   if (rows / 16 + 1 > 0x7FFFFFFF) return (int)cudaErrorInvalidValue;
   attn_prep_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(p);
-  BwdArgs a = {s, nlse, delta, bound, dq, dk, dv, shift_of<T>()};
+  BwdArgs a = {s, nlse, delta, pieces, bound, dq, dk, dv, shift_of<T>()};
   attn_dkv_kernel<T, D><<<dim3(s.Hkv, (s.Skv + kT - 1) / kT, s.B), kThreads, smem, stream>>>(tq, tk, tv, tg, a);
   attn_dq_kernel<T, D><<<dim3(s.Hq, (s.Sq + kT - 1) / kT, s.B), kThreads, smem, stream>>>(tq, tk, tv, tg, a);
   return (int)cudaGetLastError();
@@ -1154,7 +1210,7 @@ IPEX_API int ipex_attn_train_fwd(const void* q, int64_t q_b, int64_t q_h, int64_
   return (int)cudaErrorInvalidValue;
 }
 
-// g: the gradient of out, by strides like q.  work: scratch, 16-byte aligned, as many floats as nlse has and 2 B Hkv.  dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
+// g: the gradient of out, by strides like q.  work: scratch, 16-byte aligned, 9 floats for each of nlse and 2 B Hkv.  dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
 IPEX_API int ipex_attn_train_bwd(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
                                  int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, const uint32_t* mask_words,
                                  const void* out, const void* low, const float* nlse, const void* g, int64_t g_b, int64_t g_h,

@@ -89,7 +89,7 @@ class _Attention(torch.autograd.Function):
         dq = torch.empty_like(out)
         dk = torch.empty((B, Skv, Hkv, D), dtype=q.dtype, device=dev)
         dv = torch.empty_like(dk)
-        work = torch.empty(stats.numel() + 2 * B * Hkv, dtype=torch.float32, device=dev)
+        work = torch.empty(9 * stats.numel() + 2 * B * Hkv, dtype=torch.float32, device=dev)
         with _on(dev):
             rc = stream_lib("train_attn").ipex_attn_train_bwd(
                 *q_at, *k_at, *v_at, ptr(words), ptr(out), ptr(low), ptr(stats), *g_at, ptr(work), ptr(dq), ptr(dk), ptr(dv),
@@ -131,8 +131,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
 
     ``causal``: query i sees keys up to i + Skv - Sq (the queries are the last of the keys' sequence); ``window``: and only so
     many, itself among them.  ``key_mask [B, Skv]``: True (or not 0) for real keys, as a tokenizer's attention mask; what hidden
-    rows hold, NaN included, takes no part.  A query that sees no key gives zeros and gets no gradient.  ``scale`` (positive)
-    defaults to D^-1/2.
+    rows hold, NaN included, takes no part.  A query that sees no key gives zeros and gets no gradient.  ``scale`` (1e-4 to
+    1e4) defaults to D^-1/2.
 
     GPU: fp16 or bf16, D a multiple of 8 up to 128, any strides (rows that are not contiguous, or not aligned to 16 bytes, are
     copied).  Scores, sums and gradients are summed in 32 bits; probabilities and their gradients are rounded to 16 bits
@@ -148,8 +148,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
         invalidInputError(False, "attention: q, k and v should have one type and lie on one device")
     scale, window = D ** -0.5 if scale is None else float(scale), int(window)
-    if not 0.0 < scale < 1e30:
-        invalidInputError(False, f"attention: the scale has to be positive and finite, got {scale}")
+    if not 1e-4 <= scale <= 1e4:
+        invalidInputError(False, f"attention: the scale should lie between 1e-4 and 1e4, got {scale}")
     if not 0 <= window < 1 << 31 or (window and not causal):
         invalidInputError(False, f"attention: a window of {window} tokens needs causal attention and has to be positive (0: none)")
     if key_mask is not None:

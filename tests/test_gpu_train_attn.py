@@ -107,7 +107,8 @@ def test_peaked_scores():
     q, k, v, g = _inputs(1, 2, 1, 700, 700, 64, torch.float16, 6)
     _check(q * 8, k * torch.linspace(0.1, 8, 700, device="cuda").half().view(1, 1, -1, 1), v, g)
     _check(q, k, v, g, scale=3.0)
-    _check(q, k, v, g, scale=1e-6)
+    _check(q, k, v, g, scale=1e-4)
+    _check(q, k, v, g, scale=100.0)
 
 
 def test_layouts():
