@@ -47,6 +47,8 @@ constexpr int kLoader = kArith, kIssuer = kArith + 1;
 constexpr int kThreads = 32 * (kArith + 2);
 constexpr uint32_t kTmemCols = 512;
 constexpr int kShiftF16 = 12;     // P is stored times 2^12 in fp16
+template <typename T> __host__ __device__ constexpr float shift_of() { return std::is_same<T, __half>::value ? kShiftF16 : 0; }
+template <typename T> __host__ __device__ constexpr float scale_of() { return std::is_same<T, __half>::value ? 1 << kShiftF16 : 1; }
 // delta_i is the difference of all dP_ij of a row: with the rounded o its error reaches every dS_ij of the row with the same sign
 // and adds a third to the error of dq and dk (measured: 1.53 times the final rounding's instead of 1.42).  So what rounding takes
 // from o is kept too, rounded once more, times 2^11 so that it does not fall among fp16's subnormals.
@@ -104,17 +106,6 @@ __device__ __forceinline__ void tmem_ld_wait(float (&v)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int j = 0; j < N; ++j) asm volatile("" : "+f"(v[j]));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
-      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
-      "r"(v[31])
-      : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
   asm volatile(
@@ -185,6 +176,47 @@ __device__ __forceinline__ void hand_over(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
+// Two 32-bit numbers an instruction.
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // x *= a, y *= b
+  asm("{\n"
+      ".reg .b64 u, v;\n"
+      "mov.b64 u, {%0, %1};\n"
+      "mov.b64 v, {%2, %3};\n"
+      "mul.rn.f32x2 u, u, v;\n"
+      "mov.b64 {%0, %1}, u;\n"
+      "}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {   // x += a, y += b
+  asm("{\n"
+      ".reg .b64 u, v;\n"
+      "mov.b64 u, {%0, %1};\n"
+      "mov.b64 v, {%2, %3};\n"
+      "add.rn.f32x2 u, u, v;\n"
+      "mov.b64 {%0, %1}, u;\n"
+      "}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {   // x = x a + b, y = y a + b
+  asm("{\n"
+      ".reg .b64 u, v, w;\n"
+      "mov.b64 u, {%0, %1};\n"
+      "mov.b64 v, {%2, %2};\n"
+      "mov.b64 w, {%3, %3};\n"
+      "fma.rn.f32x2 u, u, v, w;\n"
+      "mov.b64 {%0, %1}, u;\n"
+      "}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -198,19 +230,34 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// 32 columns of a row out of tensor memory, times `f`, to 16-bit memory; columns from `width` on do not exist.
+// 32 rows x 32 columns of a warp, a row to a lane, times `f`, in 16 bits to shared memory (2 KB, the 64-byte swizzle), from where a
+// TMA store takes them to [b][h] of a tensor: whole sectors, where every lane storing its own row cost 2 to 6 us a tile.  What lies
+// past the tensor is not stored.
 template <typename T>
-__device__ __forceinline__ void put_row32(T* dst, const float (&v)[32], float f, int col, int width) {
+__device__ __forceinline__ void stage32(uint8_t* st, const float (&v)[32], float f, int lane) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    if (col + 8 * q >= width) break;
     uint4 w;
     w.x = pack2<T>(v[8 * q] * f, v[8 * q + 1] * f);
     w.y = pack2<T>(v[8 * q + 2] * f, v[8 * q + 3] * f);
     w.z = pack2<T>(v[8 * q + 4] * f, v[8 * q + 5] * f);
     w.w = pack2<T>(v[8 * q + 6] * f, v[8 * q + 7] * f);
-    *reinterpret_cast<uint4*>(dst + col + 8 * q) = w;
+    *reinterpret_cast<uint4*>(st + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = w;
   }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+__device__ __forceinline__ void store32(const CUtensorMap* tm, const uint8_t* st, int x, int y, int h, int b) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tm)),
+               "r"(smem_u32(st)), "r"(x), "r"(y), "r"(h), "r"(b)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Until at most N of this thread's stores have yet to read shared memory.
+template <int N>
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 
 struct Shape {
@@ -247,6 +294,13 @@ __device__ __forceinline__ void row_keys(const Shape& s, int q, int& lo, int& hi
   lo = s.window > 0 ? max(0, q + off - s.window + 1) : 0;
 }
 
+// A CTA stays on its SM and takes tiles of work, sorted from long to short, in turn with the others, every second round
+// backwards.  (A CTA to a tile cost 5 us between the last product of one and the first of the next, for barriers, tensor memory,
+// cold loads; here the ring of tiles runs on.)
+__device__ __forceinline__ unsigned item_of(int round) {
+  return round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // What a CTA takes down in every case.
 __device__ __forceinline__ void finish(uint32_t tmem_base, int warp) {
   tcgen05_fence_before();
@@ -255,12 +309,11 @@ __device__ __forceinline__ void finish(uint32_t tmem_base, int warp) {
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// Outputs go by the maps tm_o and, with nlse, tm_low: what rounding took from them, times kLowScale.
 struct FwdArgs {
   Shape s;
-  void* out;          // [B, Sq, Hq, D]
-  void* low;          // what rounding took from it, times kLowScale, for the backward pass; or null
-  float* nlse;        // [B, Hq, q_pad]: -L log2(e) (+ the shift of fp16); -inf for rows that see nothing and past Sq
-  float shift;
+  float* nlse;        // [B, Hq, q_pad]: -L log2(e) (+ the shift of fp16); -inf for rows that see nothing and past Sq; or null
+  unsigned items;
 };
 
 template <int D>
@@ -272,10 +325,29 @@ struct FwdSmem {
   static constexpr int kSize = 1024 + kBars + 512;
 };
 
+// Two tiles of queries [q0, q0 + 256) of a head.
+struct FwdItem {
+  int q0, h, b, kvh, j0[2], j1[2], ja, jb;
+  __device__ __forceinline__ FwdItem(const Shape& s, unsigned i) {
+    const int pairs = (s.Sq + 2 * kT - 1) / (2 * kT);
+    const unsigned rest = i / s.Hq;
+    h = (int)(i % s.Hq);
+    b = (int)(rest % s.B);
+    q0 = (pairs - 1 - (int)(rest / s.B)) * 2 * kT;
+    kvh = h / (s.Hq / s.Hkv);
+    key_blocks(s, q0, j0[0], j1[0]);
+    key_blocks(s, q0 + kT, j0[1], j1[1]);
+    const bool two = j1[1] > j0[1];
+    ja = two ? (j1[0] > j0[0] ? min(j0[0], j0[1]) : j0[1]) : j0[0];
+    jb = two ? max(j1[0], j1[1]) : j1[0];
+  }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FwdArgs a) {
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
+                const __grid_constant__ CUtensorMap tm_low, const __grid_constant__ FwdArgs a) {
   using L = FwdSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -283,7 +355,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint8_t* sKV = smem + 2 * L::kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* q_full = bars;
-  uint64_t* kv_full = bars + 1;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* kv_full = bars + 2;
   uint64_t* kv_empty = kv_full + L::kStages;
   uint64_t* s_full = kv_empty + L::kStages;    // [2]
   uint64_t* p_full = s_full + 2;               // [2]
@@ -294,18 +367,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
   const Shape& s = a.s;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int h = blockIdx.x, b = blockIdx.z, kvh = h / (s.Hq / s.Hkv);
-  // the longest rows first
-  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 2 * kT;
-  int j0[2], j1[2];
-  key_blocks(s, q0, j0[0], j1[0]);
-  key_blocks(s, q0 + kT, j0[1], j1[1]);
-  const int ja = j1[1] > j0[1] ? (j1[0] > j0[0] ? min(j0[0], j0[1]) : j0[1]) : j0[0];
-  const int jb = j1[1] > j0[1] ? max(j1[0], j1[1]) : j1[0];
-  const int n_tiles = q0 + kT < s.Sq ? 2 : 1;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
+    mbar_init(q_empty, kArith);
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&kv_full[i], 1);
       mbar_init(&kv_empty[i], 1);
@@ -327,23 +392,27 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
   if (warp == kLoader) {
     // ---------------- loader: keys and values of a block take a stage each, in turn ----------------
-    if (lane == 0 && ja < jb) {
+    if (lane == 0) {
       prefetch_tmap(&tm_q);
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
-      mbar_expect_tx(q_full, n_tiles * L::kTile);
-      for (int t = 0; t < n_tiles; ++t) load_tile<D>(sQ + t * L::kTile, &tm_q, q0 + t * kT, h, b, q_full);
       bool ok = true;
-      int n = 0;
-      for (int j = ja; j < jb && ok; ++j)
-        for (int w = 0; w < 2 && ok; ++w, ++n) {
+      int n = 0, w = 0;
+      for (; ok && item_of(w) < a.items; ++w) {
+        const FwdItem it(s, item_of(w));
+        if (!mbar_wait(q_empty, (w & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        const int n_tiles = it.ja >= it.jb ? 0 : it.q0 + kT < s.Sq ? 2 : 1;
+        mbar_expect_tx(q_full, n_tiles * L::kTile);
+        for (int t = 0; t < n_tiles; ++t) load_tile<D>(sQ + t * L::kTile, &tm_q, it.q0 + t * kT, it.h, it.b, q_full);
+        for (int m = 0; m < 2 * (it.jb - it.ja); ++m, ++n) {
           const int st = n % L::kStages;
           if (!mbar_wait(&kv_empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
           mbar_expect_tx(&kv_full[st], L::kTile);
-          load_tile<D>(sKV + st * L::kTile, w ? &tm_v : &tm_k, j * kT, kvh, b, &kv_full[st]);
+          load_tile<D>(sKV + st * L::kTile, m & 1 ? &tm_v : &tm_k, (it.ja + (m >> 1)) * kT, it.kvh, it.b, &kv_full[st]);
         }
+      }
       if (!ok) {
-        mbar_wait_quiet(q_full, 0, 1 << 12);
+        mbar_wait_quiet(q_full, w & 1, 1 << 12);
         for (int i = n - L::kStages < 0 ? 0 : n - L::kStages; i < n; ++i)
           mbar_wait_quiet(&kv_full[i % L::kStages], i / L::kStages & 1, 1 << 12);
       }
@@ -353,49 +422,56 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // ---------------- products ----------------
     const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
     const uint64_t qd = make_desc_sw128(smem_u32(sQ)), kd = make_desc_sw128(smem_u32(sKV)), vd = make_desc_mn(smem_u32(sKV));
-    bool ok = ja >= jb || warp_wait(q_full, 0, abort_flag);
-    auto scores = [&](int t, int j) {            // of a tile that sees block j
-      if (elect_one()) {
-        mma_rows<D>(tmem + t * kT, qd + t * (L::kTile >> 4), kd + (uint64_t)(2 * (j - ja) % L::kStages * (L::kTile >> 4)), idesc_s);
-        umma_commit(&s_full[t]);
-      }
-      __syncwarp();
-    };
-    auto has = [&](int t, int j) { return j >= j0[t] && j < j1[t]; };
+    auto slot = [&](int n) { return (uint64_t)(n % L::kStages * (L::kTile >> 4)); };
     auto wait_kv = [&](int n) { return warp_wait(&kv_full[n % L::kStages], n / L::kStages & 1, abort_flag); };
     auto free_kv = [&](int n) {
       if (elect_one()) umma_commit(&kv_empty[n % L::kStages]);
       __syncwarp();
     };
-    if (ok && ja < jb) {
-      ok = wait_kv(0);
-      tcgen05_fence_after();
-      for (int t = 0; t < 2 && ok; ++t)
-        if (has(t, ja)) scores(t, ja);
-      if (ok) free_kv(0);
-    }
-    for (int j = ja; j < jb && ok; ++j) {
-      const int n = 2 * (j - ja);
-      ok = wait_kv(n + 1);
-      if (ok && j + 1 < jb) ok = wait_kv(n + 2);
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (has(t, j)) {
-          ok = warp_wait(&p_full[t], j - j0[t] & 1, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after();
-          if (elect_one()) {
-            mma_sum<64, 64>(tmem + 2 * kT + t * kT, tmem + t * kT, vd + (uint64_t)((n + 1) % L::kStages * (L::kTile >> 4)), idesc_o,
-                    j > j0[t]);
-            umma_commit(&o_full[t]);
-          }
-          __syncwarp();
-        }
-        // over the probabilities that the product in front has read
-        if (j + 1 < jb && has(t, j + 1)) scores(t, j + 1);
-      }
+    bool ok = true;
+    int n = 0, made[2] = {0, 0};                 // tiles of keys and values before this item; probabilities waited for
+    for (int w = 0; ok && item_of(w) < a.items; ++w) {
+      const FwdItem it(s, item_of(w));
+      ok = warp_wait(q_full, w & 1, abort_flag);
       if (!ok) break;
-      free_kv(n + 1);
-      if (j + 1 < jb) free_kv(n + 2);
+      auto has = [&](int t, int j) { return j >= it.j0[t] && j < it.j1[t]; };
+      auto scores = [&](int t, int nk) {
+        if (elect_one()) {
+          mma_rows<D>(tmem + t * kT, qd + t * (L::kTile >> 4), kd + slot(nk), idesc_s);
+          umma_commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      if (it.ja < it.jb) {
+        ok = wait_kv(n);
+        tcgen05_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && has(t, it.ja)) scores(t, n);
+        if (ok) free_kv(n);
+      }
+      for (int j = it.ja; j < it.jb && ok; ++j, n += 2) {
+        ok = wait_kv(n + 1);
+        if (ok && j + 1 < it.jb) ok = wait_kv(n + 2);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && has(t, j)) ok = warp_wait(&p_full[t], made[t]++ & 1, abort_flag);
+          if (!ok) break;
+          if (has(t, j)) {
+            tcgen05_fence_after();
+            if (elect_one()) {
+              mma_sum<32, 64>(tmem + 2 * kT + t * kT, tmem + t * kT, vd + slot(n + 1), idesc_o, j > it.j0[t]);
+              umma_commit(&o_full[t]);
+            }
+            __syncwarp();
+          }
+          // over the probabilities that the product in front has read
+          if (j + 1 < it.jb && has(t, j + 1)) scores(t, n + 2);
+        }
+        if (!ok) break;
+        free_kv(n + 1);
+        if (j + 1 < it.jb) free_kv(n + 2);
+      }
     }
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
@@ -406,122 +482,158 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint32_t tS = tmem + lanes + t * kT, tO = tmem + lanes + 2 * kT + t * kT;
     uint64_t* x_bar = &x_full[t * 4 + (warp & 3)];
     float* xch = reinterpret_cast<float*>(smem + L::kXch) + t * 4 * kT;   // [2 turns][2 halves][128]
-    const int q = q0 + t * kT + r;
-    int klo, khi;
-    row_keys(s, q, klo, khi);
+    uint8_t* stage = sQ + t * L::kTile + (warp & 7) * (L::kTile / 8);     // behind the tile's last scores
     const float c = s.scale_log2;
-    float m = -INFINITY, l = 0.f;
     bool ok = true;
-    const int n = j1[t] - j0[t];
-    for (int it = 0; it < n; ++it) {
-      const int k0 = (j0[t] + it) * kT + hf * 64;
-      if (!warp_wait(&s_full[t], it & 1, abort_flag)) { ok = false; break; }
-      tcgen05_fence_after();
-      float v[64];
-      tmem_ld32(tS + hf * 64, v);
-      tmem_ld32(tS + hf * 64 + 32, v + 32);
-      uint32_t see0 = range_bits(klo, khi, k0), see1 = range_bits(klo, khi, k0 + 32);
-      if (s.mask != nullptr) {
-        const uint32_t* w = s.mask + (int64_t)b * s.k_words + (k0 >> 5);
-        see0 &= __ldg(w);
-        see1 &= __ldg(w + 1);
+    int made = 0, turns = 0;                       // scores and exchanges before this one
+    for (int w = 0; ok && item_of(w) < a.items; ++w) {
+      const FwdItem item(s, item_of(w));
+      const int first = t ? item.j0[1] : item.j0[0], n = (t ? item.j1[1] : item.j1[0]) - first;
+      const int q = item.q0 + t * kT + r, b = item.b;
+      int klo, khi;
+      row_keys(s, q, klo, khi);
+      float m = -INFINITY, l = 0.f;
+      for (int it = 0; it < n; ++it, ++made, ++turns) {
+        const int k0 = (first + it) * kT + hf * 64;
+        if (!warp_wait(&s_full[t], made & 1, abort_flag)) { ok = false; break; }
+        tcgen05_fence_after();
+        uint32_t see[2] = {range_bits(klo, khi, k0), range_bits(klo, khi, k0 + 32)};
+        if (s.mask != nullptr) {
+          const uint32_t* words = s.mask + (int64_t)b * s.k_words + (k0 >> 5);
+          see[0] &= __ldg(words);
+          see[1] &= __ldg(words + 1);
+        }
+        // The scores are read twice, for the maximum and for the exponentials: 64 of them do not stay in registers beside the rest.
+        const bool whole = __all_sync(0xffffffffu, (see[0] & see[1]) == 0xFFFFFFFFu);
+        auto read = [&](int g, float (&v)[32]) {
+          tmem_ld32(tS + hf * 64 + 32 * g, v);
+          tmem_ld_wait(v);
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = see[g] >> i & 1 ? v[i] : -INFINITY;
+          }
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float v[32];
+          read(g, v);
+          float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int i = 4; i < 28; i += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mx[u] = max3(mx[u], v[i + u], v[i + u + 4]);
+          top = max3(max3(top, v[28], v[29]), max3(mx[0], mx[1], v[30]), max3(mx[2], mx[3], v[31]));
+        }
+        // the other half's maximum
+        float* turn = xch + (turns & 1) * 2 * kT;
+        turn[hf * kT + r] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_bar);
+        if (!warp_wait(x_bar, turns & 1, abort_flag)) { ok = false; break; }
+        top = fmaxf(m, fmaxf(top, turn[(hf ^ 1) * kT + r]));
+        // The reference moves only when it falls behind by a factor of 2^8: until then sums and products stay below 2^8 times
+        // what they would be, far from the end of their range, and the outputs need not be read.
+        const bool move = (top - m) * c > 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          const float f = move ? ex2((m - top) * c) : 1.f;
+          l *= f;
+          if (move) m = top;
+          if (it > 0) {
+            if (!warp_wait(&o_full[t], (made - 1) & 1, abort_flag)) { ok = false; break; }
+            tcgen05_fence_after();
+#pragma unroll
+            for (int cc = 0; cc < D / 2; cc += 16) {
+              float o[16];
+              tmem_ld16(tO + hf * (D / 2) + cc, o);
+              tmem_ld_wait(o);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] *= f;
+              tmem_st16(tO + hf * (D / 2) + cc, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : -m * c;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float v[32], sum[4] = {0.f, 0.f, 0.f, 0.f};
+          read(g, v);
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p0 = v[2 * i], p1 = v[2 * i + 1];
+            fma2(p0, p1, c, mc);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            add2(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], p0, p1);
+            pk[i] = pack2<T>(p0, p1);
+          }
+          tmem_st16(tS + hf * 64 + 16 * g, pk);          // over scores that have been read
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        hand_over(&p_full[t], lane);
       }
-      tmem_ld_wait(v);
-      if (!__all_sync(0xffffffffu, (see0 & see1) == 0xFFFFFFFFu)) {
-#pragma unroll
-        for (int i = 0; i < 64; ++i) v[i] = (i < 32 ? see0 : see1) >> (i & 31) & 1 ? v[i] : -INFINITY;
+      if (ok && n > 0) {
+        // the row's sum, and the last product
+        float* turn = xch + (turns & 1) * 2 * kT;
+        turn[hf * kT + r] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x_bar);
+        ok = warp_wait(x_bar, turns & 1, abort_flag) && warp_wait(&o_full[t], (made - 1) & 1, abort_flag);
+        tcgen05_fence_after();
+        if (ok) l += turn[(hf ^ 1) * kT + r];
+        ++turns;
+      } else if (ok) {
+        ok = warp_wait(q_full, w & 1, abort_flag);            // nothing is loaded: the stage is free
       }
-      float mx[4] = {v[0], v[1], v[2], v[3]};
+      if (!ok) break;
+      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : NAN;   // a row without keys: zeros
+      if (a.nlse != nullptr && hf == 0 && item.q0 + t * kT < s.Sq) {
+        const bool none = q >= s.Sq || m == -INFINITY;
+        a.nlse[((int64_t)b * s.Hq + item.h) * s.q_pad + q] = none ? -INFINITY : shift_of<T>() - m * c - log2f(l);
+      }
+      const int row = item.q0 + t * kT + (warp & 3) * 32;
+      if (row < s.Sq) {
 #pragma unroll
-      for (int i = 4; i < 64; i += 4)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], v[i + u]);
-      float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      // The other half's maximum.  Behind this the other warp has read its scores too, which this one's probabilities may cover.
-      float* turn = xch + (it & 1) * 2 * kT;
-      turn[hf * kT + r] = top;
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(x_bar);
-      if (!warp_wait(x_bar, it & 1, abort_flag)) { ok = false; break; }
-      tcgen05_fence_after();
-      top = fmaxf(m, fmaxf(top, turn[(hf ^ 1) * kT + r]));
-      // The reference moves only when it falls behind by a factor of 2^8: until then sums and products stay below 2^8 times
-      // what they would be, far from the end of their range, and the outputs need not be read.
-      const bool move = (top - m) * c > 8.f;
-      if (__any_sync(0xffffffffu, move)) {
-        const float f = move ? ex2((m - top) * c) : 1.f;
-        l *= f;
-        if (move) m = top;
-        if (it > 0) {
-          if (!warp_wait(&o_full[t], (it - 1) & 1, abort_flag)) { ok = false; break; }
-          tcgen05_fence_after();
-#pragma unroll
-          for (int cc = 0; cc < D / 2; cc += 16) {       // 16 at a time: the scores stay in registers
-            float o[16];
-            tmem_ld16(tO + hf * (D / 2) + cc, o);
+        for (int i = 0; i < D / 64; ++i) {
+          const int col = i * 64 + hf * 32;
+          if (col >= s.D) break;
+          float o[32];
+          if (n > 0) {
+            tmem_ld32(tO + col, o);
             tmem_ld_wait(o);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= f;
-            tmem_st16(tO + hf * (D / 2) + cc, reinterpret_cast<const uint32_t*>(o));
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (lane == 0) stores_read<0>();
+          __syncwarp();
+          stage32<T>(stage, o, inv, lane);
+          if (lane == 0) store32(&tm_o, stage, col, row, item.h, b);
+          if (a.nlse != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float x = o[e] * inv;
+              o[e] = x - to_float<T>(from_float<T>(x));
+            }
+            uint8_t* second = stage + (D == 128 ? 2048 : 0);
+            if (lane == 0 && D != 128) stores_read<0>();
+            __syncwarp();
+            stage32<T>(second, o, kLowScale, lane);
+            if (lane == 0) store32(&tm_low, second, col, row, item.h, b);
           }
         }
       }
-      const float mc = m == -INFINITY ? 0.f : -m * c;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      uint32_t pk[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float p0 = ex2(fmaf(v[2 * i], c, mc)), p1 = ex2(fmaf(v[2 * i + 1], c, mc));
-        sum[i & 1] += p0;
-        sum[2 + (i & 1)] += p1;
-        pk[i] = pack2<T>(p0, p1);
+      tcgen05_fence_before();
+      if (lane == 0) {
+        stores_read<0>();
+        mbar_arrive(q_empty);
       }
-      tmem_st32(tS + 32 * hf, pk);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      hand_over(&p_full[t], lane);
-    }
-    if (ok && n > 0) {
-      // the row's sum, and the last product
-      float* turn = xch + (n & 1) * 2 * kT;
-      turn[hf * kT + r] = l;
       __syncwarp();
-      if (lane == 0) mbar_arrive(x_bar);
-      ok = warp_wait(x_bar, n & 1, abort_flag) && warp_wait(&o_full[t], (n - 1) & 1, abort_flag);
-      tcgen05_fence_after();
-      if (ok) l += turn[(hf ^ 1) * kT + r];
     }
     if (!ok && lane == 0) report(s.err, 73);
-    if (ok && q0 + t * kT < s.Sq) {
-      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : NAN;   // a row without keys: zeros
-      if (a.nlse != nullptr && hf == 0) {
-        const bool none = q >= s.Sq || m == -INFINITY;
-        a.nlse[((int64_t)b * s.Hq + h) * s.q_pad + q] = none ? -INFINITY : a.shift - m * c - log2f(l);
-      }
-      T* dst = reinterpret_cast<T*>(a.out) + (((int64_t)b * s.Sq + q) * s.Hq + h) * s.D;
-#pragma unroll
-      for (int cc = hf * 32; cc < D; cc += 64) {
-        float o[32];
-        if (n > 0) {
-          tmem_ld32(tO + cc, o);
-          tmem_ld_wait(o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
-        if (q < s.Sq) {
-          put_row32<T>(dst, o, inv, cc, s.D);
-          if (a.low != nullptr) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float x = o[i] * inv;
-              o[i] = x - to_float<T>(from_float<T>(x));
-            }
-            put_row32<T>(reinterpret_cast<T*>(a.low) + (dst - reinterpret_cast<T*>(a.out)), o, kLowScale, cc, s.D);
-          }
-        }
-      }
-    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   finish(tmem, warp);
 }
@@ -618,12 +730,13 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
   if (sub == 0 && a.bound != nullptr && group >= 0 && n > __uint_as_float(a.bound[group])) atomicMax(&a.bound[group], __float_as_uint(n));
 }
 
-// fp16: the power of two for dP - delta.  |dP_ij - delta_i| <= 2 max |dO_i| max |v_j| (o_i is a mean of the v_j).
-__device__ __forceinline__ float grad_factor(const uint32_t* bound, int group, float shift) {
-  if (bound == nullptr) return 1.f;
+// fp16: the power of two for dP - delta; bf16: none.  |dP_ij - delta_i| <= 2 max |dO_i| max |v_j| (o_i is a mean of the v_j).
+template <typename T>
+__device__ __forceinline__ float grad_factor(const uint32_t* bound, int group) {
+  if constexpr (!std::is_same<T, __half>::value) return 1.f;
   const float n2 = 4.f * __uint_as_float(bound[2 * group]) * __uint_as_float(bound[2 * group + 1]);
   if (!(n2 > 0.f && n2 < INFINITY)) return 1.f;
-  const int e = (int)floorf(15.f - 0.5f * log2f(n2) - shift);
+  const int e = (int)floorf(15.f - 0.5f * log2f(n2) - kShiftF16);
   return exp2f((float)min(max(e, -100), 100));
 }
 
@@ -633,39 +746,63 @@ struct BwdArgs {
   const float* delta;     // [B, Hq, q_pad]
   const uint4* pieces;
   const uint32_t* bound;  // [B, Hkv, 2] or null
-  void* dq;               // [B, Sq, Hq, D]
-  void* dk;               // [B, Skv, Hkv, D]
-  void* dv;
-  float shift;
+  unsigned items;
 };
 
 // ------------------------------------------------------------------------------------------------ dk and dv
 template <int D>
+struct DqSmem {
+  static constexpr int kTile = kT * D * 2;
+  static constexpr int kK = D == 128 ? 3 : 4, kV = D == 128 ? 2 : 4;     // tiles of k are kept for longer
+  static constexpr int kBars = (2 + kK + kV) * kTile;
+  static constexpr int kSize = 1024 + kBars + 256;
+};
+
+template <int D>
 struct BwdSmem {
   static constexpr int kTile = kT * D * 2;
   static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int kPieces = (2 + 2 * kStages) * kTile;     // of -L / scale and -delta of a stage's queries
+  static constexpr int kPieces = (2 + 2 * kStages) * kTile;     // of -L / scale, then of -delta, of the tiles' queries
   static constexpr int kWeights = kPieces + kStages * 4096;     // 16 columns of the pieces' weights, eight of them zeros
   static constexpr int kBars = kWeights + 4096;
   static constexpr int kSize = 1024 + kBars + 256;
+};
+
+// A block of keys [k0, k0 + 128), and the blocks of queries [i0, i0 + ni) of each head of its group that may see it.
+struct DkvItem {
+  int k0, kvh, b, i0, ni, total;
+  __device__ __forceinline__ DkvItem(const Shape& s, unsigned i) {
+    const unsigned rest = i / s.Hkv;
+    kvh = (int)(i % s.Hkv);
+    b = (int)(rest % s.B);
+    k0 = (int)(rest / s.B) * kT;                 // the first keys are seen by most queries, and come first
+    const int off = s.Skv - s.Sq;
+    const int qlo = s.causal ? max(0, k0 - off) : 0;
+    const int qhi = s.window > 0 ? (int)min((int64_t)s.Sq, (int64_t)min(k0 + kT, s.Skv) - 1 + s.window - off) : s.Sq;
+    i0 = qlo / kT;
+    ni = qhi > qlo ? (qhi + kT - 1) / kT - i0 : 0;
+    total = ni * (s.Hq / s.Hkv);
+  }
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
+                const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
                 const __grid_constant__ BwdArgs a) {
   using L = BwdSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = smem;
   uint8_t* sV = smem + L::kTile;
-  uint8_t* sQG = smem + 2 * L::kTile;            // stages of [q | dO]
+  uint8_t* sQG = smem + 2 * L::kTile;            // tiles of q, and as many of dO
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* kv_full = bars;
-  uint64_t* full = bars + 1;
-  uint64_t* empty = full + L::kStages;
-  uint64_t* s_full = empty + L::kStages;
+  uint64_t* kv_empty = bars + 1;
+  uint64_t* full = bars + 2;                     // [2][kStages]: q, dO
+  uint64_t* empty = full + 2 * L::kStages;
+  uint64_t* s_full = empty + 2 * L::kStages;
   uint64_t* p_full = s_full + 1;
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_full = s_full + 3;
@@ -675,18 +812,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
   const Shape& s = a.s;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int kvh = blockIdx.x, b = blockIdx.z, group = s.Hq / s.Hkv;
-  const int k0 = blockIdx.y * kT;                // the first keys are seen by most queries, and come first
-  const int off = s.Skv - s.Sq;
-  // blocks of queries that may see these keys
-  const int qlo = s.causal ? max(0, k0 - off) : 0;
-  const int qhi = s.window > 0 ? min((int64_t)s.Sq, (int64_t)min(k0 + kT, s.Skv) - 1 + s.window - off) : s.Sq;
-  const int i0 = qlo / kT, ni = qhi > qlo ? (qhi + kT - 1) / kT - i0 : 0;
-  const int total = ni * group;
+  const int group = s.Hq / s.Hkv, off = s.Skv - s.Sq;
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int i = 0; i < L::kStages; ++i) {
+    mbar_init(kv_empty, kArith);
+    for (int i = 0; i < 2 * L::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
@@ -712,26 +843,40 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const uint32_t tmem = *tmem_slot, tP = tmem + kT, tV = tmem + 2 * kT, tK = tmem + 3 * kT;
 
   if (warp == kLoader) {
-    if (lane == 0 && total > 0) {
+    if (lane == 0) {
       prefetch_tmap(&tm_q);
       prefetch_tmap(&tm_g);
-      mbar_expect_tx(kv_full, 2 * L::kTile);
-      load_tile<D>(sK, &tm_k, k0, kvh, b, kv_full);
-      load_tile<D>(sV, &tm_v, k0, kvh, b, kv_full);
+      prefetch_tmap(&tm_k);
+      prefetch_tmap(&tm_v);
+      // A tile of dO is free again half a step before the tile of q beside it: each has barriers of its own, and goes as its
+      // turn comes.
       bool ok = true;
-      int n = 0;
-      for (; n < total; ++n) {
-        const int st = n % L::kStages, h = kvh * group + n / ni, q0 = (i0 + n % ni) * kT;
-        if (!mbar_wait(&empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
-        mbar_expect_tx(&full[st], 2 * L::kTile + 4096);
-        load_tile<D>(sQG + 2 * st * L::kTile, &tm_q, q0, h, b, &full[st]);
-        load_tile<D>(sQG + (2 * st + 1) * L::kTile, &tm_g, q0, h, b, &full[st]);
-        bulk_load(smem + L::kPieces + st * 4096, a.pieces + (((int64_t)b * s.Hq + h) * s.q_pad + q0) * 2, 4096, &full[st]);
+      int n = 0, w = 0;                            // steps before this item
+      for (; ok && item_of(w) < a.items; ++w) {
+        const DkvItem it(s, item_of(w));
+        if (!mbar_wait(kv_empty, (w & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        mbar_expect_tx(kv_full, it.total > 0 ? 2 * L::kTile : 0);
+        if (it.total > 0) {
+          load_tile<D>(sK, &tm_k, it.k0, it.kvh, it.b, kv_full);
+          load_tile<D>(sV, &tm_v, it.k0, it.kvh, it.b, kv_full);
+        }
+        for (int m = 0; m < 2 * it.total; ++m) {
+          const int i = m >> 1, x = (m & 1) ^ (n + i == 0 ? 0 : 1), st = (n + i) % L::kStages, at = x * L::kStages + st;
+          const int h = it.kvh * group + i / it.ni, q0 = (it.i0 + i % it.ni) * kT;
+          if (!mbar_wait(&empty[at], ((n + i) / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+          mbar_expect_tx(&full[at], L::kTile + 2048);
+          load_tile<D>(sQG + at * L::kTile, x ? &tm_g : &tm_q, q0, h, it.b, &full[at]);
+          bulk_load(smem + L::kPieces + at * 2048, a.pieces + (((int64_t)it.b * s.Hq + h) * s.q_pad + q0) * 2 + x * kT, 2048,
+                    &full[at]);
+        }
+        n += it.total;
       }
-      if (!ok) {
-        mbar_wait_quiet(kv_full, 0, 1 << 12);
-        for (int i = n - L::kStages < 0 ? 0 : n - L::kStages; i < n; ++i)
-          mbar_wait_quiet(&full[i % L::kStages], i / L::kStages & 1, 1 << 12);
+      if (!ok) {                                   // loads in flight end before the CTA does
+        mbar_wait_quiet(kv_full, w & 1, 1 << 12);
+        for (int i = 0; i < 2 * L::kStages; ++i) {
+          mbar_wait_quiet(&full[i], 0, 1 << 12);
+          mbar_wait_quiet(&full[i], 1, 1 << 12);
+        }
       }
     }
     __syncwarp();
@@ -741,51 +886,46 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const uint64_t qg_rows = make_desc_sw128(smem_u32(sQG)), qg_sum = make_desc_mn(smem_u32(sQG));
     const uint64_t weights = make_desc_rows16(smem_u32(smem + L::kWeights), 2048);
     const uint64_t pieces = make_desc_rows16(smem_u32(smem + L::kPieces), 0);   // their second eight columns: the first once more
-    auto at = [&](int n, int which) { return (uint64_t)((2 * (n % L::kStages) + which) * (L::kTile >> 4)); };
-    auto wait_full = [&](int n) { return warp_wait(&full[n % L::kStages], n / L::kStages & 1, abort_flag); };
-    auto scores = [&](int n) {                  // k q^T
-      if (elect_one()) {
-        mma_rows<D>(tmem, kd, qg_rows + at(n, 0), idesc_s);
-        umma_f16(tmem, weights, pieces + (n % L::kStages * 4096 >> 4), idesc_s, true);
-        umma_commit(s_full);
-      }
-      __syncwarp();
-    };
-    auto grads = [&](int n) {                   // v dO^T
-      if (elect_one()) {
-        mma_rows<D>(tP, vd, qg_rows + at(n, 1), idesc_s);
-        umma_f16(tP, weights, pieces + (n % L::kStages * 4096 + 2048 >> 4), idesc_s, true);
-        umma_commit(dp_full);
-      }
-      __syncwarp();
-    };
-    bool ok = total == 0 || (warp_wait(kv_full, 0, abort_flag) && wait_full(0));
-    if (ok && total > 0) {
-      tcgen05_fence_after();
-      scores(0);
-      grads(0);
-    }
-    for (int n = 0; n < total && ok; ++n) {
-      ok = warp_wait(p_full, n & 1, abort_flag);
-      if (!ok) break;
-      tcgen05_fence_after();
-      if (elect_one()) mma_sum<16, 32>(tV, tmem, qg_sum + at(n, 1), idesc_o, n > 0);
-      __syncwarp();
-      if (n + 1 < total) {
-        ok = wait_full(n + 1);
-        if (!ok) break;
+    auto slot = [&](int n, int w) { return w * L::kStages + n % L::kStages; };
+    auto tile = [&](int n, int w) { return (uint64_t)(slot(n, w) * (L::kTile >> 4)); };
+    bool ok = true;
+    int base = 0;
+    // Half of step n of an item's `total`, of q (W 0: k q^T, and P^T dO of the step before) or of dO (W 1: v dO^T, and dS^T q): the
+    // sum, whose first operand lies where the new scores go, in front of these.
+    auto half = [&](auto which, int n, int total) {
+      constexpr int W = decltype(which)::value;
+      const uint32_t tS = W ? tP : tmem, tO = W ? tK : tV;
+      const int at = base + n;
+      if (n > 0) {
+        if (!warp_wait(W ? ds_full : p_full, (at - 1) & 1, abort_flag)) return false;
         tcgen05_fence_after();
-        scores(n + 1);
+        if (elect_one()) {
+          mma_sum<16, 32>(tO, tS, qg_sum + tile(at - 1, 1 - W), idesc_o, n > 1);
+          umma_commit(&empty[slot(at - 1, 1 - W)]);
+        }
+        __syncwarp();
       }
-      ok = warp_wait(ds_full, n & 1, abort_flag);
-      if (!ok) break;
-      tcgen05_fence_after();
-      if (elect_one()) {
-        mma_sum<16, 32>(tK, tP, qg_sum + at(n, 0), idesc_o, n > 0);
-        umma_commit(n + 1 < total ? &empty[n % L::kStages] : done);
+      if (n < total) {
+        if (!warp_wait(&full[slot(at, W)], at / L::kStages & 1, abort_flag)) return false;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          mma_rows<D>(tS, W ? vd : kd, qg_rows + tile(at, W), idesc_s);
+          umma_f16(tS, weights, pieces + (slot(at, W) * 2048 >> 4), idesc_s, true);
+          umma_commit(W ? dp_full : s_full);
+        }
+        __syncwarp();
       }
+      return true;
+    };
+    for (int w = 0; ok && item_of(w) < a.items; ++w) {
+      const DkvItem it(s, item_of(w));
+      ok = warp_wait(kv_full, w & 1, abort_flag);
+      if (it.total == 0) continue;
+      for (int n = 0; n <= it.total && ok; ++n)
+        ok = half(std::integral_constant<int, 0>(), n, it.total) && half(std::integral_constant<int, 1>(), n, it.total);
+      if (ok && elect_one()) umma_commit(done);
       __syncwarp();
-      if (n + 1 < total) grads(n + 1);
+      base += it.total;
     }
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
@@ -793,119 +933,154 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // ---------------- a key and a quarter of the queries to a thread ----------------
     const int qd = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + qd * 32;
-    const int k = k0 + r;
+    uint8_t* stage = smem + warp * (2 * L::kTile / kArith);        // in the place of the keys and values, behind the last product
     const float c = s.scale_log2;
-    const float f = a.bound != nullptr ? grad_factor(a.bound, b * s.Hkv + kvh, a.shift) : 1.f;
     bool ok = true;
-    for (int n = 0; n < total; ++n) {
-      const int q0 = (i0 + n % ni) * kT;
-      const uint32_t par = n & 1;
-      if (!warp_wait(s_full, par, abort_flag)) { ok = false; break; }
-      tcgen05_fence_after();
-      float p[32];
-      tmem_ld32(tmem + lanes, p);
-      // this key is seen by queries [lo, hi)
-      const int lo = s.causal ? k - off - q0 : -kT, hi = s.window > 0 ? min((int64_t)kT, (int64_t)k - off - q0 + s.window) : kT;
-      const uint32_t see = range_bits(lo, hi, qd * 32);
-      tmem_ld_wait(p);
+    int made = 0, items = 0;
+    for (int w = 0; ok && item_of(w) < a.items; ++w) {
+      const DkvItem it(s, item_of(w));
+      const int k = it.k0 + r;
+      const float f = grad_factor<T>(a.bound, it.b * s.Hkv + it.kvh);
+      for (int n = 0, i = 0; n < it.total; ++n, ++made) {
+        const int q0 = (it.i0 + i) * kT;
+        i = i + 1 < it.ni ? i + 1 : 0;
+        const uint32_t par = made & 1;
+        if (!warp_wait(s_full, par, abort_flag)) { ok = false; break; }
+        tcgen05_fence_after();
+        float p[32];
+        tmem_ld32(tmem + lanes, p);
+        // this key is seen by queries [lo, hi)
+        const int lo = s.causal ? k - off - q0 : -kT;
+        const int hi = s.window > 0 ? (int)min((int64_t)kT, (int64_t)k - off - q0 + s.window) : kT;
+        const uint32_t see = range_bits(lo, hi, qd * 32);
+        tmem_ld_wait(p);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) p[i] = ex2(p[i] * c);
-      if (!__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = see >> i & 1 ? p[i] : 0.f;
-      }
-      uint32_t pk[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
-      tmem_st16(tmem + lanes, pk);
-      hand_over(p_full, lane);
-      if (!warp_wait(dp_full, par, abort_flag)) { ok = false; break; }
-      tcgen05_fence_after();
-      float d[32];
-      tmem_ld32(tP + lanes, d);
-      tmem_ld_wait(d);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = p[2 * i] * d[2 * i], y = p[2 * i + 1] * d[2 * i + 1];
-        if constexpr (std::is_same<T, __half>::value) {
-          x *= f;
-          y *= f;
+        for (int i = 0; i < 32; i += 2) {
+          mul2(p[i], p[i + 1], c, c);
+          p[i] = ex2(p[i]);
+          p[i + 1] = ex2(p[i + 1]);
         }
-        pk[i] = pack2<T>(x, y);
+        if (!__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[i] = see >> i & 1 ? p[i] : 0.f;
+        }
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
+        tmem_st16(tmem + lanes, pk);
+        hand_over(p_full, lane);
+        if (!warp_wait(dp_full, par, abort_flag)) { ok = false; break; }
+        tcgen05_fence_after();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {              // 16 at a time: the probabilities stay in registers
+          float d[16];
+          tmem_ld16(tP + lanes + 16 * g, d);
+          tmem_ld_wait(d);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            mul2(d[2 * i], d[2 * i + 1], p[16 * g + 2 * i], p[16 * g + 2 * i + 1]);
+            if constexpr (std::is_same<T, __half>::value) mul2(d[2 * i], d[2 * i + 1], f, f);
+            pk[8 * g + i] = pack2<T>(d[2 * i], d[2 * i + 1]);
+          }
+        }
+        tmem_st16(tP + lanes, pk);
+        hand_over(ds_full, lane);
       }
-      tmem_st16(tP + lanes, pk);
-      hand_over(ds_full, lane);
-    }
-    if (ok && total > 0) {
-      ok = warp_wait(done, 0, abort_flag);
+      if (ok) ok = it.total > 0 ? warp_wait(done, items++ & 1, abort_flag) : warp_wait(kv_full, w & 1, abort_flag);
       tcgen05_fence_after();
+      if (!ok) break;
+      bool real = k < s.Skv && it.total > 0;
+      if (real && s.mask != nullptr) real = s.mask[(int64_t)it.b * s.k_words + (k >> 5)] >> (k & 31) & 1;
+      const int row = it.k0 + (warp & 3) * 32;
+      const float un = 1.f / scale_of<T>();
+      if (row < s.Skv) {
+        // 32 columns at a time: those of dv, then those of dk
+#pragma unroll 1
+        for (int i = 0; i < 2 * D / 128; ++i) {
+          const int x = qd + 4 * i;
+          const bool is_v = x < D / 32;
+          const int col = x % (D / 32) * 32;
+          float o[32];
+          if (it.total > 0) {
+            tmem_ld32((is_v ? tV : tK) + mine + col, o);
+            tmem_ld_wait(o);
+          }
+          if (!real) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          stage32<T>(stage + i * 2048, o, is_v ? un : s.scale * un / f, lane);
+          if (lane == 0 && col < s.D) store32(is_v ? &tm_dv : &tm_dk, stage + i * 2048, col, row, it.kvh, it.b);
+        }
+      }
+      tcgen05_fence_before();
+      if (lane == 0) {
+        stores_read<0>();
+        mbar_arrive(kv_empty);
+      }
+      __syncwarp();
     }
     if (!ok && lane == 0) report(s.err, 73);
-    if (ok) {
-      bool real = k < s.Skv && total > 0;
-      if (real && s.mask != nullptr) real = s.mask[(int64_t)b * s.k_words + (k >> 5)] >> (k & 31) & 1;
-      const int64_t row = (((int64_t)b * s.Skv + k) * s.Hkv + kvh) * s.D;
-      const float un = exp2f(-a.shift);
-      // 32 columns at a time: those of dv, then those of dk
-#pragma unroll
-      for (int i = qd; i < 2 * D / 32; i += 4) {
-        const bool is_v = i < D / 32;
-        const int col = i % (D / 32) * 32;
-        float o[32];
-        if (total > 0) {
-          tmem_ld32((is_v ? tV : tK) + mine + col, o);
-          tmem_ld_wait(o);
-        }
-        if (!real) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
-        }
-        if (k < s.Skv) put_row32<T>(reinterpret_cast<T*>(is_v ? a.dv : a.dk) + row, o, is_v ? un : s.scale * un / f, col, s.D);
-      }
-    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   finish(tmem, warp);
 }
 
 // ------------------------------------------------------------------------------------------------ dq
+// A tile of queries [q0, q0 + 128) of a head, and the blocks of keys that it may see.
+struct DqItem {
+  int q0, h, b, kvh, j0, total;
+  __device__ __forceinline__ DqItem(const Shape& s, unsigned i) {
+    const unsigned rest = i / s.Hq;
+    h = (int)(i % s.Hq);
+    b = (int)(rest % s.B);
+    q0 = ((s.Sq + kT - 1) / kT - 1 - (int)(rest / s.B)) * kT;
+    kvh = h / (s.Hq / s.Hkv);
+    int j1;
+    key_blocks(s, q0, j0, j1);
+    total = j1 - j0;
+  }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_g,
-               const __grid_constant__ BwdArgs a) {
-  using L = BwdSmem<D>;
+               const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ BwdArgs a) {
+  using L = DqSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sG = smem + L::kTile;
-  uint8_t* sKV = smem + 2 * L::kTile;            // stages of [k | v]
+  uint8_t* sKV = smem + 2 * L::kTile;            // tiles of k, then of v
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
   uint64_t* q_full = bars;
-  uint64_t* full = bars + 1;
-  uint64_t* empty = full + L::kStages;
-  uint64_t* s_full = empty + L::kStages;         // [2]
-  uint64_t* dp_full = s_full + 2;
-  uint64_t* ds_full = s_full + 3;
-  uint64_t* done = s_full + 4;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* full = bars + 2;                     // [kK] and [kV]
+  uint64_t* empty = full + L::kK + L::kV;
+  uint64_t* s_full = empty + L::kK + L::kV;      // [2]
+  uint64_t* s_free = s_full + 2;                 // [2]
+  uint64_t* dp_full = s_full + 4;
+  uint64_t* ds_full = s_full + 5;
+  uint64_t* done = s_full + 6;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const Shape& s = a.s;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int h = blockIdx.x, b = blockIdx.z, kvh = h / (s.Hq / s.Hkv);
-  const int q0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * kT;
-  int j0, j1;
-  key_blocks(s, q0, j0, j1);
-  const int total = j1 - j0;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < L::kStages; ++i) {
+    mbar_init(q_empty, kArith);
+    for (int i = 0; i < L::kK + L::kV; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(&s_full[0], 1);
-    mbar_init(&s_full[1], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], kArith);
+    }
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kArith);
     mbar_init(done, 1);
@@ -920,25 +1095,35 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   const uint32_t tmem = *tmem_slot, tP = tmem + 2 * kT, tQ = tmem + 3 * kT;
 
   if (warp == kLoader) {
-    if (lane == 0 && total > 0) {
+    if (lane == 0) {
+      prefetch_tmap(&tm_q);
+      prefetch_tmap(&tm_g);
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
-      mbar_expect_tx(q_full, 2 * L::kTile);
-      load_tile<D>(sQ, &tm_q, q0, h, b, q_full);
-      load_tile<D>(sG, &tm_g, q0, h, b, q_full);
       bool ok = true;
-      int n = 0;
-      for (; n < total; ++n) {
-        const int st = n % L::kStages;
-        if (!mbar_wait(&empty[st], (n / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
-        mbar_expect_tx(&full[st], 2 * L::kTile);
-        load_tile<D>(sKV + 2 * st * L::kTile, &tm_k, (j0 + n) * kT, kvh, b, &full[st]);
-        load_tile<D>(sKV + (2 * st + 1) * L::kTile, &tm_v, (j0 + n) * kT, kvh, b, &full[st]);
+      int n = 0, w = 0;                            // steps before this item
+      for (; ok && item_of(w) < a.items; ++w) {
+        const DqItem it(s, item_of(w));
+        if (!mbar_wait(q_empty, (w & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        mbar_expect_tx(q_full, it.total > 0 ? 2 * L::kTile : 0);
+        if (it.total > 0) {
+          load_tile<D>(sQ, &tm_q, it.q0, it.h, it.b, q_full);
+          load_tile<D>(sG, &tm_g, it.q0, it.h, it.b, q_full);
+        }
+        for (int m = 0; m < 2 * it.total; ++m) {
+          const int i = n + (m >> 1), x = m & 1, of = x ? L::kV : L::kK, at = x * L::kK + i % of;
+          if (!mbar_wait(&empty[at], (i / of & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+          mbar_expect_tx(&full[at], L::kTile);
+          load_tile<D>(sKV + at * L::kTile, x ? &tm_v : &tm_k, (it.j0 + (m >> 1)) * kT, it.kvh, it.b, &full[at]);
+        }
+        n += it.total;
       }
-      if (!ok) {
-        mbar_wait_quiet(q_full, 0, 1 << 12);
-        for (int i = n - L::kStages < 0 ? 0 : n - L::kStages; i < n; ++i)
-          mbar_wait_quiet(&full[i % L::kStages], i / L::kStages & 1, 1 << 12);
+      if (!ok) {                                   // loads in flight end before the CTA does
+        mbar_wait_quiet(q_full, w & 1, 1 << 12);
+        for (int i = 0; i < L::kK + L::kV; ++i) {
+          mbar_wait_quiet(&full[i], 0, 1 << 12);
+          mbar_wait_quiet(&full[i], 1, 1 << 12);
+        }
       }
     }
     __syncwarp();
@@ -946,45 +1131,53 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t idesc_s = make_idesc_f16<T>(kT, kT), idesc_o = make_idesc_f16<T>(kT, D) | kBMajorMN;
     const uint64_t qd = make_desc_sw128(smem_u32(sQ)), gd = make_desc_sw128(smem_u32(sG));
     const uint64_t kv_rows = make_desc_sw128(smem_u32(sKV)), kv_sum = make_desc_mn(smem_u32(sKV));
-    auto at = [&](int n, int which) { return (uint64_t)((2 * (n % L::kStages) + which) * (L::kTile >> 4)); };
-    auto wait_full = [&](int n) { return warp_wait(&full[n % L::kStages], n / L::kStages & 1, abort_flag); };
-    auto scores = [&](int n) {                  // q k^T
-      if (elect_one()) {
-        mma_rows<D>(tmem + (n & 1) * kT, qd, kv_rows + at(n, 0), idesc_s);
-        umma_commit(&s_full[n & 1]);
+    auto k_at = [&](int n) { return n % L::kK; };
+    auto v_at = [&](int n) { return L::kK + n % L::kV; };
+    bool ok = true;
+    int base = 0;
+    for (int w = 0; ok && item_of(w) < a.items; ++w) {
+      const DqItem it(s, item_of(w));
+      ok = warp_wait(q_full, w & 1, abort_flag);
+      if (it.total == 0) continue;
+      const int end = base + it.total;
+      // Scores one step ahead, into the other tile, then this step's sum (dS lies over dP) and the next dP.
+      for (int n = base - 1; n < end && ok; ++n) {
+        if (n + 1 < end) {
+          ok = warp_wait(&full[k_at(n + 1)], (n + 1) / L::kK & 1, abort_flag) &&
+               warp_wait(&s_free[n + 1 & 1], (n + 1 >> 1 & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          tcgen05_fence_after();
+          if (elect_one()) {                      // q k^T
+            mma_rows<D>(tmem + (n + 1 & 1) * kT, qd, kv_rows + (uint64_t)(k_at(n + 1) * (L::kTile >> 4)), idesc_s);
+            umma_commit(&s_full[n + 1 & 1]);
+          }
+          __syncwarp();
+        }
+        if (n >= base) {
+          ok = warp_wait(ds_full, n & 1, abort_flag);
+          if (!ok) break;
+          tcgen05_fence_after();
+          if (elect_one()) {
+            mma_sum<16, 32>(tQ, tP, kv_sum + (uint64_t)(k_at(n) * (L::kTile >> 4)), idesc_o, n > base);
+            umma_commit(&empty[k_at(n)]);
+          }
+          __syncwarp();
+        }
+        if (n + 1 < end) {                        // dO v^T
+          ok = warp_wait(&full[v_at(n + 1)], (n + 1) / L::kV & 1, abort_flag);
+          if (!ok) break;
+          tcgen05_fence_after();
+          if (elect_one()) {
+            mma_rows<D>(tP, gd, kv_rows + (uint64_t)(v_at(n + 1) * (L::kTile >> 4)), idesc_s);
+            umma_commit(dp_full);
+            umma_commit(&empty[v_at(n + 1)]);
+          }
+          __syncwarp();
+        }
       }
+      if (ok && elect_one()) umma_commit(done);
       __syncwarp();
-    };
-    auto grads = [&](int n) {                   // dO v^T
-      if (elect_one()) {
-        mma_rows<D>(tP, gd, kv_rows + at(n, 1), idesc_s);
-        umma_commit(dp_full);
-      }
-      __syncwarp();
-    };
-    bool ok = total == 0 || (warp_wait(q_full, 0, abort_flag) && wait_full(0));
-    if (ok && total > 0) {
-      tcgen05_fence_after();
-      scores(0);
-      grads(0);
-    }
-    for (int n = 0; n < total && ok; ++n) {
-      // the next scores' tile was read before dS of the step before this one was handed over
-      if (n + 1 < total) {
-        ok = wait_full(n + 1);
-        if (!ok) break;
-        tcgen05_fence_after();
-        scores(n + 1);
-      }
-      ok = warp_wait(ds_full, n & 1, abort_flag);
-      if (!ok) break;
-      tcgen05_fence_after();
-      if (elect_one()) {
-        mma_sum<16, 32>(tQ, tP, kv_sum + at(n, 0), idesc_o, n > 0);
-        umma_commit(n + 1 < total ? &empty[n % L::kStages] : done);
-      }
-      __syncwarp();
-      if (n + 1 < total) grads(n + 1);
+      base = end;
     }
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
@@ -992,58 +1185,81 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ---------------- a quarter of a query's keys to a thread ----------------
     const int qd = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + qd * 32;
-    const int q = q0 + r;
-    int klo, khi;
-    row_keys(s, q, klo, khi);
+    uint8_t* stage = sQ + (qd % (D / 32) * 4 + (warp & 3)) * 2048;     // in the place of the queries, behind the last product
     const float c = s.scale_log2;
-    const float f = a.bound != nullptr ? grad_factor(a.bound, b * s.Hkv + kvh, a.shift) : 1.f;
-    const int64_t at = ((int64_t)b * s.Hq + h) * s.q_pad + q;
-    const float nl = a.nlse[at], dl = a.delta[at] * -f;
     bool ok = true;
-    for (int n = 0; n < total; ++n) {
-      const int kb = (j0 + n) * kT + qd * 32;
-      if (!warp_wait(&s_full[n & 1], n >> 1 & 1, abort_flag)) { ok = false; break; }
-      tcgen05_fence_after();
-      float p[32];
-      tmem_ld32(tmem + lanes + (n & 1) * kT, p);
-      uint32_t see = range_bits(klo, khi, kb);
-      if (s.mask != nullptr) see &= __ldg(s.mask + (int64_t)b * s.k_words + (kb >> 5));
-      tmem_ld_wait(p);
+    int made = 0, items = 0;
+    for (int w = 0; ok && item_of(w) < a.items; ++w) {
+      const DqItem it(s, item_of(w));
+      const int q = it.q0 + r;
+      int klo, khi;
+      row_keys(s, q, klo, khi);
+      const float f = grad_factor<T>(a.bound, it.b * s.Hkv + it.kvh);
+      const int64_t at = ((int64_t)it.b * s.Hq + it.h) * s.q_pad + q;
+      const float nl = a.nlse[at], dl = a.delta[at] * -f;
+      for (int n = 0; n < it.total; ++n, ++made) {
+        const int kb = (it.j0 + n) * kT + qd * 32;
+        if (!warp_wait(&s_full[made & 1], made >> 1 & 1, abort_flag)) { ok = false; break; }
+        tcgen05_fence_after();
+        float p[32];
+        tmem_ld32(tmem + lanes + (made & 1) * kT, p);
+        uint32_t see = range_bits(klo, khi, kb);
+        if (s.mask != nullptr) see &= __ldg(s.mask + (int64_t)it.b * s.k_words + (kb >> 5));
+        tmem_ld_wait(p);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[made & 1]);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) p[i] = ex2(fmaf(p[i], c, nl));
-      if (!__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) {
+        for (int i = 0; i < 32; i += 2) {
+          fma2(p[i], p[i + 1], c, nl);
+          p[i] = ex2(p[i]);
+          p[i + 1] = ex2(p[i + 1]);
+        }
+        if (!__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = see >> i & 1 ? p[i] : 0.f;
+          for (int i = 0; i < 32; ++i) p[i] = see >> i & 1 ? p[i] : 0.f;
+        }
+        if (!warp_wait(dp_full, made & 1, abort_flag)) { ok = false; break; }
+        tcgen05_fence_after();
+        float d[32];
+        tmem_ld32(tP + lanes, d);
+        tmem_ld_wait(d);
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          fma2(d[2 * i], d[2 * i + 1], f, dl);
+          mul2(d[2 * i], d[2 * i + 1], p[2 * i], p[2 * i + 1]);
+          pk[i] = pack2<T>(d[2 * i], d[2 * i + 1]);
+        }
+        tmem_st16(tP + lanes, pk);
+        hand_over(ds_full, lane);
       }
-      if (!warp_wait(dp_full, n & 1, abort_flag)) { ok = false; break; }
+      if (ok) ok = it.total > 0 ? warp_wait(done, items++ & 1, abort_flag) : warp_wait(q_full, w & 1, abort_flag);
       tcgen05_fence_after();
-      float d[32];
-      tmem_ld32(tP + lanes, d);
-      tmem_ld_wait(d);
-      uint32_t pk[16];
+      if (!ok) break;
+      const int row = it.q0 + (warp & 3) * 32;
+      if (qd < D / 32 && qd * 32 < s.D && row < s.Sq) {
+        float o[32];
+        if (it.total > 0) {
+          tmem_ld32(tQ + mine + qd * 32, o);
+          tmem_ld_wait(o);
+        } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        pk[i] = pack2<T>(p[2 * i] * fmaf(d[2 * i], f, dl), p[2 * i + 1] * fmaf(d[2 * i + 1], f, dl));
-      tmem_st16(tP + lanes, pk);
-      hand_over(ds_full, lane);
-    }
-    if (ok && total > 0) {
-      ok = warp_wait(done, 0, abort_flag);
-      tcgen05_fence_after();
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        stage32<T>(stage, o, s.scale / (scale_of<T>() * f), lane);
+        if (lane == 0) store32(&tm_dq, stage, qd * 32, row, it.h, it.b);
+      }
+      tcgen05_fence_before();
+      if (lane == 0) {
+        stores_read<0>();
+        mbar_arrive(q_empty);
+      }
+      __syncwarp();
     }
     if (!ok && lane == 0) report(s.err, 73);
-    if (ok && qd < D / 32) {
-      T* dst = reinterpret_cast<T*>(a.dq) + (((int64_t)b * s.Sq + q) * s.Hq + h) * s.D;
-      float o[32];
-      if (total > 0) {
-        tmem_ld32(tQ + mine + qd * 32, o);
-        tmem_ld_wait(o);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.f;
-      }
-      if (q < s.Sq) put_row32<T>(dst, o, s.scale * exp2f(-a.shift) / f, qd * 32, s.D);
-    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
   }
   finish(tmem, warp);
 }
@@ -1093,7 +1309,7 @@ struct Tensor4 {
   int64_t b, h, s;
 };
 
-bool encode(CUtensorMap* tm, CUtensorMapDataType dt, const Tensor4& t, int D, int rows, int heads, int B) {
+bool encode(CUtensorMap* tm, CUtensorMapDataType dt, const Tensor4& t, int D, int rows, int heads, int B, bool store = false) {
   EncodeTiledFn enc = tensor_map_encoder();
   if (enc == nullptr) return false;
   // strides of dimensions of size 1 are never taken, but have to be multiples of 16 bytes
@@ -1101,10 +1317,34 @@ bool encode(CUtensorMap* tm, CUtensorMapDataType dt, const Tensor4& t, int D, in
   if ((reinterpret_cast<uintptr_t>(t.p) & 15) || t.p == nullptr || s <= 0 || h <= 0 || b <= 0 || ((s | h | b) & 7)) return false;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)s * 2, (cuuint64_t)h * 2, (cuuint64_t)b * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)kT, 1, 1};
+  cuuint32_t box[4] = {store ? 32u : 64u, store ? 32u : (cuuint32_t)kT, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   return enc(tm, dt, 4, const_cast<void*>(t.p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+             store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// A contiguous [B, rows, heads, D], written by tiles of 32 x 32.
+bool encode_out(CUtensorMap* tm, CUtensorMapDataType dt, void* p, int D, int rows, int heads, int B) {
+  return encode(tm, dt, {p, (int64_t)rows * heads * D, D, (int64_t)heads * D}, D, rows, heads, B, true);
+}
+
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) != 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+// Tiles of work of 128 (or 256) rows: their number, 0 where it is past what a CTA counts.
+unsigned items_of(const Shape& s, int heads, int rows, int of) {
+  const int64_t n = (int64_t)heads * ((rows + of - 1) / of) * s.B;
+  return n < (1ll << 30) ? (unsigned)n : 0;
+}
+unsigned grid_of(unsigned items) {
+  const unsigned n = (unsigned)sm_count();
+  return items < n ? items : n;
 }
 
 // The driver's encoder wants a current context, which a thread that has launched nothing yet (autograd's) need not have.
@@ -1130,7 +1370,6 @@ Shape make_shape(int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int
 template <typename T> constexpr CUtensorMapDataType map_type() {
   return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
-template <typename T> constexpr float shift_of() { return std::is_same<T, __half>::value ? (float)kShiftF16 : 0.f; }
 
 // One CTA to an SM whatever the tiles take: each allocates all of the tensor memory.
 constexpr int one_cta(int bytes) { return bytes > 120 * 1024 ? bytes : 120 * 1024; }
@@ -1138,49 +1377,56 @@ constexpr int one_cta(int bytes) { return bytes > 120 * 1024 ? bytes : 120 * 102
 template <typename T, int D>
 int run_fwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, void* out, void* low, float* nlse,
             cudaStream_t stream) {
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to, tl;
   const CUtensorMapDataType dt = map_type<T>();
   if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
-      !encode(&tv, dt, v, s.D, s.Skv, s.Hkv, s.B))
+      !encode(&tv, dt, v, s.D, s.Skv, s.Hkv, s.B) || !encode_out(&to, dt, out, s.D, s.Sq, s.Hq, s.B) ||
+      (nlse != nullptr && !encode_out(&tl, dt, low, s.D, s.Sq, s.Hq, s.B)))
     return (int)cudaErrorInvalidValue;
+  if (nlse == nullptr) tl = to;                    // not used
   constexpr int smem = one_cta(FwdSmem<D>::kSize);
   static SmemLimit limit;
   const cudaError_t e = limit((const void*)attn_fwd_kernel<T, D>, smem);
   if (e != cudaSuccess) return (int)e;
-  FwdArgs a = {s, out, low, nlse, shift_of<T>()};
-  const dim3 grid(s.Hq, (s.Sq + 2 * kT - 1) / (2 * kT), s.B);
-  attn_fwd_kernel<T, D><<<grid, kThreads, smem, stream>>>(tq, tk, tv, a);
+  const FwdArgs a = {s, nlse, items_of(s, s.Hq, s.Sq, 2 * kT)};
+  if (a.items == 0) return (int)cudaErrorInvalidValue;
+  attn_fwd_kernel<T, D><<<grid_of(a.items), kThreads, smem, stream>>>(tq, tk, tv, to, tl, a);
   return (int)cudaGetLastError();
 }
 
 template <typename T, int D>
 int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v, const Tensor4& g, const void* out,
             const void* low, const float* nlse, float* work, void* dq, void* dk, void* dv, cudaStream_t stream) {
-  CUtensorMap tq, tk, tv, tg;
+  CUtensorMap tq, tk, tv, tg, tdq, tdk, tdv;
   const CUtensorMapDataType dt = map_type<T>();
   if (!bind_context() || !encode(&tq, dt, q, s.D, s.Sq, s.Hq, s.B) || !encode(&tk, dt, k, s.D, s.Skv, s.Hkv, s.B) ||
-      !encode(&tv, dt, v, s.D, s.Skv, s.Hkv, s.B) || !encode(&tg, dt, g, s.D, s.Sq, s.Hq, s.B))
+      !encode(&tv, dt, v, s.D, s.Skv, s.Hkv, s.B) || !encode(&tg, dt, g, s.D, s.Sq, s.Hq, s.B) ||
+      !encode_out(&tdq, dt, dq, s.D, s.Sq, s.Hq, s.B) || !encode_out(&tdk, dt, dk, s.D, s.Skv, s.Hkv, s.B) ||
+      !encode_out(&tdv, dt, dv, s.D, s.Skv, s.Hkv, s.B))
     return (int)cudaErrorInvalidValue;
-  constexpr int smem = one_cta(BwdSmem<D>::kSize);
+  constexpr int smem = one_cta(BwdSmem<D>::kSize), smem_q = one_cta(DqSmem<D>::kSize);
   static SmemLimit limit_kv, limit_q;
   cudaError_t e = limit_kv((const void*)attn_dkv_kernel<T, D>, smem);
-  if (e == cudaSuccess) e = limit_q((const void*)attn_dq_kernel<T, D>, smem);
+  if (e == cudaSuccess) e = limit_q((const void*)attn_dq_kernel<T, D>, smem_q);
   if (e != cudaSuccess) return (int)e;
+  uint4* pieces = reinterpret_cast<uint4*>(work);
+  float* delta = work + (int64_t)s.B * s.Hq * s.q_pad * 8;
   uint32_t* bound = nullptr;
   if (std::is_same<T, __half>::value) {
     bound = reinterpret_cast<uint32_t*>(work + (int64_t)s.B * s.Hq * s.q_pad * 9);
     e = cudaMemsetAsync(bound, 0, (size_t)s.B * s.Hkv * 8, stream);
     if (e != cudaSuccess) return (int)e;
   }
-  uint4* pieces = reinterpret_cast<uint4*>(work);
-  float* delta = work + (int64_t)s.B * s.Hq * s.q_pad * 8;
-  PrepArgs p = {out, low, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, nlse, delta, pieces, 1.f / s.scale_log2, bound, s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
+  const PrepArgs p = {out, low, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, nlse, delta, pieces, 1.f / s.scale_log2, bound,
+                      s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
   const int64_t rows = (int64_t)s.B * s.Hq * s.q_pad + (bound != nullptr ? (int64_t)s.B * s.Hkv * s.Skv : 0);
-  if (rows / 16 + 1 > 0x7FFFFFFF) return (int)cudaErrorInvalidValue;
+  if (rows / 16 + 1 > 0x7FFFFFFF || items_of(s, s.Hkv, s.Skv, kT) == 0 || items_of(s, s.Hq, s.Sq, kT) == 0)
+    return (int)cudaErrorInvalidValue;
   attn_prep_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(p);
-  BwdArgs a = {s, nlse, delta, pieces, bound, dq, dk, dv, shift_of<T>()};
-  attn_dkv_kernel<T, D><<<dim3(s.Hkv, (s.Skv + kT - 1) / kT, s.B), kThreads, smem, stream>>>(tq, tk, tv, tg, a);
-  attn_dq_kernel<T, D><<<dim3(s.Hq, (s.Sq + kT - 1) / kT, s.B), kThreads, smem, stream>>>(tq, tk, tv, tg, a);
+  BwdArgs a = {s, nlse, delta, pieces, bound, items_of(s, s.Hkv, s.Skv, kT)};
+  attn_dkv_kernel<T, D><<<grid_of(a.items), kThreads, smem, stream>>>(tq, tk, tv, tg, tdk, tdv, a);
+  a.items = items_of(s, s.Hq, s.Sq, kT);
+  attn_dq_kernel<T, D><<<grid_of(a.items), kThreads, smem_q, stream>>>(tq, tk, tv, tg, tdq, a);
   return (int)cudaGetLastError();
 }
 
@@ -1196,8 +1442,8 @@ IPEX_API int ipex_attn_train_fwd(const void* q, int64_t q_b, int64_t q_h, int64_
                                  void* out, void* low, float* nlse, int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal,
                                  int window, float scale, int dtype, int* err, void* stream) {
   if (!shape_ok(B, Hq, Hkv, Sq, Skv, D, window, scale) || (window > 0 && !causal) || out == nullptr ||
-      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(low) | reinterpret_cast<uintptr_t>(nlse)) & 15) ||
-      (Sq + 2 * kT - 1) / (2 * kT) > 65535)
+      (nlse != nullptr && low == nullptr) ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(low) | reinterpret_cast<uintptr_t>(nlse)) & 15))
     return (int)cudaErrorInvalidValue;
   const Shape s = make_shape(B, Hq, Hkv, Sq, Skv, D, causal, window, mask_words, scale, err);
   const Tensor4 tq = {q, q_b, q_h, q_s}, tk = {k, k_b, k_h, k_s}, tv = {v, v_b, v_h, v_s};
@@ -1220,8 +1466,7 @@ IPEX_API int ipex_attn_train_bwd(const void* q, int64_t q_b, int64_t q_h, int64_
       nlse == nullptr || work == nullptr || dq == nullptr || dk == nullptr || dv == nullptr ||
       ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(low) | reinterpret_cast<uintptr_t>(nlse) |
         reinterpret_cast<uintptr_t>(work) |
-        reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) ||
-      (Sq + kT - 1) / kT > 65535 || (Skv + kT - 1) / kT > 65535)
+        reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15))
     return (int)cudaErrorInvalidValue;
   const Shape s = make_shape(B, Hq, Hkv, Sq, Skv, D, causal, window, mask_words, scale, err);
   const Tensor4 tq = {q, q_b, q_h, q_s}, tk = {k, k_b, k_h, k_s}, tv = {v, v_b, v_h, v_s}, tg = {g, g_b, g_h, g_s};
