@@ -639,7 +639,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 }
 
 // ------------------------------------------------------------------------------------------------ before the backward pass
-// delta_i = dO_i . o_i, a warp to a row (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
+// delta_i = dO_i . o_i (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
 // heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
 // Three pieces of 16 bits whose weighted sum is x, in a row of eight numbers: the third takes what the first two leave, below
 // 2^-24 of x.  fp16's weights spread the pieces over its range: numbers up to 2^23, to 2^-43.
@@ -687,47 +687,63 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
   return d;
 }
 
-// 16 lanes to a row (up to 128 columns, eight each): two rows to a warp.
+// A CTA to 128 rows of a head: 16 lanes to a row (up to 128 columns, eight each), eight rows of each half warp in flight four at a
+// time.  blockIdx.y counts the query heads, then (fp16) the key heads, whose rows only go into the bound.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
-  const int64_t rows_q = (int64_t)a.B * a.Hq * a.q_pad, rows_v = a.bound != nullptr ? (int64_t)a.B * a.Hkv * a.Skv : 0;
-  const int sub = threadIdx.x & 15;
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-  const bool in = 8 * sub < a.D;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  float d = 0.f, n = 0.f;
-  int64_t group = -1;
-  if (row < rows_q) {
-    const int64_t bh = row / a.q_pad, q = row % a.q_pad;
-    const int64_t b = bh / a.Hq, h = bh % a.Hq;
-    group = (b * a.Hkv + h / (a.Hq / a.Hkv)) * 2;
-    if (in && q < a.Sq) {
-      const uint4 g = *reinterpret_cast<const uint4*>((const T*)a.grad + b * a.g_b + h * a.g_h + q * a.g_s + 8 * sub);
-      const int64_t at = ((b * a.Sq + q) * a.Hq + h) * a.D + 8 * sub;
-      const uint4 o = *reinterpret_cast<const uint4*>((const T*)a.out + at), lo = *reinterpret_cast<const uint4*>((const T*)a.low + at);
-      d = dot8<T>(g, o) + dot8<T>(g, lo) * (1.f / kLowScale);
-      if (a.bound != nullptr) n = dot8<T>(g, g);
-    }
-  } else if (row < rows_q + rows_v) {
-    const int64_t at = row - rows_q, bh = at / a.Skv, k = at % a.Skv;
-    const int64_t b = bh / a.Hkv, h = bh % a.Hkv;
-    group = bh * 2 + 1;
-    const uint4 w = in ? *reinterpret_cast<const uint4*>((const T*)a.v + b * a.v_b + h * a.v_h + k * a.v_s + 8 * sub) : zero;
-    n = dot8<T>(w, w);
-  }
+  __shared__ float most[16];
+  const int sub = threadIdx.x & 15, half = threadIdx.x >> 4, b = blockIdx.z;
+  const bool is_q = (int)blockIdx.y < a.Hq, in = 8 * sub < a.D;
+  const int h = is_q ? blockIdx.y : blockIdx.y - a.Hq, rows = is_q ? a.Sq : a.Skv, r0 = blockIdx.x * kT + half * 8;
+  const T* x = is_q ? (const T*)a.grad + b * a.g_b + h * a.g_h : (const T*)a.v + b * a.v_b + h * a.v_h;
+  const int64_t stride = is_q ? a.g_s : a.v_s, o_row = (int64_t)a.Hq * a.D;
+  const int64_t o_at = ((int64_t)b * a.Sq * a.Hq + h) * a.D + 8 * sub;
+  if ((int)blockIdx.x * kT >= rows) return;
+  float largest = 0.f;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    d += __shfl_xor_sync(0xffffffffu, d, o);
-    n += __shfl_xor_sync(0xffffffffu, n, o);
+  for (int i = 0; i < 8; i += 4) {
+    uint4 g[4], o[4], lo[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + i + u;
+      g[u] = o[u] = lo[u] = make_uint4(0, 0, 0, 0);
+      if (in && r < rows) {
+        g[u] = ldg_nc_v4(x + r * stride + 8 * sub);
+        if (is_q) {
+          o[u] = ldg_nc_v4((const T*)a.out + o_at + r * o_row);
+          lo[u] = ldg_nc_v4((const T*)a.low + o_at + r * o_row);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + i + u;
+      float d = is_q ? dot8<T>(g[u], o[u]) + dot8<T>(g[u], lo[u]) * (1.f / kLowScale) : 0.f;
+      float n = std::is_same<T, __half>::value ? dot8<T>(g[u], g[u]) : 0.f;
+#pragma unroll
+      for (int s = 8; s > 0; s >>= 1) {
+        d += __shfl_xor_sync(0xffffffffu, d, s);
+        if (std::is_same<T, __half>::value) n += __shfl_xor_sync(0xffffffffu, n, s);
+      }
+      largest = fmaxf(largest, n);
+      if (sub == 0 && is_q) {
+        const int64_t row = ((int64_t)b * a.Hq + h) * a.q_pad + r;
+        a.delta[row] = d;
+        const float nl = a.nlse[row];
+        uint4* at = a.pieces + row / kT * (2 * kT) + row % kT;
+        at[0] = in_pieces<T>(nl == -INFINITY ? 0.f : nl * a.inv_scale_log2);
+        at[kT] = in_pieces<T>(-d);
+      }
+    }
   }
-  if (sub == 0 && row < rows_q) {
-    a.delta[row] = d;
-    const float nl = a.nlse[row];
-    uint4* at = a.pieces + row / kT * (2 * kT) + row % kT;
-    at[0] = in_pieces<T>(nl == -INFINITY ? 0.f : nl * a.inv_scale_log2);
-    at[kT] = in_pieces<T>(-d);
+  if (std::is_same<T, __half>::value) {
+    if (sub == 0) most[half] = largest;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 16; ++i) largest = fmaxf(largest, most[i]);
+      atomicMax(&a.bound[(b * a.Hkv + (is_q ? h / (a.Hq / a.Hkv) : h)) * 2 + (is_q ? 0 : 1)], __float_as_uint(largest));
+    }
   }
-  if (sub == 0 && a.bound != nullptr && group >= 0 && n > __uint_as_float(a.bound[group])) atomicMax(&a.bound[group], __float_as_uint(n));
 }
 
 // fp16: the power of two for dP - delta; bf16: none.  |dP_ij - delta_i| <= 2 max |dO_i| max |v_j| (o_i is a mean of the v_j).
@@ -1140,40 +1156,41 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       ok = warp_wait(q_full, w & 1, abort_flag);
       if (it.total == 0) continue;
       const int end = base + it.total;
-      // Scores one step ahead, into the other tile, then this step's sum (dS lies over dP) and the next dP.
-      for (int n = base - 1; n < end && ok; ++n) {
-        if (n + 1 < end) {
-          ok = warp_wait(&full[k_at(n + 1)], (n + 1) / L::kK & 1, abort_flag) &&
-               warp_wait(&s_free[n + 1 & 1], (n + 1 >> 1 & 1) ^ 1, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after();
-          if (elect_one()) {                      // q k^T
-            mma_rows<D>(tmem + (n + 1 & 1) * kT, qd, kv_rows + (uint64_t)(k_at(n + 1) * (L::kTile >> 4)), idesc_s);
-            umma_commit(&s_full[n + 1 & 1]);
-          }
-          __syncwarp();
+      auto scores = [&](int n) {                  // q k^T, into the other tile
+        if (!warp_wait(&full[k_at(n)], n / L::kK & 1, abort_flag) || !warp_wait(&s_free[n & 1], (n >> 1 & 1) ^ 1, abort_flag))
+          return false;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          mma_rows<D>(tmem + (n & 1) * kT, qd, kv_rows + (uint64_t)(k_at(n) * (L::kTile >> 4)), idesc_s);
+          umma_commit(&s_full[n & 1]);
         }
-        if (n >= base) {
-          ok = warp_wait(ds_full, n & 1, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after();
-          if (elect_one()) {
-            mma_sum<16, 32>(tQ, tP, kv_sum + (uint64_t)(k_at(n) * (L::kTile >> 4)), idesc_o, n > base);
-            umma_commit(&empty[k_at(n)]);
-          }
-          __syncwarp();
+        __syncwarp();
+        return true;
+      };
+      auto grads = [&](int n) {                   // dO v^T
+        if (!warp_wait(&full[v_at(n)], n / L::kV & 1, abort_flag)) return false;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          mma_rows<D>(tP, gd, kv_rows + (uint64_t)(v_at(n) * (L::kTile >> 4)), idesc_s);
+          umma_commit(dp_full);
+          umma_commit(&empty[v_at(n)]);
         }
-        if (n + 1 < end) {                        // dO v^T
-          ok = warp_wait(&full[v_at(n + 1)], (n + 1) / L::kV & 1, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after();
-          if (elect_one()) {
-            mma_rows<D>(tP, gd, kv_rows + (uint64_t)(v_at(n + 1) * (L::kTile >> 4)), idesc_s);
-            umma_commit(dp_full);
-            umma_commit(&empty[v_at(n + 1)]);
-          }
-          __syncwarp();
+        __syncwarp();
+        return true;
+      };
+      // What the arithmetic waits for goes first: dS of a step, its sum (dS lies over dP), the next dP.  Scores are two steps ahead.
+      ok = scores(base) && grads(base) && (base + 1 == end || scores(base + 1));
+      for (int n = base; n < end && ok; ++n) {
+        ok = warp_wait(ds_full, n & 1, abort_flag);
+        if (!ok) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          mma_sum<16, 32>(tQ, tP, kv_sum + (uint64_t)(k_at(n) * (L::kTile >> 4)), idesc_o, n > base);
+          umma_commit(&empty[k_at(n)]);
         }
+        __syncwarp();
+        if (n + 1 < end) ok = grads(n + 1);
+        if (ok && n + 2 < end) ok = scores(n + 2);
       }
       if (ok && elect_one()) umma_commit(done);
       __syncwarp();
@@ -1419,10 +1436,10 @@ int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
   }
   const PrepArgs p = {out, low, g.p, v.p, g.b, g.h, g.s, v.b, v.h, v.s, nlse, delta, pieces, 1.f / s.scale_log2, bound,
                       s.B, s.Hq, s.Hkv, s.Sq, s.Skv, s.D, s.q_pad};
-  const int64_t rows = (int64_t)s.B * s.Hq * s.q_pad + (bound != nullptr ? (int64_t)s.B * s.Hkv * s.Skv : 0);
-  if (rows / 16 + 1 > 0x7FFFFFFF || items_of(s, s.Hkv, s.Skv, kT) == 0 || items_of(s, s.Hq, s.Sq, kT) == 0)
+  if (items_of(s, s.Hkv, s.Skv, kT) == 0 || items_of(s, s.Hq, s.Sq, kT) == 0 || s.Hq + s.Hkv > 65535)
     return (int)cudaErrorInvalidValue;
-  attn_prep_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, stream>>>(p);
+  const int longest = bound != nullptr && s.Skv > s.Sq ? s.Skv : s.Sq;
+  attn_prep_kernel<T><<<dim3((longest + kT - 1) / kT, s.Hq + (bound != nullptr ? s.Hkv : 0), s.B), 256, 0, stream>>>(p);
   BwdArgs a = {s, nlse, delta, pieces, bound, items_of(s, s.Hkv, s.Skv, kT)};
   attn_dkv_kernel<T, D><<<grid_of(a.items), kThreads, smem, stream>>>(tq, tk, tv, tg, tdk, tdv, a);
   a.items = items_of(s, s.Hq, s.Sq, kT);
