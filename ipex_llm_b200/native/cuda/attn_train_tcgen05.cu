@@ -176,6 +176,10 @@ __device__ __forceinline__ void hand_over(uint64_t* bar, int lane) {
   if (lane == 0) mbar_arrive(bar);
 }
 
+// A number that is the same in the whole warp, for the compiler to know: products take their operands from uniform registers, and
+// with bounds or offsets that came out of a division every one of them took 64 clocks to issue, as long as it runs.
+__device__ __forceinline__ int uniform(int x) { return (int)__reduce_max_sync(0xffffffffu, (unsigned)x); }
+
 // Two 32-bit numbers an instruction.
 __device__ __forceinline__ void mul2(float& x, float& y, float a, float b) {   // x *= a, y *= b
   asm("{\n"
@@ -388,7 +392,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
 
   if (warp == kLoader) {
     // ---------------- loader: keys and values of a block take a stage each, in turn ----------------
@@ -431,7 +435,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     bool ok = true;
     int n = 0, made[2] = {0, 0};                 // tiles of keys and values before this item; probabilities waited for
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
-      const FwdItem it(s, item_of(w));
+      FwdItem it(s, item_of(w));
+      it.ja = uniform(it.ja);
+      it.jb = uniform(it.jb);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        it.j0[t] = uniform(it.j0[t]);
+        it.j1[t] = uniform(it.j1[t]);
+      }
       ok = warp_wait(q_full, w & 1, abort_flag);
       if (!ok) break;
       auto has = [&](int t, int j) { return j >= it.j0[t] && j < it.j1[t]; };
@@ -856,7 +867,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *tmem_slot, tP = tmem + kT, tV = tmem + 2 * kT, tK = tmem + 3 * kT;
+  const uint32_t tmem = uniform(*tmem_slot), tP = tmem + kT, tV = tmem + 2 * kT, tK = tmem + 3 * kT;
 
   if (warp == kLoader) {
     if (lane == 0) {
@@ -934,14 +945,14 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       return true;
     };
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
-      const DkvItem it(s, item_of(w));
+      const int total = uniform(DkvItem(s, item_of(w)).total);
       ok = warp_wait(kv_full, w & 1, abort_flag);
-      if (it.total == 0) continue;
-      for (int n = 0; n <= it.total && ok; ++n)
-        ok = half(std::integral_constant<int, 0>(), n, it.total) && half(std::integral_constant<int, 1>(), n, it.total);
+      if (total == 0) continue;
+      for (int n = 0; n <= total && ok; ++n)
+        ok = half(std::integral_constant<int, 0>(), n, total) && half(std::integral_constant<int, 1>(), n, total);
       if (ok && elect_one()) umma_commit(done);
       __syncwarp();
-      base += it.total;
+      base += total;
     }
     if (!ok && lane == 0) report(s.err, 72);
     __syncwarp();
@@ -1108,7 +1119,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   __syncthreads();
   tcgen05_fence_after();
   // two tiles of scores in turn, dP (and dS over it), the sum
-  const uint32_t tmem = *tmem_slot, tP = tmem + 2 * kT, tQ = tmem + 3 * kT;
+  const uint32_t tmem = uniform(*tmem_slot), tP = tmem + 2 * kT, tQ = tmem + 3 * kT;
 
   if (warp == kLoader) {
     if (lane == 0) {
@@ -1152,10 +1163,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     bool ok = true;
     int base = 0;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
-      const DqItem it(s, item_of(w));
+      const int total = uniform(DqItem(s, item_of(w)).total);
       ok = warp_wait(q_full, w & 1, abort_flag);
-      if (it.total == 0) continue;
-      const int end = base + it.total;
+      if (total == 0) continue;
+      const int end = base + total;
       auto scores = [&](int n) {                  // q k^T, into the other tile
         if (!warp_wait(&full[k_at(n)], n / L::kK & 1, abort_flag) || !warp_wait(&s_free[n & 1], (n >> 1 & 1) ^ 1, abort_flag))
           return false;
