@@ -1,18 +1,21 @@
 // What stands behind an output layer: log probabilities of given tokens with their entropy and the best alternatives, and
 // the divergence from a teacher's top logits, each with the gradient of the logits.  sm_100a.
 //
-// With y = x / T, m = max x, s = sum e^((x - m) / T), t = sum e^((x - m) / T) (x - m):
+// With c = log2(e) / T, r = fl(c max x), y = c x - r, s = sum 2^y, t = sum 2^y y (all to base 2):
 //
-//   log p_j = (x_j - m) / T - ln s            H = ln s - t / (s T)
+//   log p_j = (y_j - log2 s) ln 2             H = (log2 s - t / s) ln 2
 //   d log p_t / dx_j = (1[j = t] - p_j) / T   dH / dx_j = -p_j (log p_j + H) / T
 //
 // All of them are bound by memory: forward reads a row once, backward reads it once more and writes it once.  A row belongs
 // to one CTA (many rows; the CTAs stay and take the next row) or to a cluster of up to eight (few rows).  Each thread copies its
 // own four 16-byte vectors at a time to shared memory, asynchronously and two batches ahead, into the next row while a row's
-// parts are joined: without that, loads waited for arithmetic and arithmetic for loads (2048 rows of 32000 in bf16: 53 us).
+// parts are joined.  Fifteen warps read; a sixteenth does what a row has beside its sums (its target, the teacher's tokens, the
+// results), on this row while the others read it and on its sums while they read the next one: in their way, those latencies
+// took half of the time (2048 rows of 32000 in bf16: 58 us).
 // A thread folds the maximum of a batch into its own and rescales its sums once for all of it, so that an element costs one
 // exponential (0.73 of what the special function units do at the rate of memory, for 16-bit logits).
-// x - m is taken before the factor log2(e) / T: its rounding then does not grow with m, as that of one fma(x, c, -m c) would.
+// y is one fma: the rounding of r, common to a row, takes part everywhere alike and so cancels, as long as r is the same number
+// everywhere (it goes to the backward pass, and rescaling goes by differences of it).
 //
 // Statistics are 32-bit, 250 to 500 elements to a thread's sum and a tree above that; exponentials by ex2.approx (2 ulp).
 #include <cooperative_groups.h>
@@ -26,13 +29,15 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kNT = 512;
-constexpr int kWarps = kNT / 32;
+constexpr int kWarps = 15;        // that read rows
+constexpr int kNT = 32 * kWarps;
 constexpr int kU = 4;             // 16-byte requests of a thread in flight
 constexpr int kMaxTop = 32;
 constexpr int kMaxK = 1024;
 constexpr int kCand = 1024;       // candidates for the best tokens of a slice before it is scanned in rounds instead
 constexpr int kMaxCluster = 8;
+constexpr int kMaxTailV = 1 << 19;
+constexpr int kMaxBits = 2 * (kMaxTailV / 8 + 64);     // bytes: bits of two rows
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kErrToken = 61;     // a token outside of the vocabulary
@@ -42,14 +47,36 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// x - m, held above -1e25 (e^(-1e25 / T) is 0 for every temperature up to 1e6), so that its product with a sum of up to 2^30
-// stays finite and 0 * (x - m) is 0 for hidden tokens (-inf, or the type's lowest value); NaN stays NaN.
-__device__ __forceinline__ float below(float x, float m) {
+// An exponent, held above -1e25 (2^-1e25 is 0), so that its product with a sum of up to 2^30 stays finite and 0 times it is 0 for
+// hidden tokens (-inf, or the type's lowest value); NaN stays NaN.
+__device__ __forceinline__ float held(float y) {
   float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x - m), "f"(-1.0e25f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(y), "f"(-1.0e25f));
   return d;
 }
-
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two 32-bit numbers an instruction: x += a, y += b; x += a u, y += b v; x = x c - r, y = y c - r.
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n.reg .b64 u, v;\nmov.b64 u, {%0, %1};\nmov.b64 v, {%2, %3};\nadd.rn.f32x2 u, u, v;\nmov.b64 {%0, %1}, u;\n}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float u, float v) {
+  asm("{\n.reg .b64 p, q, r;\nmov.b64 p, {%2, %3};\nmov.b64 q, {%4, %5};\nmov.b64 r, {%0, %1};\n"
+      "fma.rn.f32x2 r, p, q, r;\nmov.b64 {%0, %1}, r;\n}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b), "f"(u), "f"(v));
+}
+__device__ __forceinline__ void exponents2(float& x, float& y, float c, float minus_r) {
+  asm("{\n.reg .b64 p, q, r;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %2};\nmov.b64 r, {%3, %3};\n"
+      "fma.rn.f32x2 p, p, q, r;\nmov.b64 {%0, %1}, p;\n}\n"
+      : "+f"(x), "+f"(y)
+      : "f"(c), "f"(minus_r));
+}
 __device__ __forceinline__ void copy_async(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
@@ -100,12 +127,6 @@ __device__ __forceinline__ void unpack(const uint4& w, float* f) {
 #pragma unroll
   for (int i = 0; i < 16 / (int)sizeof(T); ++i) f[i] = DT<T>::to_f(p[i]);
 }
-template <typename T>
-__device__ __forceinline__ uint4 hidden() {  // a vector of -inf
-  const uint32_t w = sizeof(T) == 4 ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
-  return make_uint4(w, w, w, w);
-}
-
 // Larger keys come first: by value (NaN above all), then by the lower index.  No element has key 0.
 __device__ __forceinline__ uint64_t order_key(float v, int idx) {
   const uint32_t b = v != v ? 0x7FFFFFFFu : __float_as_uint(v == 0.f ? 0.f : v);   // -0 and 0 are equal
@@ -114,20 +135,22 @@ __device__ __forceinline__ uint64_t order_key(float v, int idx) {
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
 
-// m: maximum, s: sum of e^((x - m) / T), t: that sum weighted by x - m (ENT), or over the tokens not given (TAIL).
+// r: the rounded product of c and the maximum (-inf: no token), s: sum of 2^y, t: that sum weighted by y (ENT), or over the tokens
+// not given (TAIL).
 struct Stat {
-  float m, s, t;
+  float r, s, t;
 };
+__device__ __forceinline__ float base_of(float r) { return r == -INFINITY ? 0.f : r; }
 template <bool ENT>
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
-  Stat r;
-  r.m = fmaxf(a.m, b.m);
-  const float ref = r.m == -INFINITY ? 0.f : r.m;
-  const float da = below(a.m, ref), db = below(b.m, ref);   // sums of a side without tokens are 0
-  const float ea = ex2(da * c), eb = ex2(db * c);
-  r.s = a.s * ea + b.s * eb;
-  r.t = ENT ? (a.t + a.s * da) * ea + (b.t + b.s * db) * eb : a.t * ea + b.t * eb;
-  return r;
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+  Stat o;
+  o.r = fmaxf(a.r, b.r);
+  const float to = base_of(o.r);
+  const float da = held(a.r - to), db = held(b.r - to);     // sums of a side without tokens are 0
+  const float ea = ex2(da), eb = ex2(db);
+  o.s = a.s * ea + b.s * eb;
+  o.t = ENT ? (a.t + a.s * da) * ea + (b.t + b.s * db) * eb : a.t * ea + b.t * eb;
+  return o;
 }
 
 // The vectors of a CTA's rows as a stream of batches, each thread's four to a batch, kStages batches ahead of their use.
@@ -169,22 +192,24 @@ struct Feed {
     copies_end_batch();
     slot = slot + 1 == kStages ? 0 : slot + 1;
   }
-  // The oldest batch, whose first vector is `first` of a row that ends at `last`; fetches the next one into its place.
-  __device__ void take(int first, int last, uint4 (&w)[kU]) {
+  // This thread's vectors of the oldest batch, kNT apart; fetch() overwrites them.
+  __device__ const uint4* oldest() {
     copies_wait<kStages - 1>();
-#pragma unroll
-    for (int u = 0; u < kU; ++u)
-      w[u] = first + u * kNT + (int)threadIdx.x < last ? ring[(slot * kU + u) * kNT] : hidden<T>();
-    fetch();
+    return ring + slot * kU * kNT;
   }
 };
 
-struct Shared {
-  Stat warp[kWarps];
+// A row whose largest logit is not above -2^127 has no token: -inf, or the lowest values of bf16 and of 32 bits, hide them all.
+__device__ __forceinline__ bool no_token(const Stat& st, float c) { return st.s == st.s && !(st.r > c * -0x1p127f); }
+
+struct Sums {
+  Stat warp[2][kWarps];           // by the parity of the CTA's row
   Stat part;                      // this CTA's
+};
+struct Shared : Sums {
   uint64_t best[kNT];             // the threads' best keys, sorted in each warp
   uint64_t cand[kCand];
-  uint64_t top[kMaxTop];          // this CTA's best, sorted
+  uint64_t top[2][kMaxTop];       // this CTA's best, sorted
   uint64_t thr;
   int n_cand, n_list;
   int list[kNT];                  // threads that may hold one of the best
@@ -197,10 +222,26 @@ struct Best {
   int at;
 };
 
-// A row's statistics into sh.part, TOP: this thread's best.
+// A barrier of the warps that read, and one that counts.
+__device__ __forceinline__ void sync_readers() { asm volatile("bar.sync 1, %0;" ::"n"(kNT) : "memory"); }
+__device__ __forceinline__ int sync_readers_count(bool x) {
+  int n;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.u32 p, %1, 0;\n"
+      "barrier.cta.red.popc.aligned.u32 %0, 1, %2, p;\n"
+      "}\n"
+      : "=r"(n)
+      : "r"((uint32_t)x), "n"(kNT)
+      : "memory");
+  return n;
+}
+
+// Each warp's statistics of a row into `sums`, TOP: this thread's best.
 template <typename T, bool ENT, bool TOP, bool TAIL>
-__device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, const uint32_t* given, const int* ids, int K, Shared& sh,
-                     Best& best) {
+__device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, const uint32_t* given, const int* ids, int K,
+                     Stat* sums, Best& best) {
   constexpr int VEC = Slice<T>::VEC;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Stat st = {-INFINITY, 0.f, 0.f};
@@ -210,70 +251,113 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
     bool is_given = false;
     if constexpr (TAIL)
       for (int k = 0; k < K; ++k) is_given |= ids[k] == j;
-    Stat one = {v, 1.f, TAIL && !is_given ? 1.f : 0.f};
-    if (v == -INFINITY) one.s = one.t = 0.f;
+    Stat one = {__fmul_rn(v, c), 1.f, TAIL && !is_given ? 1.f : 0.f};
+    one.s = ex2(fmaf(v, c, -base_of(one.r)));       // 1, but for the rounding of r
+    if (ENT) one.t = one.s * held(fmaf(v, c, -base_of(one.r)));
+    else if (one.t != 0.f) one.t = one.s;
     if (v != v) one.s = one.t = v;
-    st = join<ENT>(st, one, c);
+    st = join<ENT>(st, one);
     if (TOP && (best.at == -1 || order_key(v, 0) > order_key(best.v, 0))) best = {v, -2 - j};
   };
   if (tid < sl.h) single(tid);
   // as the feed does: at least one batch a row, whether it holds vectors or not
   for (int base = sl.v0; base == sl.v0 || base < sl.v1; base += kNT * kU) {
-    uint4 w[kU];
-    feed.take(base, sl.v1, w);
-    if (base + tid >= sl.v1) continue;
-    float f[kU * VEC], mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) unpack<T>(w[u], f + u * VEC);
-#pragma unroll
-    for (int i = 0; i < kU * VEC; ++i) mx = fmaxf(mx, f[i]);
-    const float m = fmaxf(st.m, mx), ref = m == -INFINITY ? 0.f : m;
-    const float down = below(st.m, ref), fac = ex2(down * c);
-    float s = 0.f, t = 0.f;
+    const uint4* w = feed.oldest();
+    if (base + tid >= sl.v1) {
+      feed.fetch();
+      continue;
+    }
+    const int n = min(kU, (sl.v1 - base - tid + kNT - 1) / kNT);    // vectors of this thread
+    float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      float sv = 0.f;
-      uint32_t bits = 0;
-      if constexpr (TAIL) {
-        const int pos = (min(base + u * kNT + tid, sl.v1 - 1) - sl.v0) * VEC;
-        bits = given[pos >> 5] >> (pos & 31) & ((1u << VEC) - 1);
-      }
+      if (u >= n) break;
+      float f[VEC];
+      unpack<T>(w[u * kNT], f);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = ENT ? below(f[u * VEC + i], ref) : f[u * VEC + i] - ref;
-        const float e = ex2(d * c);
-        sv += e;
-        if constexpr (ENT) t = fmaf(e, d, t);
-        if constexpr (TAIL) t += bits >> i & 1 ? 0.f : e;
-      }
-      s += sv;
+      for (int i = 0; i < VEC; i += 2) mx = max3(mx, f[i], f[i + 1]);
     }
+    const float r = fmaxf(st.r, __fmul_rn(mx, c)), to = base_of(r);
+    const float down = held(st.r - to), fac = ex2(down);
+    // CAREFUL: with exponents held, for what hides tokens
+    auto sums = [&](auto careful, float& s, float& t) {
+      constexpr bool CAREFUL = decltype(careful)::value;
+      float sa[2] = {0.f, 0.f}, ta[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        if (u >= n) break;
+        float f[VEC], e[VEC], v[2] = {0.f, 0.f};
+        unpack<T>(w[u * kNT], f);
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+          exponents2(f[i], f[i + 1], c, -to);
+          if (CAREFUL) {
+            f[i] = held(f[i]);
+            f[i + 1] = held(f[i + 1]);
+          }
+          e[i] = ex2(f[i]);
+          e[i + 1] = ex2(f[i + 1]);
+          add2(v[0], v[1], e[i], e[i + 1]);
+          if constexpr (ENT) fma2(ta[0], ta[1], e[i], e[i + 1], f[i], f[i + 1]);
+        }
+        add2(sa[0], sa[1], v[0], v[1]);
+        if constexpr (TAIL) {
+          const int pos = (base + u * kNT + tid - sl.v0) * VEC;
+          const uint32_t bits = given[pos >> 5] >> (pos & 31) & ((1u << VEC) - 1);
+          if (bits == 0) {
+            add2(ta[0], ta[1], v[0], v[1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) ta[i & 1] += bits >> i & 1 ? 0.f : e[i];
+          }
+        }
+      }
+      s = sa[0] + sa[1];
+      t = ta[0] + ta[1];
+    };
+    float s, t;
+    sums(std::false_type(), s, t);
+    if (ENT && t != t) sums(std::true_type(), s, t);
     if constexpr (ENT) st.t = (st.t + st.s * down) * fac + t;
     else if constexpr (TAIL) st.t = st.t * fac + t;
     st.s = st.s * fac + s;
-    st.m = m;
+    st.r = r;
     if constexpr (TOP) {
       if (s != s) {
+        for (int u = 0; u < n; ++u) {
+          float f[VEC];
+          unpack<T>(w[u * kNT], f);
 #pragma unroll
-        for (int i = 0; i < kU * VEC; ++i) mx = f[i] != f[i] ? NAN : mx;
+          for (int i = 0; i < VEC; ++i) mx = f[i] != f[i] ? NAN : mx;
+        }
       }
       if (best.at == -1 || order_key(mx, 0) > order_key(best.v, 0)) best = {mx, base + tid};
     }
+    feed.fetch();
   }
   if (tid >= kNT - sl.t) single(sl.V - (kNT - tid));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    Stat other = {__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+    Stat other = {__shfl_xor_sync(0xffffffffu, st.r, o), __shfl_xor_sync(0xffffffffu, st.s, o),
                   __shfl_xor_sync(0xffffffffu, st.t, o)};
-    st = lane & o ? join<ENT>(other, st, c) : join<ENT>(st, other, c);
+    st = lane & o ? join<ENT>(other, st) : join<ENT>(st, other);
   }
-  if (lane == 0) sh.warp[warp] = st;
-  __syncthreads();
-  if (tid == 0) {
-    Stat a = sh.warp[0];
-    for (int i = 1; i < kWarps; ++i) a = join<ENT>(a, sh.warp[i], c);
-    sh.part = a;
+  if (lane == 0) sums[warp] = st;
+}
+
+// The warps' statistics joined, in every lane of a warp.
+template <bool ENT>
+__device__ __forceinline__ Stat join_warps(const Stat* sums) {
+  const int lane = threadIdx.x & 31;
+  Stat st = {-INFINITY, 0.f, 0.f};
+  if (lane < kWarps) st = sums[lane];
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    Stat other = {__shfl_xor_sync(0xffffffffu, st.r, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+                  __shfl_xor_sync(0xffffffffu, st.t, o)};
+    st = lane & o ? join<ENT>(other, st) : join<ENT>(st, other);
   }
+  return {__shfl_sync(0xffffffffu, st.r, 0), __shfl_sync(0xffffffffu, st.s, 0), __shfl_sync(0xffffffffu, st.t, 0)};
 }
 
 // Keys of a warp: sorted from large to small over its lanes, and the 32 largest of two such rows of lanes.
@@ -314,12 +398,12 @@ __device__ __forceinline__ void elements_of(const T* x, const Slice<T>& sl, int 
 __device__ uint64_t largest32(uint64_t k, Shared& sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   k = warp_sort(k, lane);
-  __syncthreads();
+  sync_readers();
   sh.best[threadIdx.x] = k;
 #pragma unroll
-  for (int n = kWarps / 2; n > 0; n /= 2) {
-    __syncthreads();
-    if (warp < n) {
+  for (int n = 8; n > 0; n /= 2) {
+    sync_readers();
+    if (warp < n && warp + n < kWarps) {
       k = warp_merge(k, sh.best[(warp + n) * 32 + 31 - lane], lane);
       sh.best[threadIdx.x] = k;
     }
@@ -327,23 +411,23 @@ __device__ uint64_t largest32(uint64_t k, Shared& sh) {
   return k;
 }
 
-// The `top` largest keys of a slice, sorted, into sh.top (0 behind the last element).  The top-th largest of the threads' best keys
+// The `top` largest keys of a slice, sorted, into `out` (0 behind the last element).  The top-th largest of the threads' best keys
 // bounds them from below, and only the threads that reach it (top of them, keys being unique) can hold any: their elements are read
-// again, sixteen lanes to a thread, and what reaches the bound is ranked by counting.  Values nearly always decide; where several
+// again, sixteen lanes to each, and what reaches the bound is ranked by counting.  Values nearly always decide; where several
 // threads have the bound's, these look up where they have it (the lower index comes first).  Where more than kCand elements
 // reach it (a few threads hold nearly all large values), the slice is scanned once for each rank instead.
 template <typename T>
-__device__ void best_tokens(const T* x, const Slice<T>& sl, int top, const Best& best, Shared& sh) {
+__device__ void best_tokens(const T* x, const Slice<T>& sl, int top, const Best& best, uint64_t* out, Shared& sh) {
   constexpr int VEC = Slice<T>::VEC;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < kMaxTop) sh.top[tid] = 0;
+  if (tid < kMaxTop) out[tid] = 0;
   if (tid == 0) sh.n_cand = sh.n_list = 0;
   uint64_t mine = best.at == -1 ? 0 : order_key(best.v, tid);
   uint64_t k = largest32(mine, sh);
   if (tid == top - 1) sh.thr = k >> 32 << 32;       // the value alone: below every key that has it
-  __syncthreads();
+  sync_readers();
   uint64_t thr = sh.thr;
-  if (__syncthreads_count(mine != 0 && mine >= thr) > top) {
+  if (sync_readers_count(mine != 0 && mine >= thr) > top) {
     if (mine != 0 && mine >> 32 == thr >> 32) {
       if (best.at < 0) {
         mine = order_key(best.v, -2 - best.at);
@@ -363,11 +447,11 @@ __device__ void best_tokens(const T* x, const Slice<T>& sl, int top, const Best&
     }
     k = largest32(mine, sh);
     if (tid == top - 1) sh.thr = k;
-    __syncthreads();
+    sync_readers();
     thr = sh.thr;
   }
   if (mine != 0 && mine >= thr) sh.list[atomicAdd(&sh.n_list, 1)] = tid;
-  __syncthreads();
+  sync_readers();
   const int n_list = sh.n_list;
   for (int i = tid >> 4; i < n_list; i += kNT / 16)
     elements_of<T>(x, sl, sh.list[i], tid & 15, 16, [&](float v, int j) {
@@ -377,16 +461,16 @@ __device__ void best_tokens(const T* x, const Slice<T>& sl, int top, const Best&
         if (at < kCand) sh.cand[at] = key;
       }
     });
-  __syncthreads();
+  sync_readers();
   const int n = sh.n_cand;
   if (n <= kCand) {
     for (int i = tid; i < n; i += kNT) {
       const uint64_t key = sh.cand[i];
       int r = 0;
       for (int j = 0; j < n; ++j) r += sh.cand[j] > key;
-      if (r < top) sh.top[r] = key;
+      if (r < top) out[r] = key;
     }
-    __syncthreads();
+    sync_readers();
     return;
   }
   uint64_t under = ~0ull;
@@ -402,28 +486,37 @@ __device__ void best_tokens(const T* x, const Slice<T>& sl, int top, const Best&
       b = w > b ? w : b;
     }
     if (lane == 0) sh.best[warp] = b;
-    __syncthreads();
+    sync_readers();
     b = sh.best[0];
     for (int i = 1; i < kWarps; ++i) b = sh.best[i] > b ? sh.best[i] : b;
-    if (tid == 0) sh.top[r] = b;
+    if (tid == 0) out[r] = b;
     under = b;
-    __syncthreads();
+    sync_readers();
     if (b == 0) break;
   }
 }
 
-// The row's statistics from those of the cluster's CTAs, in every thread of the first one.
+// A row's statistics, in every lane of the finishing warp: those of its CTA's warps, and where a cluster has the row those of its
+// CTAs (between two barriers of the cluster, which the other warps take part in: see meet()).
 template <bool ENT>
-__device__ __forceinline__ Stat row_stat(Shared& sh, int parts, float c) {
-  if (parts == 1) {
-    __syncthreads();
-    return sh.part;
+__device__ __forceinline__ Stat row_stat(Sums& sh, int turn, int parts) {
+  Stat a = join_warps<ENT>(sh.warp[turn]);
+  if (parts > 1) {
+    if ((threadIdx.x & 31) == 0) sh.part = a;
+    __syncwarp();
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    a = *cl.map_shared_rank(&sh.part, 0);
+    for (int i = 1; i < parts; ++i) a = join<ENT>(a, *cl.map_shared_rank(&sh.part, i));
   }
-  cg::cluster_group cl = cg::this_cluster();
-  cl.sync();
-  Stat a = *cl.map_shared_rank(&sh.part, 0);
-  for (int i = 1; i < parts; ++i) a = join<ENT>(a, *cl.map_shared_rank(&sh.part, i), c);
   return a;
+}
+// The other warps' share of a row's end in a cluster: sums are there, and shared memory stays until the first CTA has read it.
+__device__ __forceinline__ void meet(int parts) {
+  if (parts > 1) {
+    cg::this_cluster().sync();
+    cg::this_cluster().sync();
+  }
 }
 
 struct ProbArgs {
@@ -431,7 +524,7 @@ struct ProbArgs {
   const int64_t* targets;
   float* logprob;
   float* entropy;      // null: not asked for
-  float* stats;        // [rows, 4]: m, 1 / s, ln s, H
+  float* stats;        // [rows, 4]: r, 1 / s, log2 s, H
   float* top_logprob;  // [rows, top]
   int64_t* top_id;
   int top, parts;
@@ -441,64 +534,58 @@ struct ProbArgs {
 };
 
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kNT, 2) token_logprobs_kernel(ProbArgs a) {
+__global__ void __launch_bounds__(kNT + 32, 2) token_logprobs_kernel(ProbArgs a) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
   const int parts = a.parts, rank = parts == 1 ? 0 : (int)(blockIdx.x % parts);
-  const int64_t step = gridDim.x / parts;
+  const int64_t first = blockIdx.x / parts, step = gridDim.x / parts;
   const float c = a.inv_t * kLog2e;
-  Feed<T> feed(a.rows, reinterpret_cast<uint4*>(dynamic), blockIdx.x / parts, step, a.n, rank, parts);
-  for (int64_t row = blockIdx.x / parts; row < a.n; row += step) {
+  if (threadIdx.x < kNT) {
+    Feed<T> feed(a.rows, reinterpret_cast<uint4*>(dynamic), first, step, a.n, rank, parts);
+    int turn = 0;
+    for (int64_t row = first; row < a.n; row += step, turn ^= 1) {
+      const T* x = row_at<T>(a.rows, row);
+      const Slice<T> sl(x, a.rows.V, rank, parts);
+      Best best;
+      scan<T, ENT, TOP, false>(x, sl, c, feed, nullptr, nullptr, 0, sh.warp[turn], best);
+      if constexpr (TOP) best_tokens<T>(x, sl, a.top, best, sh.top[turn], sh);
+      __syncthreads();
+      meet(parts);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  int turn = 0;
+  for (int64_t row = first; row < a.n; row += step, turn ^= 1) {
     const T* x = row_at<T>(a.rows, row);
-    const Slice<T> sl(x, a.rows.V, rank, parts);
-    Best best;
-    scan<T, ENT, TOP, false>(x, sl, c, feed, nullptr, nullptr, 0, sh, best);
-    if constexpr (TOP) best_tokens<T>(x, sl, a.top, best, sh);
-    const Stat st = row_stat<ENT>(sh, parts, c);
+    const int64_t t = a.targets[row];
+    const bool ignored = t == a.ignore, bad = !ignored && (t < 0 || t >= a.rows.V);
+    const float xt = ignored || bad ? 0.f : DT<T>::to_f(x[t]);
+    __syncthreads();
+    const Stat st = row_stat<ENT>(sh, turn, parts);
     if (rank == 0) {
-      const bool none = st.m == -INFINITY && st.s == 0.f;      // a row without any token
-      const float m = none ? 0.f : st.m, ln_s = none ? 0.f : log2f(st.s) * kLn2;
-      const float H = !ENT || none ? 0.f : ln_s - st.t / st.s / a.temp;
-      if (threadIdx.x == 0) {
-        const int64_t t = a.targets[row];
-        const bool ignored = t == a.ignore, bad = !ignored && (t < 0 || t >= a.rows.V);
-        float lp = 0.f;
-        if (bad) {
-          tc5::report(a.err, kErrToken);
-          lp = NAN;
-        } else if (!ignored) {
-          lp = none ? -INFINITY : (DT<T>::to_f(x[t]) - m) / a.temp - ln_s;
-        }
-        a.logprob[row] = lp;
+      const bool none = no_token(st, c);
+      const float r = none ? 0.f : st.r, log2_s = none ? 0.f : log2f(st.s);
+      const float H = !ENT || none ? 0.f : (log2_s - st.t / st.s) * kLn2;
+      auto logp = [&](float v) { return none ? -INFINITY : (fmaf(v, c, -r) - log2_s) * kLn2; };
+      if (lane == 0) {
+        if (bad) tc5::report(a.err, kErrToken);
+        a.logprob[row] = bad ? NAN : ignored ? 0.f : logp(xt);
         if (ENT) a.entropy[row] = ignored ? 0.f : bad ? NAN : H;
-        float4 s4 = make_float4(m, none ? 0.f : 1.f / st.s, ln_s, H);
-        if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[row] = s4;
+        if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r, none ? 0.f : 1.f / st.s, log2_s, H);
       }
       if constexpr (TOP) {
-        // the parts' sorted lists joined: a key's rank is the number of larger ones in all of them
-        uint64_t* all = sh.cand;
-        const int n = parts * a.top;
-        if (parts == 1) {
-          for (int i = threadIdx.x; i < n; i += kNT) all[i] = sh.top[i];
-        } else {
-          cg::cluster_group cl = cg::this_cluster();
-          for (int i = threadIdx.x; i < n; i += kNT) all[i] = cl.map_shared_rank(&sh, i / a.top)->top[i % a.top];
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kNT) {
-          const uint64_t k = all[i];
-          int r = 0;
-          for (int j = 0; j < n; ++j) r += all[j] > k;
-          if (k != 0 && r < a.top) {
-            const int id = key_index(k);
-            a.top_id[row * a.top + r] = id;
-            a.top_logprob[row * a.top + r] = none ? -INFINITY : (DT<T>::to_f(x[id]) - m) / a.temp - ln_s;
-          }
+        uint64_t k = sh.top[turn][lane];
+        for (int i = 1; i < parts; ++i)
+          k = warp_merge(k, cg::this_cluster().map_shared_rank(&sh, i)->top[turn][31 - lane], lane);
+        if (lane < a.top && k != 0) {
+          const int id = key_index(k);
+          a.top_id[row * a.top + lane] = id;
+          a.top_logprob[row * a.top + lane] = logp(DT<T>::to_f(x[id]));
         }
       }
     }
-    if (parts > 1) cg::this_cluster().sync();      // shared memory stays until the first CTA has read it
-    else __syncthreads();
+    if (parts > 1) cg::this_cluster().sync();
   }
 }
 
@@ -563,15 +650,15 @@ __global__ void __launch_bounds__(kNT) token_logprobs_grad_kernel(ProbGradArgs a
   float g = ignored || a.g == nullptr ? 0.f : a.g[row], ge = ignored || !ENT ? 0.f : a.g_ent[row];
   if (bad) g = NAN;
   if (st.y == 0.f) g = ge = 0.f;                    // no token in the row
-  const float c = a.inv_t * kLog2e, scale = -st.y * a.inv_t, lp0 = st.w - st.z;
+  const float c = a.inv_t * kLog2e, scale = -st.y * a.inv_t, lp0 = st.w - st.z * kLn2;
   if (g == 0.f && ge == 0.f) {                      // nothing flows into this row, whatever its logits hold
     map_row<T>(x, y, sl, [](float) { return 0.f; });
     return;
   }
   auto grad = [&](float v) {
-    const float d = ENT ? below(v, st.x) : v - st.x;
-    const float e = ex2(d * c) * scale;
-    return ENT ? e * fmaf(ge, fmaf(d, a.inv_t, lp0), g) : e * g;
+    const float d = ENT ? held(fmaf(v, c, -st.x)) : fmaf(v, c, -st.x);
+    const float e = ex2(d) * scale;
+    return ENT ? e * fmaf(ge, fmaf(d, kLn2, lp0), g) : e * g;
   };
   map_row<T>(x, y, sl, grad);
   __syncthreads();
@@ -591,126 +678,161 @@ struct DistillArgs {
   const float* values;     // [rows, K]
   const float* lse;        // [rows] or null
   float* loss;             // [rows]
-  float* stats;            // [rows, 8]: m, 1 / s, M, rest / left, z, share, -, -
+  float* stats;            // [rows, 8]: r, 1 / s, M, rest / left, z, share, -, -
   int64_t n;               // rows
   int K, parts;
+  int words;               // of a row's bits, a multiple of 4
   float temp, inv_t;
   int* err;
 };
 
-__device__ __forceinline__ double block_reduce(double v, bool is_max, double* buf) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const double w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = is_max ? fmax(v, w) : v + w;
-  }
-  __syncthreads();
-  if (lane == 0) buf[warp] = v;
-  __syncthreads();
-  v = buf[0];
-  for (int i = 1; i < kWarps; ++i) v = is_max ? fmax(v, buf[i]) : v + buf[i];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// The teacher's part of a row is in 64 bits (some K numbers beside V): 1 - sum q cancels, and a loss near 0 is a difference.
+// The teacher's part of a row, by the finishing warp, in 64 bits (some K numbers beside V): 1 - sum q cancels, and a loss near 0 is
+// a difference.  sum_k q_k (log q_k - log p_id) = own - ln 2 (c cross - mass (r + log2 s)) with what follows, so that it need not
+// wait for the student's sums.
+struct Teacher {
+  double own, cross, mass;   // sum q log q, sum q x_id, sum q
+  float z, share;            // q_k = e^(t_k / T - z) * share
+  bool empty, never;         // no token is given; a given one can never be the student's (its logit is -inf)
+};
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kNT, 2) distill_kernel(DistillArgs a) {
-  extern __shared__ __align__(16) uint8_t dynamic[];         // the feed's ring; TAIL: a bit for each element of this CTA's vectors
-  __shared__ Shared sh;
-  __shared__ int ids[kMaxK];
-  __shared__ double red[kWarps];
+__device__ Teacher teacher_of(const T* x, const int* ids, const float* values, const float* lse, int K, float temp_) {
+  const int lane = threadIdx.x & 31;
+  const double temp = temp_;
+  double z = TAIL ? *lse : -INFINITY;
+  bool some = false, never = false;
+  for (int k = lane; k < K; k += 32)
+    if (ids[k] >= 0) {
+      some |= values[k] != -INFINITY;
+      if (!TAIL) z = fmax(z, values[k] / temp);
+    }
+  some = __any_sync(0xffffffffu, some);
+  if (!TAIL) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z = fmax(z, __shfl_xor_sync(0xffffffffu, z, o));
+    z = (float)z;
+  }
+  double own = 0.0, cross = 0.0, mass = 0.0;
+  if (some)
+    for (int k = lane; k < K; k += 32)
+      if (ids[k] >= 0) {
+        const double d = values[k] / temp - z, q = exp(d);
+        const float v = DT<T>::to_f(x[ids[k]]);
+        if (q != 0.0) {
+          own += q * d;
+          if (v == -INFINITY) never = true;
+          else cross += q * v;
+        }
+        mass += q;
+      }
+  own = warp_sum64(own);
+  cross = warp_sum64(cross);
+  mass = warp_sum64(mass);
+  Teacher t = {own, cross, mass, (float)z, 1.f, !some, __any_sync(0xffffffffu, never) != 0};
+  if (!TAIL && some) {                              // normalised
+    t.share = (float)(1.0 / mass);
+    t.own = own / mass - log(mass);
+    t.cross = cross / mass;
+    t.mass = mass == mass ? 1.0 : mass;
+  }
+  return t;
+}
+
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kNT + 32, 2) distill_kernel(DistillArgs a) {
+  // the feed's ring; TAIL: for this row and the next one, a bit for each element of this CTA's vectors
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  __shared__ Sums sh;
+  __shared__ int ids[2][kMaxK];
   uint32_t* given = reinterpret_cast<uint32_t*>(dynamic + kRing);
-  const int parts = a.parts, rank = parts == 1 ? 0 : (int)(blockIdx.x % parts), tid = threadIdx.x, K = a.K;
-  const int64_t step = gridDim.x / parts;
+  const int parts = a.parts, rank = parts == 1 ? 0 : (int)(blockIdx.x % parts), K = a.K;
+  const int64_t first = blockIdx.x / parts, step = gridDim.x / parts;
   const float c = a.inv_t * kLog2e;
   constexpr int VEC = Slice<T>::VEC;
-  Feed<T> feed(a.rows, reinterpret_cast<uint4*>(dynamic), blockIdx.x / parts, step, a.n, rank, parts);
-  for (int64_t row = blockIdx.x / parts; row < a.n; row += step) {
-    const T* x = row_at<T>(a.rows, row);
-    const Slice<T> sl(x, a.rows.V, rank, parts);
+  if (threadIdx.x < kNT) {
+    Feed<T> feed(a.rows, reinterpret_cast<uint4*>(dynamic), first, step, a.n, rank, parts);
+    __syncthreads();
+    int turn = 0;
+    for (int64_t row = first; row < a.n; row += step, turn ^= 1) {
+      const T* x = row_at<T>(a.rows, row);
+      const Slice<T> sl(x, a.rows.V, rank, parts);
+      Best unused;
+      scan<T, false, false, TAIL>(x, sl, c, feed, given + turn * a.words, ids[turn], K, sh.warp[turn], unused);
+      __syncthreads();
+      meet(parts);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  // a row's tokens, and their bits; true where one lies outside of the vocabulary
+  auto open = [&](int64_t row, int turn) {
     bool bad = false;
-    for (int k = tid; k < K; k += kNT) {
+    for (int k = lane; k < K; k += 32) {
       const int64_t id = a.ids[row * K + k];
       bad |= id >= a.rows.V;
-      ids[k] = id < 0 || id >= a.rows.V ? -1 : (int)id;
+      ids[turn][k] = id < 0 || id >= a.rows.V ? -1 : (int)id;
     }
     if constexpr (TAIL) {
-      for (int i = tid; i < ((sl.v1 - sl.v0) * VEC + 31) / 32; i += kNT) given[i] = 0;
-    }
-    bad = __syncthreads_or(bad);
-    if constexpr (TAIL) {
-      for (int k = tid; k < K; k += kNT) {
-        const int pos = ids[k] - sl.head - sl.v0 * VEC;
-        if (ids[k] >= 0 && pos >= 0 && pos < (sl.v1 - sl.v0) * VEC) atomicOr(&given[pos >> 5], 1u << (pos & 31));
-      }
-      __syncthreads();
-    }
-    Best unused;
-    scan<T, false, false, TAIL>(x, sl, c, feed, given, ids, K, sh, unused);
-    const Stat st = row_stat<false>(sh, parts, c);
-    if (rank == 0) {
-      const bool none = st.m == -INFINITY && st.s == 0.f;
-      const float m = none ? 0.f : st.m, ln_s = none ? 0.f : log2f(st.s) * kLn2;
-      const double temp = a.temp;
-      double z = TAIL ? a.lse[row] : -INFINITY, share = 1.0;   // q_k = e^(t_k / T - z) * share
-      if constexpr (!TAIL) {
-        for (int k = tid; k < K; k += kNT)
-          if (ids[k] >= 0) z = fmax(z, a.values[row * K + k] / temp);
-        z = (float)block_reduce(z, true, red);
-      }
-      double sum = 0.0;
-      bool some = false;
-      for (int k = tid; k < K; k += kNT)
-        if (ids[k] >= 0) {
-          const float t = a.values[row * K + k];
-          some |= t != -INFINITY;
-          if (TAIL || z != -INFINITY) sum += exp(t / temp - z);
-        }
-      sum = block_reduce(sum, false, red);
-      const bool empty = !__syncthreads_or(some);              // no token given
-      const double log_share = TAIL || empty ? 0.0 : -log(sum);
-      if (!TAIL && !empty) share = 1.0 / sum;
-      double part = 0.0;
-      if (!empty)
-        for (int k = tid; k < K; k += kNT) {
-          if (ids[k] < 0) continue;
-          const double d = a.values[row * K + k] / temp - z, q = exp(d) * share;
-          const float lp = (DT<T>::to_f(x[ids[k]]) - m) / a.temp - ln_s;
-          if (q != 0.0) part += q * (d + log_share - lp);
-        }
-      part = block_reduce(part, false, red);
-      if (tid == 0) {
-        double mass = sum * share, rest = 0.0;
-        float ratio = 0.f;
-        if constexpr (TAIL) {
-          rest = fmax(1.0 - mass, 0.0);
-          const float left = none ? 0.f : st.t / st.s;
-          if (rest > 0.0 && left > 0.f) {
-            ratio = (float)rest / left;
-            part += rest * (log(rest) - (double)(log2f(left) * kLn2));
-          } else {
-            rest = 0.0;                                        // the student has no other token: the term is left out
-          }
-        }
-        if (empty) {
-          part = mass = rest = 0.0;
-          ratio = 0.f;
-        }
-        if (bad) {
-          tc5::report(a.err, kErrToken);
-          part = mass = NAN;
-        }
-        a.loss[row] = (float)(part * temp * temp);
-        if (a.stats != nullptr) {
-          float4* s4 = reinterpret_cast<float4*>(a.stats) + 2 * row;
-          s4[0] = make_float4(m, none ? 0.f : 1.f / st.s, (float)(mass + rest), ratio);
-          s4[1] = make_float4((float)z, (float)share, 0.f, 0.f);
-        }
+      const Slice<T> sl(row_at<T>(a.rows, row), a.rows.V, rank, parts);
+      uint32_t* bits = given + turn * a.words;
+      for (int i = lane; i < a.words / 4; i += 32) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+      for (int k = lane; k < K; k += 32) {
+        const int pos = ids[turn][k] - sl.head - sl.v0 * VEC;
+        if (ids[turn][k] >= 0 && pos >= 0 && pos < (sl.v1 - sl.v0) * VEC) atomicOr(&bits[pos >> 5], 1u << (pos & 31));
       }
     }
+    __syncwarp();
+    return __any_sync(0xffffffffu, bad) != 0;
+  };
+  bool bad = open(first, 0);
+  __syncthreads();
+  int turn = 0;
+  for (int64_t row = first; row < a.n; row += step, turn ^= 1) {
+    const T* x = row_at<T>(a.rows, row);
+    const Teacher te = teacher_of<T, TAIL>(x, ids[turn], a.values + row * K, TAIL ? a.lse + row : nullptr, K, a.temp);
+    const bool bad_next = row + step < a.n && open(row + step, turn ^ 1);
+    __syncthreads();
+    const Stat st = row_stat<false>(sh, turn, parts);
+    if (rank == 0 && lane == 0) {
+      const bool none = no_token(st, c);
+      const float r = none ? 0.f : st.r;
+      const double ln2 = 0.6931471805599453, log2_s = none ? 0.0 : log2((double)st.s);
+      double mass = te.mass, rest = 0.0;
+      double loss = te.never ? INFINITY : te.own - ln2 * (c * te.cross - te.mass * (r + log2_s));
+      float ratio = 0.f;
+      if constexpr (TAIL) {
+        rest = fmax(1.0 - mass, 0.0);
+        const float left = none ? 0.f : st.t / st.s;
+        if (rest > 0.0 && left > 0.f) {
+          ratio = (float)rest / left;
+          loss += rest * (log(rest) - (double)(log2f(left) * kLn2));
+        } else {
+          rest = 0.0;                                        // the student has no other token: the term is left out
+        }
+      }
+      if (te.empty) {
+        loss = mass = rest = 0.0;
+        ratio = 0.f;
+      }
+      if (bad) {
+        tc5::report(a.err, kErrToken);
+        loss = mass = NAN;
+      }
+      a.loss[row] = (float)(loss * a.temp * a.temp);
+      if (a.stats != nullptr) {
+        float4* s4 = reinterpret_cast<float4*>(a.stats) + 2 * row;
+        s4[0] = make_float4(r, none ? 0.f : 1.f / st.s, (float)(mass + rest), ratio);
+        s4[1] = make_float4(te.z, te.share, 0.f, 0.f);
+      }
+    }
+    bad = bad_next;
     if (parts > 1) cg::this_cluster().sync();
-    else __syncthreads();
   }
 }
 
@@ -748,7 +870,7 @@ __global__ void __launch_bounds__(kNT) distill_grad_kernel(DistillGradArgs a) {
     q[k] = ok ? ex2((float)(a.values[row * K + k] / (double)a.temp - z) * kLog2e) * share : 0.f;
   }
   const float other = g * st.y * (st.z - st.w), own = g * st.y * st.z;
-  map_row<T>(x, y, sl, [&](float v) { return ex2((v - st.x) * c) * other; });
+  map_row<T>(x, y, sl, [&](float v) { return ex2(fmaf(v, c, -st.x)) * other; });
   __syncthreads();
   // given tokens once more: the first of those with the same index writes for all of them
   for (int k = threadIdx.x; k < K; k += kNT) {
@@ -761,7 +883,7 @@ __global__ void __launch_bounds__(kNT) distill_grad_kernel(DistillGradArgs a) {
         first &= j >= k;
         sum += q[j];
       }
-    if (first) y[id] = DT<T>::from_f(fmaf(-g, sum, ex2((DT<T>::to_f(x[id]) - st.x) * c) * own));
+    if (first) y[id] = DT<T>::from_f(fmaf(-g, sum, ex2(fmaf(DT<T>::to_f(x[id]), c, -st.x)) * own));
   }
 }
 
@@ -784,7 +906,7 @@ int launch_rows(void (*kern)(Args), const Args& a, size_t smem, cudaStream_t s) 
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return (int)e;
   cfg.gridDim = dim3((unsigned)(a.parts > 1 || a.n < 2 * sms ? a.n * a.parts : 2 * sms));
-  cfg.blockDim = dim3(kNT);
+  cfg.blockDim = dim3(kNT + 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -854,22 +976,22 @@ IPEX_API int ipex_token_logprobs_grad(const void* logits, int64_t s0, int64_t s1
 }
 
 // ids / values [rows, K]: the teacher's tokens (below 0: none) and their logits, K up to 1024; lse [rows]: logsumexp of the
-// teacher's logits / temp, or null; loss [rows]; stats [rows, 8] (16-byte aligned) or null.  V up to 1048576 with lse.
+// teacher's logits / temp, or null; loss [rows]; stats [rows, 8] (16-byte aligned) or null.  V up to 524288 with lse.
 IPEX_API int ipex_distill(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* ids, const float* values,
                           const float* lse, float* loss, float* stats, int64_t rows, int V, int K, float temp, int dtype, int* err,
                           void* stream) {
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
-      ids == nullptr || values == nullptr || loss == nullptr || (lse != nullptr && V > (1 << 20)) || (reinterpret_cast<uintptr_t>(stats) & 15))
+      ids == nullptr || values == nullptr || loss == nullptr || (lse != nullptr && V > kMaxTailV) || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
-  DistillArgs a = {{logits, s0, s1, n1, V}, ids, values, lse, loss, stats, rows, K, 0, temp, 1.f / temp, err};
+  DistillArgs a = {{logits, s0, s1, n1, V}, ids, values, lse, loss, stats, rows, K, 0, 0, temp, 1.f / temp, err};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
   return by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
     static SmemLimit limit[2];
-    const size_t bits = lse != nullptr ? ((size_t)V / a.parts + 64) / 32 * 4 + 16 : 0;
+    if (lse != nullptr) a.words = (V / a.parts + 64 + 127) / 128 * 4;
     auto kern = lse != nullptr ? distill_kernel<T, true> : distill_kernel<T, false>;
-    const cudaError_t e = limit[lse != nullptr]((const void*)kern, kRing + (lse != nullptr ? (1 << 20) / 8 + 64 : 0));
-    return e != cudaSuccess ? (int)e : launch_rows<DistillArgs>(kern, a, kRing + bits, (cudaStream_t)stream);
+    const cudaError_t e = limit[lse != nullptr]((const void*)kern, kRing + (lse != nullptr ? kMaxBits : 0));
+    return e != cudaSuccess ? (int)e : launch_rows<DistillArgs>(kern, a, kRing + a.words * 8, (cudaStream_t)stream);
   });
 }
 

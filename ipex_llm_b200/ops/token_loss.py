@@ -21,8 +21,9 @@ from .cuda_ops import error_flag
 
 MAX_TOP = 32             # alternatives of a row
 MAX_TEACHER = 1024       # tokens of a teacher's row
-MAX_TAIL_VOCAB = 1 << 20
+MAX_TAIL_VOCAB = 1 << 19
 IGNORE = -100
+_NO_TOKEN = -2.0 ** 127   # a row whose largest logit is not above this has no token
 
 
 class TokenLogprobs(NamedTuple):
@@ -134,7 +135,7 @@ def _hidden_to_zero(logp: torch.Tensor) -> torch.Tensor:
 def _token_logprobs_plain(logits, targets, temperature, entropy, top, ignore):
     y = _wide(logits) / temperature
     real = targets != ignore
-    none = (logits == -math.inf).all(dim=-1)                       # rows without any token
+    none = logits.detach().amax(dim=-1) <= _NO_TOKEN                # rows without any token
     logp = torch.log_softmax(y.masked_fill(none.unsqueeze(-1), 0.0), dim=-1)
     lp = logp.gather(-1, targets.clamp(min=0).unsqueeze(-1)).squeeze(-1)
     lp = torch.where(real, torch.where(none, -math.inf, lp), 0.0)
@@ -156,7 +157,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: flo
     ``entropy``: that of each row as well; ``top`` (up to 32): the best tokens of each row with their log probabilities.  All
     results but the ids are 32-bit (64 for 64-bit logits on the CPU).  Rows whose target is ``ignore_index`` give a log
     probability and an entropy of 0 and no gradient, whatever their logits hold, and their alternatives all the same.  A logit
-    of -inf hides its token; a row of nothing else gives a log probability of -inf, an entropy of 0 and no gradient.  A target
+    of -inf hides its token, as the lowest value of bf16 or 32 bits does; a row of nothing else gives a log probability of -inf,
+    an entropy of 0 and no gradient.  A target
     outside of the vocabulary raises on the CPU; on the GPU its results are NaN, and ``cuda_ops.check_error_flag`` reports 61.
 
     16-bit and 32-bit logits; the gradient has the logits' type.
@@ -220,7 +222,7 @@ class _Distill(torch.autograd.Function):
 
 def _distill_plain(logits, ids, values, lse, temperature):
     y = _wide(logits) / temperature
-    none = (logits == -math.inf).all(dim=-1, keepdim=True)
+    none = logits.detach().amax(dim=-1, keepdim=True) <= _NO_TOKEN
     logp = torch.log_softmax(y.masked_fill(none, 0.0), dim=-1)
     given = ids >= 0
     at = ids.clamp(min=0)
@@ -228,7 +230,7 @@ def _distill_plain(logits, ids, values, lse, temperature):
     empty = ~(t > -math.inf).any(dim=-1, keepdim=True)             # rows without a teacher's token
     logq = t - (torch.logsumexp(t.masked_fill(empty, 0.0), dim=-1, keepdim=True) if lse is None else lse.to(y.dtype).unsqueeze(-1))
     q = torch.exp(logq)
-    own = logp.gather(-1, at)
+    own = logp.masked_fill(none, -math.inf).gather(-1, at)
     loss = torch.where(q != 0, q * (logq - torch.where(q != 0, own, 0.0)), 0.0).sum(dim=-1, keepdim=True)
     if lse is not None:
         rest = (1.0 - q.sum(dim=-1, keepdim=True)).clamp(min=0.0)
