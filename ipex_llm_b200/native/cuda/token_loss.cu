@@ -95,7 +95,10 @@ struct Rows {
 
 template <typename T>
 __device__ __forceinline__ const T* row_at(const Rows& r, int64_t row) {
-  return reinterpret_cast<const T*>(r.x) + row / r.n1 * r.s0 + row % r.n1 * r.s1;
+  const T* x = reinterpret_cast<const T*>(r.x);
+  if (row < r.n1) return x + row * r.s1;           // as all rows are where one stride goes through them (see rows_of)
+  const uint32_t outer = (uint32_t)row / (uint32_t)r.n1;
+  return x + outer * r.s0 + ((uint32_t)row - outer * (uint32_t)r.n1) * r.s1;
 }
 
 // A row [V] of any alignment: elements in front of the first 16-byte boundary, vectors, what is left.
@@ -109,10 +112,11 @@ struct Slice {
   __device__ Slice(const T* x, int V_, int rank, int parts) : V(V_) {
     const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
     head = off ? min(VEC - off, V) : 0;
-    nvec = (V - head) / VEC;
+    nvec = (unsigned)(V - head) / VEC;
     tail = V - head - nvec * VEC;
-    v0 = (int)((int64_t)nvec * rank / parts);
-    v1 = (int)((int64_t)nvec * (rank + 1) / parts);
+    const int by = __ffs(parts) - 1;                 // parts is a power of two
+    v0 = (int)((int64_t)nvec * rank >> by);
+    v1 = (int)((int64_t)nvec * (rank + 1) >> by);
     h = rank == 0 ? head : 0;
     t = rank == parts - 1 ? tail : 0;
   }
@@ -121,12 +125,25 @@ struct Slice {
   }
 };
 
+// A vector's elements.  bf16 by shifts: a conversion would go through the unit that the exponentials need.
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& w, float* f) {
-  const T* p = reinterpret_cast<const T*>(&w);
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < 16 / (int)sizeof(T); ++i) f[i] = DT<T>::to_f(p[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, float>::value) {
+      f[i] = __uint_as_float(v[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      f[2 * i] = __uint_as_float(v[i] << 16);
+      f[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    } else {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
+  }
 }
+
 // Larger keys come first: by value (NaN above all), then by the lower index.  No element has key 0.
 __device__ __forceinline__ uint64_t order_key(float v, int idx) {
   const uint32_t b = v != v ? 0x7FFFFFFFu : __float_as_uint(v == 0.f ? 0.f : v);   // -0 and 0 are equal
@@ -640,10 +657,10 @@ struct ProbGradArgs {
 
 template <typename T, bool ENT>
 __global__ void __launch_bounds__(kNT) token_logprobs_grad_kernel(ProbGradArgs a) {
-  const int64_t row = blockIdx.x / a.parts;
+  const int64_t row = blockIdx.x >> __ffs(a.parts) - 1;
   const T* x = row_at<T>(a.rows, row);
   T* y = reinterpret_cast<T*>(a.dx) + row * a.rows.V;
-  const Slice<T> sl(x, a.rows.V, (int)(blockIdx.x % a.parts), a.parts);
+  const Slice<T> sl(x, a.rows.V, (int)(blockIdx.x & a.parts - 1), a.parts);
   const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
   const int64_t t = a.targets[row];
   const bool ignored = t == a.ignore, bad = !ignored && (t < 0 || t >= a.rows.V);
@@ -851,11 +868,11 @@ template <typename T>
 __global__ void __launch_bounds__(kNT) distill_grad_kernel(DistillGradArgs a) {
   __shared__ int ids[kMaxK];
   __shared__ float q[kMaxK];
-  const int64_t row = blockIdx.x / a.parts;
+  const int64_t row = blockIdx.x >> __ffs(a.parts) - 1;
   const int K = a.K;
   const T* x = row_at<T>(a.rows, row);
   T* y = reinterpret_cast<T*>(a.dx) + row * a.rows.V;
-  const Slice<T> sl(x, a.rows.V, (int)(blockIdx.x % a.parts), a.parts);
+  const Slice<T> sl(x, a.rows.V, (int)(blockIdx.x & a.parts - 1), a.parts);
   const float4 st = reinterpret_cast<const float4*>(a.stats)[2 * row];
   const float z = a.stats[8 * row + 4], share = a.stats[8 * row + 5];
   const float g = a.g[row] * a.temp, c = a.inv_t * kLog2e;
@@ -925,6 +942,11 @@ bool rows_ok(const void* x, int64_t s0, int64_t s1, int64_t n1, int64_t rows, in
 
 bool temp_ok(float t) { return t >= 1e-6f && t <= 1e6f; }
 
+// Rows that follow one another at one stride count as one run of them.
+Rows rows_of(const void* x, int64_t s0, int64_t s1, int64_t n1, int64_t rows, int V) {
+  return {x, s0, s1, s0 == s1 * n1 || n1 > rows ? rows : n1, V};
+}
+
 template <typename F>
 int by_type(int dtype, F f) {
   if (dtype == DT_F16) return f((__half*)nullptr);
@@ -946,7 +968,7 @@ IPEX_API int ipex_token_logprobs(const void* logits, int64_t s0, int64_t s1, int
       targets == nullptr || logprob == nullptr || (top > 0 && (top_logprob == nullptr || top_id == nullptr)) ||
       (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
-  ProbArgs a = {{logits, s0, s1, n1, V}, targets, logprob, entropy, stats, top_logprob, top_id, top, 0, ignore, rows, temp, 1.f / temp, err};
+  ProbArgs a = {rows_of(logits, s0, s1, n1, rows, V), targets, logprob, entropy, stats, top_logprob, top_id, top, 0, ignore, rows, temp, 1.f / temp, err};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
   return by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
@@ -965,7 +987,7 @@ IPEX_API int ipex_token_logprobs_grad(const void* logits, int64_t s0, int64_t s1
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || !temp_ok(temp) ||
       targets == nullptr || dlogits == nullptr || stats == nullptr || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
-  ProbGradArgs a = {{logits, s0, s1, n1, V}, targets, stats, g, g_entropy, dlogits, ignore, 1.f / temp, 0};
+  ProbGradArgs a = {rows_of(logits, s0, s1, n1, rows, V), targets, stats, g, g_entropy, dlogits, ignore, 1.f / temp, 0};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
   return by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
@@ -983,7 +1005,7 @@ IPEX_API int ipex_distill(const void* logits, int64_t s0, int64_t s1, int64_t n1
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
       ids == nullptr || values == nullptr || loss == nullptr || (lse != nullptr && V > kMaxTailV) || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
-  DistillArgs a = {{logits, s0, s1, n1, V}, ids, values, lse, loss, stats, rows, K, 0, 0, temp, 1.f / temp, err};
+  DistillArgs a = {rows_of(logits, s0, s1, n1, rows, V), ids, values, lse, loss, stats, rows, K, 0, 0, temp, 1.f / temp, err};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
   return by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
@@ -1001,7 +1023,7 @@ IPEX_API int ipex_distill_grad(const void* logits, int64_t s0, int64_t s1, int64
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
       ids == nullptr || values == nullptr || dlogits == nullptr || stats == nullptr || g == nullptr || (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
-  DistillGradArgs a = {{logits, s0, s1, n1, V}, ids, values, stats, g, dlogits, K, 0, temp, 1.f / temp};
+  DistillGradArgs a = {rows_of(logits, s0, s1, n1, rows, V), ids, values, stats, g, dlogits, K, 0, temp, 1.f / temp};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
   return by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
