@@ -9,15 +9,17 @@
 // All of them are bound by memory: forward reads a row once, backward reads it once more and writes it once.  A row belongs
 // to one CTA (many rows; the CTAs stay and take the next row) or to a cluster of up to eight (few rows).  Each thread copies its
 // own four 16-byte vectors at a time to shared memory, asynchronously and two batches ahead, into the next row while a row's
-// parts are joined.  Fifteen warps read; a sixteenth does what a row has beside its sums (its target, the teacher's tokens, the
-// results), on this row while the others read it and on its sums while they read the next one: in their way, those latencies
-// took half of the time (2048 rows of 32000 in bf16: 58 us).
+// parts are joined.  Seven warps of a CTA read; an eighth does what a row has beside its sums (its target, the teacher's tokens,
+// the results), on this row while the others read it and on its sums while they read the next one: in their way, those latencies
+// took half of the time.  Four such CTAs to an SM: what is left of a row's latencies (the joining of its sums) hides behind the
+// other CTAs' rows (2048 rows of 32000 in bf16: 38 us, 3.5 TB/s; two CTAs of sixteen warps 47 us; the divergence 37 against
+// 52 us).  Backward is a plain pass of 224 threads to a row, four vectors in flight (43 us for these rows, 6.1 TB/s).
 // A thread folds the maximum of a batch into its own and rescales its sums once for all of it, so that an element costs one
 // exponential (0.73 of what the special function units do at the rate of memory, for 16-bit logits).
 // y is one fma: the rounding of r, common to a row, takes part everywhere alike and so cancels, as long as r is the same number
 // everywhere (it goes to the backward pass, and rescaling goes by differences of it).
 //
-// Statistics are 32-bit, 250 to 500 elements to a thread's sum and a tree above that; exponentials by ex2.approx (2 ulp).
+// Statistics are 32-bit, 150 to 600 elements to a thread's sum and a tree above that; exponentials by ex2.approx (2 ulp).
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -29,7 +31,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 15;        // that read rows
+constexpr int kWarps = 7;         // that read rows
+constexpr int kCtas = 4;          // to an SM
 constexpr int kNT = 32 * kWarps;
 constexpr int kU = 4;             // 16-byte requests of a thread in flight
 constexpr int kMaxTop = 32;
@@ -369,7 +372,7 @@ __device__ __forceinline__ Stat join_warps(const Stat* sums) {
   Stat st = {-INFINITY, 0.f, 0.f};
   if (lane < kWarps) st = sums[lane];
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = 4; o > 0; o >>= 1) {
     Stat other = {__shfl_xor_sync(0xffffffffu, st.r, o), __shfl_xor_sync(0xffffffffu, st.s, o),
                   __shfl_xor_sync(0xffffffffu, st.t, o)};
     st = lane & o ? join<ENT>(other, st) : join<ENT>(st, other);
@@ -418,7 +421,7 @@ __device__ uint64_t largest32(uint64_t k, Shared& sh) {
   sync_readers();
   sh.best[threadIdx.x] = k;
 #pragma unroll
-  for (int n = 8; n > 0; n /= 2) {
+  for (int n = 4; n > 0; n /= 2) {
     sync_readers();
     if (warp < n && warp + n < kWarps) {
       k = warp_merge(k, sh.best[(warp + n) * 32 + 31 - lane], lane);
@@ -551,7 +554,7 @@ struct ProbArgs {
 };
 
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kNT + 32, 2) token_logprobs_kernel(ProbArgs a) {
+__global__ void __launch_bounds__(kNT + 32, kCtas) token_logprobs_kernel(ProbArgs a) {
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Shared sh;
   const int parts = a.parts, rank = parts == 1 ? 0 : (int)(blockIdx.x % parts);
@@ -618,13 +621,13 @@ __device__ __forceinline__ void map_row(const T* x, T* y, const Slice<T>& sl, F 
   }
   const uint4* xv = reinterpret_cast<const uint4*>(x + sl.head);
   const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-  for (int base = sl.v0 + tid; base < sl.v1; base += kNT * 2) {
-    uint4 w[2];
+  for (int base = sl.v0 + tid; base < sl.v1; base += kNT * kU) {
+    uint4 w[kU];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < kU; ++u)
       if (base + u * kNT < sl.v1) w[u] = ldg_nc_v4(xv + base + u * kNT);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kU; ++u) {
       const int v = base + u * kNT;
       if (v >= sl.v1) break;
       float e[VEC];
@@ -761,7 +764,7 @@ __device__ Teacher teacher_of(const T* x, const int* ids, const float* values, c
 }
 
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kNT + 32, 2) distill_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kNT + 32, kCtas) distill_kernel(DistillArgs a) {
   // the feed's ring; TAIL: for this row and the next one, a bit for each element of this CTA's vectors
   extern __shared__ __align__(16) uint8_t dynamic[];
   __shared__ Sums sh;
@@ -914,15 +917,18 @@ int parts_of(int64_t rows, int V, int elem) {
   return parts;
 }
 
-// CTAs that stay, two to an SM, or a cluster for each row.
+// CTAs that stay, kCtas to an SM or what its 227 KB of shared memory hold (the bits of a long row's tail take some), or a cluster
+// for each row.
 template <typename Args>
-int launch_rows(void (*kern)(Args), const Args& a, size_t smem, cudaStream_t s) {
+int launch_rows(void (*kern)(Args), const Args& a, size_t smem, size_t fixed, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return (int)e;
-  cfg.gridDim = dim3((unsigned)(a.parts > 1 || a.n < 2 * sms ? a.n * a.parts : 2 * sms));
+  const size_t fit = (227 << 10) / (smem + fixed + 1024);
+  const int64_t stay = (int64_t)(fit < kCtas ? fit : kCtas) * sms;
+  cfg.gridDim = dim3((unsigned)(a.parts > 1 || a.n < stay ? a.n * a.parts : stay));
   cfg.blockDim = dim3(kNT + 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -976,7 +982,7 @@ IPEX_API int ipex_token_logprobs(const void* logits, int64_t s0, int64_t s1, int
                                    : (top ? token_logprobs_kernel<T, false, true> : token_logprobs_kernel<T, false, false>);
     static SmemLimit limit[4];
     const cudaError_t e = limit[(entropy != nullptr) * 2 + (top > 0)]((const void*)kern, kRing);
-    return e != cudaSuccess ? (int)e : launch_rows<ProbArgs>(kern, a, kRing, (cudaStream_t)stream);
+    return e != cudaSuccess ? (int)e : launch_rows<ProbArgs>(kern, a, kRing, sizeof(Shared), (cudaStream_t)stream);
   });
 }
 
@@ -1013,7 +1019,8 @@ IPEX_API int ipex_distill(const void* logits, int64_t s0, int64_t s1, int64_t n1
     if (lse != nullptr) a.words = (V / a.parts + 64 + 127) / 128 * 4;
     auto kern = lse != nullptr ? distill_kernel<T, true> : distill_kernel<T, false>;
     const cudaError_t e = limit[lse != nullptr]((const void*)kern, kRing + (lse != nullptr ? kMaxBits : 0));
-    return e != cudaSuccess ? (int)e : launch_rows<DistillArgs>(kern, a, kRing + a.words * 8, (cudaStream_t)stream);
+    return e != cudaSuccess ? (int)e
+                            : launch_rows<DistillArgs>(kern, a, kRing + a.words * 8, sizeof(Sums) + 8 * kMaxK, (cudaStream_t)stream);
   });
 }
 
