@@ -12,6 +12,8 @@ import math
 
 import torch
 
+from ..ops.token_loss import token_logprobs
+
 
 class BigDLPPL:
     def __init__(self, model_path=None, device="cuda", model=None, **model_kwargs):
@@ -31,6 +33,14 @@ class BigDLPPL:
         ids = input_ids.to(self.device)
         if ids.dim() == 1:
             ids = ids.unsqueeze(0)
+        logits = self._logits(ids)
+        logp = torch.log_softmax(logits[:, :-1].float(), dim=-1)
+        tgt = ids[:, 1:]
+        tok = logp.gather(-1, tgt.unsqueeze(-1)).squeeze(-1)
+        tok = tok[:, target_from:]
+        return float(-tok.sum()), int(tok.numel())
+
+    def _logits(self, ids: torch.Tensor) -> torch.Tensor:
         import os
         prev = os.environ.get("IPEX_LLM_LAST_LM_HEAD")
         os.environ["IPEX_LLM_LAST_LM_HEAD"] = "0"          # every position's logits are needed
@@ -44,11 +54,15 @@ class BigDLPPL:
         logits = out.logits
         if logits.shape[1] != ids.shape[1]:
             raise RuntimeError("the model returned logits for the last position only; perplexity needs all of them")
-        logp = torch.log_softmax(logits[:, :-1].float(), dim=-1)
-        tgt = ids[:, 1:]
-        tok = logp.gather(-1, tgt.unsqueeze(-1)).squeeze(-1)
-        tok = tok[:, target_from:]
-        return float(-tok.sum()), int(tok.numel())
+        return logits
+
+    @torch.no_grad()
+    def token_scores(self, input_ids: torch.Tensor, temperature: float = 1.0, entropy: bool = False, top: int = 0):
+        """Each token's log probability given its prefix, ``[batch, tokens - 1]`` in fp32, with the entropy of its distribution and
+        the ``top`` best alternatives where asked for (``ops.token_loss.TokenLogprobs``); no copy of the logits is made."""
+        ids = input_ids.to(self.device)
+        ids = ids.unsqueeze(0) if ids.dim() == 1 else ids
+        return token_logprobs(self._logits(ids)[:, :-1], ids[:, 1:], temperature, entropy, top)
 
     def perplexity_hf(self, token_stream: torch.Tensor, seq_len: int = 512, stride: int = None) -> float:
         """Perplexity of one long token stream ``[N]`` with windows of ``seq_len`` advanced by ``stride``."""

@@ -18,6 +18,7 @@ from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
 
 MAX_DIM = 128
+MAX_HEADS = 65535       # of queries and keys together
 MAX_TOKENS = 1 << 22
 _TILE = 128
 
@@ -164,6 +165,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
         invalidInputError(False, f"attention: {q.dtype} is not supported on the GPU (float16 and bfloat16 are)")
     if D > MAX_DIM or D % 8:
         invalidInputError(False, f"attention: heads of {D} are not supported (multiples of 8 up to {MAX_DIM} are)")
+    if Hq + Hkv > MAX_HEADS:
+        invalidInputError(False, f"attention: {Hq} and {Hkv} heads are too many ({MAX_HEADS} together are not)")
     if B > 65535 or Sq > MAX_TOKENS or Skv > MAX_TOKENS:
         invalidInputError(False, f"attention: {B} sequences of {Sq} queries and {Skv} keys are too many (65535 of {MAX_TOKENS} are not)")
     if q.numel() == 0 or k.numel() == 0:

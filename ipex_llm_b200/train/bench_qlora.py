@@ -8,6 +8,7 @@ directly on the device with random weights, LoRA r=8 alpha=16 dropout 0.05 on q/
 sequence 512, micro-batch 4 per GPU, random token ids, causal-LM loss.  One step = forward + backward + fused
 reduce-scatter/AdamW/all-gather kernel.  Timed with CUDA events around K steps after W warm-ups, max over ranks;
 inputs come from pinned host memory every step and the loss is read back, as a training loop does.
+``--fused-attention`` and ``--fused-loss`` swap in the attention with a gradient and the loss straight from the logits.
 ``--optimizer torch`` swaps in ``dist.all_reduce`` + ``torch.optim.AdamW`` (the library baseline).
 """
 from __future__ import annotations
@@ -41,6 +42,8 @@ def run(argv=None, timed=None):
     ap.add_argument("--layers", type=int, default=0)
     ap.add_argument("--optimizer", default="fused", choices=["fused", "torch"])
     ap.add_argument("--no-checkpointing", action="store_true")
+    ap.add_argument("--fused-attention", action="store_true")
+    ap.add_argument("--fused-loss", action="store_true")
     a = ap.parse_args(argv)
     rank, world = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1))
     local = int(os.environ.get("LOCAL_RANK", rank))
@@ -52,6 +55,7 @@ def run(argv=None, timed=None):
     from transformers import LlamaConfig
     from ..parallel.dp import FusedLoraAdamW
     from ..transformers import AutoModelForCausalLM
+    from .losses import causal_lm_loss
     from ..transformers.qlora import LoraConfig, cast_lora_weight, get_peft_model, prepare_model_for_kbit_training
     arch = dict(ARCH[a.model])
     if a.layers:
@@ -59,7 +63,8 @@ def run(argv=None, timed=None):
     cfg = LlamaConfig(tie_word_embeddings=False, **arch)
     model = AutoModelForCausalLM.from_config(cfg, load_in_low_bit="nf4", torch_dtype=torch.bfloat16, device=dev,
                                              modules_to_not_convert=["lm_head"], optimize_model=False, seed=0)
-    model = prepare_model_for_kbit_training(model, use_gradient_checkpointing=not a.no_checkpointing)
+    model = prepare_model_for_kbit_training(model, use_gradient_checkpointing=not a.no_checkpointing,
+                                            use_fused_attention=a.fused_attention)
     torch.manual_seed(0)
     pm = get_peft_model(model, LoraConfig(r=8, lora_alpha=16, lora_dropout=0.05, training_mode="qlora",
                                           target_modules=["q_proj", "k_proj", "v_proj", "o_proj", "gate_proj",
@@ -79,7 +84,7 @@ def run(argv=None, timed=None):
     def step(i):
         ids = host[i].to(dev, non_blocking=True)
         with torch.autocast("cuda", dtype=torch.bfloat16):
-            loss = pm(input_ids=ids, labels=ids).loss
+            loss = causal_lm_loss(pm(input_ids=ids).logits, ids) if a.fused_loss else pm(input_ids=ids, labels=ids).loss
         loss.backward()
         if a.optimizer == "torch" and world > 1:
             for p in params:
@@ -122,6 +127,8 @@ def run(argv=None, timed=None):
                           "micro_batch_per_gpu": a.micro_batch, "trainable_params": n_train,
                           "optimizer": "fused reduce-scatter + AdamW + all-gather kernel" if a.optimizer == "fused"
                           else "NCCL all_reduce + torch.optim.AdamW", "base": "nf4", "compute": "bf16",
+                          "attention": "fused" if a.fused_attention else "library",
+                          "loss": "fused" if a.fused_loss else "library",
                           "gradient_checkpointing": not a.no_checkpointing, "last_loss": round(last, 4),
                           "h2d_bytes_per_step": a.micro_batch * a.seq * 8, "d2h_bytes_per_step": 4})
     if world > 1:

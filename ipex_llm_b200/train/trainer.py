@@ -19,6 +19,9 @@ import torch.distributed as dist
 
 from ..parallel.dp import FusedLoraAdamW, PagedAdamW
 from ..utils.common import invalidInputError
+from .losses import TeacherTokens, causal_lm_loss, distill_lm_loss
+
+TEACHER_COLUMNS = TeacherTokens._fields
 
 
 class TrainerCallback:
@@ -108,8 +111,27 @@ class Trainer:
 
     def compute_loss(self, model, batch):
         batch = {k: v.to(self.device, non_blocking=True) for k, v in batch.items()}
+        if getattr(self.args, "fused_loss", False):
+            return self._fused_loss(model, batch)
         out = model(**batch)
         return out.loss if hasattr(out, "loss") and out.loss is not None else out[0]
+
+    def _fused_loss(self, model, batch):
+        """The loss by ``causal_lm_loss``; with a teacher's tokens in the batch, ``distill_weight`` of it by ``distill_lm_loss``."""
+        teacher = {k: batch.pop(k) for k in TEACHER_COLUMNS if k in batch}
+        invalidInputError("labels" in batch, "fused_loss: the batch has no labels")
+        labels = batch.pop("labels")
+        out = model(**batch)
+        logits = out.logits if hasattr(out, "logits") else out[0]
+        w = float(getattr(self.args, "distill_weight", 0.5)) if teacher else 0.0
+        invalidInputError(0.0 <= w <= 1.0, f"distill_weight should lie between 0 and 1, got {w}")
+        loss = causal_lm_loss(logits, labels) * (1.0 - w) if w < 1.0 else 0.0
+        if w > 0.0:
+            invalidInputError("teacher_ids" in teacher and "teacher_logits" in teacher,
+                              "a teacher's tokens need the columns teacher_ids and teacher_logits")
+            loss = loss + w * distill_lm_loss(logits, labels, temperature=float(getattr(self.args, "distill_temperature", 1.0)),
+                                              **teacher)
+        return loss
 
     def train(self, resume_from_checkpoint: Optional[str] = None):
         a = self.args
@@ -244,12 +266,25 @@ class _null:
     def __exit__(self, *a): return False
 
 
+def _pad_teacher(rows, n: int, ids: bool):
+    rows = [torch.as_tensor(r, dtype=torch.long if ids else torch.float32).cpu() for r in rows]
+    top = [max(r.shape[1] for r in rows)] if rows[0].dim() == 2 else []
+    out = torch.full((len(rows), n, *top), -1 if ids else 0, dtype=rows[0].dtype)
+    for o, r in zip(out, rows):
+        o[tuple(slice(0, s) for s in r.shape)] = r
+    return out
+
+
 def default_collator(samples):
-    """Pads ``input_ids`` / ``labels`` / ``attention_mask`` lists to the longest sample (labels padded with -100)."""
+    """Pads ``input_ids`` / ``labels`` / ``attention_mask`` lists to the longest sample (labels padded with -100); a teacher's
+    rows (``TeacherTokens``: lists or tensors [tokens, top] and [tokens]) likewise, ids with -1."""
     keys = samples[0].keys()
     n = max(len(s["input_ids"]) for s in samples)
     out = {}
     for k in keys:
+        if k in TEACHER_COLUMNS:
+            out[k] = _pad_teacher([s[k] for s in samples], n, k == "teacher_ids")
+            continue
         pad = -100 if k == "labels" else 0
         out[k] = torch.tensor([list(s[k]) + [pad] * (n - len(s[k])) for s in samples], dtype=torch.long)
     if "labels" not in out:

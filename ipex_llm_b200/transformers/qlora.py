@@ -331,9 +331,17 @@ def get_peft_model(model, peft_config: LoraConfig, adapter_name: str = "default"
     return PeftModel(model, peft_config, adapter_name)
 
 
-def prepare_model_for_kbit_training(model, use_gradient_checkpointing=True, gradient_checkpointing_kwargs=None):
+def prepare_model_for_kbit_training(model, use_gradient_checkpointing=True, gradient_checkpointing_kwargs=None,
+                                    use_fused_attention=False):
     """Freeze the base, keep 1-D parameters (norms) in fp32, make the embedding output require grad so that
-    checkpointed blocks get gradients, and switch gradient checkpointing on (reference qlora.py:304-352)."""
+    checkpointed blocks get gradients, and switch gradient checkpointing on (reference qlora.py:304-352).
+
+    ``use_fused_attention``: attention by ``ops.train_attn.attention``, which holds nothing of the size of queries x keys, where
+    the model's attention goes through transformers' registry (refused where none does)."""
+    if use_fused_attention:
+        from ..models.train_attention import use_train_attention
+        invalidInputError(use_train_attention(model), "use_fused_attention: this model's attention does not go through transformers' "
+                                                      "attention registry")
     for _, p in model.named_parameters():
         p.requires_grad_(False)
     for p in model.parameters():
@@ -409,3 +417,7 @@ class TrainingArguments:
     dataloader_num_workers: int = 0
     group_by_length: bool = False
     deepspeed: Optional[str] = None     # accepted for script compatibility; ZeRO-1 sharding is built in
+    # the loss straight from the model's logits (``train.losses``); batches may then hold a teacher's tokens, too
+    fused_loss: bool = False
+    distill_weight: float = 0.5         # of the loss, where a batch has a teacher's tokens
+    distill_temperature: float = 1.0
