@@ -234,6 +234,13 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// What rounding to 16 bits took from two numbers, in 16 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(uint32_t rounded, float lo, float hi) {
+  const T* v = reinterpret_cast<const T*>(&rounded);
+  return pack2<T>(lo - to_float<T>(v[0]), hi - to_float<T>(v[1]));
+}
+
 // 32 rows x 32 columns of a warp, a row to a lane, times `f`, in 16 bits to shared memory (2 KB, the 64-byte swizzle), from where a
 // TMA store takes them to [b][h] of a tensor: whole sectors, where every lane storing its own row cost 2 to 6 us a tile.  What lies
 // past the tensor is not stored.
@@ -296,6 +303,35 @@ __device__ __forceinline__ void row_keys(const Shape& s, int q, int& lo, int& hi
   const int off = s.Skv - s.Sq;
   hi = s.causal ? min(s.Skv, q + off + 1) : s.Skv;
   lo = s.window > 0 ? max(0, q + off - s.window + 1) : 0;
+}
+
+// Rows before this one may see fewer than kFew keys (those of a window with holes apart); the whole warp calls it.
+//
+// P and dS are rounded to 16 bits on their way into a product.  That alone takes dq and dk from one rounding to two (1.41 times
+// the error); the error of P in o, and so in delta, adds 1 / keys of a row to it, and short rows are also those with the largest
+// gradients: sequences of a few to 64 tokens came to 1.45 to 1.6 times.  So tiles with such rows give the products what rounding
+// took, too, in a second step over columns that the scores have left: the first tile of a causal sequence, or all of a short one.
+constexpr int kFew = 64;
+__device__ __forceinline__ int few_queries(const Shape& s, int b, int lane) {
+  constexpr int kAll = 0x7FFFFFFF;
+  if (s.window > 0 && s.window < kFew) return kAll;
+  int enough = s.Skv >= kFew ? kFew : kAll;        // so many keys from the front hold kFew real ones
+  if (s.mask != nullptr) {
+    const uint32_t* words = s.mask + (int64_t)b * s.k_words;
+    enough = kAll;
+    for (int w = 0, seen = 0; w < s.k_words && enough == kAll; w += 32) {
+      int n = w + lane < s.k_words ? __popc(__ldg(words + w + lane)) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int before = __shfl_up_sync(0xffffffffu, n, o);
+        n += lane >= o ? before : 0;
+      }
+      const uint32_t there = __ballot_sync(0xffffffffu, seen + n >= kFew);
+      if (there != 0) enough = min(s.Skv, (w + __ffs(there)) * 32);
+      seen += __shfl_sync(0xffffffffu, n, 31);
+    }
+  }
+  return enough == kAll ? kAll : s.causal ? max(0, enough - 1 - (s.Skv - s.Sq)) : 0;
 }
 
 // A CTA stays on its SM and takes tiles of work, sorted from long to short, in turn with the others, every second round
@@ -434,6 +470,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     };
     bool ok = true;
     int n = 0, made[2] = {0, 0};                 // tiles of keys and values before this item; probabilities waited for
+    int few_to = 0, last_b = -1;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
       FwdItem it(s, item_of(w));
       it.ja = uniform(it.ja);
@@ -443,6 +480,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         it.j0[t] = uniform(it.j0[t]);
         it.j1[t] = uniform(it.j1[t]);
       }
+      if (it.b != last_b) {
+        few_to = uniform(few_queries(s, it.b, lane));
+        last_b = it.b;
+      }
+      const int q0 = uniform(it.q0);
       ok = warp_wait(q_full, w & 1, abort_flag);
       if (!ok) break;
       auto has = [&](int t, int j) { return j >= it.j0[t] && j < it.j1[t]; };
@@ -471,7 +513,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (has(t, j)) {
             tcgen05_fence_after();
             if (elect_one()) {
-              mma_sum<32, 64>(tmem + 2 * kT + t * kT, tmem + t * kT, vd + slot(n + 1), idesc_o, j > it.j0[t]);
+              mma_sum<16, 32>(tmem + 2 * kT + t * kT, tmem + t * kT, vd + slot(n + 1), idesc_o, j > it.j0[t]);
+              if (q0 + t * kT < few_to) mma_sum<16, 32>(tmem + 2 * kT + t * kT, tmem + t * kT + 16, vd + slot(n + 1), idesc_o, true);
               umma_commit(&o_full[t]);
             }
             __syncwarp();
@@ -497,10 +540,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const float c = s.scale_log2;
     bool ok = true;
     int made = 0, turns = 0;                       // scores and exchanges before this one
+    int few_to = 0, last_b = -1;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
       const FwdItem item(s, item_of(w));
       const int first = t ? item.j0[1] : item.j0[0], n = (t ? item.j1[1] : item.j1[0]) - first;
       const int q = item.q0 + t * kT + r, b = item.b;
+      if (b != last_b) few_to = few_queries(s, b, lane);
+      last_b = b;
+      const bool few = item.q0 + t * kT < few_to;
       int klo, khi;
       row_keys(s, q, klo, khi);
       float m = -INFINITY, l = 0.f;
@@ -572,14 +619,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float p0 = v[2 * i], p1 = v[2 * i + 1];
+            float &p0 = v[2 * i], &p1 = v[2 * i + 1];
             fma2(p0, p1, c, mc);
             p0 = ex2(p0);
             p1 = ex2(p1);
             add2(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], p0, p1);
             pk[i] = pack2<T>(p0, p1);
           }
-          tmem_st16(tS + hf * 64 + 16 * g, pk);          // over scores that have been read
+          tmem_st16(tS + hf * 64 + 32 * g, pk);          // over scores that have been read
+          if (few) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = rest2<T>(pk[i], v[2 * i], v[2 * i + 1]);
+            tmem_st16(tS + hf * 64 + 32 * g + 16, pk);
+          }
           l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         hand_over(&p_full[t], lane);
@@ -916,10 +968,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     auto slot = [&](int n, int w) { return w * L::kStages + n % L::kStages; };
     auto tile = [&](int n, int w) { return (uint64_t)(slot(n, w) * (L::kTile >> 4)); };
     bool ok = true;
-    int base = 0;
+    int base = 0, few_to = 0, last_b = -1;
     // Half of step n of an item's `total`, of q (W 0: k q^T, and P^T dO of the step before) or of dO (W 1: v dO^T, and dS^T q): the
     // sum, whose first operand lies where the new scores go, in front of these.
-    auto half = [&](auto which, int n, int total) {
+    auto half = [&](auto which, int n, int total, bool few) {
       constexpr int W = decltype(which)::value;
       const uint32_t tS = W ? tP : tmem, tO = W ? tK : tV;
       const int at = base + n;
@@ -928,6 +980,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tcgen05_fence_after();
         if (elect_one()) {
           mma_sum<16, 32>(tO, tS, qg_sum + tile(at - 1, 1 - W), idesc_o, n > 1);
+          if (few) mma_sum<16, 32>(tO, tS + 16, qg_sum + tile(at - 1, 1 - W), idesc_o, true);
           umma_commit(&empty[slot(at - 1, 1 - W)]);
         }
         __syncwarp();
@@ -945,11 +998,16 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       return true;
     };
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
-      const int total = uniform(DkvItem(s, item_of(w)).total);
+      const DkvItem it(s, item_of(w));
+      const int total = uniform(it.total), ni = uniform(it.ni);
+      if (it.b != last_b) few_to = few_queries(s, it.b, lane);
+      last_b = it.b;
+      const int few_n = uniform(max(0, min(it.ni, few_to / kT + (few_to % kT != 0) - it.i0)));   // blocks of each head
       ok = warp_wait(kv_full, w & 1, abort_flag);
       if (total == 0) continue;
-      for (int n = 0; n <= total && ok; ++n)
-        ok = half(std::integral_constant<int, 0>(), n, total) && half(std::integral_constant<int, 1>(), n, total);
+      for (int n = 0, i = -1; n <= total && ok; ++n, i = i + 1 < ni ? i + 1 : 0)         // i: the block of step n - 1
+        ok = half(std::integral_constant<int, 0>(), n, total, i < few_n) &&
+             half(std::integral_constant<int, 1>(), n, total, i < few_n);
       if (ok && elect_one()) umma_commit(done);
       __syncwarp();
       base += total;
@@ -963,16 +1021,17 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     uint8_t* stage = smem + warp * (2 * L::kTile / kArith);        // in the place of the keys and values, behind the last product
     const float c = s.scale_log2;
     bool ok = true;
-    int made = 0, items = 0;
+    int made = 0, items = 0, few_to = 0, last_b = -1;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
       const DkvItem it(s, item_of(w));
+      if (it.b != last_b) few_to = few_queries(s, it.b, lane);
+      last_b = it.b;
       const int k = it.k0 + r;
       const float f = grad_factor<T>(a.bound, it.b * s.Hkv + it.kvh);
-      for (int n = 0, i = 0; n < it.total; ++n, ++made) {
-        const int q0 = (it.i0 + i) * kT;
-        i = i + 1 < it.ni ? i + 1 : 0;
+      auto step = [&](auto few, int q0) {
+        constexpr bool FEW = decltype(few)::value;
         const uint32_t par = made & 1;
-        if (!warp_wait(s_full, par, abort_flag)) { ok = false; break; }
+        if (!warp_wait(s_full, par, abort_flag)) return false;
         tcgen05_fence_after();
         float p[32];
         tmem_ld32(tmem + lanes, p);
@@ -995,8 +1054,13 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 16; ++i) pk[i] = pack2<T>(p[2 * i], p[2 * i + 1]);
         tmem_st16(tmem + lanes, pk);
+        if constexpr (FEW) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = rest2<T>(pk[i], p[2 * i], p[2 * i + 1]);
+          tmem_st16(tmem + lanes + 16, pk);
+        }
         hand_over(p_full, lane);
-        if (!warp_wait(dp_full, par, abort_flag)) { ok = false; break; }
+        if (!warp_wait(dp_full, par, abort_flag)) return false;
         tcgen05_fence_after();
 #pragma unroll
         for (int g = 0; g < 2; ++g) {              // 16 at a time: the probabilities stay in registers
@@ -1009,9 +1073,20 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             if constexpr (std::is_same<T, __half>::value) mul2(d[2 * i], d[2 * i + 1], f, f);
             pk[8 * g + i] = pack2<T>(d[2 * i], d[2 * i + 1]);
           }
+          if constexpr (FEW) {                               // in the place of probabilities that have been used
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[8 * g + i] = __uint_as_float(rest2<T>(pk[8 * g + i], d[2 * i], d[2 * i + 1]));
+          }
         }
         tmem_st16(tP + lanes, pk);
+        if constexpr (FEW) tmem_st16(tP + lanes + 16, reinterpret_cast<const uint32_t*>(p));
         hand_over(ds_full, lane);
+        return true;
+      };
+      for (int n = 0, i = 0; n < it.total && ok; ++n, ++made) {
+        const int q0 = (it.i0 + i) * kT;
+        i = i + 1 < it.ni ? i + 1 : 0;
+        ok = q0 < few_to ? step(std::true_type(), q0) : step(std::false_type(), q0);
       }
       if (ok) ok = it.total > 0 ? warp_wait(done, items++ & 1, abort_flag) : warp_wait(kv_full, w & 1, abort_flag);
       tcgen05_fence_after();
@@ -1161,9 +1236,13 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     auto k_at = [&](int n) { return n % L::kK; };
     auto v_at = [&](int n) { return L::kK + n % L::kV; };
     bool ok = true;
-    int base = 0;
+    int base = 0, few_to = 0, last_b = -1;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
-      const int total = uniform(DqItem(s, item_of(w)).total);
+      const DqItem it(s, item_of(w));
+      const int total = uniform(it.total);
+      if (it.b != last_b) few_to = few_queries(s, it.b, lane);
+      last_b = it.b;
+      const bool few = uniform(it.q0 < few_to);
       ok = warp_wait(q_full, w & 1, abort_flag);
       if (total == 0) continue;
       const int end = base + total;
@@ -1197,6 +1276,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         tcgen05_fence_after();
         if (elect_one()) {
           mma_sum<16, 32>(tQ, tP, kv_sum + (uint64_t)(k_at(n) * (L::kTile >> 4)), idesc_o, n > base);
+          if (few) mma_sum<16, 32>(tQ, tP + 16, kv_sum + (uint64_t)(k_at(n) * (L::kTile >> 4)), idesc_o, true);
           umma_commit(&empty[k_at(n)]);
         }
         __syncwarp();
@@ -1216,9 +1296,12 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     uint8_t* stage = sQ + (qd % (D / 32) * 4 + (warp & 3)) * 2048;     // in the place of the queries, behind the last product
     const float c = s.scale_log2;
     bool ok = true;
-    int made = 0, items = 0;
+    int made = 0, items = 0, few_to = 0, last_b = -1;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
       const DqItem it(s, item_of(w));
+      if (it.b != last_b) few_to = few_queries(s, it.b, lane);
+      last_b = it.b;
+      const bool few = it.q0 < few_to;
       const int q = it.q0 + r;
       int klo, khi;
       row_keys(s, q, klo, khi);
@@ -1260,6 +1343,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           pk[i] = pack2<T>(d[2 * i], d[2 * i + 1]);
         }
         tmem_st16(tP + lanes, pk);
+        if (few) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = rest2<T>(pk[i], d[2 * i], d[2 * i + 1]);
+          tmem_st16(tP + lanes + 16, pk);
+        }
         hand_over(ds_full, lane);
       }
       if (ok) ok = it.total > 0 ? warp_wait(done, items++ & 1, abort_flag) : warp_wait(q_full, w & 1, abort_flag);
