@@ -1,7 +1,7 @@
 // What stands behind an output layer: log probabilities of given tokens with their entropy and the best alternatives, and
 // the divergence from a teacher's top logits, each with the gradient of the logits.  sm_100a.
 //
-// With c = log2(e) / T, r = fl(c max x), y = c x - r, s = sum 2^y, t = sum 2^y y (all to base 2):
+// With c = log2(e) / T, r = rint(c max x), y = c x - r, s = sum 2^y, t = sum 2^y y (all to base 2):
 //
 //   log p_j = (y_j - log2 s) ln 2             H = (log2 s - t / s) ln 2
 //   d log p_t / dx_j = (1[j = t] - p_j) / T   dH / dx_j = -p_j (log p_j + H) / T
@@ -16,8 +16,9 @@
 // 52 us).  Backward is a plain pass of 224 threads to a row, four vectors in flight (43 us for these rows, 6.1 TB/s).
 // A thread folds the maximum of a batch into its own and rescales its sums once for all of it, so that an element costs one
 // exponential (0.73 of what the special function units do at the rate of memory, for 16-bit logits).
-// y is one fma: the rounding of r, common to a row, takes part everywhere alike and so cancels, as long as r is the same number
-// everywhere (it goes to the backward pass, and rescaling goes by differences of it).
+// y is one fma: what rounding takes from r, common to a row, takes part everywhere alike and so cancels, as long as r is the same
+// number everywhere (it goes to the backward pass, and rescaling goes by differences of it).  r is whole, so sums are rescaled by
+// powers of two, exactly: ex2.approx of other numbers is low by 5e-8 on average (measured), which a tree of partial sums adds up.
 //
 // Statistics are 32-bit, 150 to 600 elements to a thread's sum and a tree above that; exponentials by ex2.approx (2 ulp).
 #include <cooperative_groups.h>
@@ -271,8 +272,8 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
     bool is_given = false;
     if constexpr (TAIL)
       for (int k = 0; k < K; ++k) is_given |= ids[k] == j;
-    Stat one = {__fmul_rn(v, c), 1.f, TAIL && !is_given ? 1.f : 0.f};
-    one.s = ex2(fmaf(v, c, -base_of(one.r)));       // 1, but for the rounding of r
+    Stat one = {rintf(__fmul_rn(v, c)), 1.f, TAIL && !is_given ? 1.f : 0.f};
+    one.s = ex2(fmaf(v, c, -base_of(one.r)));    
     if (ENT) one.t = one.s * held(fmaf(v, c, -base_of(one.r)));
     else if (one.t != 0.f) one.t = one.s;
     if (v != v) one.s = one.t = v;
@@ -297,7 +298,7 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
 #pragma unroll
       for (int i = 0; i < VEC; i += 2) mx = max3(mx, f[i], f[i + 1]);
     }
-    const float r = fmaxf(st.r, __fmul_rn(mx, c)), to = base_of(r);
+    const float r = fmaxf(st.r, rintf(__fmul_rn(mx, c))), to = base_of(r);
     const float down = held(st.r - to), fac = ex2(down);
     // CAREFUL: with exponents held, for what hides tokens
     auto sums = [&](auto careful, float& s, float& t) {
@@ -539,6 +540,14 @@ __device__ __forceinline__ void meet(int parts) {
   }
 }
 
+// log sum e^(x / T).  A row's few last operations are done in 64 bits: in 32, they made the error of a log probability 1.7 times what
+// its own rounding is.  c is log2(e) / T rounded to 32 bits, and r, rounded from c max x, is taken back to the unrounded factor: what
+// is left of c's error is that of the differences to the largest logit.
+constexpr double kLn2_64 = 0.693147180559945309;
+__device__ __forceinline__ double log_sum(float r, double log2_s, float c, float temp) {
+  return r * (1.0 / ((double)temp * c)) + log2_s * kLn2_64;
+}
+
 struct ProbArgs {
   Rows rows;
   const int64_t* targets;
@@ -585,14 +594,18 @@ __global__ void __launch_bounds__(kNT + 32, kCtas) token_logprobs_kernel(ProbArg
     const Stat st = row_stat<ENT>(sh, turn, parts);
     if (rank == 0) {
       const bool none = no_token(st, c);
-      const float r = none ? 0.f : st.r, log2_s = none ? 0.f : log2f(st.s);
-      const float H = !ENT || none ? 0.f : (log2_s - st.t / st.s) * kLn2;
-      auto logp = [&](float v) { return none ? -INFINITY : (fmaf(v, c, -r) - log2_s) * kLn2; };
+      const float r = none ? 0.f : st.r;
+      const double log2_s = none ? 0.0 : log2((double)st.s), lse = log_sum(r, log2_s, c, a.temp);
+      const float H = !ENT || none ? 0.f : (float)((log2_s - (double)st.t / st.s) * kLn2_64);
+      auto logp = [&](float v) {
+        const float y = fmaf(v, c, -r);            // -inf for what hides a token
+        return none ? -INFINITY : fabsf(y) < INFINITY ? (float)(v / (double)a.temp - lse) : (y - (float)log2_s) * kLn2;
+      };
       if (lane == 0) {
         if (bad) tc5::report(a.err, kErrToken);
         a.logprob[row] = bad ? NAN : ignored ? 0.f : logp(xt);
         if (ENT) a.entropy[row] = ignored ? 0.f : bad ? NAN : H;
-        if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r, none ? 0.f : 1.f / st.s, log2_s, H);
+        if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r, none ? 0.f : 1.f / st.s, (float)log2_s, H);
       }
       if constexpr (TOP) {
         uint64_t k = sh.top[turn][lane];
@@ -713,7 +726,7 @@ __device__ __forceinline__ double warp_sum64(double v) {
 }
 
 // The teacher's part of a row, by the finishing warp, in 64 bits (some K numbers beside V): 1 - sum q cancels, and a loss near 0 is
-// a difference.  sum_k q_k (log q_k - log p_id) = own - ln 2 (c cross - mass (r + log2 s)) with what follows, so that it need not
+// a difference.  sum_k q_k (log q_k - log p_id) = own - cross / T + mass log sum e^(x / T) with what follows, so that it need not
 // wait for the student's sums.
 struct Teacher {
   double own, cross, mass;   // sum q log q, sum q x_id, sum q
@@ -822,16 +835,16 @@ __global__ void __launch_bounds__(kNT + 32, kCtas) distill_kernel(DistillArgs a)
     if (rank == 0 && lane == 0) {
       const bool none = no_token(st, c);
       const float r = none ? 0.f : st.r;
-      const double ln2 = 0.6931471805599453, log2_s = none ? 0.0 : log2((double)st.s);
       double mass = te.mass, rest = 0.0;
-      double loss = te.never ? INFINITY : te.own - ln2 * (c * te.cross - te.mass * (r + log2_s));
+      double loss = te.never ? INFINITY
+                             : te.own - te.cross / a.temp + te.mass * log_sum(r, none ? 0.0 : log2((double)st.s), c, a.temp);
       float ratio = 0.f;
       if constexpr (TAIL) {
         rest = fmax(1.0 - mass, 0.0);
         const float left = none ? 0.f : st.t / st.s;
         if (rest > 0.0 && left > 0.f) {
           ratio = (float)rest / left;
-          loss += rest * (log(rest) - (double)(log2f(left) * kLn2));
+          loss += rest * log(rest * st.s / st.t);
         } else {
           rest = 0.0;                                        // the student has no other token: the term is left out
         }
