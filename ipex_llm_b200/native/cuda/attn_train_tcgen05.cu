@@ -334,6 +334,12 @@ __device__ __forceinline__ int few_queries(const Shape& s, int b, int lane) {
   return enough == kAll ? kAll : s.causal ? max(0, enough - 1 - (s.Skv - s.Sq)) : 0;
 }
 
+// So do all rows of dq in heads below 64.  The keys that a row sees have a part along its query in common, over which dS sums to 0
+// while its rounding does not, and the fewer the dimensions the larger that part: 1.44 times the final rounding's error with 128,
+// 1.5 with 32 (1.03 so; dk, whose sums run over queries, has 1.41 to 1.44).  It costs 14 % of dq: 79 us for 4 x 1024 tokens and 32
+// heads of 56, 69 for heads of 64.
+__device__ __forceinline__ bool rest_of_dq(const Shape& s) { return s.D < 64; }
+
 // A CTA stays on its SM and takes tiles of work, sorted from long to short, in turn with the others, every second round
 // backwards.  (A CTA to a tile cost 5 us between the last product of one and the first of the next, for barriers, tensor memory,
 // cold loads; here the ring of tiles runs on.)
@@ -1242,7 +1248,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const int total = uniform(it.total);
       if (it.b != last_b) few_to = few_queries(s, it.b, lane);
       last_b = it.b;
-      const bool few = uniform(it.q0 < few_to);
+      const bool few = uniform(rest_of_dq(s) || it.q0 < few_to);
       ok = warp_wait(q_full, w & 1, abort_flag);
       if (total == 0) continue;
       const int end = base + total;
@@ -1301,7 +1307,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       const DqItem it(s, item_of(w));
       if (it.b != last_b) few_to = few_queries(s, it.b, lane);
       last_b = it.b;
-      const bool few = it.q0 < few_to;
+      const bool few = rest_of_dq(s) || it.q0 < few_to;
       const int q = it.q0 + r;
       int klo, khi;
       row_keys(s, q, klo, khi);

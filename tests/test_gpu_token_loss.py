@@ -271,3 +271,31 @@ def test_captured_and_replayed_on_another_stream():
     torch.cuda.synchronize()
     for got, want in zip(out, step()):
         assert torch.equal(got, want)
+
+
+def test_offsets_past_32_bits():
+    """2.2e9 logits and their gradients: the last rows."""
+    from ipex_llm_b200.ops import cuda_ops
+    from ipex_llm_b200.ops.token_loss import distill_loss, token_logprobs
+    R, V = 17_000, 131_072
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(R, V, dtype=torch.bfloat16, device="cuda").normal_(std=2.5, generator=g).requires_grad_()
+    t = torch.randint(0, V, (R,), generator=g, device="cuda")
+    up = torch.randn(R, generator=g, device="cuda")
+    r = token_logprobs(x, t, entropy=True, top=4)
+    got, = torch.autograd.grad((r.logprob, r.entropy), (x,), (up, up))
+    lp, ent, logp, dx = oracle.logprobs(x[-2:], t[-2:], 1.0, up[-2:], up[-2:])
+    _near(r.logprob[-2:], lp, oracle.value_tol(V, lp, 1.0), "logprob")
+    _near(r.entropy[-2:], ent, oracle.value_tol(V, ent, 1.0), "entropy")
+    assert torch.equal(r.top_ids[-2:], torch.sort(x.detach()[-2:].float(), dim=-1, descending=True, stable=True).indices[:, :4])
+    size = 2 * up[-2:].abs().double().cpu().unsqueeze(-1)
+    _near(got[-2:], dx, oracle.grad_tol(dx, x.dtype, V, size, 1.0), "dlogits")
+    del got
+    ids = r.top_ids
+    values = r.top_logprobs.detach()
+    loss = distill_loss(x, ids, values)
+    got, = torch.autograd.grad(loss, (x,), (up,))
+    want, dx = oracle.distill(x[-2:], ids[-2:], values[-2:], 1.0, None, up[-2:])
+    _near(loss[-2:], want, oracle.U * (4 * oracle.sum_steps(V) + 4 + 24 * (20 + math.log(V) + 20)), "loss")
+    _near(got[-2:], dx, oracle.grad_tol(dx, x.dtype, V, up[-2:].abs().double().cpu().unsqueeze(-1) * 2, 1.0), "dlogits")
+    cuda_ops.check_error_flag(x.device)

@@ -233,3 +233,24 @@ def test_few_keys_are_rounded_once(dtype, sizes, kw):
     for n in ("out", "dq", "dk", "dv"):
         ref = want[n][0]
         assert (got[n].double() - ref).norm() <= 0.5 * torch.finfo(dtype).eps / 2 * ref.norm(), n
+
+
+def test_more_heads_than_a_launch_takes():
+    from ipex_llm_b200.ops.train_attn import attention
+    q = torch.zeros(1, 32768, 1, 8, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="heads"):
+        attention(q, q, q)
+
+
+def test_offsets_past_32_bits():
+    """2.4e9 numbers in q, out and their gradients: the last rows of all heads, whose windows lie among the last rows."""
+    S, H, D, n = 300_000, 64, 128, 100
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, grad = (torch.empty(1, S, H, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g).transpose(1, 2) for _ in range(2))
+    k, v = (torch.empty(1, S, 1, D, dtype=torch.bfloat16, device="cuda").normal_(generator=g).transpose(1, 2) for _ in range(2))
+    got = _run(q, k, v, grad, window=64)
+    tail = slice(S - n - 136, S)
+    want = oracle.attention(*(t[:, :, tail] for t in (q, k, v, grad)), D ** -0.5, True, 64, None)
+    for name, (exact, tol) in want.items():
+        off = (got[name][:, :, -n:].double() - exact[:, :, -n:]).abs() / tol[:, :, -n:]
+        assert float(off.nan_to_num(nan=math.inf).max()) <= 1.0, name

@@ -53,8 +53,9 @@ def distill(logits, ids, values, temperature, lse=None, g=None):
 
 
 def sum_steps(V):
-    """Roundings on the way into a row's sum, in units of U: a thread adds V / 512 terms at most and a batch of 32 (each an
-    exponential of 2 ulp with a rounded argument), then come trees of 5 + 16 + 8 joins of two factors each."""
+    """Roundings on the way into a row's sum, in units of U, from above: a thread adds batches of up to 32 terms (each an
+    exponential of 2 ulp with a rounded argument) to its sum, V / 7168 of them (V / 512 is more than enough), then come trees of
+    5 + 16 + 8 joins of two factors each."""
     return V / 512 + 32 + 8 + 3 * 29
 
 

@@ -57,8 +57,6 @@ def attention(q, k, v, g, scale, causal, window, key_mask):
     floor = small * 2.0 ** -14 * 2 * float(g.norm(dim=-1).max() * vv.norm(dim=-1).max()) * see.double()
     tol["dq"] = ((size + floor) @ kk.abs()) * scale
     tol["dk"] = fold((size + floor).transpose(-1, -2) @ q.abs()) * scale
-    last = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
-    half = last[torch.float16] if eps == 2.0 ** -11 else last[torch.bfloat16]
     for name in ("dq", "dk", "dv", "out"):
-        tol[name] = tol[name] * 1.02 + eps * got[name].abs() * 1.02 + half
+        tol[name] = tol[name] * 1.02 + eps * got[name].abs() * 1.02 + small
     return {name: (got[name], tol[name]) for name in got}
