@@ -22,7 +22,9 @@
 //   dq          a pass of its own over the keys, which computes s and dP once more (7 products in all where 5 would do): the
 //               sums then need no atomics, whose order would change results, and no 32-bit dq in global memory
 // Sixteen warps of arithmetic hide each other's latencies: with eight, two to a scheduler, an exponential's chain (product,
-// special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks.
+// special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks; it takes 1700 (of two
+// tiles of queries), 2870 and 2300 now, of which the products are 1024, 2176 and 1540.  4096 tokens, 64 heads of 128 over 8 of
+// keys, causal, bf16: 300 + 40 + 485 + 380 us.
 //
 // In the transposed scores L_i and delta_i belong to columns, not to the threads' rows.  Read from shared memory, four numbers a
 // request, they took a third of its bandwidth, which the products need.  So they are summed by the products too: one more step
@@ -756,21 +758,27 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
   return d;
 }
 
-// A CTA to 128 rows of a head: 16 lanes to a row (up to 128 columns, eight each), eight rows of each half warp in flight four at a
-// time.  blockIdx.y counts the query heads, then (fp16) the key heads, whose rows only go into the bound.
-template <typename T>
+// A CTA to 128 rows of a head, LANES lanes to a row (eight columns each), the rows of a group of lanes in flight four at a time.
+// What a row gets is written by a lane of its own (in fp16 12.5 us instead of 15 for 2 x 1031 tokens in 32 heads of 80, where one lane loads
+// -L / scale and cuts numbers into pieces for all rows of its group; in bf16 the same).  blockIdx.y counts the query heads, then
+// (fp16) the key heads, whose rows only go into the bound.
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
-  __shared__ float most[16];
-  const int sub = threadIdx.x & 15, half = threadIdx.x >> 4, b = blockIdx.z;
+  constexpr int kRows = kT * LANES / 256;
+  __shared__ uint32_t most[256 / LANES];
+  const int sub = threadIdx.x % LANES, group = threadIdx.x / LANES, b = blockIdx.z;
   const bool is_q = (int)blockIdx.y < a.Hq, in = 8 * sub < a.D;
-  const int h = is_q ? blockIdx.y : blockIdx.y - a.Hq, rows = is_q ? a.Sq : a.Skv, r0 = blockIdx.x * kT + half * 8;
+  const int h = is_q ? blockIdx.y : blockIdx.y - a.Hq, rows = is_q ? a.Sq : a.Skv, r0 = blockIdx.x * kT + group * kRows;
   const T* x = is_q ? (const T*)a.grad + b * a.g_b + h * a.g_h : (const T*)a.v + b * a.v_b + h * a.v_h;
   const int64_t stride = is_q ? a.g_s : a.v_s, o_row = (int64_t)a.Hq * a.D;
   const int64_t o_at = ((int64_t)b * a.Sq * a.Hq + h) * a.D + 8 * sub;
   if ((int)blockIdx.x * kT >= rows) return;
-  float largest = 0.f;
+  const bool writes = is_q && sub < kRows;
+  const int64_t row = ((int64_t)b * a.Hq + h) * a.q_pad + r0 + sub;
+  const float nl = writes ? a.nlse[row] : 0.f;
+  float largest = 0.f, delta = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
+  for (int i = 0; i < kRows; i += 4) {
     uint4 g[4], o[4], lo[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -786,31 +794,29 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int r = r0 + i + u;
       float d = is_q ? dot8<T>(g[u], o[u]) + dot8<T>(g[u], lo[u]) * (1.f / kLowScale) : 0.f;
       float n = std::is_same<T, __half>::value ? dot8<T>(g[u], g[u]) : 0.f;
 #pragma unroll
-      for (int s = 8; s > 0; s >>= 1) {
+      for (int s = LANES / 2; s > 0; s >>= 1) {
         d += __shfl_xor_sync(0xffffffffu, d, s);
         if (std::is_same<T, __half>::value) n += __shfl_xor_sync(0xffffffffu, n, s);
       }
       largest = fmaxf(largest, n);
-      if (sub == 0 && is_q) {
-        const int64_t row = ((int64_t)b * a.Hq + h) * a.q_pad + r;
-        a.delta[row] = d;
-        const float nl = a.nlse[row];
-        uint4* at = a.pieces + row / kT * (2 * kT) + row % kT;
-        at[0] = in_pieces<T>(nl == -INFINITY ? 0.f : nl * a.inv_scale_log2);
-        at[kT] = in_pieces<T>(-d);
-      }
+      if (sub == i + u) delta = d;
     }
   }
+  if (writes) {
+    a.delta[row] = delta;
+    uint4* at = a.pieces + row / kT * (2 * kT) + row % kT;
+    at[0] = in_pieces<T>(nl == -INFINITY ? 0.f : nl * a.inv_scale_log2);
+    at[kT] = in_pieces<T>(-delta);
+  }
   if (std::is_same<T, __half>::value) {
-    if (sub == 0) most[half] = largest;
+    if (sub == 0) most[group] = __float_as_uint(largest);
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < 16; ++i) largest = fmaxf(largest, most[i]);
-      atomicMax(&a.bound[(b * a.Hkv + (is_q ? h / (a.Hq / a.Hkv) : h)) * 2 + (is_q ? 0 : 1)], __float_as_uint(largest));
+    if (threadIdx.x < 32) {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, threadIdx.x < 256 / LANES ? most[threadIdx.x] : 0u);
+      if (threadIdx.x == 0) atomicMax(&a.bound[(b * a.Hkv + (is_q ? h / (a.Hq / a.Hkv) : h)) * 2 + (is_q ? 0 : 1)], top);
     }
   }
 }
@@ -1544,7 +1550,8 @@ int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
   if (items_of(s, s.Hkv, s.Skv, kT) == 0 || items_of(s, s.Hq, s.Sq, kT) == 0 || s.Hq + s.Hkv > 65535)
     return (int)cudaErrorInvalidValue;
   const int longest = bound != nullptr && s.Skv > s.Sq ? s.Skv : s.Sq;
-  attn_prep_kernel<T><<<dim3((longest + kT - 1) / kT, s.Hq + (bound != nullptr ? s.Hkv : 0), s.B), 256, 0, stream>>>(p);
+  const dim3 prep_grid((longest + kT - 1) / kT, s.Hq + (bound != nullptr ? s.Hkv : 0), s.B);
+  attn_prep_kernel<T, D / 8><<<prep_grid, 256, 0, stream>>>(p);
   BwdArgs a = {s, nlse, delta, pieces, bound, items_of(s, s.Hkv, s.Skv, kT)};
   attn_dkv_kernel<T, D><<<grid_of(a.items), kThreads, smem, stream>>>(tq, tk, tv, tg, tdk, tdv, a);
   a.items = items_of(s, s.Hq, s.Sq, kT);
