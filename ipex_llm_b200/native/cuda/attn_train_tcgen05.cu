@@ -22,9 +22,10 @@
 //   dq          a pass of its own over the keys, which computes s and dP once more (7 products in all where 5 would do): the
 //               sums then need no atomics, whose order would change results, and no 32-bit dq in global memory
 // Sixteen warps of arithmetic hide each other's latencies: with eight, two to a scheduler, an exponential's chain (product,
-// special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks; it takes 1700 (of two
-// tiles of queries), 2870 and 2300 now, of which the products are 1024, 2176 and 1540.  4096 tokens, 64 heads of 128 over 8 of
-// keys, causal, bf16: 300 + 40 + 485 + 380 us.
+// special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks, of which the products
+// alone are 1030, 2180 and 1540.  Now, with 4096 tokens, 64 heads of 128 over 8 of keys, causal, bf16: 345, 540 and 425 us (40 for
+// the pass before the backward), 1.5, 2.1 and 1.9 us a block.  With all arithmetic taken out a block still takes 1700 (forward) and
+// 2870 clocks (dk and dv): the products' issue and arrivals between the roles are what is left to win.
 //
 // In the transposed scores L_i and delta_i belong to columns, not to the threads' rows.  Read from shared memory, four numbers a
 // request, they took a third of its bandwidth, which the products need.  So they are summed by the products too: one more step
@@ -759,9 +760,9 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
 }
 
 // A CTA to 128 rows of a head, LANES lanes to a row (eight columns each), the rows of a group of lanes in flight four at a time.
-// What a row gets is written by a lane of its own (in fp16 12.5 us instead of 15 for 2 x 1031 tokens in 32 heads of 80, where one lane loads
-// -L / scale and cuts numbers into pieces for all rows of its group; in bf16 the same).  blockIdx.y counts the query heads, then
-// (fp16) the key heads, whose rows only go into the bound.
+// What a row gets is written by a lane of its own (in fp16 12.5 us instead of 15 for 2 x 1031 tokens in 32 heads of
+// 80, where one lane loads -L / scale and cuts numbers into pieces for all rows of its group; in bf16 the same).  blockIdx.y counts
+// the query heads, then (fp16) the key heads, whose rows only go into the bound.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) attn_prep_kernel(PrepArgs a) {
   constexpr int kRows = kT * LANES / 256;
@@ -1486,7 +1487,8 @@ bool shape_ok(int B, int Hq, int Hkv, int Sq, int Skv, int D, int window, float 
          Sq <= (1 << 23) && Skv <= (1 << 23) && D >= 8 && D <= 128 && D % 8 == 0 && window >= 0 && scale >= 1e-4f && scale <= 1e4f;
 }
 
-Shape make_shape(int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window, const uint32_t* mask, float scale, int* err) {
+Shape make_shape(int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window, const uint32_t* mask, float scale,
+                 int* err) {
   Shape s;
   s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.Sq = Sq; s.Skv = Skv; s.D = D; s.causal = causal; s.window = window;
   s.q_pad = (Sq + kT - 1) / kT * kT;
@@ -1585,7 +1587,8 @@ IPEX_API int ipex_attn_train_fwd(const void* q, int64_t q_b, int64_t q_h, int64_
   return (int)cudaErrorInvalidValue;
 }
 
-// g: the gradient of out, by strides like q.  work: scratch, 16-byte aligned, 9 floats for each of nlse and 2 B Hkv.  dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
+// g: the gradient of out, by strides like q.  work: scratch, 16-byte aligned, 9 floats for each of nlse and 2 B Hkv.
+// dq [B, Sq, Hq, D], dk and dv [B, Skv, Hkv, D] contiguous.
 IPEX_API int ipex_attn_train_bwd(const void* q, int64_t q_b, int64_t q_h, int64_t q_s, const void* k, int64_t k_b, int64_t k_h,
                                  int64_t k_s, const void* v, int64_t v_b, int64_t v_h, int64_t v_s, const uint32_t* mask_words,
                                  const void* out, const void* low, const float* nlse, const void* g, int64_t g_b, int64_t g_h,
@@ -1615,7 +1618,8 @@ IPEX_API int ipex_attn_hide(const uint8_t* mask, int64_t m_b, int64_t m_s, const
                             const void* v, int64_t v_b, int64_t v_h, int64_t v_s, void* k_out, void* v_out, uint32_t* words, int B,
                             int Hkv, int Skv, int D, void* stream) {
   if (B < 1 || B > 65535 || Hkv < 1 || Skv < 1 || Skv > (1 << 23) || D < 8 || D > 128 || D % 8 ||
-      mask == nullptr || k == nullptr || v == nullptr || k_out == nullptr || v_out == nullptr || words == nullptr || ((k_b | k_h | k_s | v_b | v_h | v_s) & 7) ||
+      mask == nullptr || k == nullptr || v == nullptr || k_out == nullptr || v_out == nullptr || words == nullptr ||
+      ((k_b | k_h | k_s | v_b | v_h | v_s) & 7) ||
       ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(k_out) |
         reinterpret_cast<uintptr_t>(v_out)) & 15))
     return (int)cudaErrorInvalidValue;

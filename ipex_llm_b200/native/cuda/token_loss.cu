@@ -987,7 +987,8 @@ IPEX_API int ipex_token_logprobs(const void* logits, int64_t s0, int64_t s1, int
       targets == nullptr || logprob == nullptr || (top > 0 && (top_logprob == nullptr || top_id == nullptr)) ||
       (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
-  ProbArgs a = {rows_of(logits, s0, s1, n1, rows, V), targets, logprob, entropy, stats, top_logprob, top_id, top, 0, ignore, rows, temp, 1.f / temp, err};
+  ProbArgs a = {rows_of(logits, s0, s1, n1, rows, V), targets, logprob, entropy, stats, top_logprob, top_id, top, 0, ignore,
+                rows, temp, 1.f / temp, err};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
   return by_type(dtype, [&](auto* tag) {
     using T = std::remove_pointer_t<decltype(tag)>;
@@ -1022,7 +1023,8 @@ IPEX_API int ipex_distill(const void* logits, int64_t s0, int64_t s1, int64_t n1
                           const float* lse, float* loss, float* stats, int64_t rows, int V, int K, float temp, int dtype, int* err,
                           void* stream) {
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
-      ids == nullptr || values == nullptr || loss == nullptr || (lse != nullptr && V > kMaxTailV) || (reinterpret_cast<uintptr_t>(stats) & 15))
+      ids == nullptr || values == nullptr || loss == nullptr || (lse != nullptr && V > kMaxTailV) ||
+      (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
   DistillArgs a = {rows_of(logits, s0, s1, n1, rows, V), ids, values, lse, loss, stats, rows, K, 0, 0, temp, 1.f / temp, err};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);
@@ -1041,7 +1043,8 @@ IPEX_API int ipex_distill_grad(const void* logits, int64_t s0, int64_t s1, int64
                                const float* stats, const float* g, void* dlogits, int64_t rows, int V, int K, float temp, int dtype,
                                void* stream) {
   if (!rows_ok(logits, s0, s1, n1, rows, V, dtype == DT_F32 ? 4 : 2) || K < 1 || K > kMaxK || !temp_ok(temp) ||
-      ids == nullptr || values == nullptr || dlogits == nullptr || stats == nullptr || g == nullptr || (reinterpret_cast<uintptr_t>(stats) & 15))
+      ids == nullptr || values == nullptr || dlogits == nullptr || stats == nullptr || g == nullptr ||
+      (reinterpret_cast<uintptr_t>(stats) & 15))
     return (int)cudaErrorInvalidValue;
   DistillGradArgs a = {rows_of(logits, s0, s1, n1, rows, V), ids, values, stats, g, dlogits, K, 0, temp, 1.f / temp};
   a.parts = parts_of(rows, V, dtype == DT_F32 ? 4 : 2);

@@ -170,7 +170,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     if Hq + Hkv > MAX_HEADS:
         invalidInputError(False, f"attention: {Hq} and {Hkv} heads are too many ({MAX_HEADS} together are not)")
     if B > 65535 or Sq > MAX_TOKENS or Skv > MAX_TOKENS:
-        invalidInputError(False, f"attention: {B} sequences of {Sq} queries and {Skv} keys are too many (65535 of {MAX_TOKENS} are not)")
+        invalidInputError(False, f"attention: {B} sequences of {Sq} queries and {Skv} keys are too many (65535 of {MAX_TOKENS} "
+                                 "are not)")
     if q.numel() == 0 or k.numel() == 0:
         return q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0.0) + (k.sum() + v.sum()) * 0
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
