@@ -23,8 +23,8 @@
 //               sums then need no atomics, whose order would change results, and no 32-bit dq in global memory
 // Sixteen warps of arithmetic hide each other's latencies: with eight, two to a scheduler, an exponential's chain (product,
 // special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks, of which the products
-// alone are 1030, 2180 and 1540.  Now, with 4096 tokens, 64 heads of 128 over 8 of keys, causal, bf16: 345, 540 and 425 us (40 for
-// the pass before the backward), 1.5, 2.1 and 1.9 us a block.  With all arithmetic taken out a block still takes 1700 (forward) and
+// alone are 1030, 2180 and 1540.  Now, with 4096 tokens, 64 heads of 128 over 8 of keys, causal, bf16: 345, 540 and 415 us (41 for
+// the pass before the backward), 1.5, 2.1 and 1.8 us a block.  With all arithmetic taken out a block still takes 1700 (forward) and
 // 2870 clocks (dk and dv): the products' issue and arrivals between the roles are what is left to win.
 //
 // In the transposed scores L_i and delta_i belong to columns, not to the threads' rows.  Read from shared memory, four numbers a
@@ -838,8 +838,17 @@ struct BwdArgs {
   const float* delta;     // [B, Hq, q_pad]
   const uint4* pieces;
   const uint32_t* bound;  // [B, Hkv, 2] or null
+  void *out0, *out1;      // dk and dv, or dq: [B, rows, heads, D]
   unsigned items;
 };
+// Zeros in rows [row, row + 128) of a head of [B, rows, heads, D], by the 512 threads of the arithmetic: what no query (or key) sees.
+template <typename T>
+__device__ __forceinline__ void zero_rows(void* out, int b, int row, int rows, int h, int heads, int D) {
+  T* at = reinterpret_cast<T*>(out) + ((int64_t)b * rows * heads + h) * D;
+  const int per = D / 8, n = min(kT, rows - row) * per;
+  for (int i = threadIdx.x; i < n; i += 32 * kArith)
+    *reinterpret_cast<uint4*>(at + (int64_t)(row + i / per) * heads * D + i % per * 8) = make_uint4(0, 0, 0, 0);
+}
 
 // ------------------------------------------------------------------------------------------------ dk and dv
 template <int D>
@@ -899,7 +908,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   uint64_t* dp_full = s_full + 2;
   uint64_t* ds_full = s_full + 3;
   uint64_t* done = s_full + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* staged = done + 1;                   // [2]: by the parity of the item
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staged + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const Shape& s = a.s;
@@ -908,7 +918,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, kArith);
+    mbar_init(kv_empty, 1);
+    mbar_init(&staged[0], kArith);
+    mbar_init(&staged[1], kArith);
     for (int i = 0; i < 2 * L::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -942,19 +954,29 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       prefetch_tmap(&tm_v);
       // A tile of dO is free again half a step before the tile of q beside it: each has barriers of its own, and goes as its
       // turn comes.
+      // An item's outputs are staged where its last step's tiles were: that place is taken again by the step kStages later, in the
+      // next item or behind it.  In the place of k and v it kept the next item's from coming (4 x 512 tokens, 40 heads of 128: 61 us
+      // instead of 52.5; dq, staged over q, 48.5 instead of 45).
       bool ok = true;
-      int n = 0, w = 0;                            // steps before this item
-      for (; ok && item_of(w) < a.items; ++w) {
+      int n = 0, z = 0, waited = 0;                // steps and items before this item; items whose staging has been waited for
+      auto staged_before = [&](int item) {
+        for (; ok && waited < item; ++waited) ok = mbar_wait(&staged[waited & 1], waited >> 1 & 1, abort_flag);
+        if (!ok) report(s.err, 71);
+      };
+      for (int w = 0; ok && item_of(w) < a.items; ++w) {
         const DkvItem it(s, item_of(w));
-        if (!mbar_wait(kv_empty, (w & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
-        mbar_expect_tx(kv_full, it.total > 0 ? 2 * L::kTile : 0);
-        if (it.total > 0) {
-          load_tile<D>(sK, &tm_k, it.k0, it.kvh, it.b, kv_full);
-          load_tile<D>(sV, &tm_v, it.k0, it.kvh, it.b, kv_full);
-        }
+        if (it.total == 0) continue;
+        staged_before(z - 1);                      // so a barrier of these is never two items ahead
+        if (!ok) break;
+        if (!mbar_wait(kv_empty, (z & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        mbar_expect_tx(kv_full, 2 * L::kTile);
+        load_tile<D>(sK, &tm_k, it.k0, it.kvh, it.b, kv_full);
+        load_tile<D>(sV, &tm_v, it.k0, it.kvh, it.b, kv_full);
         for (int m = 0; m < 2 * it.total; ++m) {
           const int i = m >> 1, x = (m & 1) ^ (n + i == 0 ? 0 : 1), st = (n + i) % L::kStages, at = x * L::kStages + st;
           const int h = it.kvh * group + i / it.ni, q0 = (it.i0 + i % it.ni) * kT;
+          if (i >= L::kStages - 1) staged_before(z);
+          if (!ok) break;
           if (!mbar_wait(&empty[at], ((n + i) / L::kStages & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
           mbar_expect_tx(&full[at], L::kTile + 2048);
           load_tile<D>(sQG + at * L::kTile, x ? &tm_g : &tm_q, q0, h, it.b, &full[at]);
@@ -962,9 +984,11 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                     &full[at]);
         }
         n += it.total;
+        ++z;
       }
       if (!ok) {                                   // loads in flight end before the CTA does
-        mbar_wait_quiet(kv_full, w & 1, 1 << 12);
+        mbar_wait_quiet(kv_full, 0, 1 << 12);
+        mbar_wait_quiet(kv_full, 1, 1 << 12);
         for (int i = 0; i < 2 * L::kStages; ++i) {
           mbar_wait_quiet(&full[i], 0, 1 << 12);
           mbar_wait_quiet(&full[i], 1, 1 << 12);
@@ -981,7 +1005,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     auto slot = [&](int n, int w) { return w * L::kStages + n % L::kStages; };
     auto tile = [&](int n, int w) { return (uint64_t)(slot(n, w) * (L::kTile >> 4)); };
     bool ok = true;
-    int base = 0, few_to = 0, last_b = -1;
+    int base = 0, z = 0, few_to = 0, last_b = -1;
     // Half of step n of an item's `total`, of q (W 0: k q^T, and P^T dO of the step before) or of dO (W 1: v dO^T, and dS^T q): the
     // sum, whose first operand lies where the new scores go, in front of these.
     auto half = [&](auto which, int n, int total, bool few) {
@@ -1005,6 +1029,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           mma_rows<D>(tS, W ? vd : kd, qg_rows + tile(at, W), idesc_s);
           umma_f16(tS, weights, pieces + (slot(at, W) * 2048 >> 4), idesc_s, true);
           umma_commit(W ? dp_full : s_full);
+          if (W && n + 1 == total) umma_commit(kv_empty);      // k and v have been read: the next item's come
         }
         __syncwarp();
       }
@@ -1016,8 +1041,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (it.b != last_b) few_to = few_queries(s, it.b, lane);
       last_b = it.b;
       const int few_n = uniform(max(0, min(it.ni, few_to / kT + (few_to % kT != 0) - it.i0)));   // blocks of each head
-      ok = warp_wait(kv_full, w & 1, abort_flag);
       if (total == 0) continue;
+      ok = warp_wait(kv_full, z++ & 1, abort_flag);
       for (int n = 0, i = -1; n <= total && ok; ++n, i = i + 1 < ni ? i + 1 : 0)         // i: the block of step n - 1
         ok = half(std::integral_constant<int, 0>(), n, total, i < few_n) &&
              half(std::integral_constant<int, 1>(), n, total, i < few_n);
@@ -1031,7 +1056,6 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // ---------------- a key and a quarter of the queries to a thread ----------------
     const int qd = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + qd * 32;
-    uint8_t* stage = smem + warp * (2 * L::kTile / kArith);        // in the place of the keys and values, behind the last product
     const float c = s.scale_log2;
     bool ok = true;
     int made = 0, items = 0, few_to = 0, last_b = -1;
@@ -1039,6 +1063,11 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       const DkvItem it(s, item_of(w));
       if (it.b != last_b) few_to = few_queries(s, it.b, lane);
       last_b = it.b;
+      if (it.total == 0) {
+        zero_rows<T>(a.out0, it.b, it.k0, s.Skv, it.kvh, s.Hkv, s.D);
+        zero_rows<T>(a.out1, it.b, it.k0, s.Skv, it.kvh, s.Hkv, s.D);
+        continue;
+      }
       const int k = it.k0 + r;
       const float f = grad_factor<T>(a.bound, it.b * s.Hkv + it.kvh);
       auto step = [&](auto few, int q0) {
@@ -1101,13 +1130,15 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         i = i + 1 < it.ni ? i + 1 : 0;
         ok = q0 < few_to ? step(std::true_type(), q0) : step(std::false_type(), q0);
       }
-      if (ok) ok = it.total > 0 ? warp_wait(done, items++ & 1, abort_flag) : warp_wait(kv_full, w & 1, abort_flag);
+      if (ok) ok = warp_wait(done, items & 1, abort_flag);
       tcgen05_fence_after();
       if (!ok) break;
-      bool real = k < s.Skv && it.total > 0;
+      bool real = k < s.Skv;
       if (real && s.mask != nullptr) real = s.mask[(int64_t)it.b * s.k_words + (k >> 5)] >> (k & 31) & 1;
       const int row = it.k0 + (warp & 3) * 32;
       const float un = 1.f / scale_of<T>();
+      const int slot = (made + L::kStages - 1) % L::kStages, mine_at = warp * (2 * L::kTile / kArith);
+      uint8_t* stage = sQG + (mine_at / L::kTile * L::kStages + slot) * L::kTile + mine_at % L::kTile;
       if (row < s.Skv) {
         // 32 columns at a time: those of dv, then those of dk
 #pragma unroll 1
@@ -1116,10 +1147,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           const bool is_v = x < D / 32;
           const int col = x % (D / 32) * 32;
           float o[32];
-          if (it.total > 0) {
-            tmem_ld32((is_v ? tV : tK) + mine + col, o);
-            tmem_ld_wait(o);
-          }
+          tmem_ld32((is_v ? tV : tK) + mine + col, o);
+          tmem_ld_wait(o);
           if (!real) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0.f;
@@ -1131,8 +1160,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       tcgen05_fence_before();
       if (lane == 0) {
         stores_read<0>();
-        mbar_arrive(kv_empty);
+        mbar_arrive(&staged[items & 1]);
       }
+      ++items;
       __syncwarp();
     }
     if (!ok && lane == 0) report(s.err, 73);
@@ -1179,7 +1209,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
   uint64_t* dp_full = s_full + 4;
   uint64_t* ds_full = s_full + 5;
   uint64_t* done = s_full + 6;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* staged = done + 1;                   // [2]: by the parity of the item
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(staged + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const Shape& s = a.s;
@@ -1187,7 +1218,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, kArith);
+    mbar_init(q_empty, 1);
+    mbar_init(&staged[0], kArith);
+    mbar_init(&staged[1], kArith);
     for (int i = 0; i < L::kK + L::kV; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -1215,26 +1248,36 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       prefetch_tmap(&tm_g);
       prefetch_tmap(&tm_k);
       prefetch_tmap(&tm_v);
+      // outputs are staged where the last step's keys were, as in the other pass
       bool ok = true;
-      int n = 0, w = 0;                            // steps before this item
-      for (; ok && item_of(w) < a.items; ++w) {
+      int n = 0, z = 0, waited = 0;                // steps and items before this item; items whose staging has been waited for
+      auto staged_before = [&](int item) {
+        for (; ok && waited < item; ++waited) ok = mbar_wait(&staged[waited & 1], waited >> 1 & 1, abort_flag);
+        if (!ok) report(s.err, 71);
+      };
+      for (int w = 0; ok && item_of(w) < a.items; ++w) {
         const DqItem it(s, item_of(w));
-        if (!mbar_wait(q_empty, (w & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
-        mbar_expect_tx(q_full, it.total > 0 ? 2 * L::kTile : 0);
-        if (it.total > 0) {
-          load_tile<D>(sQ, &tm_q, it.q0, it.h, it.b, q_full);
-          load_tile<D>(sG, &tm_g, it.q0, it.h, it.b, q_full);
-        }
+        if (it.total == 0) continue;
+        staged_before(z - 1);
+        if (!ok) break;
+        if (!mbar_wait(q_empty, (z & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
+        mbar_expect_tx(q_full, 2 * L::kTile);
+        load_tile<D>(sQ, &tm_q, it.q0, it.h, it.b, q_full);
+        load_tile<D>(sG, &tm_g, it.q0, it.h, it.b, q_full);
         for (int m = 0; m < 2 * it.total; ++m) {
           const int i = n + (m >> 1), x = m & 1, of = x ? L::kV : L::kK, at = x * L::kK + i % of;
+          if (x == 0 && (m >> 1) >= L::kK - 1) staged_before(z);
+          if (!ok) break;
           if (!mbar_wait(&empty[at], (i / of & 1) ^ 1, abort_flag)) { ok = false; report(s.err, 71); break; }
           mbar_expect_tx(&full[at], L::kTile);
           load_tile<D>(sKV + at * L::kTile, x ? &tm_v : &tm_k, (it.j0 + (m >> 1)) * kT, it.kvh, it.b, &full[at]);
         }
         n += it.total;
+        ++z;
       }
       if (!ok) {                                   // loads in flight end before the CTA does
-        mbar_wait_quiet(q_full, w & 1, 1 << 12);
+        mbar_wait_quiet(q_full, 0, 1 << 12);
+        mbar_wait_quiet(q_full, 1, 1 << 12);
         for (int i = 0; i < L::kK + L::kV; ++i) {
           mbar_wait_quiet(&full[i], 0, 1 << 12);
           mbar_wait_quiet(&full[i], 1, 1 << 12);
@@ -1249,15 +1292,15 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     auto k_at = [&](int n) { return n % L::kK; };
     auto v_at = [&](int n) { return L::kK + n % L::kV; };
     bool ok = true;
-    int base = 0, few_to = 0, last_b = -1;
+    int base = 0, z = 0, few_to = 0, last_b = -1;
     for (int w = 0; ok && item_of(w) < a.items; ++w) {
       const DqItem it(s, item_of(w));
       const int total = uniform(it.total);
       if (it.b != last_b) few_to = few_queries(s, it.b, lane);
       last_b = it.b;
       const bool few = uniform(rest_of_dq(s) || it.q0 < few_to);
-      ok = warp_wait(q_full, w & 1, abort_flag);
       if (total == 0) continue;
+      ok = warp_wait(q_full, z++ & 1, abort_flag);
       const int end = base + total;
       auto scores = [&](int n) {                  // q k^T, into the other tile
         if (!warp_wait(&full[k_at(n)], n / L::kK & 1, abort_flag) || !warp_wait(&s_free[n & 1], (n >> 1 & 1) ^ 1, abort_flag))
@@ -1277,6 +1320,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           mma_rows<D>(tP, gd, kv_rows + (uint64_t)(v_at(n) * (L::kTile >> 4)), idesc_s);
           umma_commit(dp_full);
           umma_commit(&empty[v_at(n)]);
+          if (n + 1 == end) umma_commit(q_empty);          // behind all scores: the next item's q and dO come
         }
         __syncwarp();
         return true;
@@ -1306,7 +1350,6 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // ---------------- a quarter of a query's keys to a thread ----------------
     const int qd = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16, lanes = mine + qd * 32;
-    uint8_t* stage = sQ + (qd % (D / 32) * 4 + (warp & 3)) * 2048;     // in the place of the queries, behind the last product
     const float c = s.scale_log2;
     bool ok = true;
     int made = 0, items = 0, few_to = 0, last_b = -1;
@@ -1315,6 +1358,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       if (it.b != last_b) few_to = few_queries(s, it.b, lane);
       last_b = it.b;
       const bool few = rest_of_dq(s) || it.q0 < few_to;
+      if (it.total == 0) {
+        zero_rows<T>(a.out0, it.b, it.q0, s.Sq, it.h, s.Hq, s.D);
+        continue;
+      }
       const int q = it.q0 + r;
       int klo, khi;
       row_keys(s, q, klo, khi);
@@ -1363,27 +1410,24 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
         hand_over(ds_full, lane);
       }
-      if (ok) ok = it.total > 0 ? warp_wait(done, items++ & 1, abort_flag) : warp_wait(q_full, w & 1, abort_flag);
+      if (ok) ok = warp_wait(done, items & 1, abort_flag);
       tcgen05_fence_after();
       if (!ok) break;
       const int row = it.q0 + (warp & 3) * 32;
+      uint8_t* stage = sKV + (made + L::kK - 1) % L::kK * L::kTile + (qd % (D / 32) * 4 + (warp & 3)) * 2048;
       if (qd < D / 32 && qd * 32 < s.D && row < s.Sq) {
         float o[32];
-        if (it.total > 0) {
-          tmem_ld32(tQ + mine + qd * 32, o);
-          tmem_ld_wait(o);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
+        tmem_ld32(tQ + mine + qd * 32, o);
+        tmem_ld_wait(o);
         stage32<T>(stage, o, s.scale / (scale_of<T>() * f), lane);
         if (lane == 0) store32(&tm_dq, stage, qd * 32, row, it.h, it.b);
       }
       tcgen05_fence_before();
       if (lane == 0) {
         stores_read<0>();
-        mbar_arrive(q_empty);
+        mbar_arrive(&staged[items & 1]);
       }
+      ++items;
       __syncwarp();
     }
     if (!ok && lane == 0) report(s.err, 73);
@@ -1554,9 +1598,10 @@ int run_bwd(const Shape& s, const Tensor4& q, const Tensor4& k, const Tensor4& v
   const int longest = bound != nullptr && s.Skv > s.Sq ? s.Skv : s.Sq;
   const dim3 prep_grid((longest + kT - 1) / kT, s.Hq + (bound != nullptr ? s.Hkv : 0), s.B);
   attn_prep_kernel<T, D / 8><<<prep_grid, 256, 0, stream>>>(p);
-  BwdArgs a = {s, nlse, delta, pieces, bound, items_of(s, s.Hkv, s.Skv, kT)};
+  BwdArgs a = {s, nlse, delta, pieces, bound, dk, dv, items_of(s, s.Hkv, s.Skv, kT)};
   attn_dkv_kernel<T, D><<<grid_of(a.items), kThreads, smem, stream>>>(tq, tk, tv, tg, tdk, tdv, a);
   a.items = items_of(s, s.Hq, s.Sq, kT);
+  a.out0 = dq;
   attn_dq_kernel<T, D><<<grid_of(a.items), kThreads, smem_q, stream>>>(tq, tk, tv, tg, tdq, a);
   return (int)cudaGetLastError();
 }

@@ -254,3 +254,15 @@ def test_offsets_past_32_bits():
     for name, (exact, tol) in want.items():
         off = (got[name][:, :, -n:].double() - exact[:, :, -n:]).abs() / tol[:, :, -n:]
         assert float(off.nan_to_num(nan=math.inf).max()) <= 1.0, name
+
+
+@pytest.mark.parametrize("Sq,Skv,window", [(100, 1500, 30), (1500, 300, 0), (900, 700, 200)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_that_nothing_sees(Sq, Skv, window, D):
+    """Between tiles with work: blocks of keys before all windows, and blocks of queries before the first key."""
+    q, k, v, g = _inputs(3, 16, 8, Sq, Skv, D, torch.bfloat16, 17)
+    got = _check(q, k, v, g, window=window)
+    if Sq < Skv:
+        assert not got["dk"][:, :, : Skv - Sq - window].any() and not got["dv"][:, :, : Skv - Sq - window].any()
+    else:
+        assert not got["out"][:, :, : Sq - Skv].any() and not got["dq"][:, :, : Sq - Skv].any()
