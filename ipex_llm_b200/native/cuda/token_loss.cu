@@ -148,6 +148,43 @@ __device__ __forceinline__ void unpack(const uint4& w, float* f) {
   }
 }
 
+// The larger ones of two pairs of 16-bit numbers; a number before NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// The largest element of `n` (1 to kU) vectors that lie kNT apart.  16-bit numbers by pairs, as they are.
+template <typename T>
+__device__ __forceinline__ float largest_of(const uint4* w, int n) {
+  if constexpr (std::is_same<T, float>::value) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (u >= n) break;
+      float f[4];
+      unpack<T>(w[u * kNT], f);
+      mx = max3(max3(mx, f[0], f[1]), f[2], f[3]);
+    }
+    return mx;
+  } else {
+    const uint4 v = w[0];
+    uint32_t a = max2<T>(v.x, v.y), b = max2<T>(v.z, v.w);
+#pragma unroll
+    for (int u = 1; u < kU; ++u) {
+      if (u >= n) break;
+      const uint4 x = w[u * kNT];
+      a = max2<T>(a, max2<T>(x.x, x.y));
+      b = max2<T>(b, max2<T>(x.z, x.w));
+    }
+    a = max2<T>(a, b);
+    const T* e = reinterpret_cast<const T*>(&a);
+    return max3(-INFINITY, DT<T>::to_f(e[0]), DT<T>::to_f(e[1]));
+  }
+}
+
 // Larger keys come first: by value (NaN above all), then by the lower index.  No element has key 0.
 __device__ __forceinline__ uint64_t order_key(float v, int idx) {
   const uint32_t b = v != v ? 0x7FFFFFFFu : __float_as_uint(v == 0.f ? 0.f : v);   // -0 and 0 are equal
@@ -289,15 +326,7 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
       continue;
     }
     const int n = min(kU, (sl.v1 - base - tid + kNT - 1) / kNT);    // vectors of this thread
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (u >= n) break;
-      float f[VEC];
-      unpack<T>(w[u * kNT], f);
-#pragma unroll
-      for (int i = 0; i < VEC; i += 2) mx = max3(mx, f[i], f[i + 1]);
-    }
+    float mx = largest_of<T>(w, n);
     const float r = fmaxf(st.r, rintf(__fmul_rn(mx, c))), to = base_of(r);
     const float down = held(st.r - to), fac = ex2(down);
     // CAREFUL: with exponents held, for what hides tokens
