@@ -330,12 +330,12 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
     const float r = fmaxf(st.r, rintf(__fmul_rn(mx, c))), to = base_of(r);
     const float down = held(st.r - to), fac = ex2(down);
     // CAREFUL: with exponents held, for what hides tokens
-    auto sums = [&](auto careful, float& s, float& t) {
-      constexpr bool CAREFUL = decltype(careful)::value;
+    auto sums = [&](auto careful, auto whole, float& s, float& t) {
+      constexpr bool CAREFUL = decltype(careful)::value, WHOLE = decltype(whole)::value;
       float sa[2] = {0.f, 0.f}, ta[2] = {0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        if (u >= n) break;
+        if (!WHOLE && u >= n) break;
         float f[VEC], e[VEC], v[2] = {0.f, 0.f};
         unpack<T>(w[u * kNT], f);
 #pragma unroll
@@ -366,8 +366,9 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
       t = ta[0] + ta[1];
     };
     float s, t;
-    sums(std::false_type(), s, t);
-    if (ENT && t != t) sums(std::true_type(), s, t);
+    if (n == kU) sums(std::false_type(), std::true_type(), s, t);
+    else sums(std::false_type(), std::false_type(), s, t);
+    if (ENT && t != t) sums(std::true_type(), std::false_type(), s, t);
     if constexpr (ENT) st.t = (st.t + st.s * down) * fac + t;
     else if constexpr (TAIL) st.t = st.t * fac + t;
     st.s = st.s * fac + s;
