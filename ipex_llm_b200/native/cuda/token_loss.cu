@@ -157,13 +157,13 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   return d;
 }
 // The largest element of `n` (1 to kU) vectors that lie kNT apart.  16-bit numbers by pairs, as they are.
-template <typename T>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ float largest_of(const uint4* w, int n) {
   if constexpr (std::is_same<T, float>::value) {
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (u >= n) break;
+      if (!WHOLE && u >= n) break;
       float f[4];
       unpack<T>(w[u * kNT], f);
       mx = max3(max3(mx, f[0], f[1]), f[2], f[3]);
@@ -174,7 +174,7 @@ __device__ __forceinline__ float largest_of(const uint4* w, int n) {
     uint32_t a = max2<T>(v.x, v.y), b = max2<T>(v.z, v.w);
 #pragma unroll
     for (int u = 1; u < kU; ++u) {
-      if (u >= n) break;
+      if (!WHOLE && u >= n) break;
       const uint4 x = w[u * kNT];
       a = max2<T>(a, max2<T>(x.x, x.y));
       b = max2<T>(b, max2<T>(x.z, x.w));
@@ -326,7 +326,7 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
       continue;
     }
     const int n = min(kU, (sl.v1 - base - tid + kNT - 1) / kNT);    // vectors of this thread
-    float mx = largest_of<T>(w, n);
+    float mx = n == kU ? largest_of<T, true>(w, n) : largest_of<T, false>(w, n);
     const float r = fmaxf(st.r, rintf(__fmul_rn(mx, c))), to = base_of(r);
     const float down = held(st.r - to), fac = ex2(down);
     // CAREFUL: with exponents held, for what hides tokens
