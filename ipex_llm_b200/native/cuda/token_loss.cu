@@ -12,8 +12,9 @@
 // parts are joined.  Seven warps of a CTA read; an eighth does what a row has beside its sums (its target, the teacher's tokens,
 // the results), on this row while the others read it and on its sums while they read the next one: in their way, those latencies
 // took half of the time.  Four such CTAs to an SM: what is left of a row's latencies (the joining of its sums) hides behind the
-// other CTAs' rows (2048 rows of 32000 in bf16: 38 us, 3.5 TB/s; two CTAs of sixteen warps 47 us; the divergence 37 against
-// 52 us).  Backward is a plain pass of 224 threads to a row, four vectors in flight (43 us for these rows, 6.1 TB/s).
+// other CTAs' rows (2048 rows of 32000 in bf16: 38 us, with two CTAs of sixteen warps 47; the divergence 37 against 52 us).  Then
+// instructions are the bound, and maxima by pairs of 16-bit numbers, as they are, and whole batches without a test for each vector
+// make it 34 us (3.9 TB/s; both measured by themselves: 35.6 and 34).  Backward is a plain pass of 224 threads to a row, four vectors in flight (43 us for these rows, 6.1 TB/s).
 // A thread folds the maximum of a batch into its own and rescales its sums once for all of it, so that an element costs one
 // exponential (0.73 of what the special function units do at the rate of memory, for 16-bit logits).
 // y is one fma: what rounding takes from r, common to a row, takes part everywhere alike and so cancels, as long as r is the same
