@@ -265,6 +265,7 @@ def t5_dense_forward(self, hidden_states):
 # attention interface of transformers 5: every model whose attention goes through ALL_ATTENTION_FUNCTIONS
 # ------------------------------------------------------------------------------------------------
 ATTN_INTERFACE_NAME = "ipex_llm"
+TRAIN_INTERFACE_NAME = "ipex_llm_train"        # models/train_attention.py
 
 
 def attention_interface(module, query, key, value, attention_mask=None, dropout: float = 0.0, scaling=None,

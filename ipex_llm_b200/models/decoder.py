@@ -19,7 +19,7 @@ import math
 import torch
 
 from ..ops.kv_cache import CompressLayer, is_ipex_cache
-from .common import apply_rotary_pos_emb, scaled_dot_product_attention
+from .common import TRAIN_INTERFACE_NAME, apply_rotary_pos_emb, scaled_dot_product_attention
 from .utils import select_cache
 
 
@@ -124,6 +124,13 @@ def decoder_attention_forward(self, hidden_states, position_embeddings=None, att
     mask = attention_mask
     if mask is not None and mask.dim() == 4 and mask.shape[-1] != kv_len:
         mask = mask[..., :kv_len] if mask.shape[-1] > kv_len else None
+    if not alibi and getattr(self.config, "_attn_implementation", None) == TRAIN_INTERFACE_NAME:
+        from .train_attention import is_compact, train_attention_interface, whole_mask
+        if is_compact(mask) and mask.shape[1] != kv_len:
+            mask = whole_mask(mask, q_len)[..., :kv_len]
+        attn_output, _ = train_attention_interface(self, q, k, v, mask, scaling=scaling, is_causal=mask is None and q_len > 1,
+                                                   softcap=softcap, sliding_window=sliding_window)
+        return self.o_proj(attn_output.reshape(bsz, q_len, -1)), None
     if alibi:
         mask = alibi_mask(q.shape[1], q_len, kv_len, mask, q.dtype, q.device)
     attn_output = scaled_dot_product_attention(q, k, v, mask, is_causal=(mask is None and q_len > 1),

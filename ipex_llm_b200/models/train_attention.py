@@ -1,18 +1,40 @@
 """The attention with a gradient behind the transformers attention interface, for finetuning: a decoder whose attention goes
-through the registry runs ``ops.train_attn.attention`` where that can compute it, and the package's usual path elsewhere
-(soft-capped scores, dropout, masks that are neither padding nor a window, other types and head sizes, single tokens).
+through the registry, or through this package's own decoder forward, runs ``ops.train_attn.attention`` where that can compute
+it, and the package's usual path elsewhere (soft-capped scores, dropout, masks that are neither padding nor a window, other
+types and head sizes, single tokens).
 
-Masks: a causal mask, with or without a window, stays what it is, and padding stays ``[batch, keys]`` truth values; no mask of
-the size of queries x keys is made for them.
+Masks: a causal mask, with or without a window, stays what it is, and padding stays ``[batch, keys]``; no mask of the size of
+queries x keys is made for them.  Padding travels in a type that no arithmetic takes (``_compact``): a module that would use it
+in a way of its own raises, where truth values ``[batch, keys]`` would pass for a mask of scores without a causal limit.
 """
 from __future__ import annotations
 
 import torch
 
 from ..ops.train_attn import MAX_DIM, MAX_HEADS, attention
-from .common import _uses_attention_registry, attention_interface
+from .common import TRAIN_INTERFACE_NAME, _uses_attention_registry, attention_interface
+from .decoder import decoder_attention_forward
 
-TRAIN_INTERFACE_NAME = "ipex_llm_train"
+_CARRIER = torch.float8_e5m2       # the bytes of truth values; sums, products, comparisons with other types and SDPA refuse it
+
+
+def _compact(padding):
+    """Truth values [batch, keys] (or None) as this interface's masks carry them."""
+    return None if padding is None else (padding if padding.dtype == torch.bool else padding != 0).view(_CARRIER)
+
+
+def is_compact(mask) -> bool:
+    return mask is not None and mask.dtype == _CARRIER
+
+
+def whole_mask(mask, q_length: int):
+    """The truth values [batch, 1, queries, keys] that one of this interface's masks stands for; other masks as they are."""
+    if not is_compact(mask):
+        return mask
+    kv_length = mask.shape[1]
+    q = torch.arange(q_length, device=mask.device).view(-1, 1) + (kv_length - q_length)
+    key = torch.arange(kv_length, device=mask.device)
+    return mask.view(torch.bool)[:, None, None, :] & (key <= q)
 
 
 def _is_window(mask_function, q_length: int, kv_length: int, window: int, device) -> bool:
@@ -37,24 +59,11 @@ def _mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_functio
     ends = not torch.is_tensor(q_offset) and q_length > 1 and kv_offset == 0 and q_offset + q_length == kv_length
     if ends and (attention_mask is None or attention_mask.shape == (batch_size, kv_length)):
         if mask_function is causal_mask_function:
-            return attention_mask
+            return _compact(attention_mask)
         if window and _is_window(mask_function, q_length, kv_length, window, device):
-            return attention_mask
+            return _compact(attention_mask)
     return sdpa_mask(batch_size=batch_size, q_length=q_length, kv_length=kv_length, q_offset=q_offset, kv_offset=kv_offset,
                      mask_function=mask_function, attention_mask=attention_mask, **kwargs)
-
-
-def _whole_mask(key_mask, q_length: int, causal: bool, window: int):
-    """The mask [batch, 1, queries, keys] that a padding mask stands for."""
-    kv_length = key_mask.shape[1]
-    see = key_mask.bool()[:, None, None, :].expand(-1, 1, q_length, -1)
-    if causal:
-        q = torch.arange(q_length, device=key_mask.device).view(-1, 1) + (kv_length - q_length)
-        key = torch.arange(kv_length, device=key_mask.device)
-        see = see & (key <= q)
-        if window:
-            see = see & (key > q - window)
-    return see
 
 
 def train_attention_interface(module, query, key, value, attention_mask=None, dropout: float = 0.0, scaling=None,
@@ -68,7 +77,7 @@ def train_attention_interface(module, query, key, value, attention_mask=None, dr
     Hkv, Skv = k.shape[1:3]
     causal = getattr(module, "is_causal", True) if is_causal is None else bool(is_causal)
     window = int(sliding_window or 0) if causal and (sliding_window or 0) < Skv else 0
-    padding = attention_mask is not None and attention_mask.dim() == 2
+    padding = is_compact(attention_mask)
     causal = causal or padding
     scale = D ** -0.5 if scaling is None else float(scaling)
     fits = (attention_mask is None or padding) and (torch.is_grad_enabled() or module.training) and Sq > 1 \
@@ -78,16 +87,30 @@ def train_attention_interface(module, query, key, value, attention_mask=None, dr
     if fits and q.is_cuda:
         fits = q.dtype in (torch.float16, torch.bfloat16) and D <= MAX_DIM and D % 8 == 0 and Hq + Hkv <= MAX_HEADS
     if fits:
-        return attention(q, k, v, scale, causal, window, attention_mask if padding else None).transpose(1, 2), None
+        key_mask = attention_mask.view(torch.bool) if padding else None
+        return attention(q, k, v, scale, causal, window, key_mask).transpose(1, 2), None
     if padding:
-        attention_mask = _whole_mask(attention_mask, Sq, causal, window)
+        attention_mask = whole_mask(attention_mask, Sq)
+        if window:
+            at = torch.arange(Skv, device=q.device)
+            attention_mask = attention_mask & (at > at[Skv - Sq:].view(-1, 1) - window)
     return attention_interface(module, query, key, value, attention_mask, dropout, scaling, is_causal, softcap, sliding_window,
                                **kwargs)
 
 
+def _dispatches(mod) -> bool:
+    """Does the attention of this module reach the interface: by the registry, or by this package's decoder forward (which a model
+    that was optimised has bound to its attention modules)?  With linear attention biases it has masks of its own."""
+    if getattr(mod.config, "ipex_alibi", False) or not _uses_attention_registry(mod):
+        return False
+    bound = [getattr(m.forward, "__func__", m.forward) for m in mod.modules()
+             if "forward" in m.__dict__ and "Attention" in type(m).__name__]
+    return all(f is decoder_attention_forward for f in bound)
+
+
 def use_train_attention(model) -> bool:
-    """Point every sub-model whose attention goes through the registry at ``train_attention_interface``; the others keep theirs.
-    False when there is none."""
+    """Point every sub-model whose attention reaches it at ``train_attention_interface``; the others keep theirs.  False when
+    there is none."""
     try:
         from transformers import AttentionInterface, AttentionMaskInterface
     except ImportError:
@@ -97,8 +120,10 @@ def use_train_attention(model) -> bool:
     found = {}
     for mod in model.modules():
         cfg = getattr(mod, "config", None)
-        if cfg is not None and hasattr(cfg, "to_dict") and _uses_attention_registry(mod):
-            found[id(cfg)] = cfg
-    for cfg in found.values():
+        if cfg is not None and hasattr(cfg, "to_dict"):
+            found.setdefault(id(cfg), []).append(mod)
+    found = [mods[0].config for mods in found.values() if any(map(_uses_attention_registry, mods)) and
+             all(_dispatches(m) for m in mods if _uses_attention_registry(m))]
+    for cfg in found:
         cfg._attn_implementation = TRAIN_INTERFACE_NAME
     return bool(found)

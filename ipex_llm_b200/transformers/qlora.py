@@ -337,7 +337,7 @@ def prepare_model_for_kbit_training(model, use_gradient_checkpointing=True, grad
     checkpointed blocks get gradients, and switch gradient checkpointing on (reference qlora.py:304-352).
 
     ``use_fused_attention``: attention by ``ops.train_attn.attention``, which holds nothing of the size of queries x keys, where
-    the model's attention goes through transformers' registry (refused where none does)."""
+    the model's attention goes through transformers' registry or this package's decoder forward (refused where none does)."""
     if use_fused_attention:
         from ..models.train_attention import use_train_attention
         invalidInputError(use_train_attention(model), "use_fused_attention: this model's attention does not go through transformers' "

@@ -1,0 +1,139 @@
+"""The attention with a gradient inside models of other kinds and makes than plain decoders: what they compute stays what the
+library's attention computes, on the CPU."""
+import copy
+
+import pytest
+import torch
+
+from ipex_llm_b200.models import train_attention
+from ipex_llm_b200.models.train_attention import TRAIN_INTERFACE_NAME, use_train_attention
+
+# Two paths in 32 bits over the same weights: a layer of these rounds some 100 numbers on a path (norms, products of up to 96
+# terms, soft-max, residuals), each by 2^-24 of the largest number at hand; two layers, both paths, and 4 for what they amplify.
+TOL = 2 * 2 * 100 * 4 * 2.0 ** -24
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The windows that the attention with a gradient was called with."""
+    got, usual = [], train_attention.attention
+    monkeypatch.setattr(train_attention, "attention", lambda *a: got.append(a[5]) or usual(*a))
+    return got
+
+
+BASE = dict(hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, vocab_size=97,
+            max_position_embeddings=128, tie_word_embeddings=False, attn_implementation="sdpa", pad_token_id=0)
+
+
+def _model(name, **kw):
+    import transformers as tr
+    torch.manual_seed(1)
+    return getattr(tr, name + "ForCausalLM")(getattr(tr, name + "Config")(**{**BASE, **kw})).train()
+
+
+def _inputs(pad, batch=2, tokens=13):
+    ids = torch.randint(1, 97, (batch, tokens), generator=torch.Generator().manual_seed(2))
+    if pad == "none":
+        return dict(input_ids=ids)
+    real = torch.ones_like(ids)
+    if pad == "left":
+        real[-1, :4] = 0
+    if pad == "right":
+        real[-1, 9:] = 0
+    return dict(input_ids=ids, attention_mask=real)
+
+
+def _same(model, own, args):
+    x, y = (m(**args).logits for m in (model, own))
+    off = (x - y).abs()
+    if "attention_mask" in args:
+        off = off * args["attention_mask"].unsqueeze(-1)
+    assert off.max() <= TOL * x.abs().max()
+
+
+def _optimised(model):
+    from ipex_llm_b200.transformers.convert import _optimize_post, _optimize_pre
+    return _optimize_post(_optimize_pre(model))
+
+
+@pytest.mark.parametrize("name,kw", [("Llama", {}), ("Mistral", dict(sliding_window=64)), ("Qwen2", {}), ("Gemma", dict(head_dim=16)),
+                                     ("Phi3", {}), ("Glm4", dict(head_dim=16))])
+@pytest.mark.parametrize("use_cache", [False, True])
+@pytest.mark.parametrize("batch", [1, 2])
+@pytest.mark.parametrize("pad", ["none", "ones", "left", "right"])
+def test_optimised_models(name, kw, use_cache, batch, pad, calls):
+    """Models loaded with their optimisations run this package's decoder forward: it takes the attention with a gradient, too."""
+    model = _optimised(_model(name, **kw))
+    own = copy.deepcopy(model)
+    assert use_train_attention(own) and own.config._attn_implementation == TRAIN_INTERFACE_NAME
+    _same(model, own, dict(_inputs(pad, batch), use_cache=use_cache))
+    assert calls == [0, 0]
+
+
+@pytest.mark.parametrize("pad", ["none", "ones"])
+def test_no_logit_depends_on_a_later_token(pad, calls):
+    own = _optimised(_model("Llama"))
+    assert use_train_attention(own)
+    args = dict(_inputs(pad, batch=1), use_cache=False)
+    first = own(**args).logits
+    args["input_ids"] = args["input_ids"].clone()
+    args["input_ids"][0, -1] = args["input_ids"][0, -1] % 96 + 1
+    again = own(**args).logits
+    assert torch.equal(first[:, :-1], again[:, :-1]) and not torch.equal(first[:, -1], again[:, -1]) and len(calls) == 4
+
+
+def test_optimised_models_by_the_public_calls(calls):
+    """As a user loads and prepares one: the mask of ones that the collator gives, one sequence and several."""
+    from transformers import LlamaConfig
+    from ipex_llm.transformers import AutoModelForCausalLM
+    from ipex_llm.transformers.qlora import prepare_model_for_kbit_training
+
+    def load(fused):
+        torch.manual_seed(0)
+        cfg = LlamaConfig(**{**BASE, "attn_implementation": None})
+        m = AutoModelForCausalLM.from_config(cfg, load_in_low_bit="nf4", torch_dtype=torch.float32, device="cpu", seed=0,
+                                             modules_to_not_convert=["lm_head"])
+        return prepare_model_for_kbit_training(m, use_gradient_checkpointing=False, use_fused_attention=fused).train()
+
+    usual, fused = load(False), load(True)
+    for batch in (1, 2):
+        for pad in ("none", "ones", "right"):
+            args = _inputs(pad, batch)
+            calls.clear()
+            _same(usual, fused, args)
+            assert calls == [0, 0]
+
+
+def test_generation_of_optimised_models():
+    own = _optimised(_model("Llama"))
+    usual = copy.deepcopy(own)
+    assert use_train_attention(own)
+    args = _inputs("left")
+    a, b = (m.eval().generate(**args, max_new_tokens=7, do_sample=False) for m in (usual, own))
+    assert torch.equal(a, b)
+
+
+def test_attention_forwards_of_other_makes_are_left_alone():
+    """A forward bound to the attention modules that does not reach the interface keeps its masks."""
+    import types
+    model = _model("Llama")
+
+    def forward(self, hidden_states, position_embeddings=None, attention_mask=None, **kwargs):
+        return type(self).forward(self, hidden_states, position_embeddings, attention_mask, **kwargs)
+
+    model.model.layers[1].self_attn.forward = types.MethodType(forward, model.model.layers[1].self_attn)
+    assert not use_train_attention(model) and model.config._attn_implementation == "sdpa"
+    alibi = _model("Llama")
+    alibi.config.ipex_alibi = True
+    assert not use_train_attention(alibi)
+
+
+def test_padding_is_no_mask_of_scores():
+    """What carries padding cannot be added to scores, multiplied with them or handed to the library's attention."""
+    mask = train_attention._compact(torch.ones(1, 5, dtype=torch.long))
+    scores, q = torch.zeros(1, 2, 5, 5), torch.zeros(1, 2, 5, 8)
+    for use in (lambda: scores + mask, lambda: scores * mask, lambda: (1.0 - mask) * -1e4, lambda: scores.masked_fill(mask, 0.0),
+                lambda: torch.where(mask, scores, 0.0), lambda: mask[:, :, :, :5],
+                lambda: torch.nn.functional.scaled_dot_product_attention(q, q, q, attn_mask=mask)):
+        with pytest.raises((RuntimeError, NotImplementedError, IndexError)):
+            use()
