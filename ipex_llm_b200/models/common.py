@@ -282,8 +282,15 @@ def attention_interface(module, query, key, value, attention_mask=None, dropout:
     if mask is not None and mask.dim() == 4 and mask.shape[-1] > key.shape[2]:
         mask = mask[..., : key.shape[2]]
     if dropout and module.training:
-        # training with attention dropout keeps the library path
+        # training with attention dropout keeps the library path, which knows no window and counts the causal limit from the
+        # first key
         import torch.nn.functional as F_
+        q_len, kv_len = query.shape[2], key.shape[2]
+        window = sliding_window if sliding_window and sliding_window < kv_len else 0
+        if mask is None and is_causal and (window or q_len != kv_len):
+            at = torch.arange(kv_len, device=query.device)
+            last = torch.arange(kv_len - q_len, kv_len, device=query.device).view(-1, 1)
+            mask = (at <= last) & (at > last - window) if window else at <= last
         k2, v2 = repeat_kv(key, query.shape[1] // key.shape[1]), repeat_kv(value, query.shape[1] // key.shape[1])
         out = F_.scaled_dot_product_attention(query, k2, v2, attn_mask=mask, dropout_p=dropout, scale=scaling,
                                               is_causal=bool(is_causal) and mask is None)

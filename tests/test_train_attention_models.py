@@ -137,3 +137,33 @@ def test_padding_is_no_mask_of_scores():
                 lambda: torch.nn.functional.scaled_dot_product_attention(q, q, q, attn_mask=mask)):
         with pytest.raises((RuntimeError, NotImplementedError, IndexError)):
             use()
+
+
+# Attention dropout this rare drops nothing in a few thousand numbers (chance 1e-5), but takes the path that drops.
+RARELY = 1e-9
+
+
+@pytest.mark.parametrize("name,kw,window", [("Llama", {}, 0), ("Mistral", dict(sliding_window=5), 5), ("Phi3", dict(sliding_window=7), 7)])
+@pytest.mark.parametrize("pad", ["none", "ones", "left", "right"])
+def test_dropout_keeps_the_mask(name, kw, window, pad, calls):
+    model = _model(name, attention_dropout=RARELY, **kw)
+    own = copy.deepcopy(model)
+    assert use_train_attention(own)
+    _same(model, own, dict(_inputs(pad), use_cache=False))
+    assert calls == []
+
+
+@pytest.mark.parametrize("Sq,Skv,window", [(9, 9, 4), (5, 12, 0), (5, 12, 3), (5, 12, 100)])
+def test_dropout_of_windows_and_of_queries_behind_earlier_keys(Sq, Skv, window):
+    from ipex_llm_b200.models.train_attention import train_attention_interface
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(2, h, s, 16, generator=g, dtype=torch.float64) for h, s in ((4, Sq), (2, Skv), (2, Skv)))
+    module = torch.nn.Module().train()
+    for d in (0.0, RARELY):
+        got, _ = train_attention_interface(module, q, k, v, None, dropout=d, sliding_window=window or None)
+        last, key = torch.arange(Skv - Sq, Skv).view(-1, 1), torch.arange(Skv)
+        see = (key <= last) & (key > last - (window or Skv))
+        s = (q @ k.repeat_interleave(2, 1).transpose(-1, -2) / 4).masked_fill(~see, -torch.inf)
+        want = (torch.softmax(s, -1) @ v.repeat_interleave(2, 1)).transpose(1, 2)
+        # sums of a few numbers in 64 bits; what is kept is scaled by 1 / (1 - RARELY)
+        assert (got - want).abs().max() <= 1e-13 + 10 * RARELY * bool(d)
