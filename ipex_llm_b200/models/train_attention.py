@@ -4,8 +4,9 @@ it, and the package's usual path elsewhere (soft-capped scores, dropout, masks t
 types and head sizes, single tokens).
 
 Masks: a causal mask, with or without a window, stays what it is, and padding stays ``[batch, keys]``; no mask of the size of
-queries x keys is made for them.  Padding travels in a type that no arithmetic takes (``_compact``): a module that would use it
-in a way of its own raises, where truth values ``[batch, keys]`` would pass for a mask of scores without a causal limit.
+queries x keys is kept for them (a window's is looked at once, to see that it is one).  Padding and windows travel in a type
+that no arithmetic takes (``_compact``): a module that would use such a mask in a way of its own raises, where truth values
+``[batch, keys]`` would pass for a mask of scores without a causal limit.
 """
 from __future__ import annotations
 
@@ -18,23 +19,37 @@ from .decoder import decoder_attention_forward
 _CARRIER = torch.float8_e5m2       # the bytes of truth values; sums, products, comparisons with other types and SDPA refuse it
 
 
-def _compact(padding):
-    """Truth values [batch, keys] (or None) as this interface's masks carry them."""
-    return None if padding is None else (padding if padding.dtype == torch.bool else padding != 0).view(_CARRIER)
+def _compact(padding, window: int = 0, kv_length: int = 0, device=None):
+    """What this interface's masks are, beside None (causal attention over all keys): truth values [batch, keys], and with a
+    window [batch, keys, window] of stride 0, or [0, keys, window] where no key is hidden.  The window has to come with the mask:
+    not every attention module hands it on, and it goes through whatever passes a tensor's shape on."""
+    if padding is None:
+        return torch.empty((0, kv_length, window), dtype=_CARRIER, device=device) if window else None
+    padding = (padding if padding.dtype == torch.bool else padding != 0).view(_CARRIER)
+    return padding.unsqueeze(2).expand(-1, -1, window) if window else padding
 
 
 def is_compact(mask) -> bool:
     return mask is not None and mask.dtype == _CARRIER
 
 
+def _parts(mask):
+    """The truth values [batch, keys] (None: all keys) and the window (0: none) of a compact mask."""
+    if mask.dim() == 2:
+        return mask.view(torch.bool), 0
+    return mask[..., 0].view(torch.bool) if mask.shape[0] else None, mask.shape[2]
+
+
 def whole_mask(mask, q_length: int):
-    """The truth values [batch, 1, queries, keys] that one of this interface's masks stands for; other masks as they are."""
+    """The truth values [batch or 1, 1, queries, keys] that one of this interface's masks stands for; other masks as they are."""
     if not is_compact(mask):
         return mask
+    padding, window = _parts(mask)
     kv_length = mask.shape[1]
     q = torch.arange(q_length, device=mask.device).view(-1, 1) + (kv_length - q_length)
     key = torch.arange(kv_length, device=mask.device)
-    return mask.view(torch.bool)[:, None, None, :] & (key <= q)
+    see = (key <= q) & (key > q - window) if window else key <= q
+    return see[None, None] if padding is None else padding[:, None, None, :] & see
 
 
 def _is_window(mask_function, q_length: int, kv_length: int, window: int, device) -> bool:
@@ -50,8 +65,7 @@ def _is_window(mask_function, q_length: int, kv_length: int, window: int, device
 
 
 def _mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None, **kwargs):
-    """None or the padding mask [batch, keys] for causal attention over all keys or a window of them; else the mask that the usual
-    path takes."""
+    """None or a compact mask for causal attention over all keys or a window of them; else the mask that the usual path takes."""
     from transformers.masking_utils import causal_mask_function, sdpa_mask
     window, device = kwargs.get("local_size"), kwargs.get("device", "cpu")
     if attention_mask is not None:
@@ -61,7 +75,7 @@ def _mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_functio
         if mask_function is causal_mask_function:
             return _compact(attention_mask)
         if window and _is_window(mask_function, q_length, kv_length, window, device):
-            return _compact(attention_mask)
+            return _compact(attention_mask, window if window < kv_length else 0, kv_length, device)
     return sdpa_mask(batch_size=batch_size, q_length=q_length, kv_length=kv_length, q_offset=q_offset, kv_offset=kv_offset,
                      mask_function=mask_function, attention_mask=attention_mask, **kwargs)
 
@@ -75,25 +89,29 @@ def train_attention_interface(module, query, key, value, attention_mask=None, dr
         q, k, v = q.to(dt), k.to(dt), v.to(dt)
     Hq, Sq, D = q.shape[1:]
     Hkv, Skv = k.shape[1:3]
-    causal = getattr(module, "is_causal", True) if is_causal is None else bool(is_causal)
-    window = int(sliding_window or 0) if causal and (sliding_window or 0) < Skv else 0
-    padding = is_compact(attention_mask)
-    causal = causal or padding
+    compact, padding = is_compact(attention_mask), None
+    causal = compact or bool(getattr(module, "is_causal", True) if is_causal is None else is_causal)
+    window = int(sliding_window or 0)
+    if compact:
+        padding, own = _parts(attention_mask)
+        window = own or window
+    window = window if causal and window < Skv else 0
     scale = D ** -0.5 if scaling is None else float(scaling)
-    fits = (attention_mask is None or padding) and (torch.is_grad_enabled() or module.training) and Sq > 1 \
+    fits = (attention_mask is None or compact) and (torch.is_grad_enabled() or module.training) and Sq > 1 \
         and Sq <= Skv and not softcap and not (dropout and module.training) and k.shape == v.shape and Hq % Hkv == 0 \
         and 1e-4 <= scale <= 1e4 and q.dtype == k.dtype == v.dtype and q.device == k.device == v.device \
         and not any(torch.is_tensor(t) for n, t in kwargs.items() if n in ("position_bias", "s_aux", "sinks"))
     if fits and q.is_cuda:
         fits = q.dtype in (torch.float16, torch.bfloat16) and D <= MAX_DIM and D % 8 == 0 and Hq + Hkv <= MAX_HEADS
     if fits:
-        key_mask = attention_mask.view(torch.bool) if padding else None
-        return attention(q, k, v, scale, causal, window, key_mask).transpose(1, 2), None
-    if padding:
-        attention_mask = whole_mask(attention_mask, Sq)
-        if window:
-            at = torch.arange(Skv, device=q.device)
-            attention_mask = attention_mask & (at > at[Skv - Sq:].view(-1, 1) - window)
+        return attention(q, k, v, scale, causal, window, padding).transpose(1, 2), None
+    if compact:
+        if padding is None:
+            attention_mask, is_causal, sliding_window = None, True, window or None
+        else:
+            if attention_mask.dim() == 2 and window:
+                attention_mask = _compact(padding, window)
+            attention_mask = whole_mask(attention_mask, Sq)
     return attention_interface(module, query, key, value, attention_mask, dropout, scaling, is_causal, softcap, sliding_window,
                                **kwargs)
 

@@ -167,3 +167,65 @@ def test_dropout_of_windows_and_of_queries_behind_earlier_keys(Sq, Skv, window):
         want = (torch.softmax(s, -1) @ v.repeat_interleave(2, 1)).transpose(1, 2)
         # sums of a few numbers in 64 bits; what is kept is scaled by 1 / (1 - RARELY)
         assert (got - want).abs().max() <= 1e-13 + 10 * RARELY * bool(d)
+
+
+MOE = dict(num_experts=4, num_local_experts=4, num_experts_per_tok=2, moe_intermediate_size=32, sliding_window=5)
+
+
+@pytest.mark.parametrize("name,kw", [("Qwen2Moe", dict(use_sliding_window=True, max_window_layers=0, layer_types=["sliding_attention"] * 2,
+                                                       shared_expert_intermediate_size=32)),
+                                     ("Phimoe", {}), ("Mixtral", {})])
+@pytest.mark.parametrize("optimised", [False, True])
+@pytest.mark.parametrize("pad", ["none", "ones", "left", "right"])
+def test_windows_that_only_the_mask_knows(name, kw, optimised, pad, calls):
+    """Attention modules that do not hand their window to the interface: it comes with the mask."""
+    model = _model(name, **{**MOE, **kw})
+    if optimised:
+        model = _optimised(model)
+    own = copy.deepcopy(model)
+    assert use_train_attention(own)
+    _same(model, own, dict(_inputs(pad), use_cache=False))
+    assert calls == [5, 5]
+    _same(model.eval(), own.eval(), dict(_inputs(pad), use_cache=False))
+    with torch.no_grad():
+        _same(model, own, dict(_inputs(pad), use_cache=False))
+    assert len(calls) == 4
+
+
+@pytest.mark.parametrize("optimised", [False, True])
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("pad", ["none", "left"])
+def test_windows_behind_checkpoints(optimised, reentrant, pad, calls):
+    """Checkpoints hand detached tensors on: the window is in their shape."""
+    model = _model("Mistral", sliding_window=5)
+    if optimised:
+        model = _optimised(model)
+    own = copy.deepcopy(model)
+    assert use_train_attention(own)
+    own.gradient_checkpointing_enable({"use_reentrant": reentrant})
+    own.enable_input_require_grads()
+    args = _inputs(pad)
+    _same(model, own, dict(args, use_cache=False))
+    assert calls and set(calls) == {5}
+    see = args.get("attention_mask", torch.ones(2, 13)).unsqueeze(-1)
+    for m in (model, own):
+        (m(**args, use_cache=False).logits * see).square().mean().backward()
+    for (n, a), b in zip(model.named_parameters(), own.parameters()):
+        if a.grad is not None:
+            assert (a.grad - b.grad).abs().max() <= 2 * TOL * a.grad.abs().max() + TOL * 1e-3, n
+
+
+@pytest.mark.parametrize("window", [0, 4, 9, 100])
+@pytest.mark.parametrize("Sq,Skv", [(9, 9), (4, 9)])
+def test_what_masks_stand_for(window, Sq, Skv):
+    real = torch.arange(Skv) >= torch.tensor([[0], [3]])
+    last, key = torch.arange(Skv - Sq, Skv).view(-1, 1), torch.arange(Skv)
+    see = (key <= last) & (key > last - (window or Skv))
+    for padding in (real, real.long(), None):
+        mask = train_attention._compact(padding, window, Skv)
+        if mask is None:
+            assert padding is None and window == 0
+            continue
+        want = see[None, None] if padding is None else see & real[:, None, None, :]
+        assert torch.equal(train_attention.whole_mask(mask, Sq), want)
+        assert torch.equal(train_attention.whole_mask(mask.detach(), Sq), want)
