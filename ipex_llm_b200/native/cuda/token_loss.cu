@@ -18,8 +18,10 @@
 // A thread folds the maximum of a batch into its own and rescales its sums once for all of it, so that an element costs one
 // exponential (0.73 of what the special function units do at the rate of memory, for 16-bit logits).
 // y is one fma: what rounding takes from r, common to a row, takes part everywhere alike and so cancels, as long as r is the same
-// number everywhere (it goes to the backward pass, and rescaling goes by differences of it).  r is whole, so sums are rescaled by
-// powers of two, exactly: ex2.approx of other numbers is low by 5e-8 on average (measured), which a tree of partial sums adds up.
+// number everywhere (the maximum goes to the backward pass, and rescaling goes by differences of r).  r is whole, so sums are
+// rescaled by powers of two, exactly: ex2.approx of other numbers is low by 5e-8 on average (measured), which a tree of partial
+// sums adds up.  From |c max x| = 2^24 on (masks of -1e10, temperatures of 1e-6) r is no longer within a half of it, and what the
+// fma leaves may be of any size: there y = (x - max x) c.
 //
 // Statistics are 32-bit, 150 to 600 elements to a thread's sum and a tree above that; exponentials by ex2.approx (2 ulp).
 #include <cooperative_groups.h>
@@ -194,21 +196,55 @@ __device__ __forceinline__ uint64_t order_key(float v, int idx) {
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)(0xFFFFFFFFu - (uint32_t)k); }
 
-// r: the rounded product of c and the maximum (-inf: no token), s: sum of 2^y, t: that sum weighted by y (ENT), or over the tokens
-// not given (TAIL).
+// m: the largest logit (-inf: no token), s: sum of 2^y, t: that sum weighted by y (ENT), or over the tokens not given (TAIL).
 struct Stat {
-  float r, s, t;
+  float m, s, t;
 };
-__device__ __forceinline__ float base_of(float r) { return r == -INFINITY ? 0.f : r; }
+// What exponents are taken from: r = rint(c m), or c m itself where m is far from 0.
+constexpr float kFar = 0x1p24f;
+struct Base {
+  float m, r, to;      // to: r, and 0 for no token
+  bool far;
+  __device__ __forceinline__ Base(float m_, float c) {
+    m = m_;
+    r = rintf(__fmul_rn(m, c));
+    to = r == -INFINITY ? 0.f : r;
+    far = !(fabsf(r) < kFar) && m != -INFINITY;
+  }
+  __device__ __forceinline__ float exponent(float x, float c) const { return far ? (x - m) * c : fmaf(x, c, -to); }
+};
+// The exponent of the factor that takes sums from one base to another that is not below it.
+__device__ __forceinline__ float shift(const Base& from, const Base& to, float c) {
+  float d = from.r - to.to;
+  if (from.far || to.far)
+    d = !to.far ? fmaf(from.m, c, -to.to) : from.far ? (from.m - to.m) * c : -fmaf(to.m, c, -from.r);
+  return held(d);
+}
 template <bool ENT>
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
   Stat o;
-  o.r = fmaxf(a.r, b.r);
-  const float to = base_of(o.r);
-  const float da = held(a.r - to), db = held(b.r - to);     // sums of a side without tokens are 0
+  o.m = fmaxf(a.m, b.m);
+  const Base to(o.m, c);
+  const float da = shift(Base(a.m, c), to, c), db = shift(Base(b.m, c), to, c);     // sums of a side without tokens are 0
   const float ea = ex2(da), eb = ex2(db);
   o.s = a.s * ea + b.s * eb;
   o.t = ENT ? (a.t + a.s * da) * ea + (b.t + b.s * db) * eb : a.t * ea + b.t * eb;
+  return o;
+}
+
+// The statistics of the first LANES lanes joined, in the first lane: all taken to the largest base, then added up.
+template <bool ENT, int LANES>
+__device__ __forceinline__ Stat join_lanes(const Stat& a, const Base& base, float c) {
+  Stat o;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(o.m) : "f"(a.m));
+  const float d = shift(base, Base(o.m, c), c), f = ex2(d);          // sums of a lane without tokens are 0
+  o.s = a.s * f;
+  o.t = ENT ? (a.t + a.s * d) * f : a.t * f;
+#pragma unroll
+  for (int n = LANES / 2; n > 0; n /= 2) {
+    o.s += __shfl_xor_sync(0xffffffffu, o.s, n);
+    o.t += __shfl_xor_sync(0xffffffffu, o.t, n);
+  }
   return o;
 }
 
@@ -259,7 +295,7 @@ struct Feed {
 };
 
 // A row whose largest logit is not above -2^127 has no token: -inf, or the lowest values of bf16 and of 32 bits, hide them all.
-__device__ __forceinline__ bool no_token(const Stat& st, float c) { return st.s == st.s && !(st.r > c * -0x1p127f); }
+__device__ __forceinline__ bool no_token(const Stat& st) { return st.s == st.s && !(st.m > -0x1p127f); }
 
 struct Sums {
   Stat warp[2][kWarps];           // by the parity of the CTA's row
@@ -310,27 +346,29 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
     bool is_given = false;
     if constexpr (TAIL)
       for (int k = 0; k < K; ++k) is_given |= ids[k] == j;
-    Stat one = {rintf(__fmul_rn(v, c)), 1.f, TAIL && !is_given ? 1.f : 0.f};
-    one.s = ex2(fmaf(v, c, -base_of(one.r)));    
-    if (ENT) one.t = one.s * held(fmaf(v, c, -base_of(one.r)));
-    else if (one.t != 0.f) one.t = one.s;
-    if (v != v) one.s = one.t = v;
-    st = join<ENT>(st, one);
+    Stat one = {v, 1.f, 0.f};
+    const float y = held(Base(v, c).exponent(v, c));
+    one.s = ex2(y);
+    if (ENT) one.t = one.s * y;
+    else if (TAIL && !is_given) one.t = one.s;
+    if (v != v) one = {-INFINITY, v, v};
+    st = join<ENT>(st, one, c);
     if (TOP && (best.at == -1 || order_key(v, 0) > order_key(best.v, 0))) best = {v, -2 - j};
   };
   if (tid < sl.h) single(tid);
   // as the feed does: at least one batch a row, whether it holds vectors or not
-  for (int base = sl.v0; base == sl.v0 || base < sl.v1; base += kNT * kU) {
+  Base base(st.m, c);
+  for (int at = sl.v0; at == sl.v0 || at < sl.v1; at += kNT * kU) {
     const uint4* w = feed.oldest();
-    if (base + tid >= sl.v1) {
+    if (at + tid >= sl.v1) {
       feed.fetch();
       continue;
     }
-    const int n = min(kU, (sl.v1 - base - tid + kNT - 1) / kNT);    // vectors of this thread
+    const int n = min(kU, (sl.v1 - at - tid + kNT - 1) / kNT);    // vectors of this thread
     float mx = n == kU ? largest_of<T, true>(w, n) : largest_of<T, false>(w, n);
-    const float r = fmaxf(st.r, rintf(__fmul_rn(mx, c))), to = base_of(r);
-    const float down = held(st.r - to), fac = ex2(down);
-    // CAREFUL: with exponents held, for what hides tokens
+    const Base now(fmaxf(st.m, mx), c);
+    const float down = shift(base, now, c), fac = ex2(down);
+    // CAREFUL: with exponents held, for what hides tokens, and of any size
     auto sums = [&](auto careful, auto whole, float& s, float& t) {
       constexpr bool CAREFUL = decltype(careful)::value, WHOLE = decltype(whole)::value;
       float sa[2] = {0.f, 0.f}, ta[2] = {0.f, 0.f};
@@ -341,10 +379,11 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
         unpack<T>(w[u * kNT], f);
 #pragma unroll
         for (int i = 0; i < VEC; i += 2) {
-          exponents2(f[i], f[i + 1], c, -to);
           if (CAREFUL) {
-            f[i] = held(f[i]);
-            f[i + 1] = held(f[i + 1]);
+            f[i] = held(now.exponent(f[i], c));
+            f[i + 1] = held(now.exponent(f[i + 1], c));
+          } else {
+            exponents2(f[i], f[i + 1], c, -now.to);
           }
           e[i] = ex2(f[i]);
           e[i + 1] = ex2(f[i + 1]);
@@ -353,7 +392,7 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
         }
         add2(sa[0], sa[1], v[0], v[1]);
         if constexpr (TAIL) {
-          const int pos = (base + u * kNT + tid - sl.v0) * VEC;
+          const int pos = (at + u * kNT + tid - sl.v0) * VEC;
           const uint32_t bits = given[pos >> 5] >> (pos & 31) & ((1u << VEC) - 1);
           if (bits == 0) {
             add2(ta[0], ta[1], v[0], v[1]);
@@ -366,14 +405,16 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
       s = sa[0] + sa[1];
       t = ta[0] + ta[1];
     };
-    float s, t;
-    if (n == kU) sums(std::false_type(), std::true_type(), s, t);
+    float s = 0.f, t = 0.f;
+    if (now.far) sums(std::true_type(), std::false_type(), s, t);
+    else if (n == kU) sums(std::false_type(), std::true_type(), s, t);
     else sums(std::false_type(), std::false_type(), s, t);
-    if (ENT && t != t) sums(std::true_type(), std::false_type(), s, t);
+    if (ENT && !now.far && t != t) sums(std::true_type(), std::false_type(), s, t);
     if constexpr (ENT) st.t = (st.t + st.s * down) * fac + t;
     else if constexpr (TAIL) st.t = st.t * fac + t;
     st.s = st.s * fac + s;
-    st.r = r;
+    st.m = now.m;
+    base = now;
     if constexpr (TOP) {
       if (s != s) {
         for (int u = 0; u < n; ++u) {
@@ -383,33 +424,24 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
           for (int i = 0; i < VEC; ++i) mx = f[i] != f[i] ? NAN : mx;
         }
       }
-      if (best.at == -1 || order_key(mx, 0) > order_key(best.v, 0)) best = {mx, base + tid};
+      if (best.at == -1 || order_key(mx, 0) > order_key(best.v, 0)) best = {mx, at + tid};
     }
     feed.fetch();
   }
   if (tid >= kNT - sl.t) single(sl.V - (kNT - tid));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat other = {__shfl_xor_sync(0xffffffffu, st.r, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                  __shfl_xor_sync(0xffffffffu, st.t, o)};
-    st = lane & o ? join<ENT>(other, st) : join<ENT>(st, other);
-  }
+  st = join_lanes<ENT, 32>(st, Base(st.m, c), c);
   if (lane == 0) sums[warp] = st;
 }
 
 // The warps' statistics joined, in every lane of a warp.
 template <bool ENT>
-__device__ __forceinline__ Stat join_warps(const Stat* sums) {
+__device__ __forceinline__ Stat join_warps(const Stat* sums, float c) {
   const int lane = threadIdx.x & 31;
   Stat st = {-INFINITY, 0.f, 0.f};
   if (lane < kWarps) st = sums[lane];
-#pragma unroll
-  for (int o = 4; o > 0; o >>= 1) {
-    Stat other = {__shfl_xor_sync(0xffffffffu, st.r, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                  __shfl_xor_sync(0xffffffffu, st.t, o)};
-    st = lane & o ? join<ENT>(other, st) : join<ENT>(st, other);
-  }
-  return {__shfl_sync(0xffffffffu, st.r, 0), __shfl_sync(0xffffffffu, st.s, 0), __shfl_sync(0xffffffffu, st.t, 0)};
+  static_assert(kWarps <= 8, "join_lanes");
+  st = join_lanes<ENT, 8>(st, Base(st.m, c), c);
+  return {__shfl_sync(0xffffffffu, st.m, 0), __shfl_sync(0xffffffffu, st.s, 0), __shfl_sync(0xffffffffu, st.t, 0)};
 }
 
 // Keys of a warp: sorted from large to small over its lanes, and the 32 largest of two such rows of lanes.
@@ -551,15 +583,15 @@ __device__ void best_tokens(const T* x, const Slice<T>& sl, int top, const Best&
 // A row's statistics, in every lane of the finishing warp: those of its CTA's warps, and where a cluster has the row those of its
 // CTAs (between two barriers of the cluster, which the other warps take part in: see meet()).
 template <bool ENT>
-__device__ __forceinline__ Stat row_stat(Sums& sh, int turn, int parts) {
-  Stat a = join_warps<ENT>(sh.warp[turn]);
+__device__ __forceinline__ Stat row_stat(Sums& sh, int turn, int parts, float c) {
+  Stat a = join_warps<ENT>(sh.warp[turn], c);
   if (parts > 1) {
     if ((threadIdx.x & 31) == 0) sh.part = a;
     __syncwarp();
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();
     a = *cl.map_shared_rank(&sh.part, 0);
-    for (int i = 1; i < parts; ++i) a = join<ENT>(a, *cl.map_shared_rank(&sh.part, i));
+    for (int i = 1; i < parts; ++i) a = join<ENT>(a, *cl.map_shared_rank(&sh.part, i), c);
   }
   return a;
 }
@@ -571,12 +603,12 @@ __device__ __forceinline__ void meet(int parts) {
   }
 }
 
-// log sum e^(x / T).  A row's few last operations are done in 64 bits: in 32, they made the error of a log probability 1.7 times what
-// its own rounding is.  c is log2(e) / T rounded to 32 bits, and r, rounded from c max x, is taken back to the unrounded factor: what
-// is left of c's error is that of the differences to the largest logit.
+// log sum e^((x - from) / T), from = 0, or m where that is far.  A row's few last operations are done in 64 bits: in 32, they made
+// the error of a log probability 1.7 times what its own rounding is.  c is log2(e) / T rounded to 32 bits, and r, rounded from
+// c max x, is taken back to the unrounded factor: what is left of c's error is that of the differences to the largest logit.
 constexpr double kLn2_64 = 0.693147180559945309;
-__device__ __forceinline__ double log_sum(float r, double log2_s, float c, float temp) {
-  return r * (1.0 / ((double)temp * c)) + log2_s * kLn2_64;
+__device__ __forceinline__ double log_sum(const Base& base, double log2_s, float c, float temp) {
+  return (base.far ? 0.0 : base.r * (1.0 / ((double)temp * c))) + log2_s * kLn2_64;
 }
 
 struct ProbArgs {
@@ -584,7 +616,7 @@ struct ProbArgs {
   const int64_t* targets;
   float* logprob;
   float* entropy;      // null: not asked for
-  float* stats;        // [rows, 4]: r, 1 / s, log2 s, H
+  float* stats;        // [rows, 4]: m, 1 / s, log2 s, H
   float* top_logprob;  // [rows, top]
   int64_t* top_id;
   int top, parts;
@@ -622,21 +654,22 @@ __global__ void __launch_bounds__(kNT + 32, kCtas) token_logprobs_kernel(ProbArg
     const bool ignored = t == a.ignore, bad = !ignored && (t < 0 || t >= a.rows.V);
     const float xt = ignored || bad ? 0.f : DT<T>::to_f(x[t]);
     __syncthreads();
-    const Stat st = row_stat<ENT>(sh, turn, parts);
+    const Stat st = row_stat<ENT>(sh, turn, parts, c);
     if (rank == 0) {
-      const bool none = no_token(st, c);
-      const float r = none ? 0.f : st.r;
-      const double log2_s = none ? 0.0 : log2((double)st.s), lse = log_sum(r, log2_s, c, a.temp);
+      const bool none = no_token(st);
+      const Base base(none ? 0.f : st.m, c);
+      const double log2_s = none ? 0.0 : log2((double)st.s), lse = log_sum(base, log2_s, c, a.temp);
       const float H = !ENT || none ? 0.f : (float)((log2_s - (double)st.t / st.s) * kLn2_64);
       auto logp = [&](float v) {
-        const float y = fmaf(v, c, -r);            // -inf for what hides a token
-        return none ? -INFINITY : fabsf(y) < INFINITY ? (float)(v / (double)a.temp - lse) : (y - (float)log2_s) * kLn2;
+        if (none) return -INFINITY;
+        if (base.far) return (float)(((double)v - base.m) / a.temp - lse);
+        return fabsf(v) < INFINITY ? (float)(v / (double)a.temp - lse) : v - (float)log2_s;
       };
       if (lane == 0) {
         if (bad) tc5::report(a.err, kErrToken);
         a.logprob[row] = bad ? NAN : ignored ? 0.f : logp(xt);
         if (ENT) a.entropy[row] = ignored ? 0.f : bad ? NAN : H;
-        if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r, none ? 0.f : 1.f / st.s, (float)log2_s, H);
+        if (a.stats != nullptr) reinterpret_cast<float4*>(a.stats)[row] = make_float4(base.m, none ? 0.f : 1.f / st.s, (float)log2_s, H);
       }
       if constexpr (TOP) {
         uint64_t k = sh.top[turn][lane];
@@ -719,15 +752,16 @@ __global__ void __launch_bounds__(kNT) token_logprobs_grad_kernel(ProbGradArgs a
     map_row<T>(x, y, sl, [](float) { return 0.f; });
     return;
   }
-  auto grad = [&](float v) {
-    const float d = ENT ? held(fmaf(v, c, -st.x)) : fmaf(v, c, -st.x);
-    const float e = ex2(d) * scale;
+  const Base base(st.x, c);
+  auto of = [&](float y) {
+    const float d = ENT ? held(y) : y, e = ex2(d) * scale;
     return ENT ? e * fmaf(ge, fmaf(d, kLn2, lp0), g) : e * g;
   };
-  map_row<T>(x, y, sl, grad);
+  if (base.far) map_row<T>(x, y, sl, [&](float v) { return of((v - base.m) * c); });
+  else map_row<T>(x, y, sl, [&](float v) { return of(fmaf(v, c, -base.r)); });
   __syncthreads();
   if (threadIdx.x == 0 && !bad && t >= 0 && t < a.rows.V && !ignored && sl.has((int)t))
-    y[t] = DT<T>::from_f(fmaf(g, a.inv_t, grad(DT<T>::to_f(x[t]))));
+    y[t] = DT<T>::from_f(fmaf(g, a.inv_t, of(base.exponent(DT<T>::to_f(x[t]), c))));
 }
 
 // ------------------------------------------------------------------------------------------------ distillation
@@ -742,7 +776,7 @@ struct DistillArgs {
   const float* values;     // [rows, K]
   const float* lse;        // [rows] or null
   float* loss;             // [rows]
-  float* stats;            // [rows, 8]: r, 1 / s, M, rest / left, z, share, -, -
+  float* stats;            // [rows, 8]: m, 1 / s, M, rest / left, z, share, -, -
   int64_t n;               // rows
   int K, parts;
   int words;               // of a row's bits, a multiple of 4
@@ -760,12 +794,12 @@ __device__ __forceinline__ double warp_sum64(double v) {
 // a difference.  sum_k q_k (log q_k - log p_id) = own - cross / T + mass log sum e^(x / T) with what follows, so that it need not
 // wait for the student's sums.
 struct Teacher {
-  double own, cross, mass;   // sum q log q, sum q x_id, sum q
+  double own, cross, mass;   // sum q log q, sum q (x_id - from), sum q
   float z, share;            // q_k = e^(t_k / T - z) * share
   bool empty, never;         // no token is given; a given one can never be the student's (its logit is -inf)
 };
 template <typename T, bool TAIL>
-__device__ Teacher teacher_of(const T* x, const int* ids, const float* values, const float* lse, int K, float temp_) {
+__device__ Teacher teacher_of(const T* x, const int* ids, const float* values, const float* lse, int K, float temp_, double from) {
   const int lane = threadIdx.x & 31;
   const double temp = temp_;
   double z = TAIL ? *lse : -INFINITY;
@@ -790,7 +824,7 @@ __device__ Teacher teacher_of(const T* x, const int* ids, const float* values, c
         if (q != 0.0) {
           own += q * d;
           if (v == -INFINITY) never = true;
-          else cross += q * v;
+          else cross += q * (v - from);
         }
         mass += q;
       }
@@ -859,16 +893,20 @@ __global__ void __launch_bounds__(kNT + 32, kCtas) distill_kernel(DistillArgs a)
   int turn = 0;
   for (int64_t row = first; row < a.n; row += step, turn ^= 1) {
     const T* x = row_at<T>(a.rows, row);
-    const Teacher te = teacher_of<T, TAIL>(x, ids[turn], a.values + row * K, TAIL ? a.lse + row : nullptr, K, a.temp);
+    auto teacher = [&](float from) {
+      return teacher_of<T, TAIL>(x, ids[turn], a.values + row * K, TAIL ? a.lse + row : nullptr, K, a.temp, from);
+    };
+    Teacher te = teacher(0.f);
     const bool bad_next = row + step < a.n && open(row + step, turn ^ 1);
     __syncthreads();
-    const Stat st = row_stat<false>(sh, turn, parts);
+    const Stat st = row_stat<false>(sh, turn, parts, c);
+    const bool none = no_token(st);
+    const Base base(none ? 0.f : st.m, c);
+    if (base.far) te = teacher(st.m);          // differences of numbers that far from 0 would cancel
     if (rank == 0 && lane == 0) {
-      const bool none = no_token(st, c);
-      const float r = none ? 0.f : st.r;
       double mass = te.mass, rest = 0.0;
-      double loss = te.never ? INFINITY
-                             : te.own - te.cross / a.temp + te.mass * log_sum(r, none ? 0.0 : log2((double)st.s), c, a.temp);
+      double loss = te.never || (none && mass > 0.0) ? INFINITY
+                             : te.own - te.cross / a.temp + te.mass * log_sum(base, none ? 0.0 : log2((double)st.s), c, a.temp);
       float ratio = 0.f;
       if constexpr (TAIL) {
         rest = fmax(1.0 - mass, 0.0);
@@ -891,7 +929,7 @@ __global__ void __launch_bounds__(kNT + 32, kCtas) distill_kernel(DistillArgs a)
       a.loss[row] = (float)(loss * a.temp * a.temp);
       if (a.stats != nullptr) {
         float4* s4 = reinterpret_cast<float4*>(a.stats) + 2 * row;
-        s4[0] = make_float4(r, none ? 0.f : 1.f / st.s, (float)(mass + rest), ratio);
+        s4[0] = make_float4(base.m, none ? 0.f : 1.f / st.s, (float)(mass + rest), ratio);
         s4[1] = make_float4(te.z, te.share, 0.f, 0.f);
       }
     }
@@ -934,7 +972,9 @@ __global__ void __launch_bounds__(kNT) distill_grad_kernel(DistillGradArgs a) {
     q[k] = ok ? ex2((float)(a.values[row * K + k] / (double)a.temp - z) * kLog2e) * share : 0.f;
   }
   const float other = g * st.y * (st.z - st.w), own = g * st.y * st.z;
-  map_row<T>(x, y, sl, [&](float v) { return ex2(fmaf(v, c, -st.x)) * other; });
+  const Base base(st.x, c);
+  if (base.far) map_row<T>(x, y, sl, [&](float v) { return ex2((v - base.m) * c) * other; });
+  else map_row<T>(x, y, sl, [&](float v) { return ex2(fmaf(v, c, -base.r)) * other; });
   __syncthreads();
   // given tokens once more: the first of those with the same index writes for all of them
   for (int k = threadIdx.x; k < K; k += kNT) {
@@ -947,7 +987,7 @@ __global__ void __launch_bounds__(kNT) distill_grad_kernel(DistillGradArgs a) {
         first &= j >= k;
         sum += q[j];
       }
-    if (first) y[id] = DT<T>::from_f(fmaf(-g, sum, ex2(fmaf(DT<T>::to_f(x[id]), c, -st.x)) * own));
+    if (first) y[id] = DT<T>::from_f(fmaf(-g, sum, ex2(base.exponent(DT<T>::to_f(x[id]), c)) * own));
   }
 }
 
