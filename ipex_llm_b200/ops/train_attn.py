@@ -24,13 +24,13 @@ _TILE = 128
 
 
 def _fit(t: torch.Tensor):
-    """The tensor as the kernels' 4-D maps take it, rows contiguous and other strides positive multiples of 16 bytes (copied
-    where it is not), behind its pointer and strides.  The stride of a dimension of size 1 is never taken: 8 stands for it."""
+    """The tensor as the kernels' 4-D maps take it, rows contiguous, aligned to 16 bytes, and other strides positive multiples of
+    16 bytes (copied where it is not), behind its pointer and strides.  The stride of a dimension of size 1 is never taken: 8 stands for it."""
     (B, H, S, _), (b, h, s, d) = t.shape, t.stride()
     b, h, s = b if B > 1 else 8, h if H > 1 else 8, s if S > 1 else 8
     at = t.data_ptr()
     if d != 1 or at & 15 or (b | h | s) & 7 or not (b and h and s):
-        return _fit(t.contiguous())
+        return _fit(t.clone(memory_format=torch.contiguous_format))          # a contiguous one may still lie at any address
     return at, b, h, s, t
 
 

@@ -1,0 +1,52 @@
+"""Calls of the attention with a gradient that its documentation allows, on the GPU."""
+import math
+
+import pytest
+import torch
+
+import train_attn_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(B, Hq, Hkv, Sq, Skv, D, dtype, seed, grad_std=1.0 / 16):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def heads(n, s, std):
+        return (torch.randn(B, s, n, D, generator=g, device="cuda") * std).to(dtype).transpose(1, 2)
+    return heads(Hq, Sq, 1.5), heads(Hkv, Skv, 1.0), heads(Hkv, Skv, 1.0), heads(Hq, Sq, grad_std)
+
+
+def _run(q, k, v, g, **kw):
+    from ipex_llm_b200.ops import cuda_ops
+    from ipex_llm_b200.ops.train_attn import attention
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    out = attention(q, k, v, **kw)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    cuda_ops.check_error_flag(q.device)
+    return dict(zip(("out", "dq", "dk", "dv"), (out.detach(), *grads)))
+
+
+def _check(got, q, k, v, g, scale=None, causal=True, window=0, key_mask=None):
+    want = oracle.attention(q, k, v, g, scale or q.shape[-1] ** -0.5, causal, window, key_mask)
+    for name, (exact, tol) in want.items():
+        t = got[name]
+        assert t.shape == exact.shape and t.dtype == q.dtype, name
+        off = ((t.double() - exact).abs() / tol).nan_to_num(nan=math.inf)
+        assert float(off.max()) <= 1.0, (name, float(off.max()), (off > 1).sum().item(), off.argmax().item())
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("offset", [1, 4, 7])
+@pytest.mark.parametrize("which", ["q", "k", "v", "g", "qkvg"])
+def test_contiguous_tensors_at_any_address(which, offset, masked):
+    """Views of a flat buffer that begin between two 16-byte boundaries."""
+    given = dict(zip("qkvg", _inputs(2, 4, 2, 70, 70, 64, torch.bfloat16, 3)))
+    kw = dict(key_mask=torch.arange(70, device="cuda") < torch.tensor([[70], [31]], device="cuda")) if masked else {}
+    want = _run(*given.values(), **kw)
+
+    def moved(t):
+        flat = torch.zeros(offset + t.numel(), dtype=t.dtype, device="cuda")[offset:]
+        return flat.view(t.shape).copy_(t)
+    got = _run(*(moved(t) if n in which else t for n, t in given.items()), **kw)
+    assert all(torch.equal(got[n], want[n]) for n in want)
