@@ -1534,7 +1534,8 @@ bool shape_ok(int B, int Hq, int Hkv, int Sq, int Skv, int D, int window, float 
 Shape make_shape(int B, int Hq, int Hkv, int Sq, int Skv, int D, int causal, int window, const uint32_t* mask, float scale,
                  int* err) {
   Shape s;
-  s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.Sq = Sq; s.Skv = Skv; s.D = D; s.causal = causal; s.window = window;
+  s.B = B; s.Hq = Hq; s.Hkv = Hkv; s.Sq = Sq; s.Skv = Skv; s.D = D; s.causal = causal;
+  s.window = window < Skv ? window : 0;      // one of all keys hides none, and limits stay in 32 bits
   s.q_pad = (Sq + kT - 1) / kT * kT;
   s.k_words = (Skv + kT - 1) / kT * (kT / 32);
   s.mask = mask; s.scale = scale; s.scale_log2 = scale * 1.4426950408889634f; s.err = err;

@@ -23,3 +23,10 @@ def test_tensors_at_any_address_fit(layout, offset, D):
         assert stride > 0 and stride % 8 == 0
     strides = [x for n, x in zip((B, H, S), fit.stride()) if n > 1]
     assert strides == [x for n, x in zip((B, H, S), (b, h, s)) if n > 1]
+
+
+@pytest.mark.parametrize("Sq,Skv", [(6, 4), (4, 6)])
+def test_windows_of_more_than_all_keys(Sq, Skv):
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(1, 2, s, 8, generator=g, dtype=torch.float64) for s in (Sq, Skv, Skv))
+    assert torch.equal(train_attn.attention(q, k, v, window=2 ** 31 - 1), train_attn.attention(q, k, v))
