@@ -3,7 +3,8 @@ alternatives, and the divergence from a teacher's top logits, each with the grad
 
 On a CUDA tensor every function calls the package's own kernels on the current stream of the tensor's device, in the logits'
 type with 32-bit sums, and no copy of the logits in 32 bits is made; on the CPU it is plain PyTorch.  Logits may be a view with
-any strides between rows.
+any strides between rows.  Gradients are those of a backward pass; on the GPU tangents of forward-mode differentiation are
+refused.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ from ..native import cuda_api as api
 from ..native.lib import current_stream, ptr, stream_lib
 from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
+from .gradients import refuse_tangents
 
 MAX_TOP = 32             # alternatives of a row
 MAX_TEACHER = 1024       # tokens of a teacher's row
@@ -169,6 +171,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, temperature: flo
     if not 0 <= top <= most:
         invalidInputError(False, f"token_logprobs: top should be between 0 and {most}, got {top}")
     if logits.is_cuda:
+        refuse_tangents("token_logprobs", logits)
         args = (logits, targets.to(torch.int64).contiguous(), float(temperature), bool(entropy), int(top), int(ignore_index))
         if logits.requires_grad and torch.is_grad_enabled():
             return TokenLogprobs(*_TokenLogprobs.apply(*args))
@@ -270,6 +273,7 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
         if logits.shape[-1] > MAX_TAIL_VOCAB:
             invalidInputError(False, f"distill_loss: teacher_logsumexp takes vocabularies up to {MAX_TAIL_VOCAB}")
     if logits.is_cuda:
+        refuse_tangents("distill_loss", logits)
         args = (logits, teacher_ids.to(torch.int64).contiguous(), teacher_logits.detach().float().contiguous(),
                 None if lse is None else lse.detach().float().contiguous(), float(temperature))
         if logits.requires_grad and torch.is_grad_enabled():

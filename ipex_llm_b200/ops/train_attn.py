@@ -16,6 +16,7 @@ from ..native import cuda_api as api
 from ..native.lib import current_stream, ptr, stream_lib
 from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
+from .gradients import refuse_tangents
 
 MAX_DIM = 128
 MAX_HEADS = 65535       # of queries and keys together
@@ -135,11 +136,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     rows hold, NaN included, takes no part.  A query that sees no key gives zeros and gets no gradient.  ``scale`` (1e-4 to
     1e4) defaults to D^-1/2.
 
-    GPU: fp16 or bf16, D a multiple of 8 up to 128, any strides (rows that are not contiguous, or not aligned to 16 bytes, are
-    copied).  Scores, sums and gradients are summed in 32 bits; probabilities and their gradients are rounded to 16 bits
-    where they enter a product (twice as many bits for queries of few keys).  The results do not depend on the order in which
-    anything runs.  A causal limit or a window hides a key by a probability of 0: NaN and infinities in such a row may spread
-    to earlier queries, as they do in the formula; behind ``key_mask`` they do not.
+    GPU: backward gradients alone (a tangent of forward-mode differentiation is refused), fp16 or bf16, D a multiple of 8 up to
+    128, any strides (rows that are not contiguous, or not aligned to 16 bytes, are copied).  Scores, sums and gradients are
+    summed in 32 bits; probabilities and their gradients are rounded to 16 bits where they enter a product (twice as many bits
+    for queries of few keys).  The results do not depend on the order in which anything runs.  A causal limit or
+    a window hides a key by a probability of 0: NaN and infinities in such a row may spread to earlier queries, as they do in the
+    formula; behind ``key_mask`` they do not.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         invalidInputError(False, f"attention: q, k and v should be [batch, heads, tokens, dim], k and v alike; got {tuple(q.shape)}, "
@@ -163,6 +165,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     if not q.is_cuda:
         invalidInputError(q.is_floating_point(), "attention: inputs should be floating-point numbers")
         return _attention_plain(q, k, v, key_mask, scale, causal, window)
+    refuse_tangents("attention", q, k, v)
     if q.dtype not in (torch.float16, torch.bfloat16):
         invalidInputError(False, f"attention: {q.dtype} is not supported on the GPU (float16 and bfloat16 are)")
     if D > MAX_DIM or D % 8:
