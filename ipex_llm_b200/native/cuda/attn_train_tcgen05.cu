@@ -29,8 +29,8 @@
 //
 // In the transposed scores L_i and delta_i belong to columns, not to the threads' rows.  Read from shared memory, four numbers a
 // request, they took a third of its bandwidth, which the products need.  So they are summed by the products too: one more step
-// of 16 columns, in which a query's row holds -L_i / scale (or -delta_i) in three pieces of 16 bits, and every key's row the
-// pieces' weights.
+// of 16 columns, in which a query's row holds -L_i / scale (or -delta_i) in pieces of 16 bits, and every key's row the pieces'
+// weights.
 //
 // In fp16 the range of dS is what is short, not its precision: P is taken times 2^12, and dP - delta times a power of two that a
 // bound on |dO_i| |v_j| gives for each group of heads, so that the largest dS comes near 2^15.  Both go out of the results again.
@@ -713,26 +713,30 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 // ------------------------------------------------------------------------------------------------ before the backward pass
 // delta_i = dO_i . o_i (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
 // heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
-// Three pieces of 16 bits whose weighted sum is x, in a row of eight numbers: the third takes what the first two leave, below
-// 2^-24 of x.  fp16's weights spread the pieces over its range: numbers up to 2^23, to 2^-43.
+// Pieces of 16 bits whose weighted sum is x, in a row of eight numbers: each takes what those before it leave, the last below
+// 2^-24 of x.  fp16's weights spread its pieces over numbers up to 65504 x 2^15, to 2^-45: a first piece x / 2^15 leaves at most
+// 2^-12 |x| or 2^-10, and so on.  (Three pieces with weights of 2^8 and less end at 2^24, which dO_i . o_i passes where a loss is scaled; a
+// column more costs nothing, the product takes sixteen anyway.)
 template <typename T> struct Pieces;
 template <> struct Pieces<__nv_bfloat16> {
+  static constexpr int kN = 3;
   static __device__ float weight(int) { return 1.f; }
 };
 template <> struct Pieces<__half> {
-  static __device__ float weight(int i) { return i == 0 ? 256.f : i == 1 ? 0x1p-6f : 0x1p-18f; }
+  static constexpr int kN = 4;
+  static __device__ float weight(int i) { return i == 0 ? 0x1p15f : i == 1 ? 0x1p4f : i == 2 ? 0x1p-8f : 0x1p-20f; }
 };
 template <typename T>
 __device__ __forceinline__ uint4 in_pieces(float x) {
   __align__(16) T v[8];
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < Pieces<T>::kN; ++i) {
     const float w = Pieces<T>::weight(i);
     v[i] = from_float<T>(x / w);
     x -= to_float<T>(v[i]) * w;
   }
 #pragma unroll
-  for (int i = 3; i < 8; ++i) v[i] = from_float<T>(0.f);
+  for (int i = Pieces<T>::kN; i < 8; ++i) v[i] = from_float<T>(0.f);
   return *reinterpret_cast<const uint4*>(v);
 }
 
@@ -936,7 +940,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   if (threadIdx.x < 256) {
     __align__(16) T w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = from_float<T>(threadIdx.x < kT && i < 3 ? Pieces<T>::weight(i) : 0.f);
+    for (int i = 0; i < 8; ++i) w[i] = from_float<T>(threadIdx.x < kT && i < Pieces<T>::kN ? Pieces<T>::weight(i) : 0.f);
     reinterpret_cast<uint4*>(smem + L::kWeights)[threadIdx.x] = *reinterpret_cast<const uint4*>(w);
     fence_proxy_async_smem();
   }

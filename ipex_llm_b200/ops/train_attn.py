@@ -139,7 +139,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     GPU: backward gradients alone (a tangent of forward-mode differentiation is refused), fp16 or bf16, D a multiple of 8 up to
     128, any strides (rows that are not contiguous, or not aligned to 16 bytes, are copied).  Scores, sums and gradients are
     summed in 32 bits; probabilities and their gradients are rounded to 16 bits where they enter a product (twice as many bits
-    for queries of few keys).  The results do not depend on the order in which anything runs.  A causal limit or
+    for queries of few keys).  In fp16 the backward pass takes scores up to 2^30 * scale, and rows whose outputs and gradients
+    have a product up to 2^30 (NaN past 2^31).  The results do not depend on the order in which anything runs.  A causal limit or
     a window hides a key by a probability of 0: NaN and infinities in such a row may spread to earlier queries, as they do in the
     formula; behind ``key_mask`` they do not.
     """

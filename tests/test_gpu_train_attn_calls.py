@@ -63,3 +63,34 @@ def test_windows_of_more_than_all_keys(window, Sq, Skv, dtype):
     got, want = _run(*args, window=window), _run(*args)
     assert all(torch.equal(got[n], want[n]) for n in want)
     _check(got, *args, window=window)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 14, 2.0 ** 24, 2.0 ** 27, 2.0 ** 29, 2.0 ** 30.9])
+def test_rows_whose_gradient_and_output_have_a_large_product(size, D, dtype):
+    """As where a loss is scaled: delta of the first tokens, whose own dS is small, lies far past what one number of 16 bits holds."""
+    q, k, v, g = _inputs(1, 4, 2, 150, 150, D, dtype, 6)
+    v = v * 64
+    for i in (0, 3):
+        one = v[:, :, i].repeat_interleave(2, 1).float()                     # the output of row 0, and near that of row 3
+        g[:, :, i] = (one * (size / one.square().sum(-1, keepdim=True))).clamp(-6e4, 6e4).to(dtype)
+    got = _run(q, k, v, g)
+    # (row 3 is no mean of equal values: its dS and with it dk pass the range of fp16 with the larger sizes)
+    assert not any(bool(t.isnan().any()) for t in got.values())
+    _check(got, q, k, v, g)
+    delta = (g[:, :, 0].float() * got["out"][:, :, 0].float()).sum(-1)
+    assert float(delta.max()) > 0.4 * min(size, 2.0 ** 26)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [2.0 ** 23, 2.0 ** 25, 2.0 ** 30])
+def test_first_tokens_of_a_large_scaled_loss(size, D):
+    """fp16, and all gradients within its range: of the first token alone, whose dS is 0, delta is up to 2^30."""
+    q, k, v, g = _inputs(1, 2, 2, 150, 150, D, torch.float16, 6)
+    v = v * 2048
+    one = v[:, :, 0].float()
+    g[:, :, 0] = (one * (size / one.square().sum(-1, keepdim=True))).half()
+    got = _run(q, k, v, g)
+    assert all(bool(t.isfinite().all()) for t in got.values())
+    _check(got, q, k, v, g)
