@@ -123,7 +123,7 @@ def _attention_plain(q, k, v, key_mask, scale, causal, window):
     see = see if see.dim() == 2 else see.unsqueeze(2)
     s = (qg @ kf.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
     p = torch.softmax(s.masked_fill(~see.any(dim=-1, keepdim=True), 0.0), dim=-1).masked_fill(~see, 0.0)
-    return (p @ vf).reshape(B, Hq, Sq, D).to(q.dtype)
+    return (p @ vf).reshape(B, Hq, Sq, D).to(q.dtype).transpose(1, 2).contiguous().transpose(1, 2)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[float] = None, causal: bool = True,
@@ -177,7 +177,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
         invalidInputError(False, f"attention: {B} sequences of {Sq} queries and {Skv} keys are too many (65535 of {MAX_TOKENS} "
                                  "are not)")
     if q.numel() == 0 or k.numel() == 0:
-        return q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0.0) + (k.sum() + v.sum()) * 0
+        zeros = q.masked_fill(torch.ones_like(q, dtype=torch.bool), 0.0) + (k.sum() + v.sum()) * 0
+        return zeros.transpose(1, 2).contiguous().transpose(1, 2)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, key_mask, scale, bool(causal), window)
     return _forward(q, k, v, key_mask, scale, bool(causal), window, False)[0].transpose(1, 2)

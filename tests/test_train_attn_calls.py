@@ -30,3 +30,29 @@ def test_windows_of_more_than_all_keys(Sq, Skv):
     g = torch.Generator().manual_seed(1)
     q, k, v = (torch.randn(1, 2, s, 8, generator=g, dtype=torch.float64) for s in (Sq, Skv, Skv))
     assert torch.equal(train_attn.attention(q, k, v, window=2 ** 31 - 1), train_attn.attention(q, k, v))
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("Sq,Skv", [(5, 5), (1, 5), (5, 0), (0, 5)])
+def test_outputs_are_views_of_token_major_ones(device, Sq, Skv):
+    """As attention modules go on with them: `out.transpose(1, 2).view(batch, tokens, -1)`."""
+    q, k = (torch.randn(2, 4, s, 8, device=device, dtype=torch.bfloat16) for s in (Sq, Skv))
+    for learns in (False, True):
+        out = train_attn.attention(q.requires_grad_(learns), k, k, causal=False)
+        assert out.shape == (2, 4, Sq, 8) and out.transpose(1, 2).is_contiguous()
+
+
+def test_modules_that_view_the_attention():
+    """Its result in a model whose attention takes it by `view`, on the CPU."""
+    import transformers as tr
+    from ipex_llm_b200.models.train_attention import use_train_attention
+    cfg = tr.AfmoeConfig(hidden_size=32, intermediate_size=48, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                         head_dim=8, vocab_size=50, num_experts=4, num_experts_per_tok=2, moe_intermediate_size=16,
+                         max_position_embeddings=64, attn_implementation="sdpa")
+    torch.manual_seed(0)
+    model = tr.AfmoeForCausalLM(cfg)
+    ids = torch.randint(1, 50, (2, 9), generator=torch.Generator().manual_seed(2))
+    want = model(ids).logits
+    assert use_train_attention(model)
+    # 32 bits on both sides: some 100 roundings a layer on a path, two layers, either side, four for what they amplify
+    assert (model(ids).logits - want).abs().max() <= 2 * 2 * 100 * 4 * 2.0 ** -24 * want.abs().max()
