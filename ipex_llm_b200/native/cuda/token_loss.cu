@@ -48,6 +48,7 @@ constexpr int kMaxBits = 2 * (kMaxTailV / 8 + 64);     // bytes: bits of two row
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kErrToken = 61;     // a token outside of the vocabulary
+constexpr float kNothing = 0x1p-100f;  // what the student gives to no other token: rest / left stays finite, and times a gradient
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -911,11 +912,11 @@ __global__ void __launch_bounds__(kNT + 32, kCtas) distill_kernel(DistillArgs a)
       if constexpr (TAIL) {
         rest = fmax(1.0 - mass, 0.0);
         const float left = none ? 0.f : st.t / st.s;
-        if (rest > 0.0 && left > 0.f) {
+        if (rest > 0.0 && left > kNothing) {
           ratio = (float)rest / left;
           loss += rest * log(rest * st.s / st.t);
         } else {
-          rest = 0.0;                                        // the student has no other token: the term is left out
+          rest = 0.0;                                        // as good as no other token: the term is left out
         }
       }
       if (te.empty) {

@@ -26,6 +26,7 @@ MAX_TEACHER = 1024       # tokens of a teacher's row
 MAX_TAIL_VOCAB = 1 << 19
 IGNORE = -100
 _NO_TOKEN = -2.0 ** 127   # a row whose largest logit is not above this has no token
+_NOTHING = 2.0 ** -100    # a probability of all other tokens that counts as none
 
 
 class TokenLogprobs(NamedTuple):
@@ -239,7 +240,7 @@ def _distill_plain(logits, ids, values, lse, temperature):
         rest = (1.0 - q.sum(dim=-1, keepdim=True)).clamp(min=0.0)
         hide = torch.zeros(logits.shape, dtype=torch.int32, device=logits.device).scatter_add_(-1, at, given.int()) > 0
         left = torch.exp(logp).masked_fill(hide, 0.0).sum(dim=-1, keepdim=True)
-        some = (rest > 0) & (left > 0)
+        some = (rest > 0) & (left > _NOTHING)
         loss = loss + torch.where(some, rest * (torch.log(rest.clamp(min=1e-38)) - torch.log(torch.where(some, left, 1.0))), 0.0)
     loss = torch.where(empty, 0.0, loss)
     return (loss * (temperature * temperature)).squeeze(-1)
@@ -252,8 +253,8 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     temperature) at ``teacher_ids [..., K]`` (K up to 1024).
 
     With ``teacher_logsumexp [...]``, the logsumexp of all the teacher's logits / temperature, q_k are the teacher's own
-    probabilities, and what they leave is compared with what the student gives to all other tokens together (left out where the
-    student has no other token).  Ids below 0 are padding; a row of nothing else gives 0 and no gradient.  An id that occurs
+    probabilities, and what they leave is compared with what the student gives to all other tokens together (left out where that
+    is nothing: less than 2^-100).  Ids below 0 are padding; a row of nothing else gives 0 and no gradient.  An id that occurs
     twice counts twice.  An id past the vocabulary raises on the CPU; on the GPU its row is NaN, and
     ``cuda_ops.check_error_flag`` reports 61.
 
