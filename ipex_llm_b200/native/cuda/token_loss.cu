@@ -993,12 +993,23 @@ __global__ void __launch_bounds__(kNT) distill_grad_kernel(DistillGradArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ host
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) != 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 // CTAs to a row: one where the rows alone fill the SMs, else as many (up to a portable cluster) as do, while each still has a
 // batch of requests for its threads.
 int parts_of(int64_t rows, int V, int elem) {
   const int64_t batch = (int64_t)kNT * 16 / elem;
+  const int sms = sm_count();
   int parts = 1;
-  while (parts < kMaxCluster && rows * parts < 148 && (int64_t)V > batch * parts) parts *= 2;
+  while (parts < kMaxCluster && rows * parts < sms && (int64_t)V > batch * parts) parts *= 2;
   return parts;
 }
 
@@ -1007,10 +1018,8 @@ int parts_of(int64_t rows, int V, int elem) {
 template <typename Args>
 int launch_rows(void (*kern)(Args), const Args& a, size_t smem, size_t fixed, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return (int)e;
+  const int sms = sm_count();
+  if (sms == 0) return (int)cudaErrorInvalidDevice;
   const size_t fit = (227 << 10) / (smem + fixed + 1024);
   const int64_t stay = (int64_t)(fit < kCtas ? fit : kCtas) * sms;
   cfg.gridDim = dim3((unsigned)(a.parts > 1 || a.n < stay ? a.n * a.parts : stay));
