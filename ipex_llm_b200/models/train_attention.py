@@ -4,7 +4,7 @@ it, and the package's usual path elsewhere (soft-capped scores, dropout, masks t
 types and head sizes, single tokens).
 
 Masks: a causal mask, with or without a window, stays what it is, and padding stays ``[batch, keys]``; no mask of the size of
-queries x keys is kept for them (a window's is looked at once, to see that it is one).  Padding and windows travel in a type
+queries x keys is kept for them (a window's function is looked at, some rows at a time).  Padding and windows travel in a type
 that no arithmetic takes (``_compact``): a module that would use such a mask in a way of its own raises, where truth values
 ``[batch, keys]`` would pass for a mask of scores without a causal limit.
 """
@@ -16,6 +16,7 @@ from ..ops.train_attn import MAX_DIM, MAX_HEADS, attention
 from .common import TRAIN_INTERFACE_NAME, _uses_attention_registry, attention_interface
 from .decoder import decoder_attention_forward
 
+_LOOKED_AT = 1 << 24               # pairs of a query and a key at a time, where a mask function is looked at
 _CARRIER = torch.float8_e5m2       # the bytes of truth values; sums, products, comparisons with other types and SDPA refuse it
 
 
@@ -53,15 +54,18 @@ def whole_mask(mask, q_length: int):
 
 
 def _is_window(mask_function, q_length: int, kv_length: int, window: int, device) -> bool:
-    """Is this mask causal attention to the last ``window`` keys, at every query and key?"""
-    q = torch.arange(q_length, device=device).view(1, 1, -1, 1) + (kv_length - q_length)
+    """Is this mask causal attention to the last ``window`` keys, at every query and key?  Looked at some rows at a time."""
+    rows = max(1, _LOOKED_AT // kv_length)
     key = torch.arange(kv_length, device=device).view(1, 1, 1, -1)
     zero = torch.zeros((1, 1, 1, 1), dtype=torch.long, device=device)
+    same = []
     try:
-        own = mask_function(zero, zero, q, key)
+        for first in range(0, q_length, rows):
+            q = torch.arange(first, min(first + rows, q_length), device=device).view(1, 1, -1, 1) + (kv_length - q_length)
+            same.append(((key <= q) & (key > q - window) == mask_function(zero, zero, q, key)).all())
     except Exception:  # noqa: BLE001  (a function that takes single indices only)
         return False
-    return torch.is_tensor(own) and bool(((key <= q) & (key > q - window) == own).all())
+    return bool(torch.stack(same).all())
 
 
 def _mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None, **kwargs):

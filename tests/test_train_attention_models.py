@@ -229,3 +229,22 @@ def test_what_masks_stand_for(window, Sq, Skv):
         want = see[None, None] if padding is None else see & real[:, None, None, :]
         assert torch.equal(train_attention.whole_mask(mask, Sq), want)
         assert torch.equal(train_attention.whole_mask(mask.detach(), Sq), want)
+
+
+@pytest.mark.parametrize("q_length,kv_length", [(50, 50), (31, 50), (1, 7)])
+@pytest.mark.parametrize("differs", [None, (0, 0), (13, 20), (30, 49)])
+def test_windows_are_told_by_some_rows_at_a_time(q_length, kv_length, differs, monkeypatch):
+    """Nothing of the size of queries x keys is made for long sequences, and every pair counts."""
+    monkeypatch.setattr(train_attention, "_LOOKED_AT", 120)
+    pairs = []
+
+    def mask(batch, head, q, key):
+        own = (key <= q) & (key > q - 9)
+        pairs.append(own.numel())
+        if differs is not None:
+            own = own ^ ((q == differs[0] + kv_length - q_length) & (key == differs[1]))
+        return own
+    inside = differs is not None and differs[0] < q_length and differs[1] < kv_length
+    assert train_attention._is_window(mask, q_length, kv_length, 9, "cpu") == (not inside)
+    assert max(pairs) <= 120 and sum(pairs) == q_length * kv_length
+    assert q_length == 1 or not train_attention._is_window(lambda b, h, q, k: True, q_length, kv_length, 9, "cpu")
