@@ -22,10 +22,12 @@
 //   dq          a pass of its own over the keys, which computes s and dP once more (7 products in all where 5 would do): the
 //               sums then need no atomics, whose order would change results, and no 32-bit dq in global memory
 // Sixteen warps of arithmetic hide each other's latencies: with eight, two to a scheduler, an exponential's chain (product,
-// special function, conversion) showed, and a block of 128 x 128 took 2900 (forward), 3800 and 3250 clocks, of which the products
-// alone are 1030, 2180 and 1540.  Now, with 4096 tokens, 64 heads of 128 over 8 of keys, causal, bf16: 345, 540 and 415 us (41 for
-// the pass before the backward), 1.5, 2.1 and 1.8 us a block.  With all arithmetic taken out a block still takes 1700 (forward) and
-// 2870 clocks (dk and dv): the products' issue and arrivals between the roles are what is left to win.
+// special function, conversion) showed, and a block of 128 x 128 took 2900 clocks forward, 3800 for dk and dv and 3250 for dq, of
+// which the products alone are 1030, 2180 and 1540.  Now they are 2530, 3570 and 3060: 4096 tokens, 64 heads of 128 over 8 of keys,
+// causal, bf16 take 332, 515 and 395 us (37 for the pass before the backward) at 1.78 GHz, where one CTA has at most 233, 256 and 229
+// blocks (228 on average).
+// With all arithmetic taken out a block still takes 1700 (forward) and 2870 clocks (dk and dv): the products' issue and arrivals
+// between the roles are what is left to win.
 //
 // In the transposed scores L_i and delta_i belong to columns, not to the threads' rows.  Read from shared memory, four numbers a
 // request, they took a third of its bandwidth, which the products need.  So they are summed by the products too: one more step
@@ -711,12 +713,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 }
 
 // ------------------------------------------------------------------------------------------------ before the backward pass
-// delta_i = dO_i . o_i (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
-// heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
 // Pieces of 16 bits whose weighted sum is x, in a row of eight numbers: each takes what those before it leave, the last below
 // 2^-24 of x.  fp16's weights spread its pieces over numbers up to 65504 x 2^15, to 2^-45: a first piece x / 2^15 leaves at most
-// 2^-12 |x| or 2^-10, and so on.  (Three pieces with weights of 2^8 and less end at 2^24, which dO_i . o_i passes where a loss is scaled; a
-// column more costs nothing, the product takes sixteen anyway.)
+// 2^-12 |x| or 2^-10, and so on.  (Three pieces with weights of 2^8 and less end at 2^24, which dO_i . o_i passes where a loss is
+// scaled; a column more costs nothing, the product takes sixteen anyway.)
 template <typename T> struct Pieces;
 template <> struct Pieces<__nv_bfloat16> {
   static constexpr int kN = 3;
@@ -763,6 +763,9 @@ __device__ __forceinline__ float dot8(const uint4& x, const uint4& y) {
   return d;
 }
 
+// delta_i = dO_i . o_i (and zeros behind Sq); in fp16 also the largest |dO_i|^2 and |v_j|^2 of each group of
+// heads that share keys.  The maxima are of non-negative numbers, whose bits order like integers: any order gives the same.
+//
 // A CTA to 128 rows of a head, LANES lanes to a row (eight columns each), the rows of a group of lanes in flight four at a time.
 // What a row gets is written by a lane of its own (in fp16 12.5 us instead of 15 for 2 x 1031 tokens in 32 heads of
 // 80, where one lane loads -L / scale and cuts numbers into pieces for all rows of its group; in bf16 the same).  blockIdx.y counts
@@ -855,14 +858,6 @@ __device__ __forceinline__ void zero_rows(void* out, int b, int row, int rows, i
 }
 
 // ------------------------------------------------------------------------------------------------ dk and dv
-template <int D>
-struct DqSmem {
-  static constexpr int kTile = kT * D * 2;
-  static constexpr int kK = D == 128 ? 3 : 4, kV = D == 128 ? 2 : 4;     // tiles of k are kept for longer
-  static constexpr int kBars = (2 + kK + kV) * kTile;
-  static constexpr int kSize = 1024 + kBars + 256;
-};
-
 template <int D>
 struct BwdSmem {
   static constexpr int kTile = kT * D * 2;
@@ -1177,6 +1172,14 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 }
 
 // ------------------------------------------------------------------------------------------------ dq
+template <int D>
+struct DqSmem {
+  static constexpr int kTile = kT * D * 2;
+  static constexpr int kK = D == 128 ? 3 : 4, kV = D == 128 ? 2 : 4;     // tiles of k are kept for longer
+  static constexpr int kBars = (2 + kK + kV) * kTile;
+  static constexpr int kSize = 1024 + kBars + 256;
+};
+
 // A tile of queries [q0, q0 + 128) of a head, and the blocks of keys that it may see.
 struct DqItem {
   int q0, h, b, kvh, j0, total;

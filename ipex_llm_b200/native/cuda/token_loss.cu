@@ -12,9 +12,11 @@
 // parts are joined.  Seven warps of a CTA read; an eighth does what a row has beside its sums (its target, the teacher's tokens,
 // the results), on this row while the others read it and on its sums while they read the next one: in their way, those latencies
 // took half of the time.  Four such CTAs to an SM: what is left of a row's latencies (the joining of its sums) hides behind the
-// other CTAs' rows (2048 rows of 32000 in bf16: 38 us, with two CTAs of sixteen warps 47; the divergence 37 against 52 us).  Then
-// instructions are the bound, and maxima by pairs of 16-bit numbers, as they are, and whole batches without a test for each vector
-// make it 34 us (3.9 TB/s; both measured by themselves: 35.6 and 34).  Backward is a plain pass of 224 threads to a row, four vectors in flight (43 us for these rows, 6.1 TB/s).
+// other CTAs' rows.  2048 rows of 32000 in bf16 took 47 us with two CTAs of sixteen warps and 38 so (the divergence 52 and 37); maxima
+// by pairs of 16-bit numbers, as they are, whole batches without a test for each vector and a warp's sums joined at one base made it
+// 30 us (4.4 TB/s; the divergence 32).  Nothing is at its limit then: while CTAs run, 62 % of the issue slots and 60 % of what the
+// special function units do are taken, and 2048 rows are 3.46 rounds of 592 CTAs that take 4.  Backward is a plain pass of 224
+// threads to a row, four vectors in flight (43 us for these rows, 6.1 TB/s).
 // A thread folds the maximum of a batch into its own and rescales its sums once for all of it, so that an element costs one
 // exponential (0.73 of what the special function units do at the rate of memory, for 16-bit logits).
 // y is one fma: what rounding takes from r, common to a row, takes part everywhere alike and so cancels, as long as r is the same
@@ -23,7 +25,8 @@
 // sums adds up.  From |c max x| = 2^24 on (masks of -1e10, temperatures of 1e-6) r is no longer within a half of it, and what the
 // fma leaves may be of any size: there y = (x - max x) c.
 //
-// Statistics are 32-bit, 150 to 600 elements to a thread's sum and a tree above that; exponentials by ex2.approx (2 ulp).
+// Statistics are 32-bit: V / (224 x CTAs of a row) elements to a thread's sum (143 of 32000, 573 of 128256 with one CTA to a row)
+// and a tree above that; exponentials by ex2.approx (2 ulp).
 #include <cooperative_groups.h>
 
 #include <type_traits>

@@ -8,7 +8,6 @@ refused.
 """
 from __future__ import annotations
 
-import contextlib
 import math
 from typing import NamedTuple, Optional
 
@@ -19,7 +18,7 @@ from ..native import cuda_api as api
 from ..native.lib import current_stream, ptr, stream_lib
 from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
-from .gradients import refuse_tangents
+from .gradients import on, refuse_tangents
 
 MAX_TOP = 32             # alternatives of a row
 MAX_TEACHER = 1024       # tokens of a teacher's row
@@ -46,14 +45,6 @@ def _rows(logits: torch.Tensor):
     if logits.dim() == 3:
         return logits, logits.stride(0), logits.stride(1), logits.shape[1]
     return logits, 0, logits.stride(0) if logits.dim() == 2 else 0, logits.shape[0] if logits.dim() == 2 else 1
-
-
-def _on(dev: torch.device):
-    """A guard for launches on another device than the current one."""
-    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
-
-
-_HERE = contextlib.nullcontext()
 
 
 def _check_logits(logits: torch.Tensor, temperature: float, what: str):
@@ -87,7 +78,7 @@ def _token_logprobs(logits, targets, temperature, entropy, top, ignore, keep):
     top_lp = torch.empty((*shape, top), dtype=torch.float32, device=dev) if top else None
     top_id = torch.empty((*shape, top), dtype=torch.int64, device=dev) if top else None
     if rows:
-        with _on(dev):
+        with on(dev):
             rc = stream_lib("token_loss").ipex_token_logprobs(
                 ptr(x), s0, s1, n1, ptr(targets), ptr(logprob), ptr(ent), ptr(stats), ptr(top_lp), ptr(top_id), rows, V, top, ignore,
                 temperature, api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
@@ -118,7 +109,7 @@ class _TokenLogprobs(torch.autograd.Function):
         g = None if g is None else g.float().contiguous()
         g_ent = None if g_ent is None else g_ent.float().contiguous()
         if rows:
-            with _on(dev):
+            with on(dev):
                 rc = stream_lib("token_loss").ipex_token_logprobs_grad(
                     ptr(x), s0, s1, n1, ptr(targets), ptr(stats), ptr(g), ptr(g_ent), ptr(dx), rows, x.shape[-1], ctx.ignore,
                     ctx.temperature, api.dtype_code(x.dtype), current_stream())
@@ -191,7 +182,7 @@ def _distill(logits, ids, values, lse, temperature, keep):
     rows = loss.numel()
     stats = torch.empty((rows, 8), dtype=torch.float32, device=dev) if keep else None
     if rows:
-        with _on(dev):
+        with on(dev):
             rc = stream_lib("token_loss").ipex_distill(
                 ptr(x), s0, s1, n1, ptr(ids), ptr(values), ptr(lse), ptr(loss), ptr(stats), rows, V, K, temperature,
                 api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
@@ -216,7 +207,7 @@ class _Distill(torch.autograd.Function):
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
         g = g.float().contiguous()
         if g.numel():
-            with _on(dev):
+            with on(dev):
                 rc = stream_lib("token_loss").ipex_distill_grad(
                     ptr(x), s0, s1, n1, ptr(ids), ptr(values), ptr(stats), ptr(g), ptr(dx), g.numel(), x.shape[-1], ids.shape[-1],
                     ctx.temperature, api.dtype_code(x.dtype), current_stream())

@@ -5,7 +5,6 @@ On a CUDA tensor the package's own kernels run, on the current stream of the ten
 """
 from __future__ import annotations
 
-import contextlib
 import math
 from typing import Optional
 
@@ -16,7 +15,7 @@ from ..native import cuda_api as api
 from ..native.lib import current_stream, ptr, stream_lib
 from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
-from .gradients import refuse_tangents
+from .gradients import on, refuse_tangents
 
 MAX_DIM = 128
 MAX_HEADS = 65535       # of queries and keys together
@@ -35,14 +34,6 @@ def _fit(t: torch.Tensor):
     return at, b, h, s, t
 
 
-def _on(dev: torch.device):
-    """A guard for launches on another device than the current one."""
-    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
-
-
-_HERE = contextlib.nullcontext()
-
-
 def _forward(q, k, v, key_mask, scale, causal, window, keep: bool):
     """The outputs [B, Sq, Hq, D] and, with ``keep``, what the backward pass needs."""
     lib, dev = stream_lib("train_attn"), q.device
@@ -57,7 +48,7 @@ def _forward(q, k, v, key_mask, scale, causal, window, keep: bool):
     if keep:
         stats = torch.empty((B, Hq, -(-Sq // _TILE) * _TILE), dtype=torch.float32, device=dev)
         low = torch.empty_like(out)
-    with _on(dev):
+    with on(dev):
         st, err = current_stream(), ptr(error_flag(dev))
         if key_mask is not None:
             words = torch.empty((B, -(-Skv // _TILE) * (_TILE // 32)), dtype=torch.int32, device=dev)
@@ -92,7 +83,7 @@ class _Attention(torch.autograd.Function):
         dk = torch.empty((B, Skv, Hkv, D), dtype=q.dtype, device=dev)
         dv = torch.empty_like(dk)
         work = torch.empty(9 * stats.numel() + 2 * B * Hkv, dtype=torch.float32, device=dev)
-        with _on(dev):
+        with on(dev):
             rc = stream_lib("train_attn").ipex_attn_train_bwd(
                 *q_at, *k_at, *v_at, ptr(words), ptr(out), ptr(low), ptr(stats), *g_at, ptr(work), ptr(dq), ptr(dk), ptr(dv),
                 *ctx.sizes, ptr(error_flag(dev)), current_stream())
