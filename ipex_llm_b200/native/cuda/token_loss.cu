@@ -428,7 +428,7 @@ __device__ void scan(const T* x, const Slice<T>& sl, float c, Feed<T>& feed, con
           for (int i = 0; i < VEC; ++i) mx = f[i] != f[i] ? NAN : mx;
         }
       }
-      if (best.at == -1 || order_key(mx, 0) > order_key(best.v, 0)) best = {mx, at + tid};
+      if (best.at == -1 || mx > best.v || (mx != mx && best.v == best.v)) best = {mx, at + tid};   // as order_key has it
     }
     feed.fetch();
   }
