@@ -133,7 +133,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional
     for queries of few keys).  In fp16 the backward pass takes scores up to 2^30 * scale, and rows whose outputs and gradients
     have a product up to 2^30 (NaN past 2^31).  The results do not depend on the order in which anything runs.  A causal limit or
     a window hides a key by a probability of 0: NaN and infinities in such a row may spread to earlier queries, as they do in the
-    formula; behind ``key_mask`` they do not.
+    formula; behind ``key_mask`` they do not.  Those of a query, or of its output's gradient, spread to dk and dv even where the
+    query sees nothing.
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         invalidInputError(False, f"attention: q, k and v should be [batch, heads, tokens, dim], k and v alike; got {tuple(q.shape)}, "
