@@ -53,16 +53,18 @@ def whole_mask(mask, q_length: int):
     return see[None, None] if padding is None else padding[:, None, None, :] & see
 
 
-def _is_window(mask_function, q_length: int, kv_length: int, window: int, device) -> bool:
-    """Is this mask causal attention to the last ``window`` keys, at every query and key?  Looked at some rows at a time."""
-    rows = max(1, _LOOKED_AT // kv_length)
+def _is_window(mask_function, q_length: int, kv_length: int, window: int, device, batch_size: int = 1) -> bool:
+    """Is this mask causal attention to the last ``window`` keys, in every sequence, at every query and key?  Looked at some rows at
+    a time."""
+    rows = max(1, _LOOKED_AT // (kv_length * batch_size))
     key = torch.arange(kv_length, device=device).view(1, 1, 1, -1)
-    zero = torch.zeros((1, 1, 1, 1), dtype=torch.long, device=device)
+    batch = torch.arange(batch_size, device=device).view(-1, 1, 1, 1)
+    head = torch.zeros((1, 1, 1, 1), dtype=torch.long, device=device)
     same = []
     try:
         for first in range(0, q_length, rows):
             q = torch.arange(first, min(first + rows, q_length), device=device).view(1, 1, -1, 1) + (kv_length - q_length)
-            same.append(((key <= q) & (key > q - window) == mask_function(zero, zero, q, key)).all())
+            same.append(((key <= q) & (key > q - window) == mask_function(batch, head, q, key)).all())
     except Exception:  # noqa: BLE001  (a function that takes single indices only)
         return False
     return bool(torch.stack(same).all())
@@ -78,7 +80,7 @@ def _mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_functio
     if ends and (attention_mask is None or attention_mask.shape == (batch_size, kv_length)):
         if mask_function is causal_mask_function:
             return _compact(attention_mask)
-        if window and _is_window(mask_function, q_length, kv_length, window, device):
+        if window and _is_window(mask_function, q_length, kv_length, window, device, batch_size):
             return _compact(attention_mask, window if window < kv_length else 0, kv_length, device)
     return sdpa_mask(batch_size=batch_size, q_length=q_length, kv_length=kv_length, q_offset=q_offset, kv_offset=kv_offset,
                      mask_function=mask_function, attention_mask=attention_mask, **kwargs)

@@ -248,3 +248,18 @@ def test_windows_are_told_by_some_rows_at_a_time(q_length, kv_length, differs, m
     assert train_attention._is_window(mask, q_length, kv_length, 9, "cpu") == (not inside)
     assert max(pairs) <= 120 and sum(pairs) == q_length * kv_length
     assert q_length == 1 or not train_attention._is_window(lambda b, h, q, k: True, q_length, kv_length, 9, "cpu")
+
+
+@pytest.mark.parametrize("name,kw", [("Llama", {}), ("Mistral", dict(sliding_window=5)), ("Qwen2Moe", dict(
+    MOE, use_sliding_window=True, max_window_layers=0, layer_types=["sliding_attention"] * 2, shared_expert_intermediate_size=32))])
+@pytest.mark.parametrize("packed", [(0,), (1,), (0, 1)])
+def test_sequences_packed_into_some_rows(name, kw, packed, calls):
+    """A row that is one sequence says nothing about the others."""
+    model = _model(name, **kw)
+    own = copy.deepcopy(model)
+    assert use_train_attention(own)
+    at = torch.arange(13).repeat(2, 1)
+    for i in packed:
+        at[i, 4 + i:] = torch.arange(9 - i)
+    _same(model, own, dict(_inputs("none"), position_ids=at, use_cache=False))
+    assert calls == []
