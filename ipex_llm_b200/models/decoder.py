@@ -122,12 +122,14 @@ def decoder_attention_forward(self, hidden_states, position_embeddings=None, att
     scaling = getattr(self, spec.scaling_attr, None)
     kv_len = k.shape[2]
     mask = attention_mask
-    if mask is not None and mask.dim() == 4 and mask.shape[-1] != kv_len:
-        mask = mask[..., :kv_len] if mask.shape[-1] > kv_len else None
-    if not alibi and getattr(self.config, "_attn_implementation", None) == TRAIN_INTERFACE_NAME:
+    train = not alibi and getattr(self.config, "_attn_implementation", None) == TRAIN_INTERFACE_NAME
+    if train:
         from .train_attention import is_compact, train_attention_interface, whole_mask
         if is_compact(mask) and mask.shape[1] != kv_len:
-            mask = whole_mask(mask, q_len)[..., :kv_len]
+            mask = whole_mask(mask, q_len)
+    if mask is not None and mask.dim() == 4 and mask.shape[-1] != kv_len:
+        mask = mask[..., :kv_len] if mask.shape[-1] > kv_len else None
+    if train:
         attn_output, _ = train_attention_interface(self, q, k, v, mask, scaling=scaling, is_causal=mask is None and q_len > 1,
                                                    softcap=softcap, sliding_window=sliding_window)
         return self.o_proj(attn_output.reshape(bsz, q_len, -1)), None

@@ -263,3 +263,32 @@ def test_sequences_packed_into_some_rows(name, kw, packed, calls):
         at[i, 4 + i:] = torch.arange(9 - i)
     _same(model, own, dict(_inputs("none"), position_ids=at, use_cache=False))
     assert calls == []
+
+
+class _OtherLength:
+    """A cache that keeps fewer keys than the mask was made for, or gives more."""
+
+    def __init__(self, kept):
+        self.kept = kept
+
+    def update(self, k, v, layer_idx, **kw):
+        return tuple(torch.cat([t, t], 2)[:, :, :self.kept] for t in (k, v))
+
+
+@pytest.mark.parametrize("kept", [9, 13, 17])
+@pytest.mark.parametrize("window", [0, 5])
+@pytest.mark.parametrize("pad", [False, True])
+def test_caches_of_another_length_than_the_mask(kept, window, pad):
+    own = _optimised(_model("Llama")).eval()
+    usual = copy.deepcopy(own)
+    assert use_train_attention(own)
+    x = torch.randn(2, 13, 64, generator=torch.Generator().manual_seed(3))
+    rope = own.model.rotary_emb(x, torch.arange(13).unsqueeze(0))
+    real = torch.arange(13) >= torch.tensor([[0], [3]])
+    mask = train_attention._compact(real if pad else None, window, 13)
+    whole = train_attention.whole_mask(mask, 13)
+    with torch.no_grad():
+        a, b = (m.model.layers[0].self_attn(x, position_embeddings=rope, attention_mask=t, past_key_values=_OtherLength(kept))[0]
+                for m, t in ((usual, whole), (own, mask)))
+    # rows that see nothing apart, the same operations
+    assert (a - b).abs().max() <= TOL * a.abs().max()
