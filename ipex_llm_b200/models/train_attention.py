@@ -124,12 +124,16 @@ def train_attention_interface(module, query, key, value, attention_mask=None, dr
 
 def _dispatches(mod) -> bool:
     """Does the attention of this module reach the interface: by the registry, or by this package's decoder forward (which a model
-    that was optimised has bound to its attention modules)?  With linear attention biases it has masks of its own."""
+    that was optimised has bound to its attention modules)?  With linear attention biases it has masks of its own.  What a hook
+    has wrapped counts as what is inside (``_old_forward``)."""
     if getattr(mod.config, "ipex_alibi", False) or not _uses_attention_registry(mod):
         return False
-    bound = [getattr(m.forward, "__func__", m.forward) for m in mod.modules()
-             if "forward" in m.__dict__ and "Attention" in type(m).__name__]
-    return all(f is decoder_attention_forward for f in bound)
+    for m in mod.modules():
+        if "forward" in m.__dict__ and "Attention" in type(m).__name__:
+            f = getattr(m, "_old_forward", m.forward)
+            if getattr(f, "__func__", f) not in (decoder_attention_forward, type(m).forward):
+                return False
+    return True
 
 
 def use_train_attention(model) -> bool:

@@ -265,6 +265,22 @@ def test_sequences_packed_into_some_rows(name, kw, packed, calls):
     assert calls == []
 
 
+@pytest.mark.parametrize("optimised", [False, True])
+def test_hooks_around_an_attention_are_looked_through(optimised, calls):
+    """As device maps put them: the module's forward is a function of its own around the former one."""
+    model = _model("Llama")
+    if optimised:
+        model = _optimised(model)
+    own = copy.deepcopy(model)
+    for layer in own.model.layers:
+        m = layer.self_attn
+        m._old_forward = m.forward
+        m.forward = lambda *a, _m=m, **kw: _m._old_forward(*a, **kw)
+    assert use_train_attention(own)
+    _same(model, own, dict(_inputs("left"), use_cache=False))
+    assert calls == [0, 0]
+
+
 class _OtherLength:
     """A cache that keeps fewer keys than the mask was made for, or gives more."""
 
