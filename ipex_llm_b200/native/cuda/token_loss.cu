@@ -240,7 +240,7 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b, float c) {
 template <bool ENT, int LANES>
 __device__ __forceinline__ Stat join_lanes(const Stat& a, const Base& base, float c) {
   Stat o;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(o.m) : "f"(a.m));
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(o.m) : "f"(a.m));
   const float d = shift(base, Base(o.m, c), c), f = ex2(d);          // sums of a lane without tokens are 0
   o.s = a.s * f;
   o.t = ENT ? (a.t + a.s * d) * f : a.t * f;

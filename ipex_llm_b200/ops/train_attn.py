@@ -25,7 +25,8 @@ _TILE = 128
 
 def _fit(t: torch.Tensor):
     """The tensor as the kernels' 4-D maps take it, rows contiguous, aligned to 16 bytes, and other strides positive multiples of
-    16 bytes (copied where it is not), behind its pointer and strides.  The stride of a dimension of size 1 is never taken: 8 stands for it."""
+    16 bytes (copied where it is not), behind its pointer and strides.  The stride of a dimension of size 1 is never taken: 8
+    stands for it."""
     (B, H, S, _), (b, h, s, d) = t.shape, t.stride()
     b, h, s = b if B > 1 else 8, h if H > 1 else 8, s if S > 1 else 8
     at = t.data_ptr()
