@@ -48,6 +48,9 @@ COMPONENTS = {
     # training: attention with a gradient, the loss behind the output layer
     "train_attn": ("attn_train_tcgen05.cu",),
     "token_loss": ("token_loss.cu",),
+    "preference": ("preference.cu",),
+    # the update of many tensors at once
+    "adamw": ("adamw.cu",),
 }
 
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

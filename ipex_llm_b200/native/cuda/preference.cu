@@ -1,0 +1,655 @@
+// Losses of preference and policy finetuning straight from logits, with the gradient of the logits.  sm_100a.
+//
+// log p of a row's target, as in token_loss.cu: with c = log2(e) / T, r = rint(c max x) and s = sum 2^(c x - r),
+//   log p_t = x_t / T - (r / c / T + log s)            d log p_t / dx_j = (1[j = t] - p_j) / T
+//
+// preferred over rejected: S = sum (or mean) of a sequence's log p, h = (S_c - R_c) - (S_r - R_r), z = b h - margin,
+//   sigmoid  (1 - e) log(1 + e^-z) + e log(1 + e^z)    dh: b (e sig(z) - (1 - e) sig(-z))
+//   hinge    max(0, 1 - b h)                           dh: -b where b h < 1
+//   ipo      (h - 1 / 2b)^2                            dh: 2 (h - 1 / 2b)
+// policy: w = e^(log p - old), d = ref - log p,
+//   -min(w A, min(max(w, 1 - lo), 1 + hi) A) + k (e^d - d - 1)      d log p: -A w where w A is the smaller, + k (1 - e^d)
+//
+// Prompts and padding have no target: their logits are never read.  A first kernel lists the rows that have one; the second reads
+// them: batches of 32 x 4 vectors of 16 bytes, all rows' behind one another, are dealt to the warps in equal runs, whatever rows
+// they belong to, so that no warp waits for another and none has more to do; a run leaves the maximum and the sum of each row that
+// it touches.  The third joins those of a row (up to kSlots) and does what comes behind them, in 64 bits.  The backward pass deals
+// its batches the same way, from the last row to the first, whose logits are still in L2, then the rows without a target, which it
+// only writes.  All of it is bound by memory.
+#include "common/logit_rows.cuh"
+#include "common/utils.cuh"
+#include "tcgen05_common.cuh"
+
+namespace {
+
+constexpr int kNT = 256;
+constexpr int kU = 4;                       // vectors of a lane in a batch
+constexpr int kBatch = 32 * kU;             // vectors of a batch
+constexpr int kCtas = 4;                    // to an SM
+constexpr int kRun = 16;                    // batches of a warp's run, at most where a warp has many
+constexpr int kSlots = 18;                  // runs that may have a part in a row
+
+// What the forward pass keeps: the rows with a target, then those without, and each row's place among the former (-1: none); the
+// largest logit and 1 / sum of each listed row; how a listed row's loss (policy) or a sequence's (preference) moves with its log p.
+struct Keep {
+  int* count;
+  int* list;
+  int* place;
+  float2* stat;
+  float* slope;
+  float* share;      // of a row's log p in its sequence's
+};
+__host__ __device__ inline Keep keep_at(void* at, int64_t rows) {
+  char* b = reinterpret_cast<char*>(at);
+  const int64_t r = (rows + 3) / 4 * 4;
+  Keep k;
+  k.count = reinterpret_cast<int*>(b);
+  k.stat = reinterpret_cast<float2*>(b + 16);
+  k.list = reinterpret_cast<int*>(b + 16 + 8 * r);
+  k.place = k.list + r;
+  k.slope = reinterpret_cast<float*>(k.place + r);
+  k.share = k.slope + r;
+  return k;
+}
+constexpr int64_t keep_bytes(int64_t rows) { return 16 + 24 * ((rows + 3) / 4 * 4); }
+
+// How the batches of `count` rows of `per` each are dealt to `warps`: runs of `len`.
+struct Deal {
+  int64_t total;
+  int per, len, first;
+  __device__ Deal(int count, int per_, int warps) : total((int64_t)count * per_), per(per_) {
+    const int64_t rounds = max((int64_t)1, (total + (int64_t)warps * kRun - 1) / ((int64_t)warps * kRun));
+    const int least = per / (kSlots - 2) + 1;                     // so that kSlots runs reach through a row
+    const int64_t even = (total + warps * rounds - 1) / (warps * rounds);
+    len = (int)max((int64_t)least, even);
+  }
+  __device__ int64_t runs() const { return (total + len - 1) / len; }
+  __device__ int64_t run_of(int place) const { return (int64_t)place * per / len; }   // the first one with a part in a row
+};
+
+__host__ __device__ inline int batches_of(int V, int vec) {
+  const int nvec = V / vec;
+  return nvec > kBatch ? (nvec + kBatch - 1) / kBatch : 1;
+}
+
+// A row [V] of any alignment: elements in front of the first 16-byte boundary, vectors, what is left.
+template <typename T>
+struct Span {
+  static constexpr int VEC = 16 / sizeof(T);
+  int head, nvec, tail;
+  __device__ Span(const void* x, int V) {
+    const int off = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
+    head = off ? min(VEC - off, V) : 0;
+    nvec = (unsigned)(V - head) / VEC;
+    tail = V - head - nvec * VEC;
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ rows with a target
+constexpr int kListNT = 1024, kListRows = 4;
+
+__global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int64_t rows, int64_t ignore, void* keep) {
+  __shared__ int sums[kListNT / 32];
+  pdl_launch_dependents();
+  const Keep k = keep_at(keep, rows);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int have = 0;                                       // so far
+  for (int64_t at = 0; at < rows; at += kListNT * kListRows) {
+    const int64_t r0 = at + threadIdx.x * kListRows;
+    bool real[kListRows];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < kListRows; ++i) {
+      real[i] = r0 + i < rows && targets[r0 + i] != ignore;
+      mine += real[i];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int all = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, all, o);
+      if (lane >= o) all += v;
+    }
+    const int before = __shfl_sync(0xffffffffu, all, warp == 0 ? 0 : warp - 1);
+    int place = have + (warp == 0 ? 0 : before) + upto - mine;
+    have += __shfl_sync(0xffffffffu, all, 31);
+#pragma unroll
+    for (int i = 0; i < kListRows; ++i) {
+      if (r0 + i >= rows) break;
+      if (real[i]) k.list[place] = (int)(r0 + i);
+      else k.list[rows - 1 - (r0 + i - place)] = (int)(r0 + i);
+      k.place[r0 + i] = real[i] ? place : -1;
+      place += real[i];
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *k.count = have;
+}
+
+// ------------------------------------------------------------------------------------------------ sums
+// The maximum and the sum of a lane's part of a row.
+struct Part {
+  Base base;
+  float s;
+};
+template <typename T>
+__device__ __forceinline__ void add_single(Part& p, float v, float c) {
+  const Base now(fmaxf(p.base.m, v), c);              // a NaN is not the maximum, and makes the sum one
+  p.s = p.s * ex2(shift(p.base, now, c)) + ex2(held(now.exponent(v, c)));
+  if (v != v) p.s = v;
+  p.base = now;
+}
+template <typename T>
+__device__ __forceinline__ float largest(const uint4* w, int n) {
+  if constexpr (std::is_same<T, float>::value) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (u >= n) break;
+      float f[4];
+      unpack<T>(w[u], f);
+      mx = max3(max3(mx, f[0], f[1]), f[2], f[3]);
+    }
+    return mx;
+  } else {
+    uint32_t a = max2<T>(w[0].x, w[0].y), b = max2<T>(w[0].z, w[0].w);
+#pragma unroll
+    for (int u = 1; u < kU; ++u) {
+      if (u >= n) break;
+      a = max2<T>(a, max2<T>(w[u].x, w[u].y));
+      b = max2<T>(b, max2<T>(w[u].z, w[u].w));
+    }
+    a = max2<T>(a, b);
+    const T* e = reinterpret_cast<const T*>(&a);
+    return max3(-INFINITY, DT<T>::to_f(e[0]), DT<T>::to_f(e[1]));
+  }
+}
+template <typename T, bool FAR>
+__device__ __forceinline__ float sum_of(const uint4* w, int n, const Base& now, float c) {
+  constexpr int VEC = 16 / sizeof(T);
+  float a[2] = {0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    if (u >= n) break;
+    float f[VEC], v[2] = {0.f, 0.f};
+    unpack<T>(w[u], f);
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) {
+      if (FAR) {
+        f[i] = held(now.exponent(f[i], c));
+        f[i + 1] = held(now.exponent(f[i + 1], c));
+      } else {
+        exponents2(f[i], f[i + 1], c, -now.to);
+      }
+      add2(v[0], v[1], ex2(f[i]), ex2(f[i + 1]));
+    }
+    add2(a[0], a[1], v[0], v[1]);
+  }
+  return a[0] + a[1];
+}
+template <typename T>
+__device__ __forceinline__ void add_batch(Part& p, const uint4* w, int n, float c) {
+  if (n <= 0) return;
+  const Base now(fmaxf(p.base.m, largest<T>(w, n)), c);
+  const float s = now.far ? sum_of<T, true>(w, n, now, c) : sum_of<T, false>(w, n, now, c);
+  p.s = p.s * ex2(shift(p.base, now, c)) + s;
+  p.base = now;
+}
+
+struct SumArgs {
+  Rows rows;
+  int64_t n;
+  const void* keep;
+  float2* part;        // [places, kSlots]
+  float inv_t;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kNT, kCtas) row_sums(SumArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kNT / 32), warp = blockIdx.x * (kNT / 32) + (threadIdx.x >> 5);
+  const Keep k = keep_at(const_cast<void*>(a.keep), a.n);
+  const float c = a.inv_t * kLog2e;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Deal deal(*k.count, batches_of(a.rows.V, VEC), warps);
+  for (int64_t run = warp; run < deal.runs(); run += warps) {
+    int64_t at = run * deal.len;
+    const int64_t end = min(at + deal.len, deal.total);
+    int place = (int)(at / deal.per), b = (int)(at - (int64_t)place * deal.per);
+    for (; at < end; ++place, b = 0) {
+      const T* x = row_at<T>(a.rows, k.list[place]);
+      const Span<T> sp(x, a.rows.V);
+      const int b1 = (int)min((int64_t)deal.per, b + (end - at));
+      at += b1 - b;
+      const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head) + lane;
+      // vectors of this lane, 32 apart, from `from` on
+      auto count = [&](int from) { return min(kU, (sp.nvec - from - lane + 31) / 32); };
+      uint4 w[kU];
+      auto load = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (from + u * 32 + lane < sp.nvec) w[u] = ldg_nc_v4(xv + from + u * 32);
+      };
+      load(b * kBatch);
+      Part p = {Base(-INFINITY, c), 0.f};
+      if (b == 0 && lane < sp.head) add_single<T>(p, DT<T>::to_f(x[lane]), c);
+      if (b1 == deal.per && lane < sp.tail) add_single<T>(p, DT<T>::to_f(x[a.rows.V - sp.tail + lane]), c);
+      for (; b < b1; ++b) {
+        uint4 now[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) now[u] = w[u];
+        if (b + 1 < b1) load((b + 1) * kBatch);
+        add_batch<T>(p, now, count(b * kBatch), c);
+      }
+      // all taken to the largest base, then added up
+      float m;
+      asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(p.base.m));
+      float s = p.s * ex2(shift(p.base, Base(m, c), c));
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) a.part[(int64_t)place * kSlots + (int)(run - deal.run_of(place))] = make_float2(m, s);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ what comes behind the sums
+// A listed row's statistics from its parts, and log p of its target.
+struct RowArgs {
+  Rows rows;
+  const int64_t* targets;
+  int64_t n;
+  void* keep;
+  const float2* part;
+  int warps, per;      // of the sums' launch
+  float temp, inv_t;
+  int* err;
+};
+
+template <typename T>
+__device__ __forceinline__ double row_logprob(const RowArgs& a, const Keep& k, const Deal& deal, int64_t row, int place) {
+  const float c = a.inv_t * kLog2e;
+  const int64_t t = a.targets[row];
+  const bool bad = t < 0 || t >= a.rows.V;
+  const float xt = bad ? 0.f : DT<T>::to_f(row_at<T>(a.rows, row)[t]);
+  const int parts = (int)(((int64_t)(place + 1) * deal.per - 1) / deal.len - deal.run_of(place)) + 1;
+  const float2* at = a.part + (int64_t)place * kSlots;
+  Stat st = {-INFINITY, 0.f, 0.f};
+  for (int i = 0; i < parts; ++i) {
+    const float2 p = at[i];
+    st = join<false>(st, {p.x, p.y, 0.f}, c);
+  }
+  const bool none = no_token(st);
+  const Base base(none ? 0.f : st.m, c);
+  k.stat[place] = make_float2(base.m, none ? 0.f : bad ? NAN : 1.f / st.s);
+  if (bad) {
+    tc5::report(a.err, kErrToken);
+    return NAN;
+  }
+  if (none) return -INFINITY;
+  const double log2_s = log2((double)st.s), lse = log_sum(base, log2_s, c, a.temp);
+  if (base.far) return ((double)xt - base.m) / a.temp - lse;
+  return fabsf(xt) < INFINITY ? xt / (double)a.temp - lse : (double)(xt - (float)log2_s);
+}
+
+struct PolicyArgs {
+  RowArgs row;
+  const float* old;       // [rows] or null: log p itself
+  const float* ref;       // [rows] or null
+  const float* adv;       // strides of outer and inner index
+  int64_t adv0, adv1, inner;
+  float* loss;
+  float* logprob;
+  float* kl;
+  uint8_t* clipped;
+  double lo, hi, weight;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(128) policy_rows(PolicyArgs a) {
+  const Keep k = keep_at(a.row.keep, a.row.n);
+  pdl_wait();
+  const Deal deal(*k.count, a.row.per, a.row.warps);
+  const int64_t row = (int64_t)blockIdx.x * 128 + threadIdx.x;
+  if (row >= a.row.n) return;
+  const int place = k.place[row];
+  float loss = 0.f, kl = 0.f, slope = 0.f;
+  double lp = 0.0;
+  bool clipped = false;
+  if (place >= 0) {
+    lp = row_logprob<T>(a.row, k, deal, row, place);
+    const double A = a.adv[row / a.inner * a.adv0 + row % a.inner * a.adv1];
+    const double w = a.old == nullptr ? 1.0 : exp(lp - a.old[row]);
+    const double inside = w < 1.0 - a.lo ? 1.0 - a.lo : w > 1.0 + a.hi ? 1.0 + a.hi : w;      // NaN stays
+    clipped = inside * A < w * A;
+    double l = -(clipped ? inside * A : w * A), g = clipped ? 0.0 : -A * w;
+    if (a.ref != nullptr) {
+      const double d = a.ref[row] - lp, e = expm1(d);
+      kl = (float)(e - d);
+      l += a.weight * (e - d);
+      g -= a.weight * e;
+    }
+    loss = (float)l;
+    slope = (float)g;
+  }
+  a.loss[row] = loss;
+  a.logprob[row] = (float)lp;
+  a.kl[row] = kl;
+  a.clipped[row] = clipped;
+  k.slope[row] = slope;
+}
+
+enum { FORM_SIGMOID = 0, FORM_HINGE = 1, FORM_IPO = 2 };
+
+struct PairArgs {
+  RowArgs row;
+  const float* reference;   // [2 pairs] or null
+  int64_t tokens;
+  int pairs, form, average;
+  double beta, smooth, margin;
+  float* loss;              // [pairs]
+  float* logprob;           // [2 pairs]
+};
+
+constexpr int kPairNT = 1024;
+
+// A CTA to a pair.
+template <typename T>
+__global__ void __launch_bounds__(kPairNT) pair_losses(PairArgs a) {
+  __shared__ double sums[2][kPairNT / 32];
+  __shared__ int counts[2][kPairNT / 32];
+  const Keep k = keep_at(a.row.keep, a.row.n);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  const Deal deal(*k.count, a.row.per, a.row.warps);
+  for (int half = 0; half < 2; ++half) {
+    const int64_t r0 = ((int64_t)half * a.pairs + blockIdx.x) * a.tokens;
+    double s = 0.0;
+    int n = 0;
+    for (int64_t t = threadIdx.x; t < a.tokens; t += kPairNT) {
+      const int place = k.place[r0 + t];
+      if (place < 0) continue;
+      s += row_logprob<T>(a.row, k, deal, r0 + t, place);
+      ++n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      n += __shfl_xor_sync(0xffffffffu, n, o);
+    }
+    if (lane == 0) {
+      sums[half][warp] = s;
+      counts[half][warp] = n;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  double S[2], share[2];
+  for (int half = 0; half < 2; ++half) {
+    double s = 0.0;
+    int n = 0;
+    for (int w = 0; w < kPairNT / 32; ++w) {
+      s += sums[half][w];
+      n += counts[half][w];
+    }
+    share[half] = a.average ? 1.0 / max(n, 1) : 1.0;
+    S[half] = s * share[half];
+  }
+  const int c = blockIdx.x, r = blockIdx.x + a.pairs;
+  const double h = (S[0] - (a.reference == nullptr ? 0.0 : a.reference[c])) - (S[1] - (a.reference == nullptr ? 0.0 : a.reference[r]));
+  double loss, d;
+  if (a.form == FORM_SIGMOID) {
+    const double z = a.beta * h - a.margin, e = exp(-fabs(z)), near = log1p(e), small = e / (1.0 + e), large = 1.0 / (1.0 + e);
+    const double minus = near + fmax(-z, 0.0), plus = near + fmax(z, 0.0);      // log(1 + e^-z), log(1 + e^z)
+    const double up = z >= 0.0 ? large : small, down = z >= 0.0 ? small : large;
+    loss = (1.0 - a.smooth) * minus + (a.smooth == 0.0 ? 0.0 : a.smooth * plus);
+    d = a.beta * (a.smooth * up - (1.0 - a.smooth) * down);
+    if (z != z) loss = d = z;
+  } else if (a.form == FORM_HINGE) {
+    const double z = 1.0 - a.beta * h;
+    loss = z < 0.0 ? 0.0 : z;
+    d = z > 0.0 ? -a.beta : z != z ? z : 0.0;
+  } else {
+    const double z = h - 0.5 / a.beta;
+    loss = z * z;
+    d = 2.0 * z;
+  }
+  a.loss[c] = (float)loss;
+  a.logprob[c] = (float)S[0];
+  a.logprob[r] = (float)S[1];
+  k.slope[c] = (float)(d * share[0]);
+  k.slope[r] = (float)(-d * share[1]);
+  k.share[c] = (float)share[0];
+  k.share[r] = (float)share[1];
+}
+
+// ------------------------------------------------------------------------------------------------ gradient
+struct GradArgs {
+  Rows rows;
+  const int64_t* targets;
+  int64_t n;
+  const void* keep;
+  const float* g;           // of the loss: strides of outer and inner index; null: none
+  int64_t g0, g1, inner;    // inner: of g's rows; preference: tokens of a sequence
+  const float* g_seq;       // of the sequences' log p, or null
+  int pairs;                // 0: policy
+  void* dx;
+  float inv_t;
+};
+
+template <typename T>
+__device__ __forceinline__ void put(T* y, bool alike, const float* f) {
+  constexpr int VEC = 16 / sizeof(T);
+  __align__(16) T o[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) o[i] = DT<T>::from_f(f[i]);
+  if (alike) {
+    __stcs(reinterpret_cast<uint4*>(y), *reinterpret_cast<const uint4*>(o));      // nothing here reads them again
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y[i] = o[i];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kNT, kCtas) row_grads(GradArgs a) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, warps = gridDim.x * (kNT / 32), warp = blockIdx.x * (kNT / 32) + (threadIdx.x >> 5);
+  const Keep k = keep_at(const_cast<void*>(a.keep), a.n);
+  const float c = a.inv_t * kLog2e;
+  const int V = a.rows.V, count = *k.count;
+  T* dx = reinterpret_cast<T*>(a.dx);
+  const Deal deal(count, batches_of(V, VEC), warps);
+  for (int64_t back = warp; back < deal.runs(); back += warps) {
+    const int64_t run = deal.runs() - 1 - back;
+    int64_t at = run * deal.len;
+    const int64_t end = min(at + deal.len, deal.total);
+    int place = (int)(at / deal.per), b = (int)(at - (int64_t)place * deal.per);
+    for (; at < end; ++place, b = 0) {
+      const int64_t row = k.list[place];
+      const T* x = row_at<T>(a.rows, row);
+      T* y = dx + row * V;
+      const Span<T> sp(x, V);
+      const int b1 = (int)min((int64_t)deal.per, b + (end - at));
+      at += b1 - b;
+      const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head);
+      uint4 w[kU];
+      auto load = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+          if (from + u * 32 + lane < sp.nvec) w[u] = ldg_nc_v4(xv + from + u * 32 + lane);
+      };
+      load(b * kBatch);
+      const float2 st = k.stat[place];
+      const int64_t t = a.targets[row];
+      float g = 0.f;
+      if (a.pairs > 0) {
+        const int64_t seq = row / a.inner;
+        if (a.g != nullptr) g = a.g[(seq < a.pairs ? seq : seq - a.pairs) * a.g0] * k.slope[seq];
+        if (a.g_seq != nullptr) g += a.g_seq[seq] * k.share[seq];
+      } else {
+        g = a.g[row / a.inner * a.g0 + row % a.inner * a.g1] * k.slope[row];
+      }
+      if (st.y == 0.f) g = 0.f;                       // no token in the row
+      const Base base(st.x, c);
+      const float scale = -g * st.y * a.inv_t;
+      const bool nothing = g == 0.f;                  // flows into the row, whatever its logits hold
+      auto of = [&](float v) { return nothing ? 0.f : ex2(base.exponent(v, c)) * scale; };
+      auto of_target = [&](float v) { return nothing ? 0.f : fmaf(g, a.inv_t, of(v)); };
+      const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+      auto single = [&](int j) {
+        const float v = DT<T>::to_f(x[j]);
+        y[j] = DT<T>::from_f(j == t ? of_target(v) : of(v));
+      };
+      if (b == 0 && lane < sp.head) single(lane);
+      if (b1 == deal.per && lane < sp.tail) single(V - sp.tail + lane);
+      for (; b < b1; ++b) {
+        uint4 now[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) now[u] = w[u];
+        if (b + 1 < b1) load((b + 1) * kBatch);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int v = b * kBatch + u * 32 + lane;
+          if (v >= sp.nvec) break;
+          float f[VEC];
+          unpack<T>(now[u], f);
+          const int64_t hit = t - (sp.head + (int64_t)v * VEC);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) f[i] = i == hit ? of_target(f[i]) : of(f[i]);
+          put<T>(y + sp.head + (int64_t)v * VEC, alike, f);
+        }
+      }
+    }
+  }
+  // rows without a target
+  const int per = batches_of(V, VEC);
+  const int64_t rest = (a.n - count) * per;
+  for (int64_t at = warp; at < rest; at += warps) {
+    const int64_t i = at / per;
+    const int b = (int)(at - i * per);
+    T* y = dx + (int64_t)k.list[count + i] * V;
+    const Span<T> sp(y, V);
+    const T zero = DT<T>::from_f(0.f);
+    if (b == 0 && lane < sp.head) y[lane] = zero;
+    if (b == per - 1 && lane < sp.tail) y[V - sp.tail + lane] = zero;
+    uint4* yv = reinterpret_cast<uint4*>(y + sp.head);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int v = b * kBatch + u * 32 + lane;
+      if (v < sp.nvec) __stcs(yv + v, make_uint4(0, 0, 0, 0));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int elem_of(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+int grid_of(int64_t rows, int V, int elem) {
+  const int sms = sm_count();
+  const int64_t batches = rows * batches_of(V, 16 / elem), ctas = (batches + kNT / 32 - 1) / (kNT / 32);
+  return (int)(ctas < (int64_t)sms * kCtas ? ctas : (int64_t)sms * kCtas);
+}
+
+// The first two kernels; then `a` is ready for the third.
+int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
+  if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
+  list_rows<<<1, kListNT, 0, s>>>(a.targets, a.n, ignore, a.keep);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  const int grid = grid_of(a.n, a.rows.V, elem_of(dtype));
+  a.warps = grid * (kNT / 32);
+  a.per = batches_of(a.rows.V, 16 / elem_of(dtype));
+  const SumArgs sums = {a.rows, a.n, a.keep, const_cast<float2*>(a.part), a.inv_t};
+  return by_type(dtype, [&](auto* tag) {
+    return (int)launch_kernel(row_sums<std::remove_pointer_t<decltype(tag)>>, dim3(grid), dim3(kNT), 0, s, true, sums);
+  });
+}
+
+int backward(const GradArgs& a, int dtype, cudaStream_t s) {
+  if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
+  return by_type(dtype, [&](auto* tag) {
+    row_grads<std::remove_pointer_t<decltype(tag)>><<<grid_of(a.n, a.rows.V, elem_of(dtype)), kNT, 0, s>>>(a);
+    return (int)cudaGetLastError();
+  });
+}
+
+bool args_ok(const void* logits, int64_t s0, int64_t s1, int64_t n1, int64_t rows, int V, float temp, int dtype, const void* targets,
+             const void* keep) {
+  return rows_ok(logits, s0, s1, n1, rows, V, elem_of(dtype)) && temp_ok(temp) && targets != nullptr && keep != nullptr &&
+         (reinterpret_cast<uintptr_t>(keep) & 15) == 0;
+}
+
+}  // namespace
+
+// Bytes that the forward pass keeps for the backward one, and those that it works in.
+IPEX_API int64_t ipex_preference_keep_bytes(int64_t rows) { return keep_bytes(rows); }
+IPEX_API int64_t ipex_preference_work_bytes(int64_t rows) { return rows * kSlots * (int64_t)sizeof(float2); }
+
+// logits: rows of V elements, row r at (r / n1) * s0 + (r % n1) * s1; targets [rows] (`ignore`: none, all results 0); old, ref [rows] or
+// null; advantage of row r at (r / inner) * adv0 + (r % inner) * adv1; loss, logprob, kl (0 without ref), clipped [rows].  A target
+// outside of [0, V) gives NaN and sets `err`.  Returns a cudaError_t.
+IPEX_API int ipex_policy_loss(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* targets, const float* old,
+                              const float* ref, const float* adv, int64_t adv0, int64_t adv1, int64_t inner, float* loss,
+                              float* logprob, float* kl, uint8_t* clipped, void* keep, void* work, int64_t rows, int V, int64_t ignore,
+                              double lo, double hi, double weight, float temp, int dtype, int* err, void* stream) {
+  if (!args_ok(logits, s0, s1, n1, rows, V, temp, dtype, targets, keep) || work == nullptr || adv == nullptr || inner < 1 ||
+      loss == nullptr || logprob == nullptr || clipped == nullptr || kl == nullptr)
+    return (int)cudaErrorInvalidValue;
+  RowArgs r = {rows_of(logits, s0, s1, n1, rows, V), targets, rows, keep, (const float2*)work, 0, 0, temp, 1.f / temp, err};
+  const int rc = forward(r, ignore, dtype, (cudaStream_t)stream);
+  if (rc != 0) return rc;
+  const PolicyArgs a = {r, old, ref, adv, adv0, adv1, inner, loss, logprob, kl, clipped, lo, hi, weight};
+  return by_type(dtype, [&](auto* tag) {
+    return (int)launch_kernel(policy_rows<std::remove_pointer_t<decltype(tag)>>, dim3((unsigned)((rows + 127) / 128)), dim3(128), 0,
+                              (cudaStream_t)stream, true, a);
+  });
+}
+
+// g: the loss's gradient, of row r at (r / inner) * g0 + (r % inner) * g1; dlogits [rows, V].
+IPEX_API int ipex_policy_grad(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* targets, const void* keep,
+                              const float* g, int64_t g0, int64_t g1, int64_t inner, void* dlogits, int64_t rows, int V, float temp,
+                              int dtype, void* stream) {
+  if (!args_ok(logits, s0, s1, n1, rows, V, temp, dtype, targets, keep) || g == nullptr || inner < 1 || dlogits == nullptr)
+    return (int)cudaErrorInvalidValue;
+  const GradArgs a = {rows_of(logits, s0, s1, n1, rows, V), targets, rows, keep, g, g0, g1, inner, nullptr, 0, dlogits, 1.f / temp};
+  return backward(a, dtype, (cudaStream_t)stream);
+}
+
+// 2 pairs x tokens rows, the preferred sequences first; reference [2 pairs] or null; form: 0 sigmoid, 1 hinge, 2 ipo; loss [pairs],
+// logprob [2 pairs].
+IPEX_API int ipex_preference_loss(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* targets,
+                                  const float* reference, float* loss, float* logprob, void* keep, void* work, int pairs,
+                                  int64_t tokens, int V, int64_t ignore, int form, int average, double beta, double smooth,
+                                  double margin, float temp, int dtype, int* err, void* stream) {
+  const int64_t rows = 2 * (int64_t)pairs * tokens;
+  if (!args_ok(logits, s0, s1, n1, rows, V, temp, dtype, targets, keep) || work == nullptr || loss == nullptr || logprob == nullptr ||
+      pairs < 1 || form < 0 || form > 2 || !(beta > 0.0))
+    return (int)cudaErrorInvalidValue;
+  RowArgs r = {rows_of(logits, s0, s1, n1, rows, V), targets, rows, keep, (const float2*)work, 0, 0, temp, 1.f / temp, err};
+  const int rc = forward(r, ignore, dtype, (cudaStream_t)stream);
+  if (rc != 0) return rc;
+  const PairArgs a = {r, reference, tokens, pairs, form, average, beta, smooth, margin, loss, logprob};
+  return by_type(dtype, [&](auto* tag) {
+    return (int)launch_kernel(pair_losses<std::remove_pointer_t<decltype(tag)>>, dim3((unsigned)pairs), dim3(kPairNT), 0,
+                              (cudaStream_t)stream, true, a);
+  });
+}
+
+// g [pairs] (every g0-th) and g_seq [2 pairs]: gradients of the losses and of the sequences' log p; either may be null.
+IPEX_API int ipex_preference_grad(const void* logits, int64_t s0, int64_t s1, int64_t n1, const int64_t* targets, const void* keep,
+                                  const float* g, int64_t g0, const float* g_seq, void* dlogits, int pairs, int64_t tokens, int V,
+                                  float temp, int dtype, void* stream) {
+  const int64_t rows = 2 * (int64_t)pairs * tokens;
+  if (!args_ok(logits, s0, s1, n1, rows, V, temp, dtype, targets, keep) || dlogits == nullptr || pairs < 1)
+    return (int)cudaErrorInvalidValue;
+  const GradArgs a = {rows_of(logits, s0, s1, n1, rows, V), targets, rows, keep, g, g0, 0, tokens, g_seq, pairs, dlogits, 1.f / temp};
+  return backward(a, dtype, (cudaStream_t)stream);
+}

@@ -10,6 +10,8 @@ vp = ctypes.c_void_p
 ci = ctypes.c_int
 i64 = ctypes.c_int64
 cf = ctypes.c_float
+cd = ctypes.c_double
+cu = ctypes.c_uint32
 
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 WF_SYM_INT4, WF_ASYM_INT4, WF_LUT4, WF_FP8_E4M3, WF_FP8_E5M2, WF_INT8, WF_F16, WF_BF16 = range(8)
@@ -167,6 +169,17 @@ COMPONENT_SIGS = {
         "ipex_distill": [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, ci, ci, cf, ci, vp, vp],
         "ipex_distill_grad": [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, ci, ci, cf, ci, vp],
     },
+    "preference": {
+        "ipex_policy_loss": [vp, i64, i64, i64, vp, vp, vp, vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, i64, ci, i64, cd, cd, cd, cf, ci,
+                             vp, vp],
+        "ipex_policy_grad": [vp, i64, i64, i64, vp, vp, vp, i64, i64, i64, vp, i64, ci, cf, ci, vp],
+        "ipex_preference_loss": [vp, i64, i64, i64, vp, vp, vp, vp, vp, vp, ci, i64, ci, i64, ci, ci, cd, cd, cd, cf, ci, vp, vp],
+        "ipex_preference_grad": [vp, i64, i64, i64, vp, vp, vp, i64, vp, vp, ci, i64, ci, cf, ci, vp],
+    },
+    "adamw": {
+        "ipex_adamw_step": [vp, vp, vp, i64, vp, vp, vp, vp, vp, ci, vp, ci, vp, vp, cd, cd, vp, cd, cd, cd, cd, cu, ci, ci, vp],
+        "ipex_grad_norm": [vp, vp, i64, vp, vp, ci, vp],
+    },
     "linear": {
         "ipex_linear_chunks_ok": [ci, ci, ci],
         "ipex_linear_fused_ok": [ci],
@@ -183,12 +196,19 @@ _SCRATCH_FLOATS = {"delta": ("ipex_delta_scratch_floats",), "general_delta": ("i
                    "linear": ("ipex_linear_scratch_floats",), "ssd": ("ipex_ssd_group_floats", "ipex_ssd_head_floats")}
 
 
+# room that a call needs: count -> how much
+_SIZES = {"adamw": ("ipex_grad_norm_sums",), "preference": ("ipex_preference_keep_bytes", "ipex_preference_work_bytes")}
+
+
 def declare_component(lib: ctypes.CDLL, name: str):
     for fn_name, args in COMPONENT_SIGS[name].items():
         fn = getattr(lib, fn_name)
         fn.argtypes, fn.restype = args, ci
     if name == "stream":
         lib.ipex_gemv_rows_tune.argtypes, lib.ipex_gemv_rows_tune.restype = [ci], None
+    for fn_name in _SIZES.get(name, ()):
+        fn = getattr(lib, fn_name)
+        fn.argtypes, fn.restype = [i64], i64
     for fn_name in _SCRATCH_FLOATS.get(name, ()):
         fn = getattr(lib, fn_name)
         fn.argtypes, fn.restype = [ci, ci], i64
