@@ -326,16 +326,19 @@ __global__ void __launch_bounds__(128) policy_rows(PolicyArgs a) {
   if (place >= 0) {
     lp = row_logprob<T>(a.row, k, deal, row, place);
     const double A = a.adv[row / a.inner * a.adv0 + row % a.inner * a.adv1];
-    const double w = a.old == nullptr ? 1.0 : exp(lp - a.old[row]);
+    const double w = a.old != nullptr ? exp(lp - a.old[row]) : lp == lp ? 1.0 : lp;
     const double inside = w < 1.0 - a.lo ? 1.0 - a.lo : w > 1.0 + a.hi ? 1.0 + a.hi : w;      // NaN stays
     clipped = inside * A < w * A;
     double l = -(clipped ? inside * A : w * A), g = clipped ? 0.0 : -A * w;
     if (a.ref != nullptr) {
-      const double d = a.ref[row] - lp, e = expm1(d);
-      kl = (float)(e - d);
-      l += a.weight * (e - d);
-      g -= a.weight * e;
+      const double d = a.ref[row] - lp, e = expm1(d), est = e < INFINITY ? e - d : e;
+      kl = (float)est;
+      if (a.weight != 0.0) {
+        l += a.weight * est;
+        g -= a.weight * e;
+      }
     }
+    if (lp == -INFINITY) g = 0.0;                     // a hidden target: no other logit brings it back
     loss = (float)l;
     slope = (float)g;
   }

@@ -192,7 +192,8 @@ def _policy_plain(logits, targets, advantages, old, ref, lo, hi, weight, tempera
     lp = token_logprobs(logits, targets, temperature, ignore_index=ignore).logprob
     real = targets != ignore
     wide = lp.double()
-    ratio = torch.exp(wide - (wide.detach() if old is None else old.double()))
+    moved = wide.masked_fill(wide == -math.inf, 0.0) if old is None else wide        # a hidden token's ratio to itself is 1, too
+    ratio = torch.exp(moved - (moved.detach() if old is None else old.double()))
     a = advantages.double()
     held = ratio.clamp(1.0 - lo, 1.0 + hi)
     clipped = held * a < ratio * a
@@ -200,8 +201,9 @@ def _policy_plain(logits, targets, advantages, old, ref, lo, hi, weight, tempera
     kl = torch.zeros_like(wide)
     if ref is not None:
         d = ref.double() - wide
-        kl = torch.expm1(d) - d
-        loss = loss + weight * kl
+        far = d.detach() == math.inf
+        kl = torch.where(far, math.inf, torch.expm1(d.masked_fill(far, 0.0)) - d.masked_fill(far, 0.0))
+        loss = loss + weight * kl if weight else loss
     return PolicyLoss(torch.where(real, loss, 0.0).to(lp.dtype), lp.detach(), torch.where(real, kl, 0.0).detach().to(lp.dtype), clipped & real)
 
 
@@ -217,7 +219,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
 
     Without ``old_logprobs`` they are lp itself (one step for each batch): w is 1 and still has its gradient.  Targets of
     ``ignore_index`` give 0 and no gradient, and their logits are not read.  The gradient goes to the logits alone (in their type: 16
-    or 32 bits).  A hidden target (a logit of -inf) has w = 0 and an infinite KL term.  A target outside of the vocabulary raises on
+    or 32 bits).  A hidden target (a logit of -inf) has w = 0, an infinite KL term and no gradient.  A target outside of the vocabulary raises on
     the CPU; on the GPU its results are NaN, and ``cuda_ops.check_error_flag`` reports 61.
     """
     what = "policy_loss"
