@@ -1,12 +1,13 @@
 """In-tree build of the native libraries.
 
-Two shared objects and one executable are produced next to this file:
+Three shared objects and one executable are produced next to this file:
 
 * ``libipex_quant_core.so``  — C++ host library (quantizers, layout transforms, CPU matmul oracle)
 * ``libipex_llm_cuda.so``    — every sm_100a CUDA kernel of the package, plain C ABI launchers
+* ``libipex_calls.so``       — calls of training kernels with lists of tensors, autograd nodes (C++ on PyTorch's headers)
 * ``bin/ipex-quantize``      — GGUF -> k-quant GGUF rewriter on the host library (``tools/quantize_main.cpp``)
 
-Both are loaded through ctypes (``ipex_llm_b200.native.lib``).  A content hash of the sources is kept
+The first two are loaded through ctypes (``ipex_llm_b200.native.lib``), the third is a Python extension.  A content hash of the sources is kept
 beside each library so that an unchanged tree is never recompiled (the libraries travel with the
 source snapshot to GPU machines, where nothing has to be rebuilt).
 
@@ -26,12 +27,14 @@ HOST_DIR = os.path.join(HERE, "host")
 CUDA_DIR = os.path.join(HERE, "cuda")
 OBJ_DIR = os.path.join(HERE, "build")
 
+TORCH_DIR = os.path.join(HERE, "torch")
 TOOLS_DIR = os.path.join(HERE, "tools")
 BIN_DIR = os.path.join(HERE, "bin")
 QUANTIZE_BIN = os.path.join(BIN_DIR, "ipex-quantize")
 
 HOST_LIB = os.path.join(HERE, "libipex_quant_core.so")
 CUDA_LIB = os.path.join(HERE, "libipex_llm_cuda.so")
+CALLS_LIB = os.path.join(HERE, "libipex_calls.so")
 
 # Parts of the kernel library that stand on their own.  A process that needs one of them and finds no complete library
 # compiles just these sources (seconds instead of minutes); ``build_cuda`` always builds everything.
@@ -124,6 +127,31 @@ def build_tools(force=False, verbose=False):
     return QUANTIZE_BIN
 
 
+def build_calls(force=False, verbose=False):
+    """The extension on PyTorch's headers; it fits the PyTorch that it was built with alone."""
+    import sysconfig
+
+    import torch
+    srcs = _sources(TORCH_DIR, (".cpp",))
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc() or "/usr/local/cuda/bin/nvcc"))
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    digest = _hash_files(srcs, " ".join([*flags, torch.__version__, sys.version]))
+    if not force and _stamp_ok(CALLS_LIB, digest):
+        return CALLS_LIB
+    part = f"{CALLS_LIB}.{os.getpid()}"
+    cmd = ["g++", *flags, *(f"-I{d}" for d in (f"{root}/include", f"{root}/include/torch/csrc/api/include", f"{cuda}/include",
+                                               sysconfig.get_paths()["include"])),
+           "-o", part, *srcs, f"-L{root}/lib", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.check_call(cmd)
+    os.replace(part, CALLS_LIB)
+    _write_stamp(CALLS_LIB, digest)
+    return CALLS_LIB
+
+
 def cuda_flags(verbose=False):
     flags = [*NVCC_ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
              "--expt-relaxed-constexpr", "-I", CUDA_DIR]
@@ -191,7 +219,7 @@ def _build_cuda(srcs, out, force, verbose):
 
 
 def build_all(force=False, verbose=False):
-    return build_host(force, verbose), build_tools(force, verbose), build_cuda(force, verbose)
+    return build_host(force, verbose), build_tools(force, verbose), build_cuda(force, verbose), build_calls(force, verbose)
 
 
 if __name__ == "__main__":

@@ -197,7 +197,7 @@ _SCRATCH_FLOATS = {"delta": ("ipex_delta_scratch_floats",), "general_delta": ("i
 
 
 # room that a call needs: count -> how much
-_SIZES = {"adamw": ("ipex_grad_norm_sums",), "preference": ("ipex_preference_keep_bytes", "ipex_preference_work_bytes")}
+SIZES = {"adamw": ("ipex_grad_norm_sums",), "preference": ("ipex_preference_keep_bytes", "ipex_preference_work_bytes")}
 
 
 def declare_component(lib: ctypes.CDLL, name: str):
@@ -206,7 +206,7 @@ def declare_component(lib: ctypes.CDLL, name: str):
         fn.argtypes, fn.restype = args, ci
     if name == "stream":
         lib.ipex_gemv_rows_tune.argtypes, lib.ipex_gemv_rows_tune.restype = [ci], None
-    for fn_name in _SIZES.get(name, ()):
+    for fn_name in SIZES.get(name, ()):
         fn = getattr(lib, fn_name)
         fn.argtypes, fn.restype = [i64], i64
     for fn_name in _SCRATCH_FLOATS.get(name, ()):

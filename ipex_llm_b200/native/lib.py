@@ -1,4 +1,4 @@
-"""ctypes loaders for the two in-tree native libraries.
+"""Loaders of the in-tree native libraries, by ctypes but for one.
 
 ``host_lib()`` is the stand-in for the reference's ``libllama-api.so`` binding
 (python/llm/src/ipex_llm/ggml/model/llama/llama_cpp.py:946-1185): same C entry-point names
@@ -20,6 +20,7 @@ _lock = threading.Lock()
 _host = None
 _cuda = None
 _components = {}
+_calls = None
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -116,6 +117,36 @@ def prepare_components(*names: str):
     if not os.path.exists(os.environ.get("IPEX_LLM_CUDA_LIB") or _build.CUDA_LIB):
         with _lock:
             _build.build_components(names)
+
+
+def calls():
+    """The extension that calls training kernels with lists of tensors and has their autograd nodes (``torch/calls.cpp``), with
+    the kernels' addresses."""
+    global _calls
+    if _calls is None:
+        import importlib.util
+
+        import torch  # noqa: F401 (the extension's libraries)
+
+        from . import cuda_api
+        at = {}
+        for name in ("adamw", "preference"):
+            lib = stream_lib(name)
+            for fn in (*cuda_api.COMPONENT_SIGS[name], *cuda_api.SIZES[name]):
+                at[fn] = ctypes.cast(getattr(lib, fn), c_void_p).value
+        with _lock:
+            if _calls is None:
+                try:
+                    path = _build.build_calls()
+                except Exception as e:  # noqa: BLE001
+                    raise RuntimeError("ipex_llm_b200: the extension of the training kernels' calls is missing and could not be "
+                                       f"built ({e}). Run `python -m ipex_llm_b200.native.build`.") from e
+                spec = importlib.util.spec_from_file_location("libipex_calls", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.bind(at)
+                _calls = module
+    return _calls
 
 
 def ptr(t) -> ctypes.c_void_p:

@@ -7,15 +7,12 @@ plain PyTorch, operation by operation, so that both give the same bits (but for 
 from __future__ import annotations
 
 import math
-from array import array
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ..native import cuda_api as api
-from ..native.lib import current_stream, ptr, stream_lib
+from ..native.lib import calls
 from ..utils.common import invalidInputError
-from .gradients import on
 
 BLOCK = 256              # elements of a tensor are counted in these, and 8-bit moments share an exponent in each
 DTYPES = (torch.float16, torch.bfloat16, torch.float32)
@@ -82,23 +79,15 @@ def _check_gradients(grads, what):
 def grad_norm(grads: Sequence[Optional[torch.Tensor]]) -> torch.Tensor:
     """The 2-norm of all gradients together (32-bit, no dimension), ``None`` among them left out; 0 of none.  Sums are held in 64
     bits and added up in an order that depends on the sizes and the device alone."""
-    what = "grad_norm"
-    have = _check_gradients(grads, what)
+    norm = calls().grad_norm(grads) if any(g is not None and g.is_cuda for g in grads[:1]) else None
+    if norm is not None:
+        return norm
+    have = _check_gradients(grads, "grad_norm")
     if not have:
         return torch.zeros((), dtype=torch.float32)
-    dev = have[0].device
-    if dev.type != "cuda":
-        return sum(g.double().square().sum() for g in have).sqrt().float()
-    have = [g if _is_dense(g) else g.contiguous() for g in have]
-    lib = stream_lib("adamw")
-    with on(dev):
-        sums = torch.empty(lib.ipex_grad_norm_sums(len(have)), dtype=torch.float64, device=dev)
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        at, sizes = array("q", [g.data_ptr() for g in have]), array("q", [g.numel() for g in have])
-        rc = lib.ipex_grad_norm(at.buffer_info()[0], sizes.buffer_info()[0], len(have), ptr(sums), ptr(norm),
-                                api.dtype_code(have[0].dtype), current_stream())
-    api.check(rc, "grad_norm")
-    return norm
+    if have[0].is_cuda:
+        return calls().grad_norm([g if _is_dense(g) else g.contiguous() for g in have])
+    return sum(g.double().square().sum() for g in have).sqrt().float()
 
 
 def adamw_state(params: Sequence[torch.Tensor], bits: int = 32, rest: Optional[str] = None, each: bool = False) -> AdamWState:
@@ -174,6 +163,32 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         invalidInputError(False, f"{what}: {len(params)} parameters and {len(grads)} gradients")
     if not len(params):
         return
+    b1, b2 = float(betas[0]), float(betas[1])
+    lr_at = lr if isinstance(lr, torch.Tensor) else None
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0 and (lr_at is not None or lr >= 0.0)):
+        invalidInputError(False, f"{what}: betas should lie in [0, 1), lr, eps and weight_decay not below 0; got {betas}, {lr}, {eps}, "
+                                 f"{weight_decay}")
+    if not (max_grad_norm and max_grad_norm > 0.0):
+        grad_norm, max_grad_norm = None, 0.0
+    elif grad_norm is None:
+        invalidInputError(False, f"{what}: max_grad_norm needs the gradients' norm")
+    buffers = (exp_avg, exp_avg_sq, step, exp_avg_scale, exp_avg_sq_scale, rest, grad_norm)
+    numbers = (float(max_grad_norm), 0.0 if lr_at is not None else float(lr), lr_at, b1, b2, float(eps), float(weight_decay),
+               int(seed) & 0xFFFFFFFF)
+    cuda = params[0].is_cuda
+    if cuda and calls().adamw_step(params, grads, *buffers, *numbers):
+        return
+    grads = _checked(params, grads, *buffers, lr_at)          # says what is wrong, or lays the gradients out as the parameters lie
+    if not cuda:
+        with torch.no_grad():
+            _step_plain(params, grads, *buffers, *numbers)
+        torch.autograd.graph.increment_version(params)
+    elif not calls().adamw_step(list(params), grads, *buffers, *numbers):
+        invalidInputError(False, f"{what}: these tensors are not supported")
+
+
+def _checked(params, grads, exp_avg, exp_avg_sq, step, exp_avg_scale, exp_avg_sq_scale, rest, grad_norm, lr_at):
+    what = "adamw_step"
     dtype, dev = params[0].dtype, params[0].device
     _check_params(params, what)
     seen = set()
@@ -210,39 +225,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         _check_buffer(rest, "rest", torch.int16 if kind == 1 else torch.float32, n, dev)
     if step.dtype != torch.int64 or step.numel() not in (1, len(params)) or not step.is_contiguous() or step.device != dev:
         invalidInputError(False, f"{what}: step should be an int64 of 1 or {len(params)} elements on {dev}")
-    b1, b2 = float(betas[0]), float(betas[1])
-    lr_at = lr if isinstance(lr, torch.Tensor) else None
-    if lr_at is not None and (lr_at.dtype != torch.float32 or lr_at.numel() != 1 or lr_at.device != dev):
-        invalidInputError(False, f"{what}: lr should be a number, or one 32-bit number on {dev}")
-    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0 and (lr_at is not None or lr >= 0.0)):
-        invalidInputError(False, f"{what}: betas should lie in [0, 1), lr, eps and weight_decay not below 0; got {betas}, {lr}, {eps}, "
-                                 f"{weight_decay}")
-    if max_grad_norm and max_grad_norm > 0.0:
-        if grad_norm is None or grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or grad_norm.device != dev:
-            invalidInputError(False, f"{what}: max_grad_norm needs the gradients' norm, one 32-bit number on {dev}")
-    else:
-        grad_norm = None
-    args = (lr_at, 0.0 if lr_at is not None else float(lr), b1, b2, float(eps), float(weight_decay), grad_norm, float(max_grad_norm or 0.0),
-            int(seed) & 0xFFFFFFFF)
-    with torch.no_grad():
-        if dev.type != "cuda":
-            _step_plain(params, gs, exp_avg, exp_avg_sq, step, exp_avg_scale, exp_avg_sq_scale, rest, kind, *args)
-            return
-        _step_cuda(params, gs, exp_avg, exp_avg_sq, step, exp_avg_scale, exp_avg_sq_scale, rest, kind, *args)
-    torch.autograd.graph.increment_version(params)
-
-
-def _step_cuda(params, grads, m, v, step, m_scale, v_scale, rest, kind, lr_at, lr, b1, b2, eps, decay, norm, max_norm, seed):
-    dev, count = m.device, len(params)
-    with on(dev):
-        p_at, g_at = array("q", [p.data_ptr() for p in params]), array("q", [0 if g is None else g.data_ptr() for g in grads])
-        sizes = array("q", [p.numel() for p in params])
-        factors = torch.empty(4 * step.numel(), dtype=torch.float32, device=dev)
-        rc = stream_lib("adamw").ipex_adamw_step(
-            p_at.buffer_info()[0], g_at.buffer_info()[0], sizes.buffer_info()[0], count, ptr(m), ptr(v), ptr(m_scale), ptr(v_scale),
-            ptr(rest), kind, ptr(step), step.numel(), ptr(factors), ptr(norm), max_norm, lr, ptr(lr_at), b1, b2, eps, decay, seed,
-            api.dtype_code(params[0].dtype), int(m.dtype != torch.float32), current_stream())
-    api.check(rc, "adamw_step")
+    for t, name in ((lr_at, "lr"), (grad_norm, "grad_norm")):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != 1 or t.device != dev):
+            invalidInputError(False, f"{what}: {name} should be one 32-bit number on {dev}")
+    return gs
 
 
 # ---- 8-bit moments and the rest of bf16, in plain PyTorch --------------------------------------------------------------------
@@ -314,8 +300,9 @@ def _joined(high, rest):
     return _as_signed(bits, 32).to(torch.int32).view(torch.float32)
 
 
-def _step_plain(params, grads, m, v, step, m_scale, v_scale, rest, kind, lr_at, lr, b1, b2, eps, decay, norm, max_norm, seed):
+def _step_plain(params, grads, m, v, step, m_scale, v_scale, rest, norm, max_norm, lr, lr_at, b1, b2, eps, decay, seed):
     lr = float(lr_at) if lr_at is not None else lr
+    kind = 0 if rest is None else 1 if rest.dtype == torch.int16 else 2
     clip = None if norm is None else (max_norm / (norm + 1e-6)).clamp(max=1.0).reshape(())
     counted = set()
     at = 0

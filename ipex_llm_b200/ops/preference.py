@@ -12,14 +12,12 @@ import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ..native import cuda_api as api
-from ..native.lib import current_stream, ptr, stream_lib
+from ..native.lib import calls
 from ..utils.common import invalidInputError
 from .cuda_ops import error_flag
-from .gradients import on, refuse_tangents
-from .token_loss import IGNORE, _check_like, _check_logits, _rows, token_logprobs
+from .gradients import refuse_tangents
+from .token_loss import IGNORE, _check_like, _check_logits, token_logprobs
 
 FORMS = ("sigmoid", "hinge", "ipo")
 
@@ -36,57 +34,6 @@ class PolicyLoss(NamedTuple):
     logprob: torch.Tensor        # [...]: of the targets
     kl: torch.Tensor             # [...]: the estimate e^d - d - 1, d = ref - logprob (0 without a reference)
     clipped: torch.Tensor        # [...]: True where the ratio lies outside and the loss does not move with it
-
-
-def _room(lib, rows, dev):
-    """What is kept for the backward pass and what the forward pass works in: one buffer each, aligned."""
-    return (torch.empty(lib.ipex_preference_keep_bytes(rows), dtype=torch.uint8, device=dev),
-            torch.empty(lib.ipex_preference_work_bytes(rows), dtype=torch.uint8, device=dev))
-
-
-def _strides(t: torch.Tensor, shape):
-    """``t`` broadcast to ``shape``, its strides over (all but the last dimension, the last), and the last one's size."""
-    t = t.expand(shape)
-    if t.dim() != 2:
-        t = t.reshape(-1, shape[-1]) if len(shape) else t.reshape(1, 1)
-    return t, t.stride(0), t.stride(1), t.shape[1]
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, reference, beta, form, smooth, margin, average, temperature, ignore):
-        ctx.set_materialize_grads(False)
-        lib, dev = stream_lib("preference"), logits.device
-        x, s0, s1, n1 = _rows(logits)
-        n, tokens, V = logits.shape
-        loss, logprob = torch.empty(n // 2, dtype=torch.float32, device=dev), torch.empty(n, dtype=torch.float32, device=dev)
-        with on(dev):
-            keep, work = _room(lib, n * tokens, dev)
-            rc = lib.ipex_preference_loss(ptr(x), s0, s1, n1, ptr(targets), ptr(reference), ptr(loss), ptr(logprob), ptr(keep), ptr(work),
-                                          n // 2, tokens, V, ignore, FORMS.index(form), int(average), beta, smooth, margin, temperature,
-                                          api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
-        api.check(rc, "preference_loss")
-        ctx.save_for_backward(logits, targets, keep)
-        ctx.temperature = temperature
-        return loss, logprob
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, g_seq):
-        if g is None and g_seq is None:
-            return (None,) * 10
-        logits, targets, keep = ctx.saved_tensors
-        x, s0, s1, n1 = _rows(logits)
-        n, tokens, V = logits.shape
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g = None if g is None else g.float()
-        g_seq = None if g_seq is None else g_seq.float().contiguous()
-        with on(logits.device):
-            rc = stream_lib("preference").ipex_preference_grad(
-                ptr(x), s0, s1, n1, ptr(targets), ptr(keep), ptr(g), 0 if g is None else g.stride(0), ptr(g_seq), ptr(dx), n // 2,
-                tokens, V, ctx.temperature, api.dtype_code(x.dtype), current_stream())
-        api.check(rc, "preference_grad")
-        return (dx,) + (None,) * 9
 
 
 def _preference_plain(logits, targets, reference, beta, form, smooth, margin, average, temperature, ignore):
@@ -144,48 +91,11 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
         refuse_tangents(what, logits)
         if not logits.shape[1]:
             invalidInputError(False, f"{what}: no tokens")
-        return PreferenceLoss(*_Preference.apply(
+        return PreferenceLoss(*calls().preference(
             logits, targets.to(torch.int64).contiguous(), None if reference is None else reference.detach().float().contiguous(),
-            float(beta), form, float(label_smoothing), float(margin), bool(average), float(temperature), int(ignore_index)))
+            beta, FORMS.index(form), label_smoothing, margin, average, temperature, ignore_index, error_flag(logits.device).data_ptr()))
     return _preference_plain(logits, targets, None if reference is None else reference.detach(), beta, form, label_smoothing, margin,
                              average, temperature, ignore_index)
-
-
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, advantages, old, ref, lo, hi, weight, temperature, ignore):
-        lib, dev, shape = stream_lib("preference"), logits.device, targets.shape
-        x, s0, s1, n1 = _rows(logits)
-        rows = targets.numel()
-        loss, logprob, kl = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
-        clipped = torch.empty(shape, dtype=torch.bool, device=dev)
-        adv, a0, a1, inner = _strides(advantages, shape)
-        with on(dev):
-            keep, work = _room(lib, rows, dev)
-            if rows:
-                rc = lib.ipex_policy_loss(ptr(x), s0, s1, n1, ptr(targets), ptr(old), ptr(ref), ptr(adv), a0, a1, inner, ptr(loss),
-                                          ptr(logprob), ptr(kl), ptr(clipped), ptr(keep), ptr(work), rows, x.shape[-1], ignore, lo, hi,
-                                          weight, temperature, api.dtype_code(x.dtype), ptr(error_flag(dev)), current_stream())
-                api.check(rc, "policy_loss")
-        ctx.mark_non_differentiable(logprob, kl, clipped)
-        ctx.save_for_backward(logits, targets, keep)
-        ctx.temperature = temperature
-        return loss, logprob, kl, clipped
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _lp, _kl, _clipped):
-        logits, targets, keep = ctx.saved_tensors
-        x, s0, s1, n1 = _rows(logits)
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g, g0, g1, inner = _strides(g.float(), targets.shape)
-        if targets.numel():
-            with on(logits.device):
-                rc = stream_lib("preference").ipex_policy_grad(
-                    ptr(x), s0, s1, n1, ptr(targets), ptr(keep), ptr(g), g0, g1, inner, ptr(dx), targets.numel(), x.shape[-1],
-                    ctx.temperature, api.dtype_code(x.dtype), current_stream())
-            api.check(rc, "policy_grad")
-        return (dx,) + (None,) * 9
 
 
 def _policy_plain(logits, targets, advantages, old, ref, lo, hi, weight, temperature, ignore):
@@ -246,7 +156,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     old, ref = (None if t is None else t.detach() for t in (old_logprobs, ref_logprobs))
     if logits.is_cuda:
         refuse_tangents(what, logits)
-        return PolicyLoss(*_Policy.apply(
+        return PolicyLoss(*calls().policy(
             logits, targets.to(torch.int64).contiguous(), advantages.detach().float(), None if old is None else old.float().contiguous(),
-            None if ref is None else ref.float().contiguous(), lo, hi, float(kl_weight), float(temperature), int(ignore_index)))
+            None if ref is None else ref.float().contiguous(), lo, hi, kl_weight, temperature, ignore_index,
+            error_flag(logits.device).data_ptr()))
     return _policy_plain(logits, targets, advantages.detach(), old, ref, lo, hi, kl_weight, temperature, ignore_index)

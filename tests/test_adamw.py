@@ -240,7 +240,7 @@ def test_refusals():
     refused("uint8 of 2", state=adamw_state(p, 8)._replace(exp_avg_scale=torch.zeros(1, dtype=torch.uint8)))
     refused("have no rest", state=s._replace(rest=torch.zeros(512, dtype=torch.int16)))
     refused("max_grad_norm needs", max_grad_norm=1.0)
-    refused("max_grad_norm needs", max_grad_norm=1.0, grad_norm=torch.tensor(1.0, dtype=torch.float64))
+    refused("grad_norm should be one", max_grad_norm=1.0, grad_norm=torch.tensor(1.0, dtype=torch.float64))
     refused("should lie in", betas=(1.0, 0.9))
     refused("should lie in", lr=-1.0)
     refused("should lie in", eps=-1.0)

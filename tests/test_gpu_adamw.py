@@ -232,7 +232,7 @@ def test_refusals_leave_everything():
     state, before = adamw.adamw_state(p), p[0].clone()
     for kw, match in ((dict(grads=[g[0].cpu()]), "like its parameter"), (dict(state=_cpu(state)), "exp_avg should be"),
                       (dict(state=state._replace(step=state.step.cpu())), "step should be"),
-                      (dict(max_grad_norm=1.0, grad_norm=torch.tensor(1.0)), "max_grad_norm needs"),
+                      (dict(max_grad_norm=1.0, grad_norm=torch.tensor(1.0)), "grad_norm should be one"),
                       (dict(lr=torch.tensor(0.1)), "lr should be"),
                       (dict(state=state._replace(exp_avg=torch.zeros(513, device="cuda")[1:])), "exp_avg should be")):
         kw = dict(dict(params=p, grads=g, state=state), **kw)
