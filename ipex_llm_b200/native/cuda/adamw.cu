@@ -31,6 +31,8 @@ constexpr int kTile = kNT * kVec;
 constexpr int kBlock = 256;                 // elements with a common exponent: a warp's
 static_assert(kBlock == 32 * kVec, "a warp has a block");
 constexpr int kLow = 32, kHigh = 254;       // exponents of a block: 2^(e - 127)
+constexpr int kCtas = 3;                    // to an SM
+constexpr int kNormCtas = 8;                // of the norm's
 constexpr int kMost = 640;                  // tensors of a launch: 25 KB of its 32 KB of parameters
 
 enum { REST_NONE = 0, REST_16 = 1, REST_32 = 2 };
@@ -105,45 +107,117 @@ __device__ __forceinline__ int tensor_of(const Table<CAP>& tab, uint32_t tile, i
   return lo;
 }
 
-// Eight elements at a multiple of 16 bytes, as 32-bit numbers.
-__device__ __forceinline__ void load8(const float* x, float* f) {
-  const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+// ---- pairs of 32-bit numbers: one instruction, each half rounded to nearest by itself
+using Pair = float2;
+__device__ __forceinline__ Pair both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\nfma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+// A product that goes into a sum: mul.rn.f32x2 and add.rn.f32x2 would be contracted.
+__device__ __forceinline__ Pair term2(Pair a, Pair b) { return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ Pair minus(Pair a) { return make_float2(-a.x, -a.y); }
+__device__ __forceinline__ float rcp_near(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rsqrt_near(float x) {
+  float y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The largest of three by size; NaN if one is NaN.
+__device__ __forceinline__ float largest3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// ---- eight elements: as they lie in memory, and as 32-bit numbers
 template <typename T>
-__device__ __forceinline__ void load8(const T* x, float* f) {
-  const uint4 w = *reinterpret_cast<const uint4*>(x);
-  const T* e = reinterpret_cast<const T*>(&w);
+struct Raw8 {
+  uint4 w[sizeof(T) == 4 ? 2 : 1];
+  __device__ __forceinline__ void load(const T* x) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = DT<T>::to_f(e[i]);
-}
-__device__ __forceinline__ void store8(float* x, const float* f) {
-  reinterpret_cast<float4*>(x)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(x)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* x, const float* f) {
-  __align__(16) T e[8];
+    for (int i = 0; i < (int)(sizeof(w) / 16); ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(x) + i);
+  }
+  __device__ __forceinline__ void load(const T* x, int have) {      // of any alignment; 0 behind the last one
+    __align__(16) T e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = DT<T>::from_f(f[i]);
-  *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(e);
-}
+    for (int k = 0; k < 8; ++k) e[k] = k < have ? x[k] : DT<T>::from_f(0.f);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(w) / 16); ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+  }
+  __device__ __forceinline__ void store(T* x) const {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(w) / 16); ++i) __stcs(reinterpret_cast<uint4*>(x) + i, w[i]);
+  }
+  __device__ __forceinline__ void store(T* x, int have) const {
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < have) x[k] = e[k];
+  }
+  __device__ __forceinline__ void get(Pair* f) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, float>::value) {
+        const float* e = reinterpret_cast<const float*>(w);
+        f[k] = make_float2(e[2 * k], e[2 * k + 1]);
+      } else {
+        const uint32_t x = reinterpret_cast<const uint32_t*>(w)[k];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) f[k] = make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+        else f[k] = __half22float2(*reinterpret_cast<const __half2*>(&x));
+      }
+    }
+  }
+  __device__ __forceinline__ void put(const Pair* f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (std::is_same<T, float>::value) {
+        reinterpret_cast<float2*>(w)[k] = f[k];
+      } else {
+        uint32_t& x = reinterpret_cast<uint32_t*>(w)[k];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(&x) = __floats2bfloat162_rn(f[k].x, f[k].y);
+        else *reinterpret_cast<__half2*>(&x) = __floats2half2_rn(f[k].x, f[k].y);
+      }
+    }
+  }
+};
 
 // 2^k for the exponents that occur here (-126 to 127).
 __device__ __forceinline__ float pow2(int k) { return __uint_as_float((uint32_t)(k + 127) << 23); }
 // A block's exponent as it is held: 0 in moments that no step has seen.
-__device__ __forceinline__ int held(uint8_t e) { return min(max((int)e, kLow), kHigh); }
+__device__ __forceinline__ int held(int e) { return min(max(e, kLow), kHigh); }
 
 // The exponent of the largest finite number of a warp's, of 32 x 8.
-__device__ __forceinline__ int block_exponent(const float* x) {
+__device__ __noinline__ int finite_exponent(Pair a, Pair b, Pair c, Pair d) {
+  const float x[8] = {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
   uint32_t top = 0;
-#pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t b = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-    top = max(top, b < 0x7F800000u ? b : 0u);
+    const uint32_t bits = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+    top = max(top, bits < 0x7F800000u ? bits : 0u);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  return held((uint8_t)(top >> 23));
+  return held(__reduce_max_sync(0xffffffffu, top) >> 23);
 }
 
 __device__ __forceinline__ uint32_t mixed(uint32_t x) {
@@ -154,28 +228,37 @@ __device__ __forceinline__ uint32_t mixed(uint32_t x) {
 
 // A 32-bit number's bits are its exponent and fraction in a row, whatever its size: scaled so that its exponent field is the small
 // format's, adding random bits below the last kept place and cutting there rounds it up with the probability of what is cut off.
-__device__ __forceinline__ uint32_t to_e4m3(float x, float up, uint32_t chance) {
-  const float a = fabsf(x);
-  const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(a, up), 0x1p-120f));
-  const uint32_t code = (bits + (chance << 4) + 8) >> 20 | (x < 0.f ? 0x80u : 0u);
-  return a < INFINITY ? code : 0x7Fu;               // the format has no infinity
+// The codes, in the uppermost bytes.
+__device__ __forceinline__ uint32_t to_e4m3(float x, float scaled, uint32_t chance) {     // scaled: |x| times a power of two
+  const uint32_t t = (__float_as_uint(scaled) + ((chance << 4 & 0xFFFF0u) | 8u)) << 4;
+  return (t & 0x7FFFFFFFu) | (__float_as_uint(x) & 0x80000000u);
 }
-__device__ __forceinline__ uint32_t to_e5m2(float x, float up, uint32_t chance) {
-  const uint32_t bits = __float_as_uint(__fmul_rn(__fmul_rn(x, up), 0x1p-112f));
-  const uint32_t code = (bits + (chance << 5) + 16) >> 21;
-  if (!(x < INFINITY)) return x == INFINITY ? 0x7Cu : 0x7Fu;
-  return x > 0.f ? max(code, 1u) : code;
+__device__ __forceinline__ uint32_t to_e5m2(float x, float scaled, uint32_t chance) {
+  const uint32_t t = (__float_as_uint(scaled) + ((chance >> 11 & 0x1FFFE0u) | 16u)) << 3;
+  return x > 0.f ? max(t, 1u << 24) : t;            // what is not 0 does not become 0
+}
+// Of what no power of two takes there at once: numbers from 2^8 (m) and 2^15 (v) on, and what is not finite.
+__device__ __noinline__ uint32_t to_e4m3_any(float x, int e, uint32_t chance) {
+  const float a = fabsf(x);
+  return a < INFINITY ? to_e4m3(x, __fmul_rn(__fmul_rn(a, pow2(134 - e)), 0x1p-120f), chance) : 0x7F000000u;
+}
+__device__ __noinline__ uint32_t to_e5m2_any(float x, int e, uint32_t chance) {
+  if (!(x < INFINITY)) return x == INFINITY ? 0x7C000000u : 0x7F000000u;
+  return to_e5m2(x, __fmul_rn(__fmul_rn(x, pow2(141 - e)), 0x1p-112f), chance);
 }
 template <__nv_fp8_interpretation_t KIND>
-__device__ __forceinline__ void from_fp8(uint2 w, float down, float* f) {
+__device__ __forceinline__ void from_fp8(uint2 w, float down, Pair* f) {
   const uint32_t v[2] = {w.x, w.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v[i >> 1] >> (16 * (i & 1))), KIND);
-    const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    f[2 * i] = __fmul_rn(p.x, down);
-    f[2 * i + 1] = __fmul_rn(p.y, down);
+    f[i] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h)), both(down));
   }
+}
+// The uppermost bytes of eight words.
+__device__ __forceinline__ uint2 upper_bytes(const uint32_t* t) {
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0073), __byte_perm(t[2], t[3], 0x0073), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0073), __byte_perm(t[6], t[7], 0x0073), 0x5410));
 }
 
 struct StepArgs {
@@ -190,104 +273,219 @@ struct StepArgs {
   uint32_t seed;
 };
 
+// Eight elements on their way: asked for a tile ahead.
+template <typename T, bool SMALL, int REST>
+struct Eight {
+  const Entry* e;
+  int64_t off, at;     // in the tensor, in the flat buffers
+  int have;
+  bool vec, any;       // any: the warp has a block here
+  Raw8<T> g, p;
+  uint4 rest[REST == REST_32 ? 2 : 1];
+  uint4 m[SMALL ? 1 : 2], v[SMALL ? 1 : 2];
+  int em, ev;
+
+  template <int CAP>
+  __device__ __forceinline__ void load(const Table<CAP>& tab, const StepArgs& a, uint32_t tile, int& i) {
+    i = tensor_of(tab, tile, i);
+    e = &tab.e[i];
+    off = (int64_t)(tile - e->tile) * kTile + threadIdx.x * kVec;
+    any = off - (int)(threadIdx.x & 31) * kVec < e->n;
+    if (!any) return;
+    at = (int64_t)e->block * kBlock + off;
+    have = off >= e->n ? 0 : (int)min((int64_t)kVec, e->n - off);
+    vec = have == kVec && ((reinterpret_cast<uintptr_t>(e->p) | reinterpret_cast<uintptr_t>(e->g)) & 15) == 0;
+    const T *p_at = reinterpret_cast<const T*>(e->p) + off, *g_at = reinterpret_cast<const T*>(e->g) + off;
+    if (vec) {
+      g.load(g_at);
+      if constexpr (REST != REST_32) p.load(p_at);
+    } else {
+      g.load(g_at, have);
+      if constexpr (REST != REST_32) p.load(p_at, have);
+    }
+    if constexpr (REST != REST_NONE) {
+      const uint4* r = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(a.rest) + at * (REST == REST_32 ? 4 : 2));
+      rest[0] = __ldcs(r);
+      if constexpr (REST == REST_32) rest[1] = __ldcs(r + 1);
+    }
+    if constexpr (SMALL) {
+      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(a.m) + at));
+      const uint2 y = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(a.v) + at));
+      m[0].x = x.x, m[0].y = x.y, v[0].x = y.x, v[0].y = y.y;
+      em = a.m_scale[at / kBlock];
+      ev = a.v_scale[at / kBlock];
+    } else {
+      const uint4* x = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.m) + at);
+      const uint4* y = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.v) + at);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) m[k] = __ldcs(x + k), v[k] = __ldcs(y + k);
+    }
+  }
+};
+
+__device__ __forceinline__ float change_any(float m, float v, const Factors& f, float eps) {
+  return __fdiv_rn(__fmul_rn(m, f.rate), __fadd_rn(__fmul_rn(__fsqrt_rn(v), f.root), eps));
+}
+
+// The update's change m rate / (sqrt(v) root + eps) of each element, where every number is of a usual size: roots by Newton's step
+// from an approximate 1 / sqrt (2^64 v, so that no v but 0 is too small for its remainder; 0 becomes what eps absorbs), quotients
+// by Newton's step for the reciprocal and Markstein's for the quotient.  Both are the nearest numbers: the root and the reciprocal
+// for every fraction there is (tested), the quotient by Markstein's theorem; their remainders are exact while m rate is 0 or above
+// 2^-100.  20 instructions for two elements; the general root and division take twice as many, and a branch each.
+__device__ __forceinline__ Pair change_usual(Pair m, Pair v, const Factors& f, float eps) {
+  const Pair x = mul2(v, both(0x1p64f)), u = make_float2(fmaxf(x.x, 0x1p-100f), fmaxf(x.y, 0x1p-100f));
+  const Pair y = make_float2(rsqrt_near(u.x), rsqrt_near(u.y));
+  const Pair g = mul2(u, y), h = mul2(y, both(0.5f));
+  const Pair s = fma2(fma2(minus(g), g, u), h, g);
+  const Pair d = add2(term2(s, both(f.root * 0x1p-32f)), both(eps));
+  const Pair n = mul2(m, both(f.rate));
+  const Pair r0 = make_float2(rcp_near(d.x), rcp_near(d.y)), minus_d = minus(d);
+  const Pair r = fma2(fma2(minus_d, r0, both(1.f)), r0, r0);
+  const Pair q = mul2(n, r);
+  return fma2(fma2(minus_d, q, n), r, q);
+}
+
 template <typename T, bool SMALL, int REST, int CAP>
-__global__ void __launch_bounds__(kNT) adamw_step(const __grid_constant__ Table<CAP> tab, StepArgs a) {
+__global__ void __launch_bounds__(kNT, kCtas) adamw_step(const __grid_constant__ Table<CAP> tab, StepArgs a) {
   const int lane = threadIdx.x & 31;
   int i = 0;
+  Eight<T, SMALL, REST> x;
+  uint32_t tile = blockIdx.x;
+  x.load(tab, a, tile, i);       // what the launch in front of this one writes is not among it
   pdl_wait();
-  for (uint32_t tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
-    i = tensor_of(tab, tile, i);
-    const Entry& e = tab.e[i];
-    const int64_t off = (int64_t)(tile - e.tile) * kTile + threadIdx.x * kVec;      // in the tensor
-    const int64_t warp_off = off - lane * kVec;
-    if (warp_off >= e.n) continue;                                                  // whole warps: no block of theirs
-    const Factors f = a.factors[e.step];
-    const int64_t at = (int64_t)e.block * kBlock + off;                             // in the flat buffers
-    const int have = off >= e.n ? 0 : (int)min((int64_t)kVec, e.n - off);
-    T* p_at = reinterpret_cast<T*>(e.p) + off;
-    const T* g_at = reinterpret_cast<const T*>(e.g) + off;
-    const bool vec = have == kVec && ((reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g)) & 15) == 0;
-    float p[kVec], g[kVec], m[kVec], v[kVec];
-    if (vec) {
-      load8(g_at, g);
-      if constexpr (REST != REST_32) load8(p_at, p);
-    } else {
+  while (true) {
+    const Eight<T, SMALL, REST> c = x;
+    tile += gridDim.x;
+    if (tile < tab.tiles) x.load(tab, a, tile, i);
+    if (c.any) {
+      const Factors f = a.factors[c.e->step];
+      Pair p[4], g[4], m[4], v[4];
+      c.g.get(g);
+      if constexpr (REST == REST_32) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        g[k] = k < have ? DT<T>::to_f(g_at[k]) : 0.f;
-        if constexpr (REST != REST_32) p[k] = k < have ? DT<T>::to_f(p_at[k]) : 0.f;
+        for (int k = 0; k < 4; ++k) p[k] = reinterpret_cast<const float2*>(c.rest)[k];
+      } else {
+        c.p.get(p);
       }
-    }
-    if constexpr (REST == REST_32) load8(reinterpret_cast<const float*>(a.rest) + at, p);
-    if constexpr (REST == REST_16) {
-      const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const int16_t*>(a.rest) + at);
-      const int16_t* r = reinterpret_cast<const int16_t*>(&w);
+      if constexpr (REST == REST_16) {
+        const uint32_t* r = reinterpret_cast<const uint32_t*>(c.rest);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) p[k] = __uint_as_float(__float_as_uint(p[k]) + (uint32_t)(int)r[k]);
-    }
-    if constexpr (SMALL) {
-      const int64_t blk = at / kBlock;
-      from_fp8<__NV_E4M3>(*reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.m) + at), pow2(held(a.m_scale[blk]) - 134), m);
-      from_fp8<__NV_E5M2>(*reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.v) + at), pow2(held(a.v_scale[blk]) - 141), v);
-    } else {
-      load8(reinterpret_cast<const float*>(a.m) + at, m);
-      load8(reinterpret_cast<const float*>(a.v) + at, v);
-    }
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) {
-      const float x = __fmul_rn(g[k], f.clip);
-      m[k] = __fadd_rn(__fmul_rn(m[k], a.b1), __fmul_rn(x, a.c1));
-      v[k] = __fadd_rn(__fmul_rn(v[k], a.b2), __fmul_rn(__fmul_rn(x, x), a.c2));
-      const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(v[k]), f.root), a.eps);
-      p[k] = __fsub_rn(__fmul_rn(p[k], f.decay), __fdiv_rn(__fmul_rn(m[k], f.rate), d));
-      if (k >= have) m[k] = v[k] = p[k] = 0.f;      // behind the tensor's end: 0 / eps, or 0 / 0
-    }
-    if constexpr (SMALL) {
-      const int em = block_exponent(m), ev = block_exponent(v);
-      const float up_m = pow2(134 - em), up_v = pow2(141 - ev);
-      const uint32_t t = (uint32_t)a.step[e.step];
-      const uint32_t key = mixed(mixed(t) + a.seed * 0x9E3779B1u) + (uint32_t)(at >> 32) * 0xBB67AE85u;
-      uint32_t wm[2] = {0, 0}, wv[2] = {0, 0};
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const uint32_t h = mixed((uint32_t)(at + k) * 0x9E3779B1u + key);
-        wm[k >> 2] |= to_e4m3(m[k], up_m, h & 0xFFFFu) << (8 * (k & 3));
-        wv[k >> 2] |= to_e5m2(v[k], up_v, h >> 16) << (8 * (k & 3));
-      }
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.m) + at) = make_uint2(wm[0], wm[1]);
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.v) + at) = make_uint2(wv[0], wv[1]);
-      if (lane == 0) {
-        a.m_scale[at / kBlock] = (uint8_t)em;
-        a.v_scale[at / kBlock] = (uint8_t)ev;
-      }
-    } else {
-      store8(reinterpret_cast<float*>(a.m) + at, m);
-      store8(reinterpret_cast<float*>(a.v) + at, v);
-    }
-    if constexpr (REST == REST_32) store8(reinterpret_cast<float*>(a.rest) + at, p);
-    if constexpr (REST == REST_16) {
-      // bf16 nearest to p (halves up) and the difference of their bits; p is made that bf16
-      __align__(16) int16_t r[kVec];
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const uint32_t bits = __float_as_uint(p[k]);
-        uint32_t high = (bits + 0x8000u) & 0xFFFF0000u;
-        r[k] = (int16_t)(bits - high);
-        if (p[k] != p[k]) {                         // its bits may run over
-          high = 0x7FFF0000u;
-          r[k] = 0;
+        for (int k = 0; k < 4; ++k) {
+          p[k].x = __uint_as_float(__float_as_uint(p[k].x) + (uint32_t)((int)(r[k] << 16) >> 16));
+          p[k].y = __uint_as_float(__float_as_uint(p[k].y) + (uint32_t)((int)r[k] >> 16));
         }
-        p[k] = __uint_as_float(high);
       }
-      *reinterpret_cast<uint4*>(reinterpret_cast<int16_t*>(a.rest) + at) = *reinterpret_cast<const uint4*>(r);
-    }
-    if (vec) {
-      store8(p_at, p);
-    } else {
+      if constexpr (SMALL) {
+        from_fp8<__NV_E4M3>(make_uint2(c.m[0].x, c.m[0].y), pow2(held(c.em) - 134), m);
+        from_fp8<__NV_E5M2>(make_uint2(c.v[0].x, c.v[0].y), pow2(held(c.ev) - 141), v);
+      } else {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k)
-        if (k < have) p_at[k] = DT<T>::from_f(p[k]);
+        for (int k = 0; k < 4; ++k) {
+          m[k] = reinterpret_cast<const float2*>(c.m)[k];
+          v[k] = reinterpret_cast<const float2*>(c.v)[k];
+        }
+      }
+      float top_m = 0.f, top_v = 0.f, top_p = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const Pair y = mul2(g[k], both(f.clip));
+        m[k] = add2(term2(m[k], both(a.b1)), term2(y, both(a.c1)));
+        v[k] = add2(term2(v[k], both(a.b2)), term2(mul2(y, y), both(a.c2)));
+        if (c.have < kVec) {                          // behind the tensor's end
+          if (2 * k >= c.have) m[k].x = v[k].x = 0.f;
+          if (2 * k + 1 >= c.have) m[k].y = v[k].y = 0.f;
+        }
+        top_m = largest3(top_m, m[k].x, m[k].y);
+        top_v = largest3(top_v, v[k].x, v[k].y);
+      }
+      const bool usual = top_m < 0x1p60f && top_v < 0x1p60f && a.eps >= 0x1p-50f && a.eps <= 0x1p20f && f.root <= 0x1p6f &&
+                         (f.rate == 0.f || (f.rate >= 0x1p-60f && f.rate <= 0x1p10f));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const Pair d = usual ? change_usual(m[k], v[k], f, a.eps)
+                             : make_float2(change_any(m[k].x, v[k].x, f, a.eps), change_any(m[k].y, v[k].y, f, a.eps));
+        p[k] = add2(term2(p[k], both(f.decay)), minus(d));
+        top_p = largest3(top_p, p[k].x, p[k].y);
+      }
+      if (c.have < kVec) {                            // 0 / eps, or 0 / 0
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (2 * k >= c.have) p[k].x = 0.f;
+          if (2 * k + 1 >= c.have) p[k].y = 0.f;
+        }
+      }
+      if constexpr (SMALL) {
+        int em = held(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)) >> 23);
+        int ev = held(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)) >> 23);
+        const uint32_t key = mixed(mixed((uint32_t)a.step[c.e->step]) + a.seed * 0x9E3779B1u) + (uint32_t)(c.at >> 32) * 0xBB67AE85u;
+        uint32_t tm[8], tv[8];
+        if (em <= 134 && ev <= 141) {                 // all of the block below 2^8 and 2^15: one power of two is enough
+          const float up_m = pow2(14 - em), up_v = pow2(29 - ev);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t h0 = mixed((uint32_t)(c.at + 2 * k) * 0x9E3779B1u + key), h1 = mixed((uint32_t)(c.at + 2 * k + 1) * 0x9E3779B1u + key);
+            const Pair sv = mul2(v[k], both(up_v)), sm = mul2(m[k], both(up_m));
+            tm[2 * k] = to_e4m3(m[k].x, fabsf(sm.x), h0);
+            tm[2 * k + 1] = to_e4m3(m[k].y, fabsf(sm.y), h1);
+            tv[2 * k] = to_e5m2(v[k].x, sv.x, h0);
+            tv[2 * k + 1] = to_e5m2(v[k].y, sv.y, h1);
+          }
+        } else {
+          em = finite_exponent(m[0], m[1], m[2], m[3]);
+          ev = finite_exponent(v[0], v[1], v[2], v[3]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t h0 = mixed((uint32_t)(c.at + 2 * k) * 0x9E3779B1u + key), h1 = mixed((uint32_t)(c.at + 2 * k + 1) * 0x9E3779B1u + key);
+            tm[2 * k] = to_e4m3_any(m[k].x, em, h0);
+            tm[2 * k + 1] = to_e4m3_any(m[k].y, em, h1);
+            tv[2 * k] = to_e5m2_any(v[k].x, ev, h0);
+            tv[2 * k + 1] = to_e5m2_any(v[k].y, ev, h1);
+          }
+        }
+        __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.m) + c.at), upper_bytes(tm));
+        __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.v) + c.at), upper_bytes(tv));
+        if (lane == 0) {
+          a.m_scale[c.at / kBlock] = (uint8_t)em;
+          a.v_scale[c.at / kBlock] = (uint8_t)ev;
+        }
+      } else {
+        Raw8<float> w;
+        w.put(m);
+        w.store(reinterpret_cast<float*>(a.m) + c.at);
+        w.put(v);
+        w.store(reinterpret_cast<float*>(a.v) + c.at);
+      }
+      Raw8<T> w;
+      if constexpr (REST == REST_16) {
+        // bf16 nearest to p (halves up): its upper half, one more where the lower half is 2^15 or more.  What is left, from -2^15 to
+        // 2^15 - 1, is the lower half as it stands.
+        uint32_t* to = reinterpret_cast<uint32_t*>(w.w);
+        uint4 low;
+        uint32_t* r = reinterpret_cast<uint32_t*>(&low);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t lo = __float_as_uint(p[k].x), hi = __float_as_uint(p[k].y);
+          if (!(top_p < INFINITY)) {                  // NaN's bits may run over
+            if (p[k].x != p[k].x) lo = 0x7FFF0000u;
+            if (p[k].y != p[k].y) hi = 0x7FFF0000u;
+          }
+          r[k] = __byte_perm(lo, hi, 0x5410);
+          to[k] = __byte_perm(lo + 0x8000u, hi + 0x8000u, 0x7632);
+        }
+        __stcs(reinterpret_cast<uint4*>(reinterpret_cast<int16_t*>(a.rest) + c.at), low);
+      } else {
+        if constexpr (REST == REST_32) {
+          Raw8<float> copy;
+          copy.put(p);
+          copy.store(reinterpret_cast<float*>(a.rest) + c.at);
+        }
+        w.put(p);
+      }
+      T* p_at = reinterpret_cast<T*>(c.e->p) + c.off;
+      if (c.vec) w.store(p_at);
+      else w.store(p_at, c.have);
     }
+    if (tile >= tab.tiles) break;
   }
 }
 
@@ -307,20 +505,19 @@ __global__ void __launch_bounds__(kNT) grad_squares(const __grid_constant__ Tabl
     if (off >= e.n) continue;
     const int have = (int)min((int64_t)kVec, e.n - off);
     const T* at = reinterpret_cast<const T*>(e.g) + off;
-    float g[kVec];
-    if (have == kVec && (reinterpret_cast<uintptr_t>(e.g) & 15) == 0) {
-      load8(at, g);
-    } else {
+    Raw8<T> w;
+    if (have == kVec && (reinterpret_cast<uintptr_t>(e.g) & 15) == 0) w.load(at);
+    else w.load(at, have);
+    Pair g[4];
+    w.get(g);
+    Pair s = both(0.f);
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) g[k] = k < have ? DT<T>::to_f(at[k]) : 0.f;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < kVec; ++k) s = fmaf(g[k], g[k], s);
-    if (s > 1e-25f && s < 1e38f) {
-      total += (double)s;
+    for (int k = 0; k < 4; ++k) s = fma2(g[k], g[k], s);
+    const float sum = s.x + s.y;
+    if (sum > 1e-25f && sum < 1e38f) {
+      total += (double)sum;
     } else {
-      for (int k = 0; k < kVec; ++k) total += (double)g[k] * g[k];
+      for (int k = 0; k < 4; ++k) total += (double)g[k].x * g[k].x + (double)g[k].y * g[k].y;
     }
   }
 #pragma unroll
@@ -391,9 +588,7 @@ int by_type(int dtype, F f) {
   return (int)cudaErrorInvalidValue;
 }
 
-constexpr int kCtas = 4;      // to an SM
-
-int grid_of(uint32_t tiles, int sms) { return (int)(tiles < (uint32_t)(sms * kCtas) ? tiles : (uint32_t)(sms * kCtas)); }
+int grid_of(uint32_t tiles, int ctas) { return (int)(tiles < (uint32_t)ctas ? tiles : (uint32_t)ctas); }
 
 template <int CAP>
 int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count, const BeginArgs& b, const StepArgs& a, int steps,
@@ -422,7 +617,7 @@ int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count
       if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (rest == REST_16) kern = small ? adamw_step<T, true, REST_16, CAP> : adamw_step<T, false, REST_16, CAP>;
       if (kern == nullptr) return (int)cudaErrorInvalidValue;
-      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms)), dim3(kNT), 0, s, true, tab, a);
+      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * kCtas)), dim3(kNT), 0, s, true, tab, a);
     });
     if (rc != 0) return rc;
   }
@@ -440,7 +635,7 @@ int norm_all(const int64_t* g, const int64_t* n, int64_t count, double* sums, fl
     at = fill(tab, nullptr, g, n, at, count, 1, block);
     if (at < 0) return (int)cudaErrorInvalidValue;
     if (tab.n == 0) continue;
-    const int grid = grid_of(tab.tiles, sms);
+    const int grid = grid_of(tab.tiles, sms * kNormCtas);
     const int rc = by_type(dtype, [&](auto* tag) {
       grad_squares<std::remove_pointer_t<decltype(tag)>, CAP><<<grid, kNT, 0, s>>>(tab, sums + parts);
       return (int)cudaGetLastError();
@@ -457,7 +652,7 @@ constexpr int kFew = 32;
 
 // How many sums (64-bit) ipex_grad_norm needs for `count` tensors.
 IPEX_API int64_t ipex_grad_norm_sums(int64_t count) {
-  return (int64_t)sm_count() * kCtas * ((count + kMost - 1) / kMost + 1);
+  return (int64_t)sm_count() * kNormCtas * ((count + kMost - 1) / kMost + 1);
 }
 
 // p, g, n [count] (host): addresses and sizes of parameters and gradients of `dtype` (a gradient of 0: its parameter is left as it is,
