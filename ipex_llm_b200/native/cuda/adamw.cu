@@ -28,10 +28,11 @@ namespace {
 constexpr int kNT = 256;
 constexpr int kVec = 8;                     // elements of a thread
 constexpr int kTile = kNT * kVec;
+constexpr int kNormParts = 2;               // of a thread's in a tile of the norm: both are asked for before the first is worked on
 constexpr int kBlock = 256;                 // elements with a common exponent: a warp's
 static_assert(kBlock == 32 * kVec, "a warp has a block");
 constexpr int kLow = 32, kHigh = 254;       // exponents of a block: 2^(e - 127)
-constexpr int kCtas = 3;                    // to an SM
+constexpr int kCtas = 3, kCtasSmall = 4;    // to an SM, with moments in 32 and in 8 bits
 constexpr int kNormCtas = 8;                // of the norm's
 constexpr int kMost = 640;                  // tensors of a launch: 25 KB of its 32 KB of parameters
 
@@ -53,9 +54,17 @@ struct Table {
 };
 
 // What an update needs beside its numbers, for each step counter.
-struct Factors {
+struct __align__(16) Factors {
   float rate, root, clip, decay;      // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), of the gradient, 1 - lr wd
+  uint32_t key;                       // of the random bits
+  int usual;                          // whether change_usual() holds, as far as they go
 };
+
+__device__ __forceinline__ uint32_t mixed(uint32_t x) {
+  x = (x ^ (x >> 16)) * 0xBB67AE85u;                // fractions of the roots of 3 and 2
+  x = (x ^ (x >> 15)) * 0x6A09E667u;
+  return x ^ (x >> 16);
+}
 
 __device__ double power(double b, int64_t t) {
   double r = 1.0;
@@ -72,6 +81,8 @@ struct BeginArgs {
   const float* lr_at;     // or null: lr
   Factors* out;
   double max_norm, lr, b1, b2, decay;
+  float eps;
+  uint32_t seed;
 };
 
 template <int CAP>
@@ -93,6 +104,8 @@ __global__ void adamw_begin(const __grid_constant__ Table<CAP> tab, BeginArgs a)
     const float c = __fdiv_rn((float)a.max_norm, __fadd_rn(*a.norm, 1e-6f));
     f.clip = c > 1.f ? 1.f : c;                     // NaN stays
   }
+  f.key = mixed(mixed((uint32_t)t) + a.seed * 0x9E3779B1u);
+  f.usual = a.eps >= 0x1p-38f && a.eps <= 0x1p20f && f.root <= 0x1p6f && (f.rate == 0.f || (f.rate >= 0x1p-60f && f.rate <= 0x1p10f));
   a.out[at] = f;
 }
 
@@ -125,8 +138,6 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-// A product that goes into a sum: mul.rn.f32x2 and add.rn.f32x2 would be contracted.
-__device__ __forceinline__ Pair term2(Pair a, Pair b) { return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)); }
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
   Pair d;
   asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
@@ -134,7 +145,9 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
-__device__ __forceinline__ Pair minus(Pair a) { return make_float2(-a.x, -a.y); }
+// A product that goes into a sum.  The compiler contracts mul.rn.f32x2 and add.rn.f32x2 (and a fused product with a -0 that it knows);
+// it does not know that `zero`, an argument of the launch, is -0.
+__device__ __forceinline__ Pair term2(Pair a, Pair b, float zero) { return fma2(a, b, both(zero)); }
 __device__ __forceinline__ float rcp_near(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -220,18 +233,12 @@ __device__ __noinline__ int finite_exponent(Pair a, Pair b, Pair c, Pair d) {
   return held(__reduce_max_sync(0xffffffffu, top) >> 23);
 }
 
-__device__ __forceinline__ uint32_t mixed(uint32_t x) {
-  x = (x ^ (x >> 16)) * 0xBB67AE85u;                // fractions of the roots of 3 and 2
-  x = (x ^ (x >> 15)) * 0x6A09E667u;
-  return x ^ (x >> 16);
-}
-
 // A 32-bit number's bits are its exponent and fraction in a row, whatever its size: scaled so that its exponent field is the small
 // format's, adding random bits below the last kept place and cutting there rounds it up with the probability of what is cut off.
 // The codes, in the uppermost bytes.
-__device__ __forceinline__ uint32_t to_e4m3(float x, float scaled, uint32_t chance) {     // scaled: |x| times a power of two
-  const uint32_t t = (__float_as_uint(scaled) + ((chance << 4 & 0xFFFF0u) | 8u)) << 4;
-  return (t & 0x7FFFFFFFu) | (__float_as_uint(x) & 0x80000000u);
+__device__ __forceinline__ uint32_t to_e4m3(float x, float scaled, uint32_t chance) {
+  const uint32_t t = (__float_as_uint(scaled) + ((chance << 4 & 0xFFFF0u) | 8u)) << 4;    // its sign is shifted out
+  return t | (__float_as_uint(x) & 0x80000000u);
 }
 __device__ __forceinline__ uint32_t to_e5m2(float x, float scaled, uint32_t chance) {
   const uint32_t t = (__float_as_uint(scaled) + ((chance >> 11 & 0x1FFFE0u) | 16u)) << 3;
@@ -268,34 +275,50 @@ struct StepArgs {
   uint8_t* v_scale;
   void* rest;          // the 16 bits below bf16, or copies in 32 bits
   const Factors* factors;
-  const int64_t* step;
   float b1, c1, b2, c2, eps;     // c: 1 - b
-  uint32_t seed;
+  float zero;                    // -0
 };
 
-// Eight elements on their way: asked for a tile ahead.
+__device__ __forceinline__ float change_any(float m, float v, const Factors& f, float eps) {
+  return -__fdiv_rn(__fmul_rn(m, f.rate), __fadd_rn(__fmul_rn(__fsqrt_rn(v), f.root), eps));
+}
+
+// The update's change, -m rate / (sqrt(v) root + eps), where every number is of a usual size: roots by Newton's step from an
+// approximate 1 / sqrt, quotients by Newton's step for the reciprocal and Markstein's for the quotient, with signs such that none has
+// to be turned.  All are the nearest numbers: the root and the reciprocal for every fraction there is (tested), the quotient by
+// Markstein's theorem, as long as remainders are exact: while m rate is 0 or above 2^-100 in size; v is taken times 2^64, with 2^-102
+// for 0, which no other v notices, or eps absorbs.  17 instructions for two elements; the general root and division take three
+// times as many, and a branch each.
+__device__ __forceinline__ Pair change_usual(Pair m, Pair v, const Factors& f, float eps, float zero) {
+  const Pair u = fma2(v, both(-0x1p64f), both(-0x1p-102f));       // -2^64 v
+  const Pair y = make_float2(rsqrt_near(-u.x), rsqrt_near(-u.y));
+  const Pair g = mul2(u, y);                                      // about -sqrt
+  const Pair s = fma2(fma2(g, g, u), mul2(y, both(0.5f)), g);     // -sqrt
+  const Pair d = add2(term2(s, both(f.root * 0x1p-32f), zero), both(-eps));
+  const Pair n = mul2(m, both(-f.rate));
+  const Pair r0 = make_float2(rcp_near(-d.x), rcp_near(-d.y));
+  const Pair r = fma2(fma2(d, r0, both(1.f)), r0, r0);
+  const Pair q = mul2(n, r);
+  return fma2(fma2(d, q, n), r, q);
+}
+
+// A pair of bf16 numbers with what their 32-bit numbers have below them, from -2^15 to 2^15 - 1.
+__device__ __forceinline__ Pair with_rest(uint32_t p, uint32_t r) {
+  uint32_t lo;
+  asm("prmt.b32 %0, %1, 0, 0x9910;" : "=r"(lo) : "r"(r));        // the lower half with its sign
+  return make_float2(__uint_as_float(p * 65536u + lo), __uint_as_float((p & 0xFFFF0000u) + (uint32_t)((int)r >> 16)));
+}
+
+// Eight elements of a thread: what is read of them, and their update.
 template <typename T, bool SMALL, int REST>
 struct Eight {
-  const Entry* e;
-  int64_t off, at;     // in the tensor, in the flat buffers
-  int have;
-  bool vec, any;       // any: the warp has a block here
   Raw8<T> g, p;
-  uint4 rest[REST == REST_32 ? 2 : 1];
-  uint4 m[SMALL ? 1 : 2], v[SMALL ? 1 : 2];
+  Raw8<float> copy, wide_m, wide_v;
+  uint4 low;
+  uint2 m, v;
   int em, ev;
 
-  template <int CAP>
-  __device__ __forceinline__ void load(const Table<CAP>& tab, const StepArgs& a, uint32_t tile, int& i) {
-    i = tensor_of(tab, tile, i);
-    e = &tab.e[i];
-    off = (int64_t)(tile - e->tile) * kTile + threadIdx.x * kVec;
-    any = off - (int)(threadIdx.x & 31) * kVec < e->n;
-    if (!any) return;
-    at = (int64_t)e->block * kBlock + off;
-    have = off >= e->n ? 0 : (int)min((int64_t)kVec, e->n - off);
-    vec = have == kVec && ((reinterpret_cast<uintptr_t>(e->p) | reinterpret_cast<uintptr_t>(e->g)) & 15) == 0;
-    const T *p_at = reinterpret_cast<const T*>(e->p) + off, *g_at = reinterpret_cast<const T*>(e->g) + off;
+  __device__ __forceinline__ void load(const StepArgs& a, const T* g_at, const T* p_at, int64_t at, int have, bool vec) {
     if (vec) {
       g.load(g_at);
       if constexpr (REST != REST_32) p.load(p_at);
@@ -303,189 +326,168 @@ struct Eight {
       g.load(g_at, have);
       if constexpr (REST != REST_32) p.load(p_at, have);
     }
-    if constexpr (REST != REST_NONE) {
-      const uint4* r = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(a.rest) + at * (REST == REST_32 ? 4 : 2));
-      rest[0] = __ldcs(r);
-      if constexpr (REST == REST_32) rest[1] = __ldcs(r + 1);
-    }
+    if constexpr (REST == REST_32) copy.load(reinterpret_cast<const float*>(a.rest) + at);
+    if constexpr (REST == REST_16) low = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const int16_t*>(a.rest) + at));
     if constexpr (SMALL) {
-      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(a.m) + at));
-      const uint2 y = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(a.v) + at));
-      m[0].x = x.x, m[0].y = x.y, v[0].x = y.x, v[0].y = y.y;
+      m = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(a.m) + at));
+      v = __ldcs(reinterpret_cast<const uint2*>(reinterpret_cast<const char*>(a.v) + at));
       em = a.m_scale[at / kBlock];
       ev = a.v_scale[at / kBlock];
     } else {
-      const uint4* x = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.m) + at);
-      const uint4* y = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(a.v) + at);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) m[k] = __ldcs(x + k), v[k] = __ldcs(y + k);
+      wide_m.load(reinterpret_cast<const float*>(a.m) + at);
+      wide_v.load(reinterpret_cast<const float*>(a.v) + at);
     }
+  }
+
+  __device__ __forceinline__ void update(const StepArgs& a, const Factors& f, T* p_at, int64_t at, int have, bool vec) {
+    Pair w[4], d[4], mm[4], vv[4];
+    g.get(d);
+    if constexpr (REST == REST_32) {
+      copy.get(w);
+    } else if constexpr (REST == REST_16) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[k] = with_rest(reinterpret_cast<const uint32_t*>(p.w)[k], reinterpret_cast<const uint32_t*>(&low)[k]);
+    } else {
+      p.get(w);
+    }
+    if constexpr (SMALL) {
+      from_fp8<__NV_E4M3>(m, pow2(held(em) - 134), mm);
+      from_fp8<__NV_E5M2>(v, pow2(held(ev) - 141), vv);
+    } else {
+      wide_m.get(mm);
+      wide_v.get(vv);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const Pair y = mul2(d[k], both(f.clip));
+      mm[k] = add2(term2(mm[k], both(a.b1), a.zero), term2(y, both(a.c1), a.zero));
+      vv[k] = add2(term2(vv[k], both(a.b2), a.zero), term2(mul2(y, y), both(a.c2), a.zero));
+    }
+    if (have < kVec) {                                // behind the tensor's end
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (2 * k >= have) mm[k].x = vv[k].x = 0.f;
+        if (2 * k + 1 >= have) mm[k].y = vv[k].y = 0.f;
+      }
+    }
+    float top_m = 0.f, top_v = 0.f, top_p = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      top_m = largest3(top_m, mm[k].x, mm[k].y);
+      top_v = largest3(top_v, vv[k].x, vv[k].y);
+    }
+    if (f.usual && top_m < 0x1p60f && top_v < 0x1p60f) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k] = change_usual(mm[k], vv[k], f, a.eps, a.zero);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        d[k] = make_float2(change_any(mm[k].x, vv[k].x, f, a.eps), change_any(mm[k].y, vv[k].y, f, a.eps));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      w[k] = add2(term2(w[k], both(f.decay), a.zero), d[k]);
+      if constexpr (REST == REST_16) top_p = largest3(top_p, w[k].x, w[k].y);
+    }
+    if (REST != REST_NONE && have < kVec) {           // 0 / eps, or 0 / 0
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (2 * k >= have) w[k].x = 0.f;
+        if (2 * k + 1 >= have) w[k].y = 0.f;
+      }
+    }
+    if constexpr (SMALL) {
+      int e = held(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)) >> 23);
+      int h = held(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)) >> 23);
+      const uint32_t first = (uint32_t)at * 0x9E3779B1u + (uint32_t)(at >> 32) * 0xBB67AE85u + f.key;
+      uint32_t tm[8], tv[8];
+      if (e <= 134 && h <= 141) {                     // all of the block below 2^8 and 2^15: one power of two is enough
+        const float up_m = pow2(14 - e), up_v = pow2(29 - h);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t c0 = mixed(first + 2 * k * 0x9E3779B1u), c1 = mixed(first + (2 * k + 1) * 0x9E3779B1u);
+          const Pair sv = mul2(vv[k], both(up_v)), sm = mul2(mm[k], both(up_m));
+          tm[2 * k] = to_e4m3(mm[k].x, sm.x, c0);
+          tm[2 * k + 1] = to_e4m3(mm[k].y, sm.y, c1);
+          tv[2 * k] = to_e5m2(vv[k].x, sv.x, c0);
+          tv[2 * k + 1] = to_e5m2(vv[k].y, sv.y, c1);
+        }
+      } else {
+        e = finite_exponent(mm[0], mm[1], mm[2], mm[3]);
+        h = finite_exponent(vv[0], vv[1], vv[2], vv[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t c0 = mixed(first + 2 * k * 0x9E3779B1u), c1 = mixed(first + (2 * k + 1) * 0x9E3779B1u);
+          tm[2 * k] = to_e4m3_any(mm[k].x, e, c0);
+          tm[2 * k + 1] = to_e4m3_any(mm[k].y, e, c1);
+          tv[2 * k] = to_e5m2_any(vv[k].x, h, c0);
+          tv[2 * k + 1] = to_e5m2_any(vv[k].y, h, c1);
+        }
+      }
+      __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.m) + at), upper_bytes(tm));
+      __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.v) + at), upper_bytes(tv));
+      if ((threadIdx.x & 31) == 0) {
+        a.m_scale[at / kBlock] = (uint8_t)e;
+        a.v_scale[at / kBlock] = (uint8_t)h;
+      }
+    } else {
+      wide_m.put(mm);
+      wide_m.store(reinterpret_cast<float*>(a.m) + at);
+      wide_v.put(vv);
+      wide_v.store(reinterpret_cast<float*>(a.v) + at);
+    }
+    if constexpr (REST == REST_16) {
+      // bf16 nearest to p (halves up): its upper half, one more where the lower half is 2^15 or more.  What is left, from -2^15 to
+      // 2^15 - 1, is the lower half as it stands.
+      uint32_t* to = reinterpret_cast<uint32_t*>(p.w);
+      uint32_t* r = reinterpret_cast<uint32_t*>(&low);
+      if (!(top_p < INFINITY)) {                      // NaN's bits may run over
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (w[k].x != w[k].x) w[k].x = __uint_as_float(0x7FFF0000u);
+          if (w[k].y != w[k].y) w[k].y = __uint_as_float(0x7FFF0000u);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = __float_as_uint(w[k].x), hi = __float_as_uint(w[k].y);
+        r[k] = __byte_perm(lo, hi, 0x5410);
+        to[k] = __byte_perm(lo + 0x8000u, hi + 0x8000u, 0x7632);
+      }
+      __stcs(reinterpret_cast<uint4*>(reinterpret_cast<int16_t*>(a.rest) + at), low);
+    } else {
+      if constexpr (REST == REST_32) {
+        copy.put(w);
+        copy.store(reinterpret_cast<float*>(a.rest) + at);
+      }
+      p.put(w);
+    }
+    if (vec) p.store(p_at);
+    else p.store(p_at, have);
   }
 };
 
-__device__ __forceinline__ float change_any(float m, float v, const Factors& f, float eps) {
-  return __fdiv_rn(__fmul_rn(m, f.rate), __fadd_rn(__fmul_rn(__fsqrt_rn(v), f.root), eps));
-}
-
-// The update's change m rate / (sqrt(v) root + eps) of each element, where every number is of a usual size: roots by Newton's step
-// from an approximate 1 / sqrt (2^64 v, so that no v but 0 is too small for its remainder; 0 becomes what eps absorbs), quotients
-// by Newton's step for the reciprocal and Markstein's for the quotient.  Both are the nearest numbers: the root and the reciprocal
-// for every fraction there is (tested), the quotient by Markstein's theorem; their remainders are exact while m rate is 0 or above
-// 2^-100.  20 instructions for two elements; the general root and division take twice as many, and a branch each.
-__device__ __forceinline__ Pair change_usual(Pair m, Pair v, const Factors& f, float eps) {
-  const Pair x = mul2(v, both(0x1p64f)), u = make_float2(fmaxf(x.x, 0x1p-100f), fmaxf(x.y, 0x1p-100f));
-  const Pair y = make_float2(rsqrt_near(u.x), rsqrt_near(u.y));
-  const Pair g = mul2(u, y), h = mul2(y, both(0.5f));
-  const Pair s = fma2(fma2(minus(g), g, u), h, g);
-  const Pair d = add2(term2(s, both(f.root * 0x1p-32f)), both(eps));
-  const Pair n = mul2(m, both(f.rate));
-  const Pair r0 = make_float2(rcp_near(d.x), rcp_near(d.y)), minus_d = minus(d);
-  const Pair r = fma2(fma2(minus_d, r0, both(1.f)), r0, r0);
-  const Pair q = mul2(n, r);
-  return fma2(fma2(minus_d, q, n), r, q);
-}
-
 template <typename T, bool SMALL, int REST, int CAP>
-__global__ void __launch_bounds__(kNT, kCtas) adamw_step(const __grid_constant__ Table<CAP> tab, StepArgs a) {
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(kNT, SMALL ? kCtasSmall : kCtas) adamw_step(const __grid_constant__ Table<CAP> tab, StepArgs a) {
   int i = 0;
-  Eight<T, SMALL, REST> x;
-  uint32_t tile = blockIdx.x;
-  x.load(tab, a, tile, i);       // what the launch in front of this one writes is not among it
-  pdl_wait();
-  while (true) {
-    const Eight<T, SMALL, REST> c = x;
-    tile += gridDim.x;
-    if (tile < tab.tiles) x.load(tab, a, tile, i);
-    if (c.any) {
-      const Factors f = a.factors[c.e->step];
-      Pair p[4], g[4], m[4], v[4];
-      c.g.get(g);
-      if constexpr (REST == REST_32) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) p[k] = reinterpret_cast<const float2*>(c.rest)[k];
-      } else {
-        c.p.get(p);
-      }
-      if constexpr (REST == REST_16) {
-        const uint32_t* r = reinterpret_cast<const uint32_t*>(c.rest);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          p[k].x = __uint_as_float(__float_as_uint(p[k].x) + (uint32_t)((int)(r[k] << 16) >> 16));
-          p[k].y = __uint_as_float(__float_as_uint(p[k].y) + (uint32_t)((int)r[k] >> 16));
-        }
-      }
-      if constexpr (SMALL) {
-        from_fp8<__NV_E4M3>(make_uint2(c.m[0].x, c.m[0].y), pow2(held(c.em) - 134), m);
-        from_fp8<__NV_E5M2>(make_uint2(c.v[0].x, c.v[0].y), pow2(held(c.ev) - 141), v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          m[k] = reinterpret_cast<const float2*>(c.m)[k];
-          v[k] = reinterpret_cast<const float2*>(c.v)[k];
-        }
-      }
-      float top_m = 0.f, top_v = 0.f, top_p = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const Pair y = mul2(g[k], both(f.clip));
-        m[k] = add2(term2(m[k], both(a.b1)), term2(y, both(a.c1)));
-        v[k] = add2(term2(v[k], both(a.b2)), term2(mul2(y, y), both(a.c2)));
-        if (c.have < kVec) {                          // behind the tensor's end
-          if (2 * k >= c.have) m[k].x = v[k].x = 0.f;
-          if (2 * k + 1 >= c.have) m[k].y = v[k].y = 0.f;
-        }
-        top_m = largest3(top_m, m[k].x, m[k].y);
-        top_v = largest3(top_v, v[k].x, v[k].y);
-      }
-      const bool usual = top_m < 0x1p60f && top_v < 0x1p60f && a.eps >= 0x1p-50f && a.eps <= 0x1p20f && f.root <= 0x1p6f &&
-                         (f.rate == 0.f || (f.rate >= 0x1p-60f && f.rate <= 0x1p10f));
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const Pair d = usual ? change_usual(m[k], v[k], f, a.eps)
-                             : make_float2(change_any(m[k].x, v[k].x, f, a.eps), change_any(m[k].y, v[k].y, f, a.eps));
-        p[k] = add2(term2(p[k], both(f.decay)), minus(d));
-        top_p = largest3(top_p, p[k].x, p[k].y);
-      }
-      if (c.have < kVec) {                            // 0 / eps, or 0 / 0
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (2 * k >= c.have) p[k].x = 0.f;
-          if (2 * k + 1 >= c.have) p[k].y = 0.f;
-        }
-      }
-      if constexpr (SMALL) {
-        int em = held(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)) >> 23);
-        int ev = held(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)) >> 23);
-        const uint32_t key = mixed(mixed((uint32_t)a.step[c.e->step]) + a.seed * 0x9E3779B1u) + (uint32_t)(c.at >> 32) * 0xBB67AE85u;
-        uint32_t tm[8], tv[8];
-        if (em <= 134 && ev <= 141) {                 // all of the block below 2^8 and 2^15: one power of two is enough
-          const float up_m = pow2(14 - em), up_v = pow2(29 - ev);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t h0 = mixed((uint32_t)(c.at + 2 * k) * 0x9E3779B1u + key), h1 = mixed((uint32_t)(c.at + 2 * k + 1) * 0x9E3779B1u + key);
-            const Pair sv = mul2(v[k], both(up_v)), sm = mul2(m[k], both(up_m));
-            tm[2 * k] = to_e4m3(m[k].x, fabsf(sm.x), h0);
-            tm[2 * k + 1] = to_e4m3(m[k].y, fabsf(sm.y), h1);
-            tv[2 * k] = to_e5m2(v[k].x, sv.x, h0);
-            tv[2 * k + 1] = to_e5m2(v[k].y, sv.y, h1);
-          }
-        } else {
-          em = finite_exponent(m[0], m[1], m[2], m[3]);
-          ev = finite_exponent(v[0], v[1], v[2], v[3]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t h0 = mixed((uint32_t)(c.at + 2 * k) * 0x9E3779B1u + key), h1 = mixed((uint32_t)(c.at + 2 * k + 1) * 0x9E3779B1u + key);
-            tm[2 * k] = to_e4m3_any(m[k].x, em, h0);
-            tm[2 * k + 1] = to_e4m3_any(m[k].y, em, h1);
-            tv[2 * k] = to_e5m2_any(v[k].x, ev, h0);
-            tv[2 * k + 1] = to_e5m2_any(v[k].y, ev, h1);
-          }
-        }
-        __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.m) + c.at), upper_bytes(tm));
-        __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(a.v) + c.at), upper_bytes(tv));
-        if (lane == 0) {
-          a.m_scale[c.at / kBlock] = (uint8_t)em;
-          a.v_scale[c.at / kBlock] = (uint8_t)ev;
-        }
-      } else {
-        Raw8<float> w;
-        w.put(m);
-        w.store(reinterpret_cast<float*>(a.m) + c.at);
-        w.put(v);
-        w.store(reinterpret_cast<float*>(a.v) + c.at);
-      }
-      Raw8<T> w;
-      if constexpr (REST == REST_16) {
-        // bf16 nearest to p (halves up): its upper half, one more where the lower half is 2^15 or more.  What is left, from -2^15 to
-        // 2^15 - 1, is the lower half as it stands.
-        uint32_t* to = reinterpret_cast<uint32_t*>(w.w);
-        uint4 low;
-        uint32_t* r = reinterpret_cast<uint32_t*>(&low);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t lo = __float_as_uint(p[k].x), hi = __float_as_uint(p[k].y);
-          if (!(top_p < INFINITY)) {                  // NaN's bits may run over
-            if (p[k].x != p[k].x) lo = 0x7FFF0000u;
-            if (p[k].y != p[k].y) hi = 0x7FFF0000u;
-          }
-          r[k] = __byte_perm(lo, hi, 0x5410);
-          to[k] = __byte_perm(lo + 0x8000u, hi + 0x8000u, 0x7632);
-        }
-        __stcs(reinterpret_cast<uint4*>(reinterpret_cast<int16_t*>(a.rest) + c.at), low);
-      } else {
-        if constexpr (REST == REST_32) {
-          Raw8<float> copy;
-          copy.put(p);
-          copy.store(reinterpret_cast<float*>(a.rest) + c.at);
-        }
-        w.put(p);
-      }
-      T* p_at = reinterpret_cast<T*>(c.e->p) + c.off;
-      if (c.vec) w.store(p_at);
-      else w.store(p_at, c.have);
-    }
-    if (tile >= tab.tiles) break;
+  bool first = true;
+  for (uint32_t tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
+    i = tensor_of(tab, tile, i);
+    const Entry& e = tab.e[i];
+    const int64_t off = (int64_t)(tile - e.tile) * kTile + threadIdx.x * kVec, at = (int64_t)e.block * kBlock + off;
+    const int64_t left = e.n - off;
+    if (left + (int)(threadIdx.x & 31) * kVec <= 0) continue;      // no block of the warp's
+    T* p_at = reinterpret_cast<T*>(e.p) + off;
+    const T* g_at = reinterpret_cast<const T*>(e.g) + off;
+    const int have = (int)max((int64_t)0, min((int64_t)kVec, left));
+    const bool vec = have == kVec && ((reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g)) & 15) == 0;
+    Eight<T, SMALL, REST> x;
+    x.load(a, g_at, p_at, at, have, vec);
+    if (first) pdl_wait();                            // what the launch in front of this one writes is not among it
+    first = false;
+    const Factors f = a.factors[e.step];
+    x.update(a, f, p_at, at, have, vec);
   }
 }
 
@@ -501,23 +503,28 @@ __global__ void __launch_bounds__(kNT) grad_squares(const __grid_constant__ Tabl
   for (uint32_t tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
     i = tensor_of(tab, tile, i);
     const Entry& e = tab.e[i];
-    const int64_t off = (int64_t)(tile - e.tile) * kTile + threadIdx.x * kVec;
-    if (off >= e.n) continue;
-    const int have = (int)min((int64_t)kVec, e.n - off);
+    const int64_t off = (int64_t)(tile - e.tile) * (kTile * kNormParts) + threadIdx.x * kVec;
     const T* at = reinterpret_cast<const T*>(e.g) + off;
-    Raw8<T> w;
-    if (have == kVec && (reinterpret_cast<uintptr_t>(e.g) & 15) == 0) w.load(at);
-    else w.load(at, have);
-    Pair g[4];
-    w.get(g);
-    Pair s = both(0.f);
+    const bool aligned = (reinterpret_cast<uintptr_t>(e.g) & 15) == 0;
+    Raw8<T> w[kNormParts];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s = fma2(g[k], g[k], s);
-    const float sum = s.x + s.y;
-    if (sum > 1e-25f && sum < 1e38f) {
-      total += (double)sum;
-    } else {
-      for (int k = 0; k < 4; ++k) total += (double)g[k].x * g[k].x + (double)g[k].y * g[k].y;
+    for (int h = 0; h < kNormParts; ++h) {
+      const int have = (int)max((int64_t)0, min((int64_t)kVec, e.n - off - h * kTile));
+      if (have == kVec && aligned) w[h].load(at + h * kTile);
+      else w[h].load(at + h * kTile, have);
+    }
+#pragma unroll
+    for (int h = 0; h < kNormParts; ++h) {
+      Pair g[4], s = both(0.f);
+      w[h].get(g);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s = fma2(g[k], g[k], s);
+      const float sum = s.x + s.y;
+      if (sum > 1e-25f && sum < 1e38f) {
+        total += (double)sum;
+      } else {
+        for (int k = 0; k < 4; ++k) total += (double)g[k].x * g[k].x + (double)g[k].y * g[k].y;
+      }
     }
   }
 #pragma unroll
@@ -556,16 +563,17 @@ int sm_count() {
   return n;
 }
 
-// The tensors [from, to) that have a gradient, at most CAP of them, as a table; `block`: where the moments of tensor `from` begin.
+// The tensors [from, to) that have a gradient, at most CAP of them, as a table of tiles of `tile` elements; `block`: where the moments of tensor `from` begin.
 // Returns the tensor behind the last one, -1 for a size that is not allowed.
 template <int CAP>
-int64_t fill(Table<CAP>& tab, const int64_t* p, const int64_t* g, const int64_t* n, int64_t from, int64_t to, int steps, uint64_t& block) {
+int64_t fill(Table<CAP>& tab, const int64_t* p, const int64_t* g, const int64_t* n, int64_t from, int64_t to, int steps, int tile,
+             uint64_t& block) {
   tab.n = 0;
   tab.tiles = 0;
   int64_t i = from;
   for (; i < to && tab.n < CAP; ++i) {
-    const uint64_t blocks = ((uint64_t)n[i] + kBlock - 1) / kBlock, tiles = ((uint64_t)n[i] + kTile - 1) / kTile;
-    if (n[i] < 0 || block + blocks > 0xFFFFFFFFull) return -1;
+    const uint64_t blocks = ((uint64_t)n[i] + kBlock - 1) / kBlock, tiles = ((uint64_t)n[i] + tile - 1) / tile;
+    if (n[i] < 0 || n[i] > (int64_t)1 << 40 || block + blocks > 0xFFFFFFFFull) return -1;
     if (g[i] != 0 && n[i] > 0) {
       if (tiles + tab.tiles > 0x7FFFFFFFull) {
         if (tab.n == 0) return -1;
@@ -599,7 +607,7 @@ int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count
   uint64_t block = 0;
   bool begun = false;
   for (int64_t at = 0; at < count;) {
-    at = fill(tab, p, g, n, at, count, steps, block);
+    at = fill(tab, p, g, n, at, count, steps, kTile, block);
     if (at < 0) return (int)cudaErrorInvalidValue;
     if (tab.n == 0) continue;
     if (!begun || steps > 1) {                      // a common counter moves once
@@ -617,7 +625,7 @@ int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count
       if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (rest == REST_16) kern = small ? adamw_step<T, true, REST_16, CAP> : adamw_step<T, false, REST_16, CAP>;
       if (kern == nullptr) return (int)cudaErrorInvalidValue;
-      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * kCtas)), dim3(kNT), 0, s, true, tab, a);
+      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * (small ? kCtasSmall : kCtas))), dim3(kNT), 0, s, true, tab, a);
     });
     if (rc != 0) return rc;
   }
@@ -632,7 +640,7 @@ int norm_all(const int64_t* g, const int64_t* n, int64_t count, double* sums, fl
   uint64_t block = 0;
   int parts = 0;
   for (int64_t at = 0; at < count;) {
-    at = fill(tab, nullptr, g, n, at, count, 1, block);
+    at = fill(tab, nullptr, g, n, at, count, 1, kTile * kNormParts, block);
     if (at < 0) return (int)cudaErrorInvalidValue;
     if (tab.n == 0) continue;
     const int grid = grid_of(tab.tiles, sms * kNormCtas);
@@ -658,7 +666,7 @@ IPEX_API int64_t ipex_grad_norm_sums(int64_t count) {
 // p, g, n [count] (host): addresses and sizes of parameters and gradients of `dtype` (a gradient of 0: its parameter is left as it is,
 // and so is its step counter).  Flat buffers of sum(ceil(n / 256)) * 256 elements, aligned to 16 bytes: m, v in 32 bits or (small) in 8,
 // with an exponent for each 256 of them; rest: none (0), int16 (1, bf16 alone) or 32-bit (2, 16-bit parameters).  step: one counter, or
-// `count` of them; factors: 16 bytes for each.  lr_at (device) stands for lr.  Returns a cudaError_t.
+// `count` of them; factors: 32 bytes for each.  lr_at (device) stands for lr.  Returns a cudaError_t.
 IPEX_API int ipex_adamw_step(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count, void* m, void* v, uint8_t* m_scale,
                              uint8_t* v_scale, void* rest, int rest_kind, int64_t* step, int steps, void* factors, const float* norm,
                              double max_norm, double lr, const float* lr_at, double b1, double b2, double eps, double decay,
@@ -669,9 +677,9 @@ IPEX_API int ipex_adamw_step(const int64_t* p, const int64_t* g, const int64_t* 
       ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(rest) |
         reinterpret_cast<uintptr_t>(factors)) & 15))
     return (int)cudaErrorInvalidValue;
-  const BeginArgs b = {step, norm, lr_at, (Factors*)factors, max_norm, lr, b1, b2, decay};
-  const StepArgs a = {m, v, m_scale, v_scale, rest, (const Factors*)factors, step, (float)b1, (float)(1.0 - b1), (float)b2,
-                      (float)(1.0 - b2), (float)eps, seed};
+  const BeginArgs b = {step, norm, lr_at, (Factors*)factors, max_norm, lr, b1, b2, decay, (float)eps, seed};
+  const StepArgs a = {m, v, m_scale, v_scale, rest, (const Factors*)factors, (float)b1, (float)(1.0 - b1), (float)b2,
+                      (float)(1.0 - b2), (float)eps, -0.f};
   return count <= kFew ? step_all<kFew>(p, g, n, count, b, a, steps, dtype, small != 0, rest_kind, (cudaStream_t)stream)
                        : step_all<kMost>(p, g, n, count, b, a, steps, dtype, small != 0, rest_kind, (cudaStream_t)stream);
 }

@@ -151,7 +151,7 @@ bool adamw_step(py::handle params_, py::handle grads_, const Tensor& m, const Te
   }
   if ((norm && !one_of(*norm, dev)) || (lr_at && !one_of(*lr_at, dev))) return false;
   const c10::cuda::OptionalCUDAGuard guard(dev);
-  const Tensor factors = at::empty({4 * step.numel()}, at::TensorOptions().dtype(at::kFloat).device(dev));
+  const Tensor factors = at::empty({8 * step.numel()}, at::TensorOptions().dtype(at::kFloat).device(dev));
   check(entries.adamw_step(p_at, g_at, sizes, n, m.data_ptr(), v.data_ptr(), at_of<uint8_t>(m_scale), at_of<uint8_t>(v_scale),
                            at_of<void>(rest), kind, step.data_ptr<int64_t>(), (int)step.numel(), factors.data_ptr(),
                            at_of<const float>(norm), max_norm, lr, at_of<const float>(lr_at), b1, b2, eps, decay, seed, type_code(type),
