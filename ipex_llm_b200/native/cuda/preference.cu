@@ -16,16 +16,20 @@
 // it touches.  The third joins those of a row (up to kSlots) and does what comes behind them, in 64 bits.  The backward pass deals
 // its batches the same way, from the last row to the first, whose logits are still in L2, then the rows without a target, which it
 // only writes.  All of it is bound by memory.
+#include <cooperative_groups.h>
+
 #include "common/logit_rows.cuh"
 #include "common/utils.cuh"
 #include "tcgen05_common.cuh"
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kNT = 256;
 constexpr int kU = 4;                       // vectors of a lane in a batch
 constexpr int kBatch = 32 * kU;             // vectors of a batch
-constexpr int kCtas = 4;                    // to an SM
+constexpr int kCtas = 4, kGradCtas = 3;     // to an SM
 constexpr int kRun = 16;                    // batches of a warp's run, at most where a warp has many
 constexpr int kSlots = 18;                  // runs that may have a part in a row
 
@@ -134,25 +138,27 @@ __global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int
 }
 
 // ------------------------------------------------------------------------------------------------ sums
-// The maximum and the sum of a lane's part of a row.
+// A lane's part of a row: the sum of 2^(c x - r), r of a logit that none passes by more than 2^kSlack times its share.  It moves, and
+// the sum with it, only when one does: a sum's error is relative, wherever r lies.
+constexpr float kSlack = 16.f;
 struct Part {
   Base base;
   float s;
 };
-template <typename T>
 __device__ __forceinline__ void add_single(Part& p, float v, float c) {
   const Base now(fmaxf(p.base.m, v), c);              // a NaN is not the maximum, and makes the sum one
   p.s = p.s * ex2(shift(p.base, now, c)) + ex2(held(now.exponent(v, c)));
   if (v != v) p.s = v;
   p.base = now;
 }
-template <typename T>
+// The largest element of the first `n` vectors; a number before NaN.  16-bit numbers by pairs, as they are.
+template <typename T, bool WHOLE>
 __device__ __forceinline__ float largest(const uint4* w, int n) {
   if constexpr (std::is_same<T, float>::value) {
     float mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      if (u >= n) break;
+      if (!WHOLE && u >= n) break;
       float f[4];
       unpack<T>(w[u], f);
       mx = max3(max3(mx, f[0], f[1]), f[2], f[3]);
@@ -162,7 +168,7 @@ __device__ __forceinline__ float largest(const uint4* w, int n) {
     uint32_t a = max2<T>(w[0].x, w[0].y), b = max2<T>(w[0].z, w[0].w);
 #pragma unroll
     for (int u = 1; u < kU; ++u) {
-      if (u >= n) break;
+      if (!WHOLE && u >= n) break;
       a = max2<T>(a, max2<T>(w[u].x, w[u].y));
       b = max2<T>(b, max2<T>(w[u].z, w[u].w));
     }
@@ -171,13 +177,13 @@ __device__ __forceinline__ float largest(const uint4* w, int n) {
     return max3(-INFINITY, DT<T>::to_f(e[0]), DT<T>::to_f(e[1]));
   }
 }
-template <typename T, bool FAR>
+template <typename T, bool FAR, bool WHOLE>
 __device__ __forceinline__ float sum_of(const uint4* w, int n, const Base& now, float c) {
   constexpr int VEC = 16 / sizeof(T);
   float a[2] = {0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
-    if (u >= n) break;
+    if (!WHOLE && u >= n) break;
     float f[VEC], v[2] = {0.f, 0.f};
     unpack<T>(w[u], f);
 #pragma unroll
@@ -194,13 +200,20 @@ __device__ __forceinline__ float sum_of(const uint4* w, int n, const Base& now, 
   }
   return a[0] + a[1];
 }
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void add_vectors(Part& p, const uint4* w, int n, float c) {
+  const float mx = largest<T, WHOLE>(w, n);
+  if (!(fmaf(mx, c, -p.base.to) <= kSlack) || p.base.far || p.base.m == -INFINITY) {
+    const Base now(fmaxf(p.base.m, mx), c);
+    p.s *= ex2(shift(p.base, now, c));
+    p.base = now;
+  }
+  p.s += p.base.far ? sum_of<T, true, false>(w, n, p.base, c) : sum_of<T, false, WHOLE>(w, n, p.base, c);
+}
 template <typename T>
 __device__ __forceinline__ void add_batch(Part& p, const uint4* w, int n, float c) {
-  if (n <= 0) return;
-  const Base now(fmaxf(p.base.m, largest<T>(w, n)), c);
-  const float s = now.far ? sum_of<T, true>(w, n, now, c) : sum_of<T, false>(w, n, now, c);
-  p.s = p.s * ex2(shift(p.base, now, c)) + s;
-  p.base = now;
+  if (n == kU) add_vectors<T, true>(p, w, n, c);
+  else if (n > 0) add_vectors<T, false>(p, w, n, c);
 }
 
 struct SumArgs {
@@ -232,22 +245,24 @@ __global__ void __launch_bounds__(kNT, kCtas) row_sums(SumArgs a) {
       const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head) + lane;
       // vectors of this lane, 32 apart, from `from` on
       auto count = [&](int from) { return min(kU, (sp.nvec - from - lane + 31) / 32); };
-      uint4 w[kU];
-      auto load = [&](int from) {
+      auto load = [&](uint4* w, int b) {
+        const int from = b * kBatch;
 #pragma unroll
         for (int u = 0; u < kU; ++u)
           if (from + u * 32 + lane < sp.nvec) w[u] = ldg_nc_v4(xv + from + u * 32);
       };
-      load(b * kBatch);
+      uint4 w[kU], v[kU];
+      load(w, b);
       Part p = {Base(-INFINITY, c), 0.f};
-      if (b == 0 && lane < sp.head) add_single<T>(p, DT<T>::to_f(x[lane]), c);
-      if (b1 == deal.per && lane < sp.tail) add_single<T>(p, DT<T>::to_f(x[a.rows.V - sp.tail + lane]), c);
-      for (; b < b1; ++b) {
-        uint4 now[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) now[u] = w[u];
-        if (b + 1 < b1) load((b + 1) * kBatch);
-        add_batch<T>(p, now, count(b * kBatch), c);
+      if (b == 0 && lane < sp.head) add_single(p, DT<T>::to_f(x[lane]), c);
+      if (b1 == deal.per && lane < sp.tail) add_single(p, DT<T>::to_f(x[a.rows.V - sp.tail + lane]), c);
+      while (true) {                                  // a batch is asked for while the one in front of it is added
+        if (b + 1 < b1) load(v, b + 1);
+        add_batch<T>(p, w, count(b * kBatch), c);
+        if (++b >= b1) break;
+        if (b + 1 < b1) load(w, b + 1);
+        add_batch<T>(p, v, count(b * kBatch), c);
+        if (++b >= b1) break;
       }
       // all taken to the largest base, then added up
       float m;
@@ -281,11 +296,18 @@ __device__ __forceinline__ double row_logprob(const RowArgs& a, const Keep& k, c
   const float xt = bad ? 0.f : DT<T>::to_f(row_at<T>(a.rows, row)[t]);
   const int parts = (int)(((int64_t)(place + 1) * deal.per - 1) / deal.len - deal.run_of(place)) + 1;
   const float2* at = a.part + (int64_t)place * kSlots;
+  float2 p[kSlots];
   Stat st = {-INFINITY, 0.f, 0.f};
-  for (int i = 0; i < parts; ++i) {
-    const float2 p = at[i];
-    st = join<false>(st, {p.x, p.y, 0.f}, c);
-  }
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i)
+    if (i < parts) p[i] = at[i];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i)
+    if (i < parts) st.m = fmaxf(st.m, p[i].x);
+  const Base to(st.m, c);
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i)
+    if (i < parts) st.s += p[i].y * ex2(shift(Base(p[i].x, c), to, c));
   const bool none = no_token(st);
   const Base base(none ? 0.f : st.m, c);
   k.stat[place] = make_float2(base.m, none ? 0.f : bad ? NAN : 1.f / st.s);
@@ -361,51 +383,64 @@ struct PairArgs {
   float* logprob;           // [2 pairs]
 };
 
-constexpr int kPairNT = 1024;
+constexpr int kPairNT = 256, kPairCtas = 8;
 
-// A CTA to a pair.
+// A cluster of eight CTAs to a pair: half of them to each sequence.
 template <typename T>
-__global__ void __launch_bounds__(kPairNT) pair_losses(PairArgs a) {
-  __shared__ double sums[2][kPairNT / 32];
-  __shared__ int counts[2][kPairNT / 32];
+__global__ void __cluster_dims__(kPairCtas, 1, 1) __launch_bounds__(kPairNT) pair_losses(PairArgs a) {
+  __shared__ double sums[kPairNT / 32];
+  __shared__ int counts[kPairNT / 32];
+  __shared__ double sum;
+  __shared__ int count;
   const Keep k = keep_at(a.row.keep, a.row.n);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x % kPairCtas, pair = blockIdx.x / kPairCtas;
+  const int half = rank / (kPairCtas / 2), part = rank % (kPairCtas / 2);
   pdl_wait();
   const Deal deal(*k.count, a.row.per, a.row.warps);
-  for (int half = 0; half < 2; ++half) {
-    const int64_t r0 = ((int64_t)half * a.pairs + blockIdx.x) * a.tokens;
-    double s = 0.0;
-    int n = 0;
-    for (int64_t t = threadIdx.x; t < a.tokens; t += kPairNT) {
-      const int place = k.place[r0 + t];
-      if (place < 0) continue;
-      s += row_logprob<T>(a.row, k, deal, r0 + t, place);
-      ++n;
-    }
+  const int64_t r0 = ((int64_t)half * a.pairs + pair) * a.tokens;
+  double s = 0.0;
+  int n = 0;
+  for (int64_t t = part * kPairNT + threadIdx.x; t < a.tokens; t += kPairNT * (kPairCtas / 2)) {
+    const int place = k.place[r0 + t];
+    if (place < 0) continue;
+    s += row_logprob<T>(a.row, k, deal, r0 + t, place);
+    ++n;
+  }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      n += __shfl_xor_sync(0xffffffffu, n, o);
-    }
-    if (lane == 0) {
-      sums[half][warp] = s;
-      counts[half][warp] = n;
-    }
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+  if (lane == 0) {
+    sums[warp] = s;
+    counts[warp] = n;
   }
   __syncthreads();
-  if (threadIdx.x != 0) return;
-  double S[2], share[2];
-  for (int half = 0; half < 2; ++half) {
-    double s = 0.0;
-    int n = 0;
-    for (int w = 0; w < kPairNT / 32; ++w) {
-      s += sums[half][w];
-      n += counts[half][w];
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kPairNT / 32; ++w) {
+      s += sums[w];
+      n += counts[w];
     }
-    share[half] = a.average ? 1.0 / max(n, 1) : 1.0;
-    S[half] = s * share[half];
+    sum = s;
+    count = n;
   }
-  const int c = blockIdx.x, r = blockIdx.x + a.pairs;
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  double S[2] = {0.0, 0.0};
+  int N[2] = {0, 0};
+  if (rank == 0 && threadIdx.x == 0)
+    for (int i = 0; i < kPairCtas; ++i) {
+      S[i / (kPairCtas / 2)] += *cl.map_shared_rank(&sum, i);
+      N[i / (kPairCtas / 2)] += *cl.map_shared_rank(&count, i);
+    }
+  cl.sync();
+  if (rank != 0 || threadIdx.x != 0) return;
+  double share[2];
+  for (int h = 0; h < 2; ++h) {
+    share[h] = a.average ? 1.0 / max(N[h], 1) : 1.0;
+    S[h] *= share[h];
+  }
+  const int c = pair, r = pair + a.pairs;
   const double h = (S[0] - (a.reference == nullptr ? 0.0 : a.reference[c])) - (S[1] - (a.reference == nullptr ? 0.0 : a.reference[r]));
   double loss, d;
   if (a.form == FORM_SIGMOID) {
@@ -447,22 +482,37 @@ struct GradArgs {
   float inv_t;
 };
 
+__device__ __forceinline__ void times2(float& x, float& y, float a) {
+  asm("{\n.reg .b64 p, q;\nmov.b64 p, {%0, %1};\nmov.b64 q, {%2, %2};\nmul.rn.f32x2 p, p, q;\nmov.b64 {%0, %1}, p;\n}\n" : "+f"(x), "+f"(y) : "f"(a));
+}
+// scale 2^(c x - r) of a vector's elements.
 template <typename T>
-__device__ __forceinline__ void put(T* y, bool alike, const float* f) {
+__device__ __forceinline__ uint4 shares(const uint4& w, float c, float minus_r, float scale) {
   constexpr int VEC = 16 / sizeof(T);
-  __align__(16) T o[VEC];
+  float f[VEC];
+  unpack<T>(w, f);
+  uint4 o;
+  T* to = reinterpret_cast<T*>(&o);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) o[i] = DT<T>::from_f(f[i]);
-  if (alike) {
-    __stcs(reinterpret_cast<uint4*>(y), *reinterpret_cast<const uint4*>(o));      // nothing here reads them again
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) y[i] = o[i];
+  for (int i = 0; i < VEC; i += 2) {
+    exponents2(f[i], f[i + 1], c, minus_r);
+    f[i] = ex2(f[i]);
+    f[i + 1] = ex2(f[i + 1]);
+    times2(f[i], f[i + 1], scale);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      *reinterpret_cast<__nv_bfloat162*>(to + i) = __floats2bfloat162_rn(f[i], f[i + 1]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      *reinterpret_cast<__half2*>(to + i) = __floats2half2_rn(f[i], f[i + 1]);
+    } else {
+      to[i] = f[i];
+      to[i + 1] = f[i + 1];
+    }
   }
+  return o;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kNT, kCtas) row_grads(GradArgs a) {
+__global__ void __launch_bounds__(kNT, kGradCtas) row_grads(GradArgs a) {
   constexpr int VEC = 16 / sizeof(T);
   const int lane = threadIdx.x & 31, warps = gridDim.x * (kNT / 32), warp = blockIdx.x * (kNT / 32) + (threadIdx.x >> 5);
   const Keep k = keep_at(const_cast<void*>(a.keep), a.n);
@@ -482,14 +532,16 @@ __global__ void __launch_bounds__(kNT, kCtas) row_grads(GradArgs a) {
       const Span<T> sp(x, V);
       const int b1 = (int)min((int64_t)deal.per, b + (end - at));
       at += b1 - b;
-      const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head);
-      uint4 w[kU];
-      auto load = [&](int from) {
+      const uint4* xv = reinterpret_cast<const uint4*>(x + sp.head) + lane;
+      uint4* yv = reinterpret_cast<uint4*>(y + sp.head) + lane;
+      auto load = [&](uint4* w, int b) {
+        const int from = b * kBatch;
 #pragma unroll
         for (int u = 0; u < kU; ++u)
-          if (from + u * 32 + lane < sp.nvec) w[u] = ldg_nc_v4(xv + from + u * 32 + lane);
+          if (from + u * 32 + lane < sp.nvec) w[u] = ldg_nc_v4(xv + from + u * 32);
       };
-      load(b * kBatch);
+      uint4 w[kU], v[kU];
+      load(w, b);
       const float2 st = k.stat[place];
       const int64_t t = a.targets[row];
       float g = 0.f;
@@ -504,36 +556,49 @@ __global__ void __launch_bounds__(kNT, kCtas) row_grads(GradArgs a) {
       const Base base(st.x, c);
       const float scale = -g * st.y * a.inv_t;
       const bool nothing = g == 0.f;                  // flows into the row, whatever its logits hold
-      auto of = [&](float v) { return nothing ? 0.f : ex2(base.exponent(v, c)) * scale; };
-      auto of_target = [&](float v) { return nothing ? 0.f : fmaf(g, a.inv_t, of(v)); };
       const bool alike = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
-      auto single = [&](int j) {
-        const float v = DT<T>::to_f(x[j]);
-        y[j] = DT<T>::from_f(j == t ? of_target(v) : of(v));
+      auto one = [&](int j) {
+        const float f = DT<T>::to_f(x[j]);
+        const float e = nothing ? 0.f : ex2(base.exponent(f, c)) * scale;
+        y[j] = DT<T>::from_f(j == t && !nothing ? fmaf(g, a.inv_t, e) : e);
       };
-      if (b == 0 && lane < sp.head) single(lane);
-      if (b1 == deal.per && lane < sp.tail) single(V - sp.tail + lane);
-      for (; b < b1; ++b) {
-        uint4 now[kU];
-#pragma unroll
-        for (int u = 0; u < kU; ++u) now[u] = w[u];
-        if (b + 1 < b1) load((b + 1) * kBatch);
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-          const int v = b * kBatch + u * 32 + lane;
-          if (v >= sp.nvec) break;
-          float f[VEC];
-          unpack<T>(now[u], f);
-          const int64_t hit = t - (sp.head + (int64_t)v * VEC);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) f[i] = i == hit ? of_target(f[i]) : of(f[i]);
-          put<T>(y + sp.head + (int64_t)v * VEC, alike, f);
+      if (b == 0 && lane < sp.head) one(lane);
+      if (b1 == deal.per && lane < sp.tail) one(V - sp.tail + lane);
+      const int v0 = b * kBatch, v1 = min(b1 * kBatch, sp.nvec);
+      if (nothing) {
+        for (int i = v0 + lane; i < v1; i += 32) {
+          if (alike) {
+            __stcs(yv + i - lane, make_uint4(0, 0, 0, 0));
+          } else {
+            for (int e = 0; e < VEC; ++e) y[sp.head + (int64_t)i * VEC + e] = DT<T>::from_f(0.f);
+          }
         }
+      } else if (alike && !base.far) {
+        auto store = [&](const uint4* w, int b) {
+          const int from = b * kBatch;
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+            if (from + u * 32 + lane < sp.nvec) __stcs(yv + from + u * 32, shares<T>(w[u], c, -base.r, scale));     // nothing here reads them again
+        };
+        while (true) {                                // a batch is asked for while the one in front of it is worked on
+          if (b + 1 < b1) load(v, b + 1);
+          store(w, b);
+          if (++b >= b1) break;
+          if (b + 1 < b1) load(w, b + 1);
+          store(v, b);
+          if (++b >= b1) break;
+        }
+      } else {
+        for (int i = v0 + lane; i < v1; i += 32)
+          for (int e = 0; e < VEC; ++e) one(sp.head + i * VEC + e);
       }
+      // the target once more, by the lane that has written it
+      const int64_t at_t = t - sp.head;
+      if (!nothing && at_t >= (int64_t)v0 * VEC && at_t < (int64_t)v1 * VEC && (at_t / VEC - v0) % 32 == lane) one((int)t);
     }
   }
   // rows without a target
-  const int per = batches_of(V, VEC);
+  const int per = deal.per;
   const int64_t rest = (a.n - count) * per;
   for (int64_t at = warp; at < rest; at += warps) {
     const int64_t i = at / per;
@@ -555,10 +620,10 @@ __global__ void __launch_bounds__(kNT, kCtas) row_grads(GradArgs a) {
 // ------------------------------------------------------------------------------------------------ host
 int elem_of(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
-int grid_of(int64_t rows, int V, int elem) {
+int grid_of(int64_t rows, int V, int elem, int per_sm) {
   const int sms = sm_count();
   const int64_t batches = rows * batches_of(V, 16 / elem), ctas = (batches + kNT / 32 - 1) / (kNT / 32);
-  return (int)(ctas < (int64_t)sms * kCtas ? ctas : (int64_t)sms * kCtas);
+  return (int)(ctas < (int64_t)sms * per_sm ? ctas : (int64_t)sms * per_sm);
 }
 
 // The first two kernels; then `a` is ready for the third.
@@ -567,7 +632,7 @@ int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
   list_rows<<<1, kListNT, 0, s>>>(a.targets, a.n, ignore, a.keep);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  const int grid = grid_of(a.n, a.rows.V, elem_of(dtype));
+  const int grid = grid_of(a.n, a.rows.V, elem_of(dtype), kCtas);
   a.warps = grid * (kNT / 32);
   a.per = batches_of(a.rows.V, 16 / elem_of(dtype));
   const SumArgs sums = {a.rows, a.n, a.keep, const_cast<float2*>(a.part), a.inv_t};
@@ -579,7 +644,7 @@ int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
 int backward(const GradArgs& a, int dtype, cudaStream_t s) {
   if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
   return by_type(dtype, [&](auto* tag) {
-    row_grads<std::remove_pointer_t<decltype(tag)>><<<grid_of(a.n, a.rows.V, elem_of(dtype)), kNT, 0, s>>>(a);
+    row_grads<std::remove_pointer_t<decltype(tag)>><<<grid_of(a.n, a.rows.V, elem_of(dtype), kGradCtas), kNT, 0, s>>>(a);
     return (int)cudaGetLastError();
   });
 }
@@ -641,7 +706,7 @@ IPEX_API int ipex_preference_loss(const void* logits, int64_t s0, int64_t s1, in
   if (rc != 0) return rc;
   const PairArgs a = {r, reference, tokens, pairs, form, average, beta, smooth, margin, loss, logprob};
   return by_type(dtype, [&](auto* tag) {
-    return (int)launch_kernel(pair_losses<std::remove_pointer_t<decltype(tag)>>, dim3((unsigned)pairs), dim3(kPairNT), 0,
+    return (int)launch_kernel(pair_losses<std::remove_pointer_t<decltype(tag)>>, dim3((unsigned)pairs * kPairCtas), dim3(kPairNT), 0,
                               (cudaStream_t)stream, true, a);
   });
 }

@@ -141,10 +141,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     if advantages.device != logits.device or not advantages.is_floating_point():
         invalidInputError(False, f"{what}: advantages should hold floating-point numbers on {logits.device}, got {advantages.dtype} on "
                                  f"{advantages.device}")
-    try:
-        fits = torch.broadcast_shapes(advantages.shape, targets.shape) == targets.shape
-    except RuntimeError:
-        fits = False
+    fits = advantages.dim() <= targets.dim() and all(
+        m in (1, n) for m, n in zip(reversed(advantages.shape), reversed(targets.shape)))
     if not fits:
         invalidInputError(False, f"{what}: advantages of shape {tuple(advantages.shape)} do not fit targets of {tuple(targets.shape)}")
     lo, hi = float(clip[0]), float(clip[1])
