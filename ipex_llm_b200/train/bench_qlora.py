@@ -9,6 +9,7 @@ sequence 512, micro-batch 4 per GPU, random token ids, causal-LM loss.  One step
 reduce-scatter/AdamW/all-gather kernel.  Timed with CUDA events around K steps after W warm-ups, max over ranks;
 inputs come from pinned host memory every step and the loss is read back, as a training loop does.
 ``--fused-attention`` and ``--fused-loss`` swap in the attention with a gradient and the loss straight from the logits.
+``--optimizer tensors`` and ``8bit`` step the adapters where they lie, with moments in 32 or 8 bits (one GPU).
 ``--optimizer torch`` swaps in ``dist.all_reduce`` + ``torch.optim.AdamW`` (the library baseline).
 """
 from __future__ import annotations
@@ -40,7 +41,7 @@ def run(argv=None, timed=None):
     ap.add_argument("--seq", type=int, default=512)
     ap.add_argument("--micro-batch", type=int, default=4)
     ap.add_argument("--layers", type=int, default=0)
-    ap.add_argument("--optimizer", default="fused", choices=["fused", "torch"])
+    ap.add_argument("--optimizer", default="fused", choices=["fused", "tensors", "8bit", "torch"])
     ap.add_argument("--no-checkpointing", action="store_true")
     ap.add_argument("--fused-attention", action="store_true")
     ap.add_argument("--fused-loss", action="store_true")
@@ -56,6 +57,7 @@ def run(argv=None, timed=None):
     from ..parallel.dp import FusedLoraAdamW
     from ..transformers import AutoModelForCausalLM
     from .losses import causal_lm_loss
+    from .optim import MultiTensorAdamW
     from ..transformers.qlora import LoraConfig, cast_lora_weight, get_peft_model, prepare_model_for_kbit_training
     arch = dict(ARCH[a.model])
     if a.layers:
@@ -75,6 +77,10 @@ def run(argv=None, timed=None):
     n_train = sum(p.numel() for p in params)
     if a.optimizer == "fused":
         opt = FusedLoraAdamW(params, lr=2e-4, max_grad_norm=0.0)
+    elif a.optimizer in ("tensors", "8bit"):
+        if world > 1:
+            raise SystemExit("--optimizer tensors and 8bit do not average gradients: one GPU")
+        opt = MultiTensorAdamW(params, lr=2e-4, bits=8 if a.optimizer == "8bit" else 32)
     else:
         opt = torch.optim.AdamW(params, lr=2e-4)
     g = torch.Generator().manual_seed(100 + rank)
@@ -125,8 +131,9 @@ def run(argv=None, timed=None):
                           "tokens_per_s": round(world * a.micro_batch * a.seq * 1000.0 / ms, 1),
                           "ms_per_step": round(ms, 3), "steps": a.steps, "warmup": a.warmup, "seq_len": a.seq,
                           "micro_batch_per_gpu": a.micro_batch, "trainable_params": n_train,
-                          "optimizer": "fused reduce-scatter + AdamW + all-gather kernel" if a.optimizer == "fused"
-                          else "NCCL all_reduce + torch.optim.AdamW", "base": "nf4", "compute": "bf16",
+                          "optimizer": {"fused": "fused reduce-scatter + AdamW + all-gather kernel",
+                                        "tensors": "AdamW over many tensors", "8bit": "AdamW over many tensors, 8-bit moments",
+                                        "torch": "NCCL all_reduce + torch.optim.AdamW"}[a.optimizer], "base": "nf4", "compute": "bf16",
                           "attention": "fused" if a.fused_attention else "library",
                           "loss": "fused" if a.fused_loss else "library",
                           "gradient_checkpointing": not a.no_checkpointing, "last_loss": round(last, 4),

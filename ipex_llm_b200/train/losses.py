@@ -2,10 +2,11 @@
 gradient is written once, in the logits' type (``ops.token_loss``)."""
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
+from ..ops.preference import policy_loss, preference_loss
 from ..ops.token_loss import IGNORE, distill_loss, token_logprobs
 from ..utils.common import invalidInputError
 
@@ -56,3 +57,44 @@ def teacher_tokens(logits: torch.Tensor, top: int = 32, temperature: float = 1.0
     best = token_logprobs(logits, torch.zeros(logits.shape[:-1], dtype=torch.int64, device=logits.device), temperature, top=top)
     return TeacherTokens(best.top_ids, best.top_logprobs.float() * temperature,
                          torch.zeros(logits.shape[:-1], dtype=torch.float32, device=logits.device))
+
+
+@torch.no_grad()
+def sequence_logprobs(logits: torch.Tensor, labels: torch.Tensor, average: bool = False) -> torch.Tensor:
+    """Log probability of each sequence's labels, ``[batch]`` (``average``: the mean over them): what ``preference_lm_loss`` takes of a
+    reference model."""
+    _check(logits, labels, "sequence_logprobs")
+    targets = next_tokens(labels)
+    total = token_logprobs(logits, targets).logprob.double().sum(dim=1)
+    return (total / (targets != IGNORE).sum(dim=1).clamp(min=1) if average else total).float()
+
+
+def preference_lm_loss(logits: torch.Tensor, labels: torch.Tensor, reference: Optional[torch.Tensor] = None, beta: float = 0.1,
+                       form: str = "sigmoid", label_smoothing: float = 0.0, margin: float = 0.0, average: bool = False,
+                       likelihood_weight: float = 0.0) -> torch.Tensor:
+    """Mean loss of preferred over rejected sequences (``ops.preference.preference_loss``): the first half of the batch is preferred to
+    the second, in order; labels of -100 (prompts, padding) take no part.  ``likelihood_weight`` of the preferred sequences' mean
+    negative log probability a token is added."""
+    _check(logits, labels, "preference_lm_loss")
+    targets = next_tokens(labels)
+    got = preference_loss(logits, targets, reference, beta, form, label_smoothing, margin, average)
+    loss = got.loss.mean()
+    if likelihood_weight:
+        pairs = got.loss.shape[0]
+        likely = got.logprob[:pairs]
+        if not average:
+            likely = likely / (targets[:pairs] != IGNORE).sum(dim=1).clamp(min=1)
+        loss = loss - likelihood_weight * likely.mean()
+    return loss
+
+
+def policy_lm_loss(logits: torch.Tensor, labels: torch.Tensor, advantages: torch.Tensor, old_logprobs: Optional[torch.Tensor] = None,
+                   ref_logprobs: Optional[torch.Tensor] = None, clip: Tuple[float, float] = (0.2, 0.2), kl_weight: float = 0.0,
+                   temperature: float = 1.0) -> torch.Tensor:
+    """Mean clipped policy loss (``ops.preference.policy_loss``) over the positions that predict a label.  What belongs to a token stands
+    in the row that predicts it: ``old_logprobs``, ``ref_logprobs`` and ``advantages [batch, tokens]`` (or ``[batch, 1]``).  0 where no
+    position is left."""
+    _check(logits, labels, "policy_lm_loss")
+    targets = next_tokens(labels)
+    loss = policy_loss(logits, targets, advantages, old_logprobs, ref_logprobs, clip, kl_weight, temperature).loss
+    return loss.sum() / (targets != IGNORE).sum().clamp(min=1)

@@ -19,9 +19,11 @@ import torch.distributed as dist
 
 from ..parallel.dp import FusedLoraAdamW, PagedAdamW
 from ..utils.common import invalidInputError
-from .losses import TeacherTokens, causal_lm_loss, distill_lm_loss
+from .losses import TeacherTokens, causal_lm_loss, distill_lm_loss, policy_lm_loss, preference_lm_loss, sequence_logprobs
+from .optim import MultiTensorAdamW
 
 TEACHER_COLUMNS = TeacherTokens._fields
+POLICY_COLUMNS = ("advantages", "old_logprobs", "ref_logprobs")
 
 
 class TrainerCallback:
@@ -82,6 +84,10 @@ class Trainer:
         if a.optim == "adamw_torch":
             invalidInputError(self.world == 1, "adamw_torch has no gradient averaging: use fused_lora_adamw")
             self.optimizer = torch.optim.AdamW(params, **kw)
+        elif a.optim in ("adamw_multi", "adamw_8bit"):
+            invalidInputError(self.world == 1, f"{a.optim} has no gradient averaging: use fused_lora_adamw")
+            self.optimizer = MultiTensorAdamW(params, max_grad_norm=a.max_grad_norm, bits=8 if a.optim == "adamw_8bit" else 32,
+                                              seed=a.seed, **kw)
         elif a.optim == "paged_adamw" and self.world == 1 and self.device.type == "cuda" and \
                 sum(p.numel() for p in params) > (1 << 28):
             self.optimizer = PagedAdamW(params, **kw)
@@ -117,7 +123,13 @@ class Trainer:
         return out.loss if hasattr(out, "loss") and out.loss is not None else out[0]
 
     def _fused_loss(self, model, batch):
-        """The loss by ``causal_lm_loss``; with a teacher's tokens in the batch, ``distill_weight`` of it by ``distill_lm_loss``."""
+        """The loss by ``causal_lm_loss``; with a teacher's tokens in the batch, ``distill_weight`` of it by ``distill_lm_loss``.  With
+        ``preference_form`` batches are pairs, and the loss ``preference_lm_loss``; with advantages in the batch it is
+        ``policy_lm_loss``."""
+        if getattr(self.args, "preference_form", None):
+            return self._preference_loss(model, batch)
+        if "advantages" in batch:
+            return self._policy_loss(model, batch)
         teacher = {k: batch.pop(k) for k in TEACHER_COLUMNS if k in batch}
         invalidInputError("labels" in batch, "fused_loss: the batch has no labels")
         labels = batch.pop("labels")
@@ -132,6 +144,33 @@ class Trainer:
             loss = loss + w * distill_lm_loss(logits, labels, temperature=float(getattr(self.args, "distill_temperature", 1.0)),
                                               **teacher)
         return loss
+
+    def _preference_loss(self, model, batch):
+        a = self.args
+        invalidInputError("labels" in batch, "preference_form: the batch has no labels")
+        labels, reference = batch.pop("labels"), batch.pop("reference_logprobs", None)
+        average = bool(getattr(a, "preference_average", False))
+        if reference is None and getattr(a, "preference_reference", True):
+            invalidInputError(hasattr(model, "disable_adapter_layers"), "preference_form: without adapters the batch needs "
+                                                                        "reference_logprobs (or preference_reference=False)")
+            model.disable_adapter_layers(True)                 # the model that finetuning began with
+            try:
+                with torch.no_grad():
+                    reference = sequence_logprobs(_logits_of(model(**batch)), labels, average)
+            finally:
+                model.disable_adapter_layers(False)
+        return preference_lm_loss(_logits_of(model(**batch)), labels, reference, float(getattr(a, "preference_beta", 0.1)),
+                                  a.preference_form, float(getattr(a, "preference_label_smoothing", 0.0)),
+                                  float(getattr(a, "preference_margin", 0.0)), average,
+                                  float(getattr(a, "preference_likelihood_weight", 0.0)))
+
+    def _policy_loss(self, model, batch):
+        a = self.args
+        invalidInputError("labels" in batch, "a policy's batch has no labels")
+        given = {k: batch.pop(k) for k in POLICY_COLUMNS if k in batch}
+        labels = batch.pop("labels")
+        return policy_lm_loss(_logits_of(model(**batch)), labels, clip=tuple(getattr(a, "policy_clip", (0.2, 0.2))),
+                              kl_weight=float(getattr(a, "policy_kl_weight", 0.0)), **given)
 
     def train(self, resume_from_checkpoint: Optional[str] = None):
         a = self.args
@@ -171,7 +210,7 @@ class Trainer:
                 loss_acc += float(loss.detach())
                 tokens += int(batch["input_ids"].numel())
                 self.state.data_cursor = cursor
-            if not isinstance(self.optimizer, FusedLoraAdamW) and a.max_grad_norm and a.max_grad_norm > 0:
+            if not isinstance(self.optimizer, (FusedLoraAdamW, MultiTensorAdamW)) and a.max_grad_norm and a.max_grad_norm > 0:
                 torch.nn.utils.clip_grad_norm_([p for p in self.model.parameters() if p.requires_grad],
                                                a.max_grad_norm)
             self.optimizer.step()
@@ -266,6 +305,10 @@ class _null:
     def __exit__(self, *a): return False
 
 
+def _logits_of(out):
+    return out.logits if hasattr(out, "logits") else out[0]
+
+
 def _pad_teacher(rows, n: int, ids: bool):
     rows = [torch.as_tensor(r, dtype=torch.long if ids else torch.float32).cpu() for r in rows]
     top = [max(r.shape[1] for r in rows)] if rows[0].dim() == 2 else []
@@ -277,7 +320,13 @@ def _pad_teacher(rows, n: int, ids: bool):
 
 def default_collator(samples):
     """Pads ``input_ids`` / ``labels`` / ``attention_mask`` lists to the longest sample (labels padded with -100); a teacher's
-    rows (``TeacherTokens``: lists or tensors [tokens, top] and [tokens]) likewise, ids with -1."""
+    rows (``TeacherTokens``: lists or tensors [tokens, top] and [tokens]) likewise, ids with -1, and a policy's numbers (advantages may
+    be one for each sample) with 0.
+
+    Pairs, with ``chosen_input_ids`` and ``rejected_input_ids`` (and labels of either name, -100 for the prompt), become a batch of the
+    chosen samples, then of the rejected ones; ``reference_logprobs`` hold two numbers, the chosen one's first."""
+    if "chosen_input_ids" in samples[0]:
+        return _pairs(samples)
     keys = samples[0].keys()
     n = max(len(s["input_ids"]) for s in samples)
     out = {}
@@ -285,8 +334,26 @@ def default_collator(samples):
         if k in TEACHER_COLUMNS:
             out[k] = _pad_teacher([s[k] for s in samples], n, k == "teacher_ids")
             continue
+        if k in POLICY_COLUMNS:
+            rows = [torch.as_tensor(s[k], dtype=torch.float32).cpu().reshape(-1) for s in samples]
+            one = k == "advantages" and all(r.numel() == 1 for r in rows)
+            out[k] = torch.stack(rows) if one else _pad_teacher(rows, n, False)
+            continue
         pad = -100 if k == "labels" else 0
         out[k] = torch.tensor([list(s[k]) + [pad] * (n - len(s[k])) for s in samples], dtype=torch.long)
     if "labels" not in out:
         out["labels"] = out["input_ids"].clone()
+    return out
+
+
+def _pairs(samples):
+    both = []
+    for name in ("chosen", "rejected"):
+        for s in samples:
+            ids = list(s[f"{name}_input_ids"])
+            both.append({"input_ids": ids, "labels": list(s.get(f"{name}_labels", ids)),
+                         "attention_mask": list(s.get(f"{name}_attention_mask", [1] * len(ids)))})
+    out = default_collator(both)
+    if "reference_logprobs" in samples[0]:
+        out["reference_logprobs"] = torch.tensor([[float(x) for x in s["reference_logprobs"]] for s in samples]).t().reshape(-1)
     return out

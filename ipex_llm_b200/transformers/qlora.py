@@ -15,7 +15,7 @@ import math
 import os
 import re
 from dataclasses import asdict, dataclass, field
-from typing import List, Optional, Union
+from typing import List, Optional, Tuple, Union
 
 import torch
 from torch import nn
@@ -408,7 +408,7 @@ class TrainingArguments:
     save_total_limit: Optional[int] = None
     bf16: bool = True
     fp16: bool = False
-    optim: str = "paged_adamw"          # adamw_torch | paged_adamw | fused_lora_adamw
+    optim: str = "paged_adamw"          # adamw_torch | paged_adamw | fused_lora_adamw | adamw_multi | adamw_8bit
     gradient_checkpointing: bool = False
     ddp_backend: str = "nccl"
     seed: int = 42
@@ -421,3 +421,15 @@ class TrainingArguments:
     fused_loss: bool = False
     distill_weight: float = 0.5         # of the loss, where a batch has a teacher's tokens
     distill_temperature: float = 1.0
+    # with fused_loss: pairs of samples ("chosen_input_ids", "rejected_input_ids") by "sigmoid", "hinge" or "ipo"; the reference is the
+    # batch's reference_logprobs, or the model with its adapters disabled
+    preference_form: Optional[str] = None
+    preference_beta: float = 0.1
+    preference_label_smoothing: float = 0.0
+    preference_margin: float = 0.0
+    preference_average: bool = False
+    preference_reference: bool = True
+    preference_likelihood_weight: float = 0.0
+    # with fused_loss and advantages in the batch: a policy's step
+    policy_clip: Tuple[float, float] = (0.2, 0.2)
+    policy_kl_weight: float = 0.0

@@ -100,6 +100,10 @@ def load_weight_checkpoint(model, checkpoint_path: str):
 def reset_optimizer(optimizer, prune_ratio: float = 0.9):
     """Zero the smallest ``prune_ratio`` fraction (by magnitude) of the Adam moments after a restart."""
     from ..parallel.dp import FusedLoraAdamW
+    from ..train.optim import MultiTensorAdamW
+    if isinstance(optimizer, MultiTensorAdamW):
+        optimizer.prune_moments(prune_ratio)
+        return
     if isinstance(optimizer, FusedLoraAdamW):
         tensors = [optimizer.exp_avg, optimizer.exp_avg_sq]
     else:
@@ -151,6 +155,8 @@ class ReLoRACallback(TrainerCallback):
                 # the adapters were re-initialised in place inside the flat parameter buffer
                 lo = optimizer.rank * optimizer.shard
                 optimizer.master.copy_(optimizer.flat_params[lo:lo + optimizer.shard].float())
+            elif hasattr(optimizer, "parameters_changed"):
+                optimizer.parameters_changed()
             self.num_restarts = state.global_step // self.relora_steps
         # applied on top of the trainer's own schedule
         if optimizer is not None:
