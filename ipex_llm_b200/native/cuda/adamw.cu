@@ -33,6 +33,10 @@ constexpr int kBlock = 256;                 // elements with a common exponent: 
 static_assert(kBlock == 32 * kVec, "a warp has a block");
 constexpr int kLow = 32, kHigh = 254;       // exponents of a block: 2^(e - 127)
 constexpr int kCtas = 3, kCtasSmall = 4;    // to an SM, with moments in 32 and in 8 bits
+// SMs do not all run at one speed: 64 times as many CTAs are launched at most, of a few tiles each (one tile to a CTA where there are
+// fewer).  202M elements with 8-bit moments took 597 us with the CTAs that stay and 565 so, 240 x 40960 with 32-bit ones 46 and 43, 12.6M
+// of fp16 with copies and 8-bit moments 56 and 44.
+constexpr int kDealt = 64;
 constexpr int kNormCtas = 8;                // of the norm's
 constexpr int kMost = 640;                  // tensors of a launch: 25 KB of its 32 KB of parameters
 
@@ -625,7 +629,7 @@ int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count
       if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (rest == REST_16) kern = small ? adamw_step<T, true, REST_16, CAP> : adamw_step<T, false, REST_16, CAP>;
       if (kern == nullptr) return (int)cudaErrorInvalidValue;
-      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * (small ? kCtasSmall : kCtas))), dim3(kNT), 0, s, true, tab, a);
+      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * (small ? kCtasSmall : kCtas) * kDealt)), dim3(kNT), 0, s, true, tab, a);
     });
     if (rc != 0) return rc;
   }

@@ -620,10 +620,18 @@ __global__ void __launch_bounds__(kNT, kGradCtas) row_grads(GradArgs a) {
 // ------------------------------------------------------------------------------------------------ host
 int elem_of(int dtype) { return dtype == DT_F32 ? 4 : 2; }
 
-int grid_of(int64_t rows, int V, int elem, int per_sm) {
-  const int sms = sm_count();
+// CTAs that stay, or as many as there are batches for.
+int grid_of(int64_t rows, int V, int elem, int64_t most) {
   const int64_t batches = rows * batches_of(V, 16 / elem), ctas = (batches + kNT / 32 - 1) / (kNT / 32);
-  return (int)(ctas < (int64_t)sms * per_sm ? ctas : (int64_t)sms * per_sm);
+  return (int)(ctas < most ? ctas : most);
+}
+
+// CTAs of the backward pass: SMs do not all run at one speed, so that more are launched than stay, up to eight times as many, while
+// each warp still has eight batches (2042 rows of 128256: 148 us with those that stay, 139 with four times as many, 133 with eight;
+// 2048 of 32000: 35.8, 35.8 and 37.7, and 35.2 with twice as many).  The sums gain nothing (69 to 72 us): their ends cost more.
+int grad_grid_of(int64_t rows, int V, int elem) {
+  const int64_t stay = (int64_t)sm_count() * kGradCtas, times = rows * batches_of(V, 16 / elem) / (stay * (kNT / 32) * 8);
+  return grid_of(rows, V, elem, stay * (times < 1 ? 1 : times > 8 ? 8 : times));
 }
 
 // The first two kernels; then `a` is ready for the third.
@@ -632,7 +640,7 @@ int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
   list_rows<<<1, kListNT, 0, s>>>(a.targets, a.n, ignore, a.keep);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
-  const int grid = grid_of(a.n, a.rows.V, elem_of(dtype), kCtas);
+  const int grid = grid_of(a.n, a.rows.V, elem_of(dtype), (int64_t)sm_count() * kCtas);
   a.warps = grid * (kNT / 32);
   a.per = batches_of(a.rows.V, 16 / elem_of(dtype));
   const SumArgs sums = {a.rows, a.n, a.keep, const_cast<float2*>(a.part), a.inv_t};
@@ -644,7 +652,7 @@ int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
 int backward(const GradArgs& a, int dtype, cudaStream_t s) {
   if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
   return by_type(dtype, [&](auto* tag) {
-    row_grads<std::remove_pointer_t<decltype(tag)>><<<grid_of(a.n, a.rows.V, elem_of(dtype), kGradCtas), kNT, 0, s>>>(a);
+    row_grads<std::remove_pointer_t<decltype(tag)>><<<grad_grid_of(a.n, a.rows.V, elem_of(dtype)), kNT, 0, s>>>(a);
     return (int)cudaGetLastError();
   });
 }
