@@ -33,10 +33,11 @@ constexpr int kBlock = 256;                 // elements with a common exponent: 
 static_assert(kBlock == 32 * kVec, "a warp has a block");
 constexpr int kLow = 32, kHigh = 254;       // exponents of a block: 2^(e - 127)
 constexpr int kCtas = 3, kCtasSmall = 4;    // to an SM, with moments in 32 and in 8 bits
-// SMs do not all run at one speed: 64 times as many CTAs are launched at most, of a few tiles each (one tile to a CTA where there are
-// fewer).  202M elements with 8-bit moments took 597 us with the CTAs that stay and 565 so, 240 x 40960 with 32-bit ones 46 and 43, 12.6M
-// of fp16 with copies and 8-bit moments 56 and 44.
-constexpr int kDealt = 64;
+// SMs do not all run at one speed: 32 times as many CTAs are launched at most, of a few tiles each (one tile to a CTA where there are
+// fewer).  202M elements with 8-bit moments took 597 us with the CTAs that stay and 547 so, 240 x 40960 with 32-bit ones 46 and 43, 12.6M
+// of fp16 with copies and 8-bit moments 56 and 44.  A CTA's tiles lie far apart: with two neighbours to a CTA, what is read at a time has
+// gaps, and the first of these took 1210 us.
+constexpr int kDealt = 32;
 constexpr int kNormCtas = 8;                // of the norm's
 constexpr int kMost = 640;                  // tensors of a launch: 25 KB of its 32 KB of parameters
 
@@ -241,7 +242,7 @@ __device__ __noinline__ int finite_exponent(Pair a, Pair b, Pair c, Pair d) {
 // format's, adding random bits below the last kept place and cutting there rounds it up with the probability of what is cut off.
 // The codes, in the uppermost bytes.
 __device__ __forceinline__ uint32_t to_e4m3(float x, float scaled, uint32_t chance) {
-  const uint32_t t = (__float_as_uint(scaled) + ((chance << 4 & 0xFFFF0u) | 8u)) << 4;    // its sign is shifted out
+  const uint32_t t = (__float_as_uint(scaled) + (chance << 4 & 0xFFFF0u) + 8u) << 4;      // its sign is shifted out
   return t | (__float_as_uint(x) & 0x80000000u);
 }
 __device__ __forceinline__ uint32_t to_e5m2(float x, float scaled, uint32_t chance) {
