@@ -65,9 +65,13 @@ struct __align__(16) Factors {
   int usual;                          // whether change_usual() holds, as far as they go
 };
 
+// A hash: multiplications by the fractions of the roots of 3 and 2, upper bits brought down before each and behind them.
+__device__ __forceinline__ uint32_t almost_mixed(uint32_t x) {
+  x = (x ^ (x >> 16)) * 0xBB67AE85u;
+  return (x ^ (x >> 15)) * 0x6A09E667u;
+}
 __device__ __forceinline__ uint32_t mixed(uint32_t x) {
-  x = (x ^ (x >> 16)) * 0xBB67AE85u;                // fractions of the roots of 3 and 2
-  x = (x ^ (x >> 15)) * 0x6A09E667u;
+  x = almost_mixed(x);
   return x ^ (x >> 16);
 }
 
@@ -240,9 +244,10 @@ __device__ __noinline__ int finite_exponent(Pair a, Pair b, Pair c, Pair d) {
 
 // A 32-bit number's bits are its exponent and fraction in a row, whatever its size: scaled so that its exponent field is the small
 // format's, adding random bits below the last kept place and cutting there rounds it up with the probability of what is cut off.
-// The codes, in the uppermost bytes.
+// The codes, in the uppermost bytes; `chance` is the hash but for its last step: that leaves the upper half (v's bits) as it is, and
+// for the lower one (m's) it is taken here, with the shift.
 __device__ __forceinline__ uint32_t to_e4m3(float x, float scaled, uint32_t chance) {
-  const uint32_t t = (__float_as_uint(scaled) + (chance << 4 & 0xFFFF0u) + 8u) << 4;      // its sign is shifted out
+  const uint32_t t = (__float_as_uint(scaled) + ((chance << 4 ^ chance >> 12) & 0xFFFF0u) + 8u) << 4;      // its sign is shifted out
   return t | (__float_as_uint(x) & 0x80000000u);
 }
 __device__ __forceinline__ uint32_t to_e5m2(float x, float scaled, uint32_t chance) {
@@ -411,7 +416,7 @@ struct Eight {
         const float up_m = pow2(14 - e), up_v = pow2(29 - h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t c0 = mixed(first + 2 * k * 0x9E3779B1u), c1 = mixed(first + (2 * k + 1) * 0x9E3779B1u);
+          const uint32_t c0 = almost_mixed(first + 2 * k * 0x9E3779B1u), c1 = almost_mixed(first + (2 * k + 1) * 0x9E3779B1u);
           const Pair sv = mul2(vv[k], both(up_v)), sm = mul2(mm[k], both(up_m));
           tm[2 * k] = to_e4m3(mm[k].x, sm.x, c0);
           tm[2 * k + 1] = to_e4m3(mm[k].y, sm.y, c1);
@@ -423,7 +428,7 @@ struct Eight {
         h = finite_exponent(vv[0], vv[1], vv[2], vv[3]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t c0 = mixed(first + 2 * k * 0x9E3779B1u), c1 = mixed(first + (2 * k + 1) * 0x9E3779B1u);
+          const uint32_t c0 = almost_mixed(first + 2 * k * 0x9E3779B1u), c1 = almost_mixed(first + (2 * k + 1) * 0x9E3779B1u);
           tm[2 * k] = to_e4m3_any(mm[k].x, e, c0);
           tm[2 * k + 1] = to_e4m3_any(mm[k].y, e, c1);
           tv[2 * k] = to_e5m2_any(vv[k].x, h, c0);
