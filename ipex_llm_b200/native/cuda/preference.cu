@@ -31,7 +31,7 @@ constexpr int kU = 4;                       // vectors of a lane in a batch
 constexpr int kBatch = 32 * kU;             // vectors of a batch
 constexpr int kCtas = 4, kGradCtas = 3;     // to an SM
 constexpr int kRun = 16;                    // batches of a warp's run, at most where a warp has many
-constexpr int kSlots = 18;                  // runs that may have a part in a row
+constexpr int kSlots = 18;                  // runs that may have a part in a row, at most; one of its batches each
 
 // What the forward pass keeps: the rows with a target, then those without, and each row's place among the former (-1: none); the
 // largest logit and 1 / sum of each listed row; how a listed row's loss (policy) or a sequence's (preference) moves with its log p.
@@ -70,6 +70,8 @@ struct Deal {
   __device__ int64_t runs() const { return (total + len - 1) / len; }
   __device__ int64_t run_of(int place) const { return (int64_t)place * per / len; }   // the first one with a part in a row
 };
+
+__host__ __device__ inline int slots_of(int per) { return per < kSlots ? per : kSlots; }
 
 __host__ __device__ inline int batches_of(int V, int vec) {
   const int nvec = V / vec;
@@ -139,8 +141,8 @@ __global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int
 
 // ------------------------------------------------------------------------------------------------ sums
 // A lane's part of a row: the sum of 2^(c x - r), r of a logit that none passes by more than 2^kSlack times its share.  It moves, and
-// the sum with it, only when one does: a sum's error is relative, wherever r lies.
-constexpr float kSlack = 16.f;
+// the sum with it, only when one does (with sixteen octaves, the largest terms' exponents lost a place of the result: 7e-7).
+constexpr float kSlack = 4.f;
 struct Part {
   Base base;
   float s;
@@ -220,7 +222,7 @@ struct SumArgs {
   Rows rows;
   int64_t n;
   const void* keep;
-  float2* part;        // [places, kSlots]
+  float2* part;        // [places, slots_of(batches of a row)]
   float inv_t;
 };
 
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(kNT, kCtas) row_sums(SumArgs a) {
       float s = p.s * ex2(shift(p.base, Base(m, c), c));
 #pragma unroll
       for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0) a.part[(int64_t)place * kSlots + (int)(run - deal.run_of(place))] = make_float2(m, s);
+      if (lane == 0) a.part[(int64_t)place * slots_of(deal.per) + (int)(run - deal.run_of(place))] = make_float2(m, s);
     }
   }
 }
@@ -295,7 +297,7 @@ __device__ __forceinline__ double row_logprob(const RowArgs& a, const Keep& k, c
   const bool bad = t < 0 || t >= a.rows.V;
   const float xt = bad ? 0.f : DT<T>::to_f(row_at<T>(a.rows, row)[t]);
   const int parts = (int)(((int64_t)(place + 1) * deal.per - 1) / deal.len - deal.run_of(place)) + 1;
-  const float2* at = a.part + (int64_t)place * kSlots;
+  const float2* at = a.part + (int64_t)place * slots_of(deal.per);
   float2 p[kSlots];
   Stat st = {-INFINITY, 0.f, 0.f};
 #pragma unroll
@@ -667,7 +669,9 @@ bool args_ok(const void* logits, int64_t s0, int64_t s1, int64_t n1, int64_t row
 
 // Bytes that the forward pass keeps for the backward one, and those that it works in.
 IPEX_API int64_t ipex_preference_keep_bytes(int64_t rows) { return keep_bytes(rows); }
-IPEX_API int64_t ipex_preference_work_bytes(int64_t rows) { return rows * kSlots * (int64_t)sizeof(float2); }
+IPEX_API int64_t ipex_preference_work_bytes(int64_t rows, int V, int dtype) {
+  return rows * slots_of(batches_of(V, 16 / elem_of(dtype))) * (int64_t)sizeof(float2);
+}
 
 // logits: rows of V elements, row r at (r / n1) * s0 + (r % n1) * s1; targets [rows] (`ignore`: none, all results 0); old, ref [rows] or
 // null; advantage of row r at (r / inner) * adv0 + (r % inner) * adv1; loss, logprob, kl (0 without ref), clipped [rows].  A target

@@ -196,8 +196,9 @@ _SCRATCH_FLOATS = {"delta": ("ipex_delta_scratch_floats",), "general_delta": ("i
                    "linear": ("ipex_linear_scratch_floats",), "ssd": ("ipex_ssd_group_floats", "ipex_ssd_head_floats")}
 
 
-# room that a call needs: count -> how much
-SIZES = {"adamw": ("ipex_grad_norm_sums",), "preference": ("ipex_preference_keep_bytes", "ipex_preference_work_bytes")}
+# how much room a call needs
+SIZES = {"adamw": {"ipex_grad_norm_sums": [i64]},
+         "preference": {"ipex_preference_keep_bytes": [i64], "ipex_preference_work_bytes": [i64, ci, ci]}}
 
 
 def declare_component(lib: ctypes.CDLL, name: str):
@@ -206,9 +207,9 @@ def declare_component(lib: ctypes.CDLL, name: str):
         fn.argtypes, fn.restype = args, ci
     if name == "stream":
         lib.ipex_gemv_rows_tune.argtypes, lib.ipex_gemv_rows_tune.restype = [ci], None
-    for fn_name in SIZES.get(name, ()):
+    for fn_name, args in SIZES.get(name, {}).items():
         fn = getattr(lib, fn_name)
-        fn.argtypes, fn.restype = [i64], i64
+        fn.argtypes, fn.restype = args, i64
     for fn_name in _SCRATCH_FLOATS.get(name, ()):
         fn = getattr(lib, fn_name)
         fn.argtypes, fn.restype = [ci, ci], i64

@@ -31,6 +31,7 @@ using AdamwStep = int (*)(const int64_t*, const int64_t*, const int64_t*, int64_
                           void*);
 using GradNorm = int (*)(const int64_t*, const int64_t*, int64_t, double*, float*, int, void*);
 using Size = int64_t (*)(int64_t);
+using RowSize = int64_t (*)(int64_t, int, int);
 using PolicyLoss = int (*)(const void*, int64_t, int64_t, int64_t, const int64_t*, const float*, const float*, const float*, int64_t,
                            int64_t, int64_t, float*, float*, float*, uint8_t*, void*, void*, int64_t, int, int64_t, double, double, double,
                            float, int, int*, void*);
@@ -44,7 +45,8 @@ using PreferenceGrad = int (*)(const void*, int64_t, int64_t, int64_t, const int
 struct Entries {
   AdamwStep adamw_step = nullptr;
   GradNorm grad_norm = nullptr;
-  Size grad_norm_sums = nullptr, keep_bytes = nullptr, work_bytes = nullptr;
+  Size grad_norm_sums = nullptr, keep_bytes = nullptr;
+  RowSize work_bytes = nullptr;
   PolicyLoss policy_loss = nullptr;
   PolicyGrad policy_grad = nullptr;
   PreferenceLoss preference_loss = nullptr;
@@ -232,9 +234,10 @@ struct Preference : torch::autograd::Function<Preference> {
     const c10::cuda::OptionalCUDAGuard guard(dev);
     const Rows r(logits);
     const int64_t n = logits.size(0), tokens = logits.size(1);
+    const int type = type_code(logits.scalar_type());
     const at::TensorOptions opt = at::TensorOptions().dtype(at::kFloat).device(dev);
     Tensor loss = at::empty({n / 2}, opt), logprob = at::empty({n}, opt);
-    const Tensor keep = bytes(entries.keep_bytes(n * tokens), dev), work = bytes(entries.work_bytes(n * tokens), dev);
+    const Tensor keep = bytes(entries.keep_bytes(n * tokens), dev), work = bytes(entries.work_bytes(n * tokens, (int)logits.size(2), type), dev);
     check(entries.preference_loss(r.x.data_ptr(), r.s0, r.s1, r.n1, targets.data_ptr<int64_t>(), at_of<const float>(reference),
                                   loss.data_ptr<float>(), logprob.data_ptr<float>(), keep.data_ptr(), work.data_ptr(), (int)(n / 2), tokens,
                                   (int)logits.size(2), ignore, (int)form, average, beta, smooth, margin, (float)temperature,
@@ -283,7 +286,7 @@ struct Policy : torch::autograd::Function<Policy> {
     Tensor clipped = at::empty(targets.sizes(), opt.dtype(at::kBool));
     const Tensor keep = bytes(entries.keep_bytes(rows), dev);
     if (rows > 0) {
-      const Tensor work = bytes(entries.work_bytes(rows), dev);
+      const Tensor work = bytes(entries.work_bytes(rows, (int)logits.size(-1), type_code(logits.scalar_type())), dev);
       const PerRow a(advantages, targets.sizes());
       check(entries.policy_loss(r.x.data_ptr(), r.s0, r.s1, r.n1, targets.data_ptr<int64_t>(), at_of<const float>(old),
                                 at_of<const float>(ref), a.t.data_ptr<float>(), a.s0, a.s1, a.inner, loss.data_ptr<float>(),

@@ -77,6 +77,8 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
     _check_logits(logits, temperature, what)
     if logits.dim() != 3 or logits.shape[0] % 2 or not logits.shape[0]:
         invalidInputError(False, f"{what}: logits should be [2 pairs, tokens, vocabulary], got {tuple(logits.shape)}")
+    if not logits.shape[1]:
+        invalidInputError(False, f"{what}: no tokens")
     _check_like(targets, logits.shape[:2], logits.device, f"{what}: targets", True)
     if reference is not None:
         _check_like(reference, logits.shape[:1], logits.device, f"{what}: reference", False)
@@ -89,8 +91,6 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
         invalidInputError(False, f"{what}: label_smoothing and margin belong to the form 'sigmoid'")
     if logits.is_cuda:
         refuse_tangents(what, logits)
-        if not logits.shape[1]:
-            invalidInputError(False, f"{what}: no tokens")
         return PreferenceLoss(*calls().preference(
             logits, targets.to(torch.int64).contiguous(), None if reference is None else reference.detach().float().contiguous(),
             beta, FORMS.index(form), label_smoothing, margin, average, temperature, ignore_index, error_flag(logits.device).data_ptr()))

@@ -156,6 +156,34 @@ def test_norm_of_views():
     assert float(adamw.grad_norm([x[:0], None])) == 0.0 and float(adamw.grad_norm([None])) == 0.0
 
 
+@pytest.mark.parametrize("eps,exponents", [(1e-8, (-149, 60)), (1e-8, (-149, 127)), (2.0 ** -38, (-149, 60)), (1e-12, (-149, 100)),
+                                           (0.0, (-100, 60)), (1.0, (-20, 20))])
+def test_roots_and_quotients_are_the_nearest_numbers(eps, exponents):
+    """Moments of every size, none, and not finite: what the kernel takes for roots and divisions against the library's, bit by bit.
+    Gradients of 0 and betas of a half leave half of each moment; parameters of 0 show the change."""
+    n = 1 << 22
+    g = torch.Generator(device="cuda").manual_seed(int(eps * 1e9) + exponents[1])
+    size = lambda lo, hi: torch.exp2(torch.rand(n, generator=g, device="cuda") * (hi - lo) + lo)      # noqa: E731
+    v = size(*exponents)
+    m = size(-60, min(exponents[1], 58)) * torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    v[:1000], m[500:1500] = 0.0, 0.0
+    if exponents[1] > 100:
+        v[2000], v[3000], m[4000], m[5000] = math.inf, math.nan, math.inf, math.nan
+    p, zero = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    state = adamw.adamw_state([p])
+    state.exp_avg.copy_(m)
+    state.exp_avg_sq.copy_(v)
+    state.step.fill_(2)
+    _step([p], [zero], state, betas=(0.5, 0.5), eps=eps, weight_decay=0.0)
+    rate = torch.tensor(KW["lr"] / (1 - 0.5 ** 3), dtype=torch.float64).float().cuda()
+    root = torch.tensor(1 / math.sqrt(1 - 0.5 ** 3), dtype=torch.float64).float().cuda()
+    m1, v1 = m * 0.5, v * 0.5
+    want = zero - (m1 * rate) / (v1.sqrt() * root + eps)
+    _same(p, want, "change")
+    _same(state.exp_avg, m1, "m")
+    _same(state.exp_avg_sq, v1, "v")
+
+
 def test_captured_steps_count_on():
     """Replays take the step counter, the rate and the gradients as they are then; two graphs of the same parameters, and an eager
     step between them, share nothing but the state."""

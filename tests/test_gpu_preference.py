@@ -344,6 +344,32 @@ def test_rows_past_32_bits():
     assert int((dx != 0).sum()) == 2 * V
 
 
+def test_a_gradients_gradient_is_refused():
+    x, t = torch.randn(2, 3, 9, device="cuda", requires_grad=True), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
+    for call in (lambda: preference_loss(x, t).loss, lambda: policy_loss(x, t, torch.ones(2, 3, device="cuda")).loss):
+        want, = torch.autograd.grad(call().sum(), x)
+        dx, = torch.autograd.grad(call().sum(), x, create_graph=True)
+        assert torch.equal(dx.detach(), want)
+        with pytest.raises(RuntimeError, match="used in the graph"):
+            torch.autograd.grad(dx.sum(), x, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            dx.sum().backward()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 5])
+def test_a_dominant_token_among_many(rows):
+    """One logit 60 octaves above thousands that come before it, and after it: the sums' reference moves once, or not at all."""
+    g = _gen(rows)
+    x = _logits((2, rows, 40000), torch.float32, g)
+    t = torch.randint(0, 40000, (2, rows), generator=g, device="cuda")
+    for at in (0, 20011, 39999):
+        y = x.clone()
+        y[:, :, at] += 42.0
+        _check_preference(y, t)
+        y[:, :, at] = 9.0                                  # a few octaves above the largest others
+        _check_preference(y, torch.full_like(t, at))
+
+
 def test_tangents_are_refused():
     from torch.autograd import forward_ad
     x, t = torch.randn(2, 3, 9, device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda")

@@ -159,6 +159,7 @@ def test_refusals():
     refused("2 pairs", x[:3], t[:3])
     refused("2 pairs", x[0], t[0])
     refused("2 pairs", x[:0], t[:0])
+    refused("no tokens", x[:, :0], t[:, :0])
     refused("targets should have shape", x, t[:, :3])
     refused("targets should hold token ids", x, t.float())
     refused("reference should have shape", x, t, ref[:2])
