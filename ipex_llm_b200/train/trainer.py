@@ -74,6 +74,11 @@ class Trainer:
         self.rank = dist.get_rank() if dist.is_initialized() else 0
         self.world = dist.get_world_size() if dist.is_initialized() else 1
         self.device = next(p for p in model.parameters()).device
+        pairs = bool(getattr(args, "preference_form", None))
+        invalidInputError(not pairs or getattr(args, "fused_loss", False), "preference_form needs fused_loss=True")
+        if not pairs and data_collator is None and train_dataset is not None and len(train_dataset):
+            first = train_dataset[0]
+            invalidInputError(not (isinstance(first, dict) and "chosen_input_ids" in first), "pairs of samples need preference_form")
 
     # ------------------------------------------------------------------------------------------------
     def create_optimizer(self):

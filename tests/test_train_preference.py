@@ -153,6 +153,12 @@ def test_trainer_refuses(tmp_path):
     model = _adapters()
     plain = torch.nn.Module()
     plain.register_parameter("w", torch.nn.Parameter(torch.zeros(1)))
+    with pytest.raises(RuntimeError, match="pairs of samples need"):
+        Trainer(model, _args(tmp_path), train_dataset=data)
+    plain_loss = _args(tmp_path, preference_form="ipo")
+    plain_loss.fused_loss = False
+    with pytest.raises(RuntimeError, match="needs fused_loss"):
+        Trainer(model, plain_loss, train_dataset=data)
     tr = Trainer(model, _args(tmp_path, preference_form="ipo"), train_dataset=data)
     with pytest.raises(RuntimeError, match="disable_adapter|adapters"):
         tr._preference_loss(plain, {"labels": torch.zeros(2, 3, dtype=torch.int64)})
@@ -259,3 +265,31 @@ def test_trainer_resumes_with_it(tmp_path):
     for (k, a), (_, b) in zip(one.state_dict().items(), two.state_dict().items()):
         if "lora_" in k:
             assert torch.equal(a, b), k
+
+
+def test_layers_that_take_turns(tmp_path):
+    """Layer-wise sampling: layers without a gradient stay, moments and step counters too."""
+    from ipex_llm.transformers.lisa import DynamicLayerActivationCallback
+    from transformers import LlamaConfig, LlamaForCausalLM
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(LlamaConfig(hidden_size=32, intermediate_size=64, num_hidden_layers=3, num_attention_heads=2,
+                                         num_key_value_heads=2, vocab_size=64, tie_word_embeddings=False))
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    data = [{"input_ids": torch.randint(0, 64, (9,), generator=_gen(i)).tolist()} for i in range(8)]
+    args = _args(tmp_path, optim="adamw_8bit")
+    args.max_steps = 2
+    turns = DynamicLayerActivationCallback(n_layers=1, interval_steps=1, model=model, seed=1)
+    tr = Trainer(model, args, train_dataset=data, callbacks=[turns])
+    tr.create_optimizer()
+    seen = set()
+    turns.switch = turns.switch_active_layers
+    turns.switch_active_layers = lambda: (turns.switch(), seen.update(turns.active_layers_indices))
+    tr.train()
+    (b,) = tr.optimizer.buckets()
+    for (name, p), steps in zip(((n, p) for n, p in model.named_parameters()), b["state"].step.tolist()):
+        layer = int(name.split(".")[2]) if ".layers." in name else None
+        if layer is None:
+            assert steps == 2
+        else:
+            assert (steps > 0) == (layer in seen)
+            assert torch.equal(p, before[name]) == (layer not in seen), name
