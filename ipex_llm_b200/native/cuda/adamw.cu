@@ -96,7 +96,8 @@ struct BeginArgs {
 
 template <int CAP>
 __global__ void adamw_begin(const __grid_constant__ Table<CAP> tab, BeginArgs a) {
-  pdl_launch_dependents();
+  pdl_wait();
+  pdl_launch_dependents();      // not before the wait: the step's first loads do not wait for more than this launch's begin
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= tab.n) return;
   const int at = tab.e[i].step;
@@ -507,6 +508,7 @@ __global__ void __launch_bounds__(kNT, SMALL ? kCtasSmall : kCtas) adamw_step(co
 template <typename T, int CAP>
 __global__ void __launch_bounds__(kNT) grad_squares(const __grid_constant__ Table<CAP> tab, double* sums) {
   __shared__ double part[kNT / 32];
+  pdl_wait();
   pdl_launch_dependents();
   double total = 0.0;
   int i = 0;
@@ -621,8 +623,14 @@ int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count
     if (at < 0) return (int)cudaErrorInvalidValue;
     if (tab.n == 0) continue;
     if (!begun || steps > 1) {                      // a common counter moves once
-      adamw_begin<CAP><<<(tab.n + 127) / 128, 128, 0, s>>>(tab, b);
-      const cudaError_t e = cudaGetLastError();
+      cudaError_t e;
+      if (steps > 1) {
+        e = launch_kernel(adamw_begin<CAP>, dim3((tab.n + 127) / 128), dim3(128), 0, s, true, tab, b);
+      } else {                                      // and needs no table: 25 KB of parameters less
+        Table<1> one = {};
+        one.n = 1;
+        e = launch_kernel(adamw_begin<1>, dim3(1), dim3(32), 0, s, true, one, b);
+      }
       if (e != cudaSuccess) return (int)e;
       begun = true;
     }
@@ -655,8 +663,7 @@ int norm_all(const int64_t* g, const int64_t* n, int64_t count, double* sums, fl
     if (tab.n == 0) continue;
     const int grid = grid_of(tab.tiles, sms * kNormCtas);
     const int rc = by_type(dtype, [&](auto* tag) {
-      grad_squares<std::remove_pointer_t<decltype(tag)>, CAP><<<grid, kNT, 0, s>>>(tab, sums + parts);
-      return (int)cudaGetLastError();
+      return (int)launch_kernel(grad_squares<std::remove_pointer_t<decltype(tag)>, CAP>, dim3(grid), dim3(kNT), 0, s, true, tab, sums + parts);
     });
     if (rc != 0) return rc;
     parts += grid;

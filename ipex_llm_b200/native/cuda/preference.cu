@@ -96,6 +96,7 @@ constexpr int kListNT = 1024, kListRows = 4;
 
 __global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int64_t rows, int64_t ignore, void* keep) {
   __shared__ int sums[kListNT / 32];
+  pdl_wait();
   pdl_launch_dependents();
   const Keep k = keep_at(keep, rows);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -519,6 +520,7 @@ __global__ void __launch_bounds__(kNT, kGradCtas) row_grads(GradArgs a) {
   const int lane = threadIdx.x & 31, warps = gridDim.x * (kNT / 32), warp = blockIdx.x * (kNT / 32) + (threadIdx.x >> 5);
   const Keep k = keep_at(const_cast<void*>(a.keep), a.n);
   const float c = a.inv_t * kLog2e;
+  pdl_wait();
   const int V = a.rows.V, count = *k.count;
   T* dx = reinterpret_cast<T*>(a.dx);
   const Deal deal(count, batches_of(V, VEC), warps);
@@ -639,8 +641,7 @@ int grad_grid_of(int64_t rows, int V, int elem) {
 // The first two kernels; then `a` is ready for the third.
 int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
   if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
-  list_rows<<<1, kListNT, 0, s>>>(a.targets, a.n, ignore, a.keep);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_kernel(list_rows, dim3(1), dim3(kListNT), 0, s, true, a.targets, a.n, ignore, a.keep);
   if (e != cudaSuccess) return (int)e;
   const int grid = grid_of(a.n, a.rows.V, elem_of(dtype), (int64_t)sm_count() * kCtas);
   a.warps = grid * (kNT / 32);
@@ -654,8 +655,8 @@ int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
 int backward(const GradArgs& a, int dtype, cudaStream_t s) {
   if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
   return by_type(dtype, [&](auto* tag) {
-    row_grads<std::remove_pointer_t<decltype(tag)>><<<grad_grid_of(a.n, a.rows.V, elem_of(dtype)), kNT, 0, s>>>(a);
-    return (int)cudaGetLastError();
+    return (int)launch_kernel(row_grads<std::remove_pointer_t<decltype(tag)>>, dim3(grad_grid_of(a.n, a.rows.V, elem_of(dtype))), dim3(kNT),
+                              0, s, true, a);
   });
 }
 
