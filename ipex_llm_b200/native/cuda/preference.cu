@@ -12,10 +12,12 @@
 //
 // Prompts and padding have no target: their logits are never read.  A first kernel lists the rows that have one; the second reads
 // them: batches of 32 x 4 vectors of 16 bytes, all rows' behind one another, are dealt to the warps in equal runs, whatever rows
-// they belong to, so that no warp waits for another and none has more to do; a run leaves the maximum and the sum of each row that
-// it touches.  The third joins those of a row (up to kSlots) and does what comes behind them, in 64 bits.  The backward pass deals
-// its batches the same way, from the last row to the first, whose logits are still in L2, then the rows without a target, which it
-// only writes.  All of it is bound by memory.
+// they belong to, so that no warp waits for another and none has more to do; a run leaves a sum, and what its exponents were taken
+// from, for each row that it touches.  The third joins those of a row (up to kSlots) and does what comes behind them, in 64 bits.  The
+// backward pass deals its batches the same way, from the last row to the first, then the rows without a target, which it only writes.
+// All of it is bound by memory: 2042 rows of 128256 in bf16, 1329 of them with a target, take 70 us for the sums (341 MB, and what the
+// pass before has left in L2 to be written: 6.3 TB/s) and 133 us for the gradient (865 MB: 6.5 TB/s; writes alone reach 3.9); 2048 of
+// 32000, 1287 of them with one, 21 and 35.
 #include <cooperative_groups.h>
 
 #include "common/logit_rows.cuh"
@@ -34,7 +36,8 @@ constexpr int kRun = 16;                    // batches of a warp's run, at most 
 constexpr int kSlots = 18;                  // runs that may have a part in a row, at most; one of its batches each
 
 // What the forward pass keeps: the rows with a target, then those without, and each row's place among the former (-1: none); the
-// largest logit and 1 / sum of each listed row; how a listed row's loss (policy) or a sequence's (preference) moves with its log p.
+// what a listed row's exponents are taken from, and 1 / its sum; how a listed row's loss (policy) or a sequence's (preference) moves
+// with its log p.
 struct Keep {
   int* count;
   int* list;
@@ -60,7 +63,7 @@ constexpr int64_t keep_bytes(int64_t rows) { return 16 + 24 * ((rows + 3) / 4 * 
 // How the batches of `count` rows of `per` each are dealt to `warps`: runs of `len`.
 struct Deal {
   int64_t total;
-  int per, len, first;
+  int per, len;
   __device__ Deal(int count, int per_, int warps) : total((int64_t)count * per_), per(per_) {
     const int64_t rounds = max((int64_t)1, (total + (int64_t)warps * kRun - 1) / ((int64_t)warps * kRun));
     const int least = per / (kSlots - 2) + 1;                     // so that kSlots runs reach through a row

@@ -2,8 +2,8 @@
 // hundreds of tensors, and the backward passes (a node of the autograd graph in C++ needs no interpreter on autograd's thread).
 // The kernels' addresses come from the library that ctypes has loaded (`bind`), so that there is one of them in a process.
 //
-// Arguments are checked by the callers in Python, which name what is wrong; where a list holds anything out of the ordinary (another
-// type, device or order of memory, a tensor twice), the functions here answer so and do nothing.
+// Where an argument is not as it should be, or a list holds anything out of the ordinary (another type, device or order of memory, a
+// tensor twice), the functions here answer so and do nothing; their callers in Python name what is wrong, or put it right.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -13,7 +13,9 @@
 #include <torch/types.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
+#include <tuple>
 #include <unordered_map>
 #include <vector>
 
@@ -326,20 +328,61 @@ struct Policy : torch::autograd::Function<Policy> {
   }
 };
 
+// Whether arguments are as the documentation asks for; else the caller finds out what is wrong with them.
+bool logits_fit(const Tensor& x, double temperature) {
+  return x.is_cuda() && x.layout() == at::kStrided && type_code(x.scalar_type()) >= 0 && x.dim() >= 1 && x.size(-1) >= 1 &&
+         x.size(-1) <= (int64_t)1 << 30 && x.numel() / x.size(-1) <= (int64_t)1 << 27 && temperature >= 1e-6 && temperature <= 1e6;
+}
+bool targets_fit(const Tensor& t, at::IntArrayRef shape, const Tensor& x) {
+  return t.device() == x.device() && t.layout() == at::kStrided && at::isIntegralType(t.scalar_type(), false) &&
+         t.sizes() == shape;
+}
+bool numbers_fit(const std::optional<Tensor>& t, at::IntArrayRef shape, const Tensor& x) {
+  return !t || (t->device() == x.device() && t->layout() == at::kStrided && t->is_floating_point() && t->sizes() == shape);
+}
+Tensor whole(const Tensor& t) { return t.scalar_type() == at::kLong && t.is_contiguous() ? t : t.to(at::kLong).contiguous(); }
+Tensor single(const Tensor& t) {      // a constant, in 32 bits
+  const Tensor d = t.requires_grad() ? t.detach() : t;
+  return d.scalar_type() == at::kFloat ? d : d.to(at::kFloat);
+}
+std::optional<Tensor> single(const std::optional<Tensor>& t) {
+  return t ? std::optional<Tensor>(single(*t).contiguous()) : std::nullopt;
+}
+
+std::optional<std::tuple<Tensor, Tensor>> preference(const Tensor& logits, const Tensor& targets, const std::optional<Tensor>& reference,
+                                                     double beta, int64_t form, double smooth, double margin, bool average,
+                                                     double temperature, int64_t ignore, int64_t err) {
+  if (!logits_fit(logits, temperature) || logits.dim() != 3 || logits.size(0) < 2 || logits.size(0) % 2 || logits.size(1) < 1 ||
+      !targets_fit(targets, logits.sizes().slice(0, 2), logits) || !numbers_fit(reference, logits.sizes().slice(0, 1), logits) || form < 0 ||
+      !(beta > 0.0 && beta < INFINITY && smooth >= 0.0 && smooth <= 1.0 && std::isfinite(margin)) ||
+      (form > 0 && (smooth != 0.0 || margin != 0.0)))
+    return std::nullopt;
+  const auto out = Preference::apply(logits, whole(targets), single(reference), beta, form, smooth, margin, average, temperature, ignore, err);
+  return std::make_tuple(out[0], out[1]);
+}
+
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> policy(const Tensor& logits, const Tensor& targets, const Tensor& advantages,
+                                                                 const std::optional<Tensor>& old, const std::optional<Tensor>& ref,
+                                                                 double lo, double hi, double weight, double temperature, int64_t ignore,
+                                                                 int64_t err) {
+  if (!logits_fit(logits, temperature)) return std::nullopt;
+  const at::IntArrayRef shape = logits.sizes().slice(0, logits.dim() - 1);
+  if (!targets_fit(targets, shape, logits) || !numbers_fit(old, shape, logits) || !numbers_fit(ref, shape, logits) ||
+      !numbers_fit(advantages, advantages.sizes(), logits) || advantages.dim() > (int64_t)shape.size() ||
+      !(lo >= 0.0 && lo <= 1.0 && hi >= 0.0 && weight >= 0.0 && weight < INFINITY) || (weight != 0.0 && !ref))
+    return std::nullopt;
+  for (int64_t i = 1; i <= advantages.dim(); ++i)
+    if (advantages.size(-i) != 1 && advantages.size(-i) != shape[shape.size() - i]) return std::nullopt;
+  const auto out = Policy::apply(logits, whole(targets), single(advantages), single(old), single(ref), lo, hi, weight, temperature, ignore, err);
+  return std::make_tuple(out[0], out[1], out[2], out[3]);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(libipex_calls, m) {
   m.def("bind", &bind);
   m.def("adamw_step", &adamw_step);
   m.def("grad_norm", &grad_norm);
-  m.def("preference", [](const Tensor& logits, const Tensor& targets, const std::optional<Tensor>& reference, double beta, int64_t form,
-                         double smooth, double margin, bool average, double temperature, int64_t ignore, int64_t err) {
-    auto out = Preference::apply(logits, targets, reference, beta, form, smooth, margin, average, temperature, ignore, err);
-    return std::make_tuple(out[0], out[1]);
-  });
-  m.def("policy", [](const Tensor& logits, const Tensor& targets, const Tensor& advantages, const std::optional<Tensor>& old,
-                     const std::optional<Tensor>& ref, double lo, double hi, double weight, double temperature, int64_t ignore, int64_t err) {
-    auto out = Policy::apply(logits, targets, advantages, old, ref, lo, hi, weight, temperature, ignore, err);
-    return std::make_tuple(out[0], out[1], out[2], out[3]);
-  });
+  m.def("preference", &preference);
+  m.def("policy", &policy);
 }

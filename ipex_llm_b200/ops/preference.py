@@ -20,6 +20,7 @@ from .gradients import refuse_tangents
 from .token_loss import IGNORE, _check_like, _check_logits, token_logprobs
 
 FORMS = ("sigmoid", "hinge", "ipo")
+_FORM_CODES = {f: i for i, f in enumerate(FORMS)}
 
 
 class PreferenceLoss(NamedTuple):
@@ -74,6 +75,13 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
     reports 61.
     """
     what = "preference_loss"
+    cuda = logits.is_cuda
+    if cuda:
+        refuse_tangents(what, logits)
+        got = calls().preference(logits, targets, reference, beta, _FORM_CODES.get(form, -1), label_smoothing, margin, average, temperature,
+                                 ignore_index, error_flag(logits.device).data_ptr())
+        if got is not None:
+            return PreferenceLoss(*got)
     _check_logits(logits, temperature, what)
     if logits.dim() != 3 or logits.shape[0] % 2 or not logits.shape[0]:
         invalidInputError(False, f"{what}: logits should be [2 pairs, tokens, vocabulary], got {tuple(logits.shape)}")
@@ -89,11 +97,8 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
                                  f"{label_smoothing}, {margin}")
     if form != "sigmoid" and (label_smoothing or margin):
         invalidInputError(False, f"{what}: label_smoothing and margin belong to the form 'sigmoid'")
-    if logits.is_cuda:
-        refuse_tangents(what, logits)
-        return PreferenceLoss(*calls().preference(
-            logits, targets.to(torch.int64).contiguous(), None if reference is None else reference.detach().float().contiguous(),
-            beta, FORMS.index(form), label_smoothing, margin, average, temperature, ignore_index, error_flag(logits.device).data_ptr()))
+    if cuda:
+        invalidInputError(False, f"{what}: these tensors are not supported")
     return _preference_plain(logits, targets, None if reference is None else reference.detach(), beta, form, label_smoothing, margin,
                              average, temperature, ignore_index)
 
@@ -133,6 +138,14 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     the CPU; on the GPU its results are NaN, and ``cuda_ops.check_error_flag`` reports 61.
     """
     what = "policy_loss"
+    lo, hi = float(clip[0]), float(clip[1])
+    cuda = logits.is_cuda
+    if cuda:
+        refuse_tangents(what, logits)
+        got = calls().policy(logits, targets, advantages, old_logprobs, ref_logprobs, lo, hi, kl_weight, temperature, ignore_index,
+                             error_flag(logits.device).data_ptr())
+        if got is not None:
+            return PolicyLoss(*got)
     _check_logits(logits, temperature, what)
     _check_like(targets, logits.shape[:-1], logits.device, f"{what}: targets", True)
     for t, name in ((old_logprobs, "old_logprobs"), (ref_logprobs, "ref_logprobs")):
@@ -145,17 +158,12 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
         m in (1, n) for m, n in zip(reversed(advantages.shape), reversed(targets.shape)))
     if not fits:
         invalidInputError(False, f"{what}: advantages of shape {tuple(advantages.shape)} do not fit targets of {tuple(targets.shape)}")
-    lo, hi = float(clip[0]), float(clip[1])
     if not (0.0 <= lo <= 1.0 and 0.0 <= hi and 0.0 <= kl_weight < math.inf):
         invalidInputError(False, f"{what}: clip should hold a number in [0, 1] and one not below 0, kl_weight be finite and not below 0; "
                                  f"got {clip}, {kl_weight}")
     if kl_weight and ref_logprobs is None:
         invalidInputError(False, f"{what}: kl_weight needs ref_logprobs")
+    if cuda:
+        invalidInputError(False, f"{what}: these tensors are not supported")
     old, ref = (None if t is None else t.detach() for t in (old_logprobs, ref_logprobs))
-    if logits.is_cuda:
-        refuse_tangents(what, logits)
-        return PolicyLoss(*calls().policy(
-            logits, targets.to(torch.int64).contiguous(), advantages.detach().float(), None if old is None else old.float().contiguous(),
-            None if ref is None else ref.float().contiguous(), lo, hi, kl_weight, temperature, ignore_index,
-            error_flag(logits.device).data_ptr()))
     return _policy_plain(logits, targets, advantages.detach(), old, ref, lo, hi, kl_weight, temperature, ignore_index)
