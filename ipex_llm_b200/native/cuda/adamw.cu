@@ -32,9 +32,9 @@ constexpr int kNormParts = 2;               // of a thread's in a tile of the no
 constexpr int kBlock = 256;                 // elements with a common exponent: a warp's
 static_assert(kBlock == 32 * kVec, "a warp has a block");
 constexpr int kLow = 32, kHigh = 254;       // exponents of a block: 2^(e - 127)
-constexpr int kCtas = 3, kCtasSmall = 4;    // to an SM, with moments in 32 and in 8 bits
+constexpr int kCtas = 4;                    // to an SM (three, with more registers, take 3 % longer for 240 x 40960 with 32-bit moments)
 // SMs do not all run at one speed: 32 times as many CTAs are launched at most, of a few tiles each (one tile to a CTA where there are
-// fewer).  202M elements with 8-bit moments took 597 us with the CTAs that stay and 547 so, 240 x 40960 with 32-bit ones 46 and 43, 12.6M
+// fewer).  202M elements with 8-bit moments took 597 us with the CTAs that stay and 547 so, 240 x 40960 with 32-bit ones 46 and 42, 12.6M
 // of fp16 with copies and 8-bit moments 56 and 44.  A CTA's tiles lie far apart: with two neighbours to a CTA, what is read at a time has
 // gaps, and the first of these took 1210 us.
 constexpr int kDealt = 32;
@@ -480,7 +480,7 @@ struct Eight {
 };
 
 template <typename T, bool SMALL, int REST, int CAP>
-__global__ void __launch_bounds__(kNT, SMALL ? kCtasSmall : kCtas) adamw_step(const __grid_constant__ Table<CAP> tab, StepArgs a) {
+__global__ void __launch_bounds__(kNT, kCtas) adamw_step(const __grid_constant__ Table<CAP> tab, StepArgs a) {
   int i = 0;
   bool first = true;
   for (uint32_t tile = blockIdx.x; tile < tab.tiles; tile += gridDim.x) {
@@ -643,7 +643,7 @@ int step_all(const int64_t* p, const int64_t* g, const int64_t* n, int64_t count
       if constexpr (std::is_same<T, __nv_bfloat16>::value)
         if (rest == REST_16) kern = small ? adamw_step<T, true, REST_16, CAP> : adamw_step<T, false, REST_16, CAP>;
       if (kern == nullptr) return (int)cudaErrorInvalidValue;
-      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * (small ? kCtasSmall : kCtas) * kDealt)), dim3(kNT), 0, s, true, tab, a);
+      return (int)launch_kernel(kern, dim3(grid_of(tab.tiles, sms * kCtas * kDealt)), dim3(kNT), 0, s, true, tab, a);
     });
     if (rc != 0) return rc;
   }
