@@ -10,14 +10,15 @@
 // policy: w = e^(log p - old), d = ref - log p,
 //   -min(w A, min(max(w, 1 - lo), 1 + hi) A) + k (e^d - d - 1)      d log p: -A w where w A is the smaller, + k (1 - e^d)
 //
-// Prompts and padding have no target: their logits are never read.  A first kernel lists the rows that have one; the second reads
-// them: batches of 32 x 4 vectors of 16 bytes, all rows' behind one another, are dealt to the warps in equal runs, whatever rows
-// they belong to, so that no warp waits for another and none has more to do; a run leaves a sum, and what its exponents were taken
-// from, for each row that it touches.  The third joins those of a row (up to kSlots) and does what comes behind them, in 64 bits.  The
-// backward pass deals its batches the same way, from the last row to the first, then the rows without a target, which it only writes.
-// All of it is bound by memory: 2042 rows of 128256 in bf16, 1329 of them with a target, take 70 us for the sums (341 MB, and what the
-// pass before has left in L2 to be written: 6.3 TB/s) and 133 us for the gradient (865 MB: 6.5 TB/s; writes alone reach 3.9); 2048 of
-// 32000, 1287 of them with one, 21 and 35.
+// Prompts and padding have no target: their logits are never read.  A first kernel (or, for few rows, each CTA of the second for itself)
+// lists the rows that have one; the second reads them: batches of 32 x 4 vectors of 16 bytes, all rows' behind one another, are dealt to
+// the warps in equal runs, whatever rows they belong to, so that no warp waits for another and none has more to do; a run leaves a sum,
+// and what its exponents were taken from, for each row that it touches.  The third joins those of a row (up to kSlots) and does what
+// comes behind them, in 64 bits.  The backward pass deals its batches the same way, from the last row to the first, then the rows
+// without a target, which it only writes.
+// All of it is bound by memory: 2042 rows of 128256 in bf16, 1329 of them with a target, take 71 us for the list and the sums (341 MB,
+// and what the pass before has left in L2 to be written: 6.3 TB/s) and 133 us for the gradient (865 MB: 6.5 TB/s; writes alone reach
+// 3.9); 2048 of 32000, 1287 of them with one, 24 and 35.
 #include <cooperative_groups.h>
 
 #include "common/logit_rows.cuh"
@@ -95,21 +96,18 @@ struct Span {
 };
 
 // ------------------------------------------------------------------------------------------------ rows with a target
-constexpr int kListNT = 1024, kListRows = 4;
-
-__global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int64_t rows, int64_t ignore, void* keep) {
-  __shared__ int sums[kListNT / 32];
-  pdl_wait();
-  pdl_launch_dependents();
-  const Keep k = keep_at(keep, rows);
+// Calls put(row, place among the rows with a target so far, whether it has one) for each row, in order of the rows for each thread;
+// returns how many have one.  PER rows to a thread at a time.
+template <int NT, int PER, typename F>
+__device__ __forceinline__ int for_rows(const int64_t* targets, int64_t rows, int64_t ignore, int* sums, F put) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int have = 0;                                       // so far
-  for (int64_t at = 0; at < rows; at += kListNT * kListRows) {
-    const int64_t r0 = at + threadIdx.x * kListRows;
-    bool real[kListRows];
+  for (int64_t at = 0; at < rows; at += NT * PER) {
+    const int64_t r0 = at + threadIdx.x * PER;
+    bool real[PER];
     int mine = 0;
 #pragma unroll
-    for (int i = 0; i < kListRows; ++i) {
+    for (int i = 0; i < PER; ++i) {
       real[i] = r0 + i < rows && targets[r0 + i] != ignore;
       mine += real[i];
     }
@@ -121,7 +119,7 @@ __global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    int all = sums[lane];
+    int all = lane < NT / 32 ? sums[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const int v = __shfl_up_sync(0xffffffffu, all, o);
@@ -131,15 +129,29 @@ __global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int
     int place = have + (warp == 0 ? 0 : before) + upto - mine;
     have += __shfl_sync(0xffffffffu, all, 31);
 #pragma unroll
-    for (int i = 0; i < kListRows; ++i) {
+    for (int i = 0; i < PER; ++i) {
       if (r0 + i >= rows) break;
-      if (real[i]) k.list[place] = (int)(r0 + i);
-      else k.list[rows - 1 - (r0 + i - place)] = (int)(r0 + i);
-      k.place[r0 + i] = real[i] ? place : -1;
+      put(r0 + i, place, real[i]);
       place += real[i];
     }
     __syncthreads();
   }
+  return have;
+}
+__device__ __forceinline__ void keep_row(const Keep& k, int64_t rows, int64_t row, int place, bool real) {
+  k.list[real ? place : rows - 1 - (row - place)] = (int)row;
+  k.place[row] = real ? place : -1;
+}
+
+constexpr int kListNT = 1024;
+
+__global__ void __launch_bounds__(kListNT) list_rows(const int64_t* targets, int64_t rows, int64_t ignore, void* keep) {
+  __shared__ int sums[kListNT / 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const Keep k = keep_at(keep, rows);
+  const int have = for_rows<kListNT, 4>(targets, rows, ignore, sums,
+                                        [&](int64_t row, int place, bool real) { keep_row(k, rows, row, place, real); });
   if (threadIdx.x == 0) *k.count = have;
 }
 
@@ -225,26 +237,45 @@ __device__ __forceinline__ void add_batch(Part& p, const uint4* w, int n, float 
 struct SumArgs {
   Rows rows;
   int64_t n;
-  const void* keep;
+  const int64_t* targets;
+  int64_t ignore;
+  void* keep;
   float2* part;        // [places, slots_of(batches of a row)]
   float inv_t;
 };
 
-template <typename T>
+// LIST: of up to kListed rows, each CTA lists those with a target for itself, and the first one keeps the list: a launch less (2048 rows
+// of 32000: 25.0 us with a launch for the list, 24.4 so, and 2 us less of host time; 48 rows of 1000: 5.5 and 4.3).
+constexpr int kListed = 2048;
+
+template <typename T, bool LIST>
 __global__ void __launch_bounds__(kNT, kCtas) row_sums(SumArgs a) {
   constexpr int VEC = 16 / sizeof(T);
+  __shared__ int sums[kNT / 32];
+  __shared__ int own[LIST ? kListed : 1];
   const int lane = threadIdx.x & 31, warps = gridDim.x * (kNT / 32), warp = blockIdx.x * (kNT / 32) + (threadIdx.x >> 5);
-  const Keep k = keep_at(const_cast<void*>(a.keep), a.n);
+  const Keep k = keep_at(a.keep, a.n);
   const float c = a.inv_t * kLog2e;
-  pdl_launch_dependents();
   pdl_wait();
-  const Deal deal(*k.count, batches_of(a.rows.V, VEC), warps);
+  pdl_launch_dependents();
+  int count;
+  if constexpr (LIST) {
+    count = for_rows<kNT, kListed / kNT>(a.targets, a.n, a.ignore, sums, [&](int64_t row, int place, bool real) {
+      if (real) own[place] = (int)row;
+      if (blockIdx.x == 0) keep_row(k, a.n, row, place, real);
+    });
+    if (blockIdx.x == 0 && threadIdx.x == 0) *k.count = count;
+  } else {
+    count = *k.count;
+  }
+  const int* list = LIST ? own : k.list;
+  const Deal deal(count, batches_of(a.rows.V, VEC), warps);
   for (int64_t run = warp; run < deal.runs(); run += warps) {
     int64_t at = run * deal.len;
     const int64_t end = min(at + deal.len, deal.total);
     int place = (int)(at / deal.per), b = (int)(at - (int64_t)place * deal.per);
     for (; at < end; ++place, b = 0) {
-      const T* x = row_at<T>(a.rows, k.list[place]);
+      const T* x = row_at<T>(a.rows, list[place]);
       const Span<T> sp(x, a.rows.V);
       const int b1 = (int)min((int64_t)deal.per, b + (end - at));
       at += b1 - b;
@@ -641,17 +672,21 @@ int grad_grid_of(int64_t rows, int V, int elem) {
   return grid_of(rows, V, elem, stay * (times < 1 ? 1 : times > 8 ? 8 : times));
 }
 
-// The first two kernels; then `a` is ready for the third.
+// The list and the sums; then `a` is ready for the kernel behind them.
 int forward(RowArgs& a, int64_t ignore, int dtype, cudaStream_t s) {
   if (sm_count() == 0) return (int)cudaErrorInvalidDevice;
-  const cudaError_t e = launch_kernel(list_rows, dim3(1), dim3(kListNT), 0, s, true, a.targets, a.n, ignore, a.keep);
-  if (e != cudaSuccess) return (int)e;
   const int grid = grid_of(a.n, a.rows.V, elem_of(dtype), (int64_t)sm_count() * kCtas);
   a.warps = grid * (kNT / 32);
   a.per = batches_of(a.rows.V, 16 / elem_of(dtype));
-  const SumArgs sums = {a.rows, a.n, a.keep, const_cast<float2*>(a.part), a.inv_t};
+  const bool list = a.n <= kListed;
+  if (!list) {
+    const cudaError_t e = launch_kernel(list_rows, dim3(1), dim3(kListNT), 0, s, true, a.targets, a.n, ignore, a.keep);
+    if (e != cudaSuccess) return (int)e;
+  }
+  const SumArgs sums = {a.rows, a.n, a.targets, ignore, a.keep, const_cast<float2*>(a.part), a.inv_t};
   return by_type(dtype, [&](auto* tag) {
-    return (int)launch_kernel(row_sums<std::remove_pointer_t<decltype(tag)>>, dim3(grid), dim3(kNT), 0, s, true, sums);
+    using T = std::remove_pointer_t<decltype(tag)>;
+    return (int)launch_kernel(list ? row_sums<T, true> : row_sums<T, false>, dim3(grid), dim3(kNT), 0, s, true, sums);
   });
 }
 

@@ -102,6 +102,18 @@ def test_policy_by_size(dtype, shape):
     _check_policy(x, t, *_policy_inputs(x, t, g), kl_weight=0.2)
 
 
+@pytest.mark.parametrize("tokens", [1, 127, 128, 129, 1023, 1024, 1025, 2048, 2049, 5000])
+def test_lists_of_rows(tokens):
+    """Around the number of rows up to which each CTA lists them for itself, and that which one pass over the targets takes."""
+    g = _gen(tokens)
+    x, t = _logits((2, tokens, 40), torch.float32, g), _targets((2, tokens), 40, g)
+    _check_preference(x, t, average=True)
+    _check_policy(x, t, *_policy_inputs(x, t, g), kl_weight=0.2)
+    t[:] = -100
+    t[1, -1] = 3
+    _check_preference(x, t)
+
+
 @pytest.mark.parametrize("kind", ["some", "prompts", "none", "one", "all"])
 def test_which_rows_have_a_target(kind):
     g = _gen(kind)
