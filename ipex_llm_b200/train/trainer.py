@@ -29,6 +29,8 @@ POLICY_COLUMNS = ("advantages", "old_logprobs", "ref_logprobs")
 class TrainerCallback:
     """Hook points (same names as HF ``TrainerCallback`` for the ones used by ReLoRA / LISA)."""
 
+    folds_adapters = False               # True: adapters are folded into their base while it trains
+
     def on_train_begin(self, args, state, control, **kw): ...
     def on_step_begin(self, args, state, control, **kw): ...
     def on_step_end(self, args, state, control, **kw): ...
@@ -74,6 +76,7 @@ class Trainer:
         self.rank = dist.get_rank() if dist.is_initialized() else 0
         self.world = dist.get_world_size() if dist.is_initialized() else 1
         self.device = next(p for p in model.parameters()).device
+        self._folds = None               # how often adapters had been folded into their base, at the first loss that compares with it
         pairs = bool(getattr(args, "preference_form", None))
         invalidInputError(not pairs or getattr(args, "fused_loss", False), "preference_form needs fused_loss=True")
         if not pairs and data_collator is None and train_dataset is not None and len(train_dataset):
@@ -150,15 +153,27 @@ class Trainer:
                                               **teacher)
         return loss
 
+    def _check_base(self, model):
+        """The model without its adapters is a reference as long as nothing moves it."""
+        how = "give the pairs reference_logprobs (or preference_reference=False)"
+        invalidInputError(hasattr(model, "disable_adapter_layers"), f"preference_form: there are no adapters to disable: {how}")
+        folds = getattr(model, "adapter_folds", 0)
+        if self._folds is None:
+            self._folds = folds
+        if folds != self._folds or any(getattr(cb, "folds_adapters", False) for cb in self.callbacks):
+            invalidInputError(False, f"preference_form: adapters are folded into their base, which is no reference any more: {how}")
+        for name, p in model.named_parameters():
+            if p.requires_grad and "lora_" not in name:
+                invalidInputError(False, f"preference_form: outside of the adapters {name} is trained, too, and the base is no reference: {how}")
+
     def _preference_loss(self, model, batch):
         a = self.args
         invalidInputError("labels" in batch, "preference_form: the batch has no labels")
         labels, reference = batch.pop("labels"), batch.pop("reference_logprobs", None)
         average = bool(getattr(a, "preference_average", False))
         if reference is None and getattr(a, "preference_reference", True):
-            invalidInputError(hasattr(model, "disable_adapter_layers"), "preference_form: without adapters the batch needs "
-                                                                        "reference_logprobs (or preference_reference=False)")
-            model.disable_adapter_layers(True)                 # the model that finetuning began with
+            self._check_base(model)
+            model.disable_adapter_layers(True)
             try:
                 with torch.no_grad():
                     reference = sequence_logprobs(_logits_of(model(**batch)), labels, average)

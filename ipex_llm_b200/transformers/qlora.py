@@ -422,7 +422,7 @@ class TrainingArguments:
     distill_weight: float = 0.5         # of the loss, where a batch has a teacher's tokens
     distill_temperature: float = 1.0
     # with fused_loss: pairs of samples ("chosen_input_ids", "rejected_input_ids") by "sigmoid", "hinge" or "ipo"; the reference is the
-    # batch's reference_logprobs, or the model with its adapters disabled
+    # batch's reference_logprobs, or the model with its adapters disabled, as long as nothing trains that or folds adapters into it
     preference_form: Optional[str] = None
     preference_beta: float = 0.1
     preference_label_smoothing: float = 0.0

@@ -77,6 +77,7 @@ def merge_and_requantize(model, reinit: bool = True):
         else:
             w = base.weight.detach().float()
         update_weights(layer, w + delta, reinit, dev)
+    model.adapter_folds = getattr(model, "adapter_folds", 0) + 1
 
 
 def merge_and_save(model, dst_dir: str, reinit: bool = False, **_unused):
@@ -132,6 +133,8 @@ class ReLoRAScheduler:
 
 
 class ReLoRACallback(TrainerCallback):
+    folds_adapters = True
+
     def __init__(self, relora_steps=150, relora_warmup_steps=10, relora_cpu_offload=False, prune_ratio=0.9,
                  resume_from_checkpoint=None):
         self.relora_steps = relora_steps

@@ -1,0 +1,110 @@
+"""Calls of preference and policy finetuning that are easy to make and hard to notice: references that move, batches of another kind."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from ipex_llm_b200.train import Trainer, TrainerCallback, default_collator, sequence_logprobs
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _adapters(seed=0):
+    from ipex_llm.transformers import AutoModelForCausalLM
+    from ipex_llm.transformers.qlora import LoraConfig, get_peft_model, prepare_model_for_kbit_training
+    from transformers import LlamaConfig
+    cfg = LlamaConfig(hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                      vocab_size=256, max_position_embeddings=128, tie_word_embeddings=False)
+    torch.manual_seed(0)
+    model = AutoModelForCausalLM.from_config(cfg, load_in_low_bit="nf4", torch_dtype=torch.float32,
+                                             modules_to_not_convert=["lm_head"], optimize_model=False, device="cpu")
+    model = get_peft_model(prepare_model_for_kbit_training(model, use_gradient_checkpointing=False),
+                           LoraConfig(r=4, lora_alpha=8, lora_dropout=0.0, target_modules=["q_proj", "v_proj"]))
+    for i, p in enumerate(p for p in model.parameters() if p.requires_grad):
+        torch.nn.init.normal_(p, std=0.05, generator=_gen(seed + i))
+    return model
+
+
+def _args(tmp_path, **kw):
+    from ipex_llm.transformers.qlora import TrainingArguments
+    kw = {"fused_loss": True, "max_steps": 5, "per_device_train_batch_size": 4, "optim": "adamw_multi", **kw}
+    return TrainingArguments(output_dir=str(tmp_path), logging_steps=1, bf16=False, learning_rate=1e-2, **kw)
+
+
+def _pairs(n=4, vocab=256):
+    out = []
+    for i in range(n):
+        g = _gen(i)
+        prompt, a, b = (torch.randint(0, vocab, (k,), generator=g).tolist() for k in (3, 4, 2 + i))
+        out.append({"chosen_input_ids": prompt + a, "chosen_labels": [-100] * 3 + a, "rejected_input_ids": prompt + b,
+                    "rejected_labels": [-100] * 3 + b})
+    return out
+
+
+def _with_reference(model, data):
+    """Pairs with the log probabilities of the model without its adapters, as it is now."""
+    batch = default_collator(data)
+    model.disable_adapter_layers(True)
+    with torch.no_grad():
+        got = sequence_logprobs(model(input_ids=batch["input_ids"], attention_mask=batch["attention_mask"]).logits, batch["labels"])
+    model.disable_adapter_layers(False)
+    return [dict(s, reference_logprobs=[float(got[i]), float(got[len(data) + i])]) for i, s in enumerate(data)]
+
+
+# ---- the reference of pairs --------------------------------------------------------------------------------------------------
+def test_a_reference_that_restarts_would_move(tmp_path):
+    """Restarts fold the adapters into the base, which then is no reference any more: it has to be given with the pairs."""
+    from ipex_llm.transformers.relora import ReLoRATrainer
+    model, data = _adapters(), _pairs()
+    args = _args(tmp_path, preference_form="sigmoid", preference_beta=0.5)
+    before = [p.detach().clone() for p in model.parameters() if p.requires_grad]
+    with pytest.raises(RuntimeError, match="fold"):
+        ReLoRATrainer(model, args, train_dataset=data, relora_steps=2).train()
+    assert all(torch.equal(p, q) for p, q in zip((p for p in model.parameters() if p.requires_grad), before))
+    args.preference_reference = False
+    assert ReLoRATrainer(_adapters(), args, train_dataset=data, relora_steps=2).train()["train_loss"] > 0
+    args.preference_reference = True
+    given = _with_reference(model, data)
+    batch = default_collator(given)
+    seen = []
+
+    class Watch(TrainerCallback):
+        """The loss of the batch by its definition, before each step."""
+
+        def on_step_begin(self, args, state, control, model=None, **kw):
+            with torch.no_grad():
+                logits = model(input_ids=batch["input_ids"], attention_mask=batch["attention_mask"]).logits
+            h = sequence_logprobs(logits, batch["labels"]) - batch["reference_logprobs"]
+            seen.append(float(-F.logsigmoid(0.5 * (h[:4] - h[4:])).mean()))
+    trainer = ReLoRATrainer(model, args, train_dataset=given, relora_steps=2)
+    trainer.callbacks.append(Watch())                 # behind the restarts
+    trainer.train()
+    assert trainer.relora.num_restarts == 2
+    losses = [r["loss"] for r in trainer.state.log_history]
+    # the batch's order is the only difference: sums of 32-bit numbers below 100
+    assert losses == pytest.approx(seen, abs=1e-4)
+
+
+def test_a_reference_whose_base_is_trained_would_move(tmp_path):
+    model, data = _adapters(), _pairs()
+    model.base_model.get_output_embeddings().weight.requires_grad_(True)
+    trainer = Trainer(model, _args(tmp_path, preference_form="sigmoid"), train_dataset=data)
+    with pytest.raises(RuntimeError, match="outside of the adapters.*lm_head"):
+        trainer.compute_loss(model, default_collator(data))
+    trainer.compute_loss(model, default_collator(_with_reference(model, data))).backward()
+    trainer.args.preference_reference = False
+    trainer.compute_loss(model, default_collator(data)).backward()
+
+
+def test_a_base_that_took_the_adapters_in_is_no_reference(tmp_path):
+    """Whoever folds the adapters in; a base that had them before the first loss is what finetuning begins with."""
+    from ipex_llm.transformers.relora import merge_and_requantize
+    model, data = _adapters(), _pairs()
+    merge_and_requantize(model, reinit=True)
+    trainer = Trainer(model, _args(tmp_path, preference_form="sigmoid"), train_dataset=data)
+    trainer.compute_loss(model, default_collator(data)).backward()
+    merge_and_requantize(model, reinit=True)
+    with pytest.raises(RuntimeError, match="fold"):
+        trainer.compute_loss(model, default_collator(data))
+    trainer.compute_loss(model, default_collator(_with_reference(model, data))).backward()
