@@ -5,7 +5,7 @@ from typing import Dict, List, Optional, Union
 
 import torch
 
-from ..ops.adamw import AdamWState, adamw_state, adamw_step, grad_norm, moments
+from ..ops.adamw import AdamWState, adamw_state, adamw_step, flat_size, grad_norm, moments
 from ..utils.common import invalidInputError
 
 
@@ -85,13 +85,15 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def prune_moments(self, ratio: float):
-        """Zeroes the smallest ``ratio`` of each kind of moment."""
+        """Zeroes the smallest ``ratio`` of each kind of moment (with what equals the last one of them)."""
         for b in self.buckets():
-            s = b["state"]
-            for codes, wide in zip(s[:2], moments(s.exp_avg, s.exp_avg_sq, s.exp_avg_scale, s.exp_avg_sq_scale)):
-                k = int(ratio * wide.numel())
-                if k > 0:
-                    limit = torch.kthvalue(wide.abs().cpu(), k).values.to(wide.device)
+            s, sizes = b["state"], [p.numel() for p in b["params"]]
+            k = int(ratio * sum(sizes))
+            if k > 0:
+                for codes, wide in zip(s[:2], moments(s.exp_avg, s.exp_avg_sq, s.exp_avg_scale, s.exp_avg_sq_scale)):
+                    # the zeros that fill a parameter's last 256 are none of its moments
+                    real = [x[:n] for x, n in zip(wide.split([flat_size([n]) for n in sizes]), sizes)]
+                    limit = torch.kthvalue(torch.cat(real).abs().cpu(), k).values.to(wide.device)
                     bits = codes.view(torch.uint8 if codes.element_size() == 1 else torch.int32)
                     bits.mul_((wide.abs() > limit).to(bits.dtype))
 
