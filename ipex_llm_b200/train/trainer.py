@@ -8,6 +8,7 @@ bit-for-bit on the same world size.
 """
 from __future__ import annotations
 
+import inspect
 import json
 import math
 import os
@@ -123,7 +124,24 @@ class Trainer:
             cursor = (epoch + 1) * n
             epoch += 1
 
+    def _check_columns(self, model, batch):
+        """Columns of a policy's or of pairs' batches belong to their losses: a model that takes any would pass over them."""
+        fused, form = getattr(self.args, "fused_loss", False), getattr(self.args, "preference_form", None)
+        given = [k for k in (*POLICY_COLUMNS, "reference_logprobs") if k in batch]
+        if given and not fused:
+            named = inspect.signature(model.forward).parameters      # of a model that has a loss for them
+            given = [k for k in given if k not in named]
+            invalidInputError(not given, f"{', '.join(given)} in the batch: this loss needs fused_loss=True")
+        if not (given and fused):
+            return
+        invalidInputError(not form or given == ["reference_logprobs"], f"{', '.join(given)} in the batch: preference_form is for pairs")
+        invalidInputError(form or "reference_logprobs" not in given, "reference_logprobs in the batch: pairs need preference_form")
+        if not form:
+            invalidInputError("advantages" in batch, f"{', '.join(given)} in the batch, without advantages")
+            invalidInputError(not any(k in batch for k in TEACHER_COLUMNS), "a policy's batch takes no teacher's tokens")
+
     def compute_loss(self, model, batch):
+        self._check_columns(model, batch)
         batch = {k: v.to(self.device, non_blocking=True) for k, v in batch.items()}
         if getattr(self.args, "fused_loss", False):
             return self._fused_loss(model, batch)

@@ -108,3 +108,63 @@ def test_a_base_that_took_the_adapters_in_is_no_reference(tmp_path):
     with pytest.raises(RuntimeError, match="fold"):
         trainer.compute_loss(model, default_collator(data))
     trainer.compute_loss(model, default_collator(_with_reference(model, data))).backward()
+
+
+# ---- batches of a policy -----------------------------------------------------------------------------------------------------
+def _drawn(n=4, **kw):
+    out = []
+    for i in range(n):
+        ids = torch.randint(0, 256, (6 + i,), generator=_gen(i)).tolist()
+        out.append({"input_ids": ids, "labels": [-100] * 2 + ids[2:], "attention_mask": [1] * len(ids), "advantages": float(i - 1.5), **kw})
+    return out
+
+
+@pytest.mark.parametrize("args,match", [(dict(fused_loss=False), "fused_loss=True"), (dict(preference_form="sigmoid"), "preference_form")],
+                         ids=["usual loss", "pairs"])
+@pytest.mark.parametrize("columns", [("advantages",), ("advantages", "old_logprobs", "ref_logprobs"), ("old_logprobs",)], ids=str)
+def test_a_policys_numbers_are_not_passed_over(tmp_path, args, match, columns):
+    """A loss that does not know them would make completions of a negative advantage more likely."""
+    model = _adapters()
+    batch = default_collator(_drawn())
+    for k in ("old_logprobs", "ref_logprobs"):
+        batch[k] = torch.full(batch["input_ids"].shape, -5.0)
+    batch = {k: v for k, v in batch.items() if k in columns or k in ("input_ids", "labels", "attention_mask")}
+    trainer = Trainer(model, _args(tmp_path, **args), train_dataset=None, data_collator=lambda s: batch)
+    with pytest.raises(RuntimeError, match=match):
+        trainer.compute_loss(model, dict(batch))
+    assert set(batch) == {"input_ids", "labels", "attention_mask", *columns}
+    if "advantages" in columns:
+        Trainer(model, _args(tmp_path)).compute_loss(model, dict(batch)).backward()
+
+
+def test_old_log_probabilities_need_advantages(tmp_path):
+    model = _adapters()
+    batch = default_collator(_drawn(old_logprobs=[-5.0] * 6))
+    del batch["advantages"]
+    with pytest.raises(RuntimeError, match="without advantages"):
+        Trainer(model, _args(tmp_path)).compute_loss(model, batch)
+
+
+def test_a_teachers_tokens_and_references_are_not_passed_over(tmp_path):
+    model = _adapters()
+    batch = default_collator(_drawn())
+    batch["teacher_ids"] = torch.zeros(*batch["input_ids"].shape, 2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="no teacher"):
+        Trainer(model, _args(tmp_path)).compute_loss(model, batch)
+    batch = default_collator(_with_reference(model, _pairs()))
+    for args in (dict(fused_loss=False), dict()):
+        with pytest.raises(RuntimeError, match="reference_logprobs in the batch"):
+            Trainer(model, _args(tmp_path, **args)).compute_loss(model, dict(batch))
+
+
+def test_a_model_with_a_loss_of_its_own_gets_them(tmp_path):
+    class Own(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.Parameter(torch.ones(1))
+
+        def forward(self, input_ids, labels, attention_mask=None, advantages=None):
+            return ((self.w * advantages).sum(),)
+    batch = default_collator(_drawn())
+    loss = Trainer(Own(), _args(tmp_path, fused_loss=False)).compute_loss(Own(), batch)
+    assert float(loss.detach()) == float(batch["advantages"].sum())
