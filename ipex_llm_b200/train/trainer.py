@@ -359,7 +359,7 @@ def _pad_teacher(rows, n: int, ids: bool):
 def default_collator(samples):
     """Pads ``input_ids`` / ``labels`` / ``attention_mask`` lists to the longest sample (labels padded with -100); a teacher's
     rows (``TeacherTokens``: lists or tensors [tokens, top] and [tokens]) likewise, ids with -1, and a policy's numbers (advantages may
-    be one for each sample) with 0.
+    be one for each sample, or for some of them) with 0.
 
     Pairs, with ``chosen_input_ids`` and ``rejected_input_ids`` (and labels of either name, -100 for the prompt), become a batch of the
     chosen samples, then of the rejected ones; ``reference_logprobs`` hold two numbers, the chosen one's first."""
@@ -375,6 +375,8 @@ def default_collator(samples):
         if k in POLICY_COLUMNS:
             rows = [torch.as_tensor(s[k], dtype=torch.float32).cpu().reshape(-1) for s in samples]
             one = k == "advantages" and all(r.numel() == 1 for r in rows)
+            if k == "advantages" and not one:
+                rows = [r.expand(len(s["input_ids"])) if r.numel() == 1 else r for r, s in zip(rows, samples)]
             out[k] = torch.stack(rows) if one else _pad_teacher(rows, n, False)
             continue
         pad = -100 if k == "labels" else 0

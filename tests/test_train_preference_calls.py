@@ -168,3 +168,12 @@ def test_a_model_with_a_loss_of_its_own_gets_them(tmp_path):
     batch = default_collator(_drawn())
     loss = Trainer(Own(), _args(tmp_path, fused_loss=False)).compute_loss(Own(), batch)
     assert float(loss.detach()) == float(batch["advantages"].sum())
+
+
+def test_advantages_of_both_kinds_in_a_batch():
+    """One number for a sample counts at each of its positions, also where another sample has one for each."""
+    samples = [{"input_ids": [1, 2, 3], "labels": [1, 2, 3], "advantages": -1.0},
+               {"input_ids": [1, 2, 3, 4], "labels": [1, 2, 3, 4], "advantages": [1.0, 2.0, 3.0, 4.0]},
+               {"input_ids": [5], "labels": [5], "advantages": [0.5]}]
+    assert default_collator(samples)["advantages"].tolist() == [[-1.0, -1.0, -1.0, 0.0], [1.0, 2.0, 3.0, 4.0], [0.5, 0.0, 0.0, 0.0]]
+    assert default_collator([samples[0], samples[2]])["advantages"].tolist() == [[-1.0], [0.5]]
