@@ -363,6 +363,9 @@ def default_collator(samples):
 
     Pairs, with ``chosen_input_ids`` and ``rejected_input_ids`` (and labels of either name, -100 for the prompt), become a batch of the
     chosen samples, then of the rejected ones; ``reference_logprobs`` hold two numbers, the chosen one's first."""
+    for k in (*POLICY_COLUMNS, "reference_logprobs"):
+        have = sum(k in s for s in samples)
+        invalidInputError(have in (0, len(samples)), f"{k} of some samples of a batch, but not of all")
     if "chosen_input_ids" in samples[0]:
         return _pairs(samples)
     keys = samples[0].keys()

@@ -177,3 +177,14 @@ def test_advantages_of_both_kinds_in_a_batch():
                {"input_ids": [5], "labels": [5], "advantages": [0.5]}]
     assert default_collator(samples)["advantages"].tolist() == [[-1.0, -1.0, -1.0, 0.0], [1.0, 2.0, 3.0, 4.0], [0.5, 0.0, 0.0, 0.0]]
     assert default_collator([samples[0], samples[2]])["advantages"].tolist() == [[-1.0], [0.5]]
+
+
+def test_columns_that_some_samples_lack():
+    plain, drawn = {"input_ids": [1, 2], "labels": [1, 2]}, {"input_ids": [1, 2], "labels": [1, 2], "advantages": 1.0}
+    pairs = _pairs(2)
+    pairs[1]["reference_logprobs"] = [-1.0, -2.0]
+    for samples, match in (([plain, drawn], "advantages"), ([drawn, plain], "advantages"), ([drawn, dict(drawn, ref_logprobs=[0.0, 0.0])],
+                                                                                           "ref_logprobs"),
+                           (pairs, "reference_logprobs"), (pairs[::-1], "reference_logprobs")):
+        with pytest.raises(RuntimeError, match=f"{match} of some samples"):
+            default_collator(samples)
