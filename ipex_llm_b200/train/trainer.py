@@ -208,7 +208,8 @@ class Trainer:
         given = {k: batch.pop(k) for k in POLICY_COLUMNS if k in batch}
         labels = batch.pop("labels")
         return policy_lm_loss(_logits_of(model(**batch)), labels, clip=tuple(getattr(a, "policy_clip", (0.2, 0.2))),
-                              kl_weight=float(getattr(a, "policy_kl_weight", 0.0)), **given)
+                              kl_weight=float(getattr(a, "policy_kl_weight", 0.0)),
+                              temperature=float(getattr(a, "policy_temperature", 1.0)), **given)
 
     def train(self, resume_from_checkpoint: Optional[str] = None):
         a = self.args

@@ -433,3 +433,4 @@ class TrainingArguments:
     # with fused_loss and advantages in the batch: a policy's step
     policy_clip: Tuple[float, float] = (0.2, 0.2)
     policy_kl_weight: float = 0.0
+    policy_temperature: float = 1.0     # that the completions, and their old log probabilities, were sampled at

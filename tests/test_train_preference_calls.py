@@ -188,3 +188,15 @@ def test_columns_that_some_samples_lack():
                            (pairs, "reference_logprobs"), (pairs[::-1], "reference_logprobs")):
         with pytest.raises(RuntimeError, match=f"{match} of some samples"):
             default_collator(samples)
+
+
+def test_the_temperature_a_policy_was_sampled_at(tmp_path):
+    from ipex_llm_b200.train import policy_lm_loss
+    model = _adapters()
+    batch = default_collator(_drawn(old_logprobs=[-5.0] * 6, ref_logprobs=[-5.5] * 6))
+    trainer = Trainer(model, _args(tmp_path, policy_temperature=0.7, policy_kl_weight=0.1))
+    loss = trainer.compute_loss(model, dict(batch))
+    logits = model(input_ids=batch["input_ids"], attention_mask=batch["attention_mask"]).logits
+    numbers = [batch[k] for k in ("advantages", "old_logprobs", "ref_logprobs")]
+    assert torch.equal(loss, policy_lm_loss(logits, batch["labels"], *numbers, kl_weight=0.1, temperature=0.7))
+    assert not torch.equal(loss, policy_lm_loss(logits, batch["labels"], *numbers, kl_weight=0.1))
