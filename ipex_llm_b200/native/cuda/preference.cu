@@ -9,6 +9,7 @@
 //   ipo      (h - 1 / 2b)^2                            dh: 2 (h - 1 / 2b)
 // policy: w = e^(log p - old), d = ref - log p,
 //   -min(w A, min(max(w, 1 - lo), 1 + hi) A) + k (e^d - d - 1)      d log p: -A w where w A is the smaller, + k (1 - e^d)
+// (differences of equal numbers are 0, also where both policies hide a target: of -inf)
 //
 // Prompts and padding have no target: their logits are never read.  A first kernel (or, for few rows, each CTA of the second for itself)
 // lists the rows that have one; the second reads them: batches of 32 x 4 vectors of 16 bytes, all rows' behind one another, are dealt to
@@ -371,6 +372,8 @@ struct PolicyArgs {
   double lo, hi, weight;
 };
 
+__device__ __forceinline__ double apart(double a, double b) { return a == b ? 0.0 : a - b; }
+
 template <typename T>
 __global__ void __launch_bounds__(128) policy_rows(PolicyArgs a) {
   const Keep k = keep_at(a.row.keep, a.row.n);
@@ -385,12 +388,12 @@ __global__ void __launch_bounds__(128) policy_rows(PolicyArgs a) {
   if (place >= 0) {
     lp = row_logprob<T>(a.row, k, deal, row, place);
     const double A = a.adv[row / a.inner * a.adv0 + row % a.inner * a.adv1];
-    const double w = a.old != nullptr ? exp(lp - a.old[row]) : lp == lp ? 1.0 : lp;
+    const double w = a.old != nullptr ? exp(apart(lp, a.old[row])) : lp == lp ? 1.0 : lp;
     const double inside = w < 1.0 - a.lo ? 1.0 - a.lo : w > 1.0 + a.hi ? 1.0 + a.hi : w;      // NaN stays
     clipped = inside * A < w * A;
     double l = -(clipped ? inside * A : w * A), g = clipped ? 0.0 : -A * w;
     if (a.ref != nullptr) {
-      const double d = a.ref[row] - lp, e = expm1(d), est = e < INFINITY ? e - d : e;
+      const double d = apart(a.ref[row], lp), e = expm1(d), est = e < INFINITY ? e - d : e;
       kl = (float)est;
       if (a.weight != 0.0) {
         l += a.weight * est;

@@ -103,19 +103,24 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
                              average, temperature, ignore_index)
 
 
+def _apart(a, b):
+    """a - b: 0, and without a gradient, where both are the same infinity."""
+    same = (a == b) & a.isinf()
+    return a.masked_fill(same, 0.0) - b.masked_fill(same, 0.0)
+
+
 def _policy_plain(logits, targets, advantages, old, ref, lo, hi, weight, temperature, ignore):
     lp = token_logprobs(logits, targets, temperature, ignore_index=ignore).logprob
     real = targets != ignore
     wide = lp.double()
-    moved = wide.masked_fill(wide == -math.inf, 0.0) if old is None else wide        # a hidden token's ratio to itself is 1, too
-    ratio = torch.exp(moved - (moved.detach() if old is None else old.double()))
+    ratio = torch.exp(_apart(wide, wide.detach() if old is None else old.double()))
     a = advantages.double()
     held = ratio.clamp(1.0 - lo, 1.0 + hi)
     clipped = held * a < ratio * a
     loss = -torch.where(clipped, held.detach() * a, ratio * a)
     kl = torch.zeros_like(wide)
     if ref is not None:
-        d = ref.double() - wide
+        d = _apart(ref.double(), wide)
         far = d.detach() == math.inf
         kl = torch.where(far, math.inf, torch.expm1(d.masked_fill(far, 0.0)) - d.masked_fill(far, 0.0))
         loss = loss + weight * kl if weight else loss
@@ -134,8 +139,9 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
 
     Without ``old_logprobs`` they are lp itself (one step for each batch): w is 1 and still has its gradient.  Targets of
     ``ignore_index`` give 0 and no gradient, and their logits are not read.  The gradient goes to the logits alone (in their type: 16
-    or 32 bits).  A hidden target (a logit of -inf) has w = 0, an infinite KL term and no gradient.  A target outside of the vocabulary raises on
-    the CPU; on the GPU its results are NaN, and ``cuda_ops.check_error_flag`` reports 61.
+    or 32 bits).  A hidden target (a logit of -inf) has no gradient; its w is 0, or 1 without ``old_logprobs`` and where they hide it,
+    too, and its KL term is infinite, or 0 where the reference hides it, too.  A target outside of the vocabulary raises on the CPU; on
+    the GPU its results are NaN, and ``cuda_ops.check_error_flag`` reports 61.
     """
     what = "policy_loss"
     lo, hi = float(clip[0]), float(clip[1])
