@@ -115,7 +115,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                     raw = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}[t.element_size()]
                     t.view(raw).copy_(a.view(raw))
         for g, s in zip(self.param_groups, sd["param_groups"]):
+            rate = g["lr"]
             g.update(s)
+            if isinstance(rate, torch.Tensor):               # steps that were captured read it where it is
+                g["lr"] = rate.fill_(float(s["lr"]))
+            else:
+                g["lr"] = float(s["lr"])
 
 
 __all__ = ["AdamWState", "MultiTensorAdamW"]

@@ -49,3 +49,28 @@ def test_pruned_moments_are_the_smallest_real_ones(bits, sizes, ratio):
         assert torch.equal(y, torch.where(x.abs() > limit, x, 0.0))          # ties with the last one go, too
         if bits == 32:
             assert int((y != 0).sum()) == x.numel() - k
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_rate_on_the_device_stays_there(device, tmp_path):
+    """Steps that are captured read the rate's tensor: loading a state writes into it."""
+    params = [torch.nn.Parameter(p.detach().to(device)) for p in _params([300, 7])]
+    rate = torch.tensor(0.25, device=device)
+    opt = MultiTensorAdamW([{"params": params[:1]}, {"params": params[1:], "lr": 0.125}], lr=rate)
+    _set = lambda t: [setattr(p, "grad", torch.full_like(p, float(t))) for p in params]      # noqa: E731
+    _set(1)
+    opt.step()
+    torch.save(opt.state_dict(), tmp_path / "o.pt")
+    saved = torch.load(tmp_path / "o.pt", map_location="cpu", weights_only=False)
+    rate.fill_(9.0)
+    opt.param_groups[1]["lr"] = 9.0
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] is rate and float(rate) == 0.25 and opt.param_groups[1]["lr"] == 0.125
+    assert rate.device.type == device
+    opt.step()                                                    # takes the rate where it is
+    # a rate that was saved from a tensor, for an optimizer with a number, and the other way round
+    other = MultiTensorAdamW([{"params": params[:1]}, {"params": params[1:], "lr": torch.tensor(3.0, device=device)}], lr=1.0)
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["lr"] == 0.25 and isinstance(other.param_groups[0]["lr"], float)
+    assert float(other.param_groups[1]["lr"]) == 0.125 and other.param_groups[1]["lr"].device.type == device
+    other.step()
