@@ -99,8 +99,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     # state for checkpoint / resume -------------------------------------------------------------------
     def state_dict(self):
-        return {"bits": self.bits, "buckets": [[None if t is None else t.cpu() for t in b["state"]] for b in self.buckets()],
-                "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
+        """The state as it is now: copies, on the CPU, that later steps do not change."""
+        return {"bits": self.bits, "buckets": [[None if t is None else t.to("cpu", copy=True) for t in b["state"]] for b in self.buckets()],
+                "param_groups": [{k: v.detach().to("cpu", copy=True) if isinstance(v, torch.Tensor) else v for k, v in g.items()
+                                  if k != "params"} for g in self.param_groups]}
 
     @torch.no_grad()
     def load_state_dict(self, sd):

@@ -74,3 +74,30 @@ def test_a_rate_on_the_device_stays_there(device, tmp_path):
     assert other.param_groups[0]["lr"] == 0.25 and isinstance(other.param_groups[0]["lr"], float)
     assert float(other.param_groups[1]["lr"]) == 0.125 and other.param_groups[1]["lr"].device.type == device
     other.step()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_state_that_was_taken_does_not_move(bits):
+    """Of parameters on the CPU, too, and a rate in a tensor with it: an earlier state can be gone back to."""
+    params, rate = _params([300, 7], torch.bfloat16), torch.tensor(0.25)
+    opt = MultiTensorAdamW(params, lr=rate, bits=bits)
+    _set_grads(params, 0)
+    opt.step()
+    held = [p.detach().clone() for p in params]
+    taken = opt.state_dict()
+
+    def go_on():
+        out = []
+        for t in range(1, 3):
+            _set_grads(params, t)
+            opt.step()
+            out += [p.detach().clone() for p in params]
+            rate.mul_(0.5)
+        return out
+    first = go_on()
+    with torch.no_grad():
+        for p, q in zip(params, held):
+            p.copy_(q)
+    opt.load_state_dict(taken)
+    assert float(rate) == 0.25
+    assert all(torch.equal(p, q) for p, q in zip(first, go_on()))
