@@ -100,7 +100,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     # state for checkpoint / resume -------------------------------------------------------------------
     def state_dict(self):
         """The state as it is now: copies, on the CPU, that later steps do not change."""
-        return {"bits": self.bits, "buckets": [[None if t is None else t.to("cpu", copy=True) for t in b["state"]] for b in self.buckets()],
+        return {"bits": self.bits, "seed": self.seed,
+                "buckets": [[None if t is None else t.to("cpu", copy=True) for t in b["state"]] for b in self.buckets()],
                 "param_groups": [{k: v.detach().to("cpu", copy=True) if isinstance(v, torch.Tensor) else v for k, v in g.items()
                                   if k != "params"} for g in self.param_groups]}
 
@@ -116,6 +117,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 if t is not None:
                     raw = {1: torch.uint8, 2: torch.int16, 4: torch.int32, 8: torch.int64}[t.element_size()]
                     t.view(raw).copy_(a.view(raw))
+        self.seed = sd.get("seed", self.seed)
         for g, s in zip(self.param_groups, sd["param_groups"]):
             rate = g["lr"]
             g.update(s)

@@ -101,3 +101,26 @@ def test_a_state_that_was_taken_does_not_move(bits):
     opt.load_state_dict(taken)
     assert float(rate) == 0.25
     assert all(torch.equal(p, q) for p, q in zip(first, go_on()))
+
+
+def test_a_resumed_state_rounds_as_the_saved_one():
+    """8-bit moments are rounded by a hash of the seed: it comes with the state."""
+    a, b = _params([300, 7]), _params([300, 7])
+    one, other = MultiTensorAdamW(a, lr=1e-2, bits=8, seed=3), MultiTensorAdamW(b, lr=1e-2, bits=8, seed=4)
+    _set_grads(a, 0)
+    one.step()
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    other.load_state_dict(one.state_dict())
+    assert other.seed == 3
+    for t in range(1, 4):
+        _set_grads(a, t)
+        _set_grads(b, t)
+        one.step()
+        other.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    older = one.state_dict()
+    del older["seed"]                                             # as states were saved before
+    other.load_state_dict(older)
+    assert other.seed == 3
