@@ -97,10 +97,13 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                     bits = codes.view(torch.uint8 if codes.element_size() == 1 else torch.int32)
                     bits.mul_((wide.abs() > limit).to(bits.dtype))
 
+    def _sizes(self):
+        return [[p.numel() for p in b["params"]] for b in self.buckets()]
+
     # state for checkpoint / resume -------------------------------------------------------------------
     def state_dict(self):
         """The state as it is now: copies, on the CPU, that later steps do not change."""
-        return {"bits": self.bits, "seed": self.seed,
+        return {"bits": self.bits, "seed": self.seed, "sizes": self._sizes(),
                 "buckets": [[None if t is None else t.to("cpu", copy=True) for t in b["state"]] for b in self.buckets()],
                 "param_groups": [{k: v.detach().to("cpu", copy=True) if isinstance(v, torch.Tensor) else v for k, v in g.items()
                                   if k != "params"} for g in self.param_groups]}
@@ -108,7 +111,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, sd):
         mine = self.buckets()
-        fits = len(sd["buckets"]) == len(mine) and all(
+        fits = len(sd["buckets"]) == len(mine) and len(sd["param_groups"]) == len(self.param_groups) and \
+            sd.get("sizes", self._sizes()) == self._sizes() and all(
             (a is None) == (t is None) and (t is None or (a.shape == t.shape and a.dtype == t.dtype))
             for saved, b in zip(sd["buckets"], mine) for a, t in zip(saved, b["state"]))
         invalidInputError(fits, "MultiTensorAdamW: the state was saved for other parameters, or with other bits")

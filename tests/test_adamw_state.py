@@ -124,3 +124,29 @@ def test_a_resumed_state_rounds_as_the_saved_one():
     del older["seed"]                                             # as states were saved before
     other.load_state_dict(older)
     assert other.seed == 3
+
+
+def test_a_state_of_other_parameters_is_refused():
+    """Also where all of them take as much room, or fall into as many buckets."""
+    def of(*groups):
+        params = [_params(sizes, dtype) for sizes, dtype in groups]
+        opt = MultiTensorAdamW([{"params": p} for p in params], lr=1e-3)
+        _set_grads([p for g in params for p in g], 1)
+        opt.step()
+        return opt
+    f32, bf16 = torch.float32, torch.bfloat16
+    saved = of(([300, 7], f32))
+    for other in (of(([7, 300], f32)), of(([(2, 300), 7], f32)), of(([301, 7], f32))):
+        before = [p.detach().clone() for p in other.param_groups[0]["params"]]
+        kept = [t.clone() for t in other.buckets()[0]["state"] if t is not None]
+        with pytest.raises(RuntimeError, match="other parameters"):
+            other.load_state_dict(saved.state_dict())
+        assert all(torch.equal(a, b) for a, b in zip(before, other.param_groups[0]["params"]))
+        assert all(torch.equal(a, b) for a, b in zip(kept, (t for t in other.buckets()[0]["state"] if t is not None)))
+    two = of(([300], f32), ([300], bf16))
+    both = MultiTensorAdamW([*_params([300], f32), *_params([300], bf16)], lr=1e-3)
+    with pytest.raises(RuntimeError, match="other parameters"):
+        both.load_state_dict(two.state_dict())
+    older = saved.state_dict()
+    del older["sizes"]                                            # as states were saved before
+    of(([300, 7], f32)).load_state_dict(older)
