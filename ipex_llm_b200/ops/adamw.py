@@ -172,6 +172,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         grad_norm, max_grad_norm = None, 0.0
     elif grad_norm is None:
         invalidInputError(False, f"{what}: max_grad_norm needs the gradients' norm")
+    elif all(g is None for g in grads):
+        grad_norm = None                                      # of none: it is on no device
     buffers = (exp_avg, exp_avg_sq, step, exp_avg_scale, exp_avg_sq_scale, rest, grad_norm)
     numbers = (float(max_grad_norm), 0.0 if lr_at is not None else float(lr), lr_at, b1, b2, float(eps), float(weight_decay),
                int(seed) & 0xFFFFFFFF)

@@ -1,0 +1,20 @@
+"""Calls of the optimizer's operators that hold nothing, or less than usual."""
+import pytest
+import torch
+
+from ipex_llm_b200.ops.adamw import adamw_state, adamw_step, grad_norm
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_without_any_gradient(device, bits):
+    """The norm of no gradients has no device to be on but the CPU; a step that clips by it does nothing."""
+    params, grads = [torch.ones(300, device=device), torch.ones(7, device=device)], [None, None]
+    state = adamw_state(params, bits)
+    adamw_step(params, grads, **state._asdict(), lr=1.0, grad_norm=grad_norm(grads), max_grad_norm=1.0)
+    assert all(bool((p == 1.0).all()) for p in params) and state.step.tolist() == [0]
+    with pytest.raises(RuntimeError, match="exp_avg should be"):
+        adamw_step(params, grads, **state._replace(exp_avg=state.exp_avg[:256])._asdict(), lr=1.0, grad_norm=grad_norm(grads), max_grad_norm=1.0)
+    if device == "cuda":                                          # of gradients that are there, it is read where they are
+        with pytest.raises(RuntimeError, match="grad_norm should be"):
+            adamw_step(params, [torch.ones_like(p) for p in params], **state._asdict(), lr=1.0, grad_norm=torch.ones(()), max_grad_norm=1.0)
