@@ -93,8 +93,7 @@ class Trainer:
         if a.optim == "adamw_torch":
             invalidInputError(self.world == 1, "adamw_torch has no gradient averaging: use fused_lora_adamw")
             self.optimizer = torch.optim.AdamW(params, **kw)
-        elif a.optim in ("adamw_multi", "adamw_8bit"):
-            invalidInputError(self.world == 1, f"{a.optim} has no gradient averaging: use fused_lora_adamw")
+        elif a.optim in ("adamw_multi", "adamw_8bit") and self.world == 1:      # ranks share moments in 32 bits among them
             self.optimizer = MultiTensorAdamW(params, max_grad_norm=a.max_grad_norm, bits=8 if a.optim == "adamw_8bit" else 32,
                                               seed=a.seed, **kw)
         elif a.optim == "paged_adamw" and self.world == 1 and self.device.type == "cuda" and \
