@@ -248,7 +248,9 @@ class Trainer:
                 loss_acc += float(loss.detach())
                 tokens += int(batch["input_ids"].numel())
                 self.state.data_cursor = cursor
-            if not isinstance(self.optimizer, (FusedLoraAdamW, MultiTensorAdamW)) and a.max_grad_norm and a.max_grad_norm > 0:
+            clips = isinstance(self.optimizer, FusedLoraAdamW) or (isinstance(self.optimizer, MultiTensorAdamW) and
+                                                                   self.optimizer.max_grad_norm)
+            if not clips and a.max_grad_norm and a.max_grad_norm > 0:
                 torch.nn.utils.clip_grad_norm_([p for p in self.model.parameters() if p.requires_grad],
                                                a.max_grad_norm)
             self.optimizer.step()

@@ -200,3 +200,23 @@ def test_the_temperature_a_policy_was_sampled_at(tmp_path):
     numbers = [batch[k] for k in ("advantages", "old_logprobs", "ref_logprobs")]
     assert torch.equal(loss, policy_lm_loss(logits, batch["labels"], *numbers, kl_weight=0.1, temperature=0.7))
     assert not torch.equal(loss, policy_lm_loss(logits, batch["labels"], *numbers, kl_weight=0.1))
+
+
+# ---- optimizers of the caller's own ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("own", [0.0, 1e-3])
+def test_gradients_are_clipped_for_an_optimizer_that_does_not(tmp_path, own):
+    from ipex_llm_b200.train import MultiTensorAdamW
+
+    class Watch(MultiTensorAdamW):
+        def step(self, closure=None):
+            self.norm = float(torch.cat([p.grad.flatten() for g in self.param_groups for p in g["params"]]).norm())
+            return super().step(closure)
+    norms = []
+    for limit in (0.0, 1e-3):
+        model = _adapters()
+        opt = Watch([p for p in model.parameters() if p.requires_grad], max_grad_norm=own)
+        args = _args(tmp_path, max_grad_norm=limit, max_steps=1)
+        Trainer(model, args, train_dataset=_drawn(), optimizers=(opt, None)).train()
+        norms.append(opt.norm)
+    # an optimizer that clips gets its gradients as they are
+    assert norms[0] > 1e-2 and norms[1] == (norms[0] if own else pytest.approx(1e-3, rel=1e-3))
