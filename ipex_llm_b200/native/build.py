@@ -128,7 +128,7 @@ def build_tools(force=False, verbose=False):
 
 
 def build_calls(force=False, verbose=False):
-    """The extension on PyTorch's headers; it fits the PyTorch that it was built with alone."""
+    """The extension on PyTorch's headers; it fits the PyTorch that it was built with alone, and the version of Python."""
     import sysconfig
 
     import torch
@@ -137,7 +137,7 @@ def build_calls(force=False, verbose=False):
     cuda = os.path.dirname(os.path.dirname(_nvcc() or "/usr/local/cuda/bin/nvcc"))
     flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    digest = _hash_files(srcs, " ".join([*flags, torch.__version__, sys.version]))
+    digest = _hash_files(srcs, " ".join([*flags, torch.__version__, sysconfig.get_config_var("EXT_SUFFIX")]))
     if not force and _stamp_ok(CALLS_LIB, digest):
         return CALLS_LIB
     part = f"{CALLS_LIB}.{os.getpid()}"

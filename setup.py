@@ -8,7 +8,7 @@ setup(
     version="0.1.0",
     description="Blackwell-native low-bit LLM library with the API surface of ipex-llm",
     packages=find_packages(include=["ipex_llm_b200*", "ipex_llm*", "bigdl*"]),
-    package_data={"ipex_llm_b200": ["native/*.so", "native/cuda/*.cu", "native/cuda/*.cuh", "native/cuda/*.h",
+    package_data={"ipex_llm_b200": ["native/*.so", "native/*.so.hash", "native/cuda/*.cu", "native/cuda/*.cuh", "native/cuda/*.h",
                                     "native/cuda/common/*.cuh", "native/host/*.cpp", "native/host/*.h", "native/torch/*.cpp", "native/tools/*.cpp", "native/bin/*"]},
     python_requires=">=3.10",
     install_requires=["torch", "transformers", "numpy"],
