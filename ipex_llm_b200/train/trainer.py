@@ -80,8 +80,8 @@ class Trainer:
         self._folds = None               # how often adapters had been folded into their base, at the first loss that compares with it
         pairs = bool(getattr(args, "preference_form", None))
         invalidInputError(not pairs or getattr(args, "fused_loss", False), "preference_form needs fused_loss=True")
-        if not pairs and data_collator is None and train_dataset is not None and len(train_dataset):
-            first = train_dataset[0]
+        if not pairs and data_collator is None:
+            first = _first_of(train_dataset)
             invalidInputError(not (isinstance(first, dict) and "chosen_input_ids" in first), "pairs of samples need preference_form")
 
     # ------------------------------------------------------------------------------------------------
@@ -343,6 +343,14 @@ class Trainer:
 class _null:
     def __enter__(self): return None
     def __exit__(self, *a): return False
+
+
+def _first_of(dataset):
+    """A dataset's first sample; None where it is empty, or has no length or no places."""
+    try:
+        return dataset[0] if len(dataset) else None
+    except (TypeError, NotImplementedError):
+        return None
 
 
 def _logits_of(out):

@@ -220,3 +220,19 @@ def test_gradients_are_clipped_for_an_optimizer_that_does_not(tmp_path, own):
         norms.append(opt.norm)
     # an optimizer that clips gets its gradients as they are
     assert norms[0] > 1e-2 and norms[1] == (norms[0] if own else pytest.approx(1e-3, rel=1e-3))
+
+
+# ---- datasets ----------------------------------------------------------------------------------------------------------------
+def test_datasets_without_a_length_or_places(tmp_path):
+    """A trainer can be made of them, as for a loop of one's own over compute_loss."""
+    class Stream(torch.utils.data.IterableDataset):
+        def __iter__(self):
+            return iter(_drawn())
+
+    class Places(torch.utils.data.Dataset):
+        def __len__(self):
+            return 4
+    model = _adapters()
+    for data in (Stream(), iter(_drawn()), Places(), [], None):
+        trainer = Trainer(model, _args(tmp_path), train_dataset=data)
+    trainer.compute_loss(model, default_collator(list(Stream()))).backward()
