@@ -80,9 +80,11 @@ class Trainer:
         self._folds = None               # how often adapters had been folded into their base, at the first loss that compares with it
         pairs = bool(getattr(args, "preference_form", None))
         invalidInputError(not pairs or getattr(args, "fused_loss", False), "preference_form needs fused_loss=True")
-        if not pairs and data_collator is None:
-            first = _first_of(train_dataset)
-            invalidInputError(not (isinstance(first, dict) and "chosen_input_ids" in first), "pairs of samples need preference_form")
+        first = _first_of(train_dataset) if data_collator is None else None
+        if isinstance(first, dict):
+            paired = "chosen_input_ids" in first
+            invalidInputError(pairs or not paired, "pairs of samples need preference_form")
+            invalidInputError(paired or not pairs, "preference_form needs pairs of samples (chosen_input_ids, rejected_input_ids)")
 
     # ------------------------------------------------------------------------------------------------
     def create_optimizer(self):

@@ -236,3 +236,16 @@ def test_datasets_without_a_length_or_places(tmp_path):
     for data in (Stream(), iter(_drawn()), Places(), [], None):
         trainer = Trainer(model, _args(tmp_path), train_dataset=data)
     trainer.compute_loss(model, default_collator(list(Stream()))).backward()
+
+
+def test_pairs_are_not_made_of_single_samples(tmp_path):
+    """Halves of a shuffled batch of samples are no preferred and rejected ones."""
+    model = _adapters()
+    args = _args(tmp_path, preference_form="sigmoid")
+    single = [{k: v for k, v in s.items() if k != "advantages"} for s in _drawn()]
+    with pytest.raises(RuntimeError, match="needs pairs"):
+        Trainer(model, args, train_dataset=single)
+    # a collator of one's own makes them of what it is given
+    given = default_collator(_pairs())
+    trainer = Trainer(model, args, train_dataset=single, data_collator=lambda samples: given)
+    trainer.compute_loss(model, trainer.collate(single)).backward()
