@@ -46,7 +46,7 @@ def _preference_plain(logits, targets, reference, beta, form, smooth, margin, av
     if form == "ipo":
         loss = (h - 0.5 / beta).square()
     elif form == "hinge":
-        loss = (1.0 - beta * h).clamp(min=0.0)
+        loss = (1.0 - beta * h).relu()                  # its gradient at 0 is 0
     else:
         z = beta * h - margin
         loss = -(1.0 - smooth) * torch.nn.functional.logsigmoid(z)
