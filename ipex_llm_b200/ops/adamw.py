@@ -305,7 +305,8 @@ def _joined(high, rest):
 def _step_plain(params, grads, m, v, step, m_scale, v_scale, rest, norm, max_norm, lr, lr_at, b1, b2, eps, decay, seed):
     lr = float(lr_at) if lr_at is not None else lr
     kind = 0 if rest is None else 1 if rest.dtype == torch.int16 else 2
-    clip = None if norm is None else (max_norm / (norm + 1e-6)).clamp(max=1.0).reshape(())
+    # by a tensor: of a number and a tensor, the library takes the reciprocal and a product, which round twice
+    clip = None if norm is None else (norm.new_tensor(max_norm) / (norm + 1e-6)).clamp(max=1.0).reshape(())
     counted = set()
     at = 0
     for i, (p, g) in enumerate(zip(params, grads)):

@@ -18,3 +18,19 @@ def test_a_step_without_any_gradient(device, bits):
     if device == "cuda":                                          # of gradients that are there, it is read where they are
         with pytest.raises(RuntimeError, match="grad_norm should be"):
             adamw_step(params, [torch.ones_like(p) for p in params], **state._asdict(), lr=1.0, grad_norm=torch.ones(()), max_grad_norm=1.0)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_the_clipping_factor_is_a_quotient_rounded_once(device):
+    """With beta 0 and gradients of 1, the first moment is the factor: max_norm / (norm + 1e-6) in 32 bits, its sum and its quotient
+    rounded to nearest, and 1 at most."""
+    params, grads = [torch.zeros(1, device=device)], [torch.ones(1, device=device)]
+    state = adamw_state(params)
+    norms = (torch.rand(500, generator=torch.Generator().manual_seed(0)) * 3).tolist() + [0.0, 0.05, 1e30, float("inf")]
+    for norm in norms:
+        norm = torch.tensor(norm)
+        adamw_step(params, grads, **state._asdict(), lr=0.0, betas=(0.0, 0.5), grad_norm=norm.to(device), max_grad_norm=0.05)
+        # 64 bits hold the quotient of two 32-bit numbers to more than twice their places: rounding it again is rounding it once
+        below = (norm + torch.tensor(1e-6)).double()
+        want = min(1.0, float((torch.tensor(0.05).double() / below).float()))
+        assert float(state.exp_avg[0]) == want, float(norm)
