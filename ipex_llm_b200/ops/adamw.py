@@ -277,7 +277,7 @@ def _to_small(m, v, chance_m, chance_v):
     em, ev = _block_exponents(m), _block_exponents(v)
     bits = (m.abs() * _power(134 - em) * 2.0 ** -120).view(torch.int32).long()
     cm = (bits + (chance_m << 4) + 8) >> 20
-    cm = torch.where(m.isfinite(), torch.where(m < 0, cm + 128, cm), 0x7F)
+    cm = torch.where(m.isfinite(), torch.where(m.signbit(), cm + 128, cm), 0x7F)
     bits = (v * _power(141 - ev) * 2.0 ** -112).view(torch.int32).long()
     cv = (bits + (chance_v << 5) + 16) >> 21
     cv = torch.where(v > 0, cv.clamp(min=1), cv)

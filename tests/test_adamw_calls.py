@@ -34,3 +34,24 @@ def test_the_clipping_factor_is_a_quotient_rounded_once(device):
         below = (norm + torch.tensor(1e-6)).double()
         want = min(1.0, float((torch.tensor(0.05).double() / below).float()))
         assert float(state.exp_avg[0]) == want, float(norm)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("largest", [0.0, 1.0, float("inf")])
+def test_zeros_keep_their_sign(device, largest):
+    """Of first moments in 8 bits, as in 32: codes are the same on both sides."""
+    grads = [torch.zeros(300, device=device)]
+    grads[0][1::2] = -0.0
+    grads[0][0] = largest                                         # the block's exponent, or what does not count for it
+    params = [torch.zeros(300, device=device)]
+    state = adamw_state(params, 8)
+    for _ in range(2):
+        adamw_step(params, grads, **state._asdict(), lr=0.1, betas=(0.0, 0.5))
+        codes = state.exp_avg.view(torch.uint8).tolist()
+        # with beta 0, moments are (0 m) + g: of -0 after 0 it is 0, of -0 after -0 it is -0
+        assert not any(codes[2:300:2]) and not any(codes[300:])
+    state = adamw_state(params, 8)
+    state.exp_avg.view(torch.uint8)[:300] = 0x80
+    adamw_step(params, grads, **state._asdict(), lr=0.1, betas=(0.5, 0.5))
+    codes = state.exp_avg.view(torch.uint8).tolist()
+    assert codes[1:300:2] == [0x80] * 150 and not any(codes[2:300:2]) and not any(codes[300:])
