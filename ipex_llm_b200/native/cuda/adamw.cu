@@ -9,7 +9,8 @@
 // sizes come with the launch, as its parameters, and CTAs take tiles of 2048 elements, each of one tensor.
 //
 // Every operation is one of IEEE's, rounded to nearest, in the order written above, none contracted: results do not depend on how
-// the work is split, and 8-bit moments can be told bit by bit.
+// the work is split, and 8-bit moments can be told bit by bit.  The one exception: a change below 2^-62 in size, which no parameter
+// from 2^-37 on notices, may be off in its last bits (see change_usual).
 //
 // Moments in 8 bits: 256 elements (a warp's) share an exponent e, that of the largest of them; m / 2^(e - 134) is held in e4m3, so
 // that the largest lies in [2^7, 2^8), and v / 2^(e - 141) in e5m2 (the largest in [2^14, 2^15): v spans twice m's octaves).  A step
@@ -32,7 +33,9 @@ constexpr int kNormParts = 2;               // of a thread's in a tile of the no
 constexpr int kBlock = 256;                 // elements with a common exponent: a warp's
 static_assert(kBlock == 32 * kVec, "a warp has a block");
 constexpr int kLow = 32, kHigh = 254;       // exponents of a block: 2^(e - 127)
-constexpr int kCtas = 4;                    // to an SM (three, with more registers, take 3 % longer for 240 x 40960 with 32-bit moments)
+// To an SM: 64 registers, at which the forms with 8-bit moments spill 16 to 24 bytes a thread.  Three, with up to 80 and no spills, are
+// slower all the same: 240 x 40960 with 32-bit moments 40.9 -> 42.2 us, with 8-bit ones 31.7 -> 34.1, 202M with 8-bit ones 537 -> 658.
+constexpr int kCtas = 4;
 // SMs do not all run at one speed: 32 times as many CTAs are launched at most, of a few tiles each (one tile to a CTA where there are
 // fewer).  202M elements with 8-bit moments took 597 us with the CTAs that stay and 547 so, 240 x 40960 with 32-bit ones 46 and 42, 12.6M
 // of fp16 with copies and 8-bit moments 56 and 44.  A CTA's tiles lie far apart: with two neighbours to a CTA, what is read at a time has
@@ -297,8 +300,9 @@ __device__ __forceinline__ float change_any(float m, float v, const Factors& f, 
 // The update's change, -m rate / (sqrt(v) root + eps), where every number is of a usual size: roots by Newton's step from an
 // approximate 1 / sqrt, quotients by Newton's step for the reciprocal and Markstein's for the quotient, with signs such that none has
 // to be turned.  All are the nearest numbers: the root and the reciprocal for every fraction there is (tested), the quotient by
-// Markstein's theorem, as long as remainders are exact: while m rate is 0 or above 2^-100 in size; v is taken times 2^64, with 2^-102
-// for 0, which no other v notices, or eps absorbs.  17 instructions for two elements; the general root and division take three
+// Markstein's theorem, as long as remainders are exact: while m rate is 0 or above 2^-100 in size (below, the quotient by a divisor of
+// 2^-38 or more is below 2^-62, and its last bits may be others); v is taken times 2^64, with 2^-102 for 0, which no other v
+// notices, or eps absorbs.  17 instructions for two elements; the general root and division take three
 // times as many, and a branch each.
 __device__ __forceinline__ Pair change_usual(Pair m, Pair v, const Factors& f, float eps, float zero) {
   const Pair u = fma2(v, both(-0x1p64f), both(-0x1p-102f));       // -2^64 v

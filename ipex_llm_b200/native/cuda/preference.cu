@@ -33,7 +33,10 @@ namespace cg = cooperative_groups;
 constexpr int kNT = 256;
 constexpr int kU = 4;                       // vectors of a lane in a batch
 constexpr int kBatch = 32 * kU;             // vectors of a batch
-constexpr int kCtas = 4, kGradCtas = 3;     // to an SM
+// To an SM: 64 registers for the sums, which spill 36 to 52 bytes a thread there, 80 for gradients (8 to 24 bytes).  One CTA less of
+// each, without spills, is as fast within 2 %: 2048 x 32000 68 and 67 us for both passes, 4096 x 32000 118 and 119.5, 2048 x 128256 214
+// and 210.
+constexpr int kCtas = 4, kGradCtas = 3;
 constexpr int kRun = 16;                    // batches of a warp's run, at most where a warp has many
 constexpr int kSlots = 18;                  // runs that may have a part in a row, at most; one of its batches each
 

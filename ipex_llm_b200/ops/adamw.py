@@ -2,7 +2,8 @@
 all gradients.
 
 On CUDA tensors the package's own kernels run, on the current stream of the tensors' device; on the CPU it is the same arithmetic in
-plain PyTorch, operation by operation, so that both give the same bits (but for a root or a power of the factors common to all).
+plain PyTorch, operation by operation, so that both give the same bits (but for a root or a power of the factors common to all, and
+the last bits of changes below 2^-62).
 """
 from __future__ import annotations
 
