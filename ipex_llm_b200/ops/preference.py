@@ -71,8 +71,8 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, reference: Opti
     - "ipo": ``(h - 1 / (2 beta))^2``
 
     The gradient goes to the logits alone (in their type: 16 or 32 bits), from the losses and from the sequences' log probabilities.
-    A target outside of the vocabulary raises on the CPU; on the GPU its pair's results are NaN, and ``cuda_ops.check_error_flag``
-    reports 61.
+    A hidden target (a logit of -inf) makes its sequence's log probability -inf, and a loss that compares two such numbers NaN.  A target
+    outside of the vocabulary raises on the CPU; on the GPU its pair's results are NaN, and ``cuda_ops.check_error_flag`` reports 61.
     """
     what = "preference_loss"
     cuda = logits.is_cuda
